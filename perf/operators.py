@@ -5,7 +5,7 @@ power-of-two fp32 scale per page and head, [pages, Hk]; a value is code * scale.
 [B, W] names each sequence's pages in order (-1: none).  The three operators:
 
 append     count[b] new tokens of sequence b go to positions start[b], start[b] + 1, ...  Per
-           page and head the scale is the smallest 2^e (|e| <= 120) with max |x| <= 448 * 2^e
+           page and head the scale is the smallest 2^e (-120 <= e <= 119) with max |x| <= 448 * 2^e
            over every token written since the page was empty; tokens already in a page whose
            scale grows are rounded again to the new one.
 read       the values of positions 0 .. max_len - 1 in bf16, zero past a sequence's length.
@@ -21,7 +21,7 @@ import torch
 own = False
 
 D = 128
-E_MIN, E_MAX = -120, 120
+E_MIN, E_MAX = -120, 119
 
 
 # ------------------------------------------------------------------------------------ cases
