@@ -43,6 +43,7 @@ EXPORTED = (
     "demon_nvfp4_linear_noalloc", "demon_test_arm_gemm_stall",
     "demon_bf16_linear", "demon_adanorm_quantize", "demon_silu_mul_quantize", "demon_head_norm_rope",
     "demon_attention", "demon_attention_args_size",
+    "demon_kv_append", "demon_kv_read", "demon_kv_attention", "demon_kv_struct_sizes",
 )
 
 _vp = ctypes.c_void_p
@@ -98,6 +99,44 @@ class DemonAttnArgs(ctypes.Structure):
     ]
 
 
+class DemonKvCache(ctypes.Structure):
+    _fields_ = [
+        ("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp),
+        ("pages", _i64), ("heads", _i32), ("page_size", _i32), ("head_dim", _i32), ("reserved", _i32),
+    ]
+
+
+class DemonKvAppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", DemonKvCache),
+        ("k", _vp), ("k_seq", _i64), ("k_row", _i64), ("k_head", _i64),
+        ("v", _vp), ("v_seq", _i64), ("v_row", _i64), ("v_head", _i64),
+        ("table", _vp), ("ld_table", _i64), ("start", _vp), ("count", _vp),
+        ("B", _i32), ("S", _i32), ("W", _i32), ("reserved", _i32),
+    ]
+
+
+class DemonKvReadArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", DemonKvCache),
+        ("k_out", _vp), ("k_seq", _i64), ("k_row", _i64),
+        ("v_out", _vp), ("v_seq", _i64), ("v_row", _i64),
+        ("table", _vp), ("ld_table", _i64), ("lens", _vp),
+        ("B", _i32), ("max_len", _i32), ("W", _i32), ("reserved", _i32),
+    ]
+
+
+class DemonKvAttnArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", DemonKvCache),
+        ("q", _vp), ("q_seq", _i64), ("q_row", _i64), ("q_head", _i64),
+        ("o", _vp), ("o_seq", _i64), ("o_row", _i64), ("o_head", _i64),
+        ("table", _vp), ("ld_table", _i64), ("lens", _vp), ("q_lens", _vp),
+        ("B", _i32), ("Sq", _i32), ("Hq", _i32), ("W", _i32),
+        ("causal", _i32), ("window", _i32), ("scale", _f32), ("reserved", _i32),
+    ]
+
+
 class DemonError(RuntimeError):
     """A C-ABI call returned a non-zero status (message from demon_last_error)."""
 
@@ -143,6 +182,10 @@ def load() -> ctypes.CDLL:
         L.demon_silu_mul_quantize.argtypes = [_vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp]
         L.demon_head_norm_rope.argtypes = [_vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _f32, _vp]
         L.demon_attention.argtypes = [ctypes.POINTER(DemonAttnArgs), _vp]
+        L.demon_kv_append.argtypes = [ctypes.POINTER(DemonKvAppendArgs), _vp]
+        L.demon_kv_read.argtypes = [ctypes.POINTER(DemonKvReadArgs), _vp]
+        L.demon_kv_attention.argtypes = [ctypes.POINTER(DemonKvAttnArgs), _vp]
+        L.demon_kv_struct_sizes.argtypes = [ctypes.POINTER(_i64)] * 3
         for name in EXPORTED:
             getattr(L, name).restype = (_i64 if name in ("demon_nvfp4_sf_bytes", "demon_nvfp4_noalloc_scratch_bytes",
                                                          "demon_attention_args_size") else ctypes.c_int)
@@ -155,6 +198,11 @@ def load() -> ctypes.CDLL:
         if L.demon_attention_args_size() != ctypes.sizeof(DemonAttnArgs):
             raise RuntimeError(f"ABI mismatch: C sizeof(DemonAttnArgs)={L.demon_attention_args_size()} vs "
                                f"{ctypes.sizeof(DemonAttnArgs)}")
+        kv = (_i64(), _i64(), _i64())
+        L.demon_kv_struct_sizes(*map(ctypes.byref, kv))
+        for c, py in zip(kv, (DemonKvAppendArgs, DemonKvReadArgs, DemonKvAttnArgs)):
+            if c.value != ctypes.sizeof(py):
+                raise RuntimeError(f"ABI mismatch: C sizeof({py.__name__})={c.value} vs {ctypes.sizeof(py)}")
         _lib = L
     return _lib
 

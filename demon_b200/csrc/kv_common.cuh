@@ -1,0 +1,49 @@
+// kv_common.cuh -- device helpers of the paged E4M3 K/V cache kernels.
+#pragma once
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "demon_common.cuh"
+#include "kv_index.h"
+
+namespace demon {
+namespace kv {
+
+// The cache as the kernels see it.  Page p, head h: P x 128 codes at ((p * heads + h) * P) * 128,
+// one scale at p * heads + h.
+struct Cache {
+  uint8_t* codes[2];  // K, V
+  float* scale[2];
+  int64_t pages;
+  int heads, P;
+};
+
+// Four E4M3 codes -> two packed f16 pairs (exact: E4M3 values are f16 values).
+__device__ __forceinline__ void e4m3x4_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(w));
+}
+__device__ __forceinline__ float2 f16x2_f32(uint32_t h) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+// Two fp32 values -> E4M3 codes, nearest even, saturating at +-448 (infinities too); NaN stays
+// NaN.  `a` in the low byte.
+__device__ __forceinline__ uint32_t e4m3x2(float a, float b) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(b), "f"(a));
+  return r;
+}
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+  return e4m3x2(a, b) | (e4m3x2(c, d) << 16);
+}
+// 2^e for -126 <= e <= 127.
+__device__ __forceinline__ float exp2i(int e) { return __int_as_float((e + 127) << 23); }
+// Exponent of a power-of-two scale, brought into the range that the cache uses.
+__device__ __forceinline__ int scale_exp(float s) {
+  return imin(imax((int)((__float_as_uint(s) >> 23) & 255u) - 127, kMinExp), kMaxExp);
+}
+
+}  // namespace kv
+}  // namespace demon

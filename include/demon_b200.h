@@ -367,6 +367,105 @@ typedef struct DemonAttnArgs {
 DEMON_API int demon_attention(const DemonAttnArgs* args, void* stream);
 DEMON_API int64_t demon_attention_args_size(void);
 
+/*
+ * Paged 8-bit K/V cache.  Page p holds page_size tokens (16, 32, 64 or 128) of every kv head:
+ * E4M3 codes k / v [pages, heads, page_size, 128], contiguous, and one fp32 scale per page and
+ * head, k_scale / v_scale [pages, heads], a power of two 2^e, -120 <= e <= 119.  A value is
+ * code * scale (exact in bf16).  A page table [B, W] (row pitch ld_table entries) lists each
+ * sequence's pages in order: token t of sequence b lies in page table[b][t / page_size], at
+ * t % page_size.  Sequences may share pages that are only read.
+ * Stands next to the bf16 K / V that DemonDiT keeps for the cross attention of a condition
+ * (acestep/models/modeling_acestep_v15_turbo.py:320-345 recomputes them per call).
+ * Lengths, starts, counts and table entries are read on the device.  One out of range (a length
+ * outside [0, W * page_size], a page id outside [0, pages) where a page is needed) sets
+ * DEMON_DEV_BAD_ARG in the status word; what it concerns is left out: nothing is appended for
+ * the sequence or page, a read gives zeros, attention clamps the length and does not see the
+ * page's keys.
+ */
+typedef struct DemonKvCache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int64_t pages;
+  int32_t heads, page_size, head_dim, reserved;
+} DemonKvCache;
+
+/*
+ * Append: tokens i < count[b] (count NULL: all S) of k / v [B, S, heads, 128] bf16 go to
+ * positions start[b] + i of sequence b.  Element (b, i, h, d) of k sits at
+ * k + b * k_seq + i * k_row + h * k_head + d (strides in elements, multiples of 8).
+ * Per page, head and half (K, V): e is the smallest exponent with max |x| <= 448 * 2^e over the
+ * finite new values (at most 119), at least the page's present e when it holds tokens before
+ * start[b]; codes are x * 2^-e rounded to nearest even (infinities, and magnitudes above
+ * 448 * 2^119, saturate; NaN stays NaN), and when e grew the earlier tokens' codes are rounded
+ * to it.  Tokens of a page at or after start[b] + count[b]
+ * keep their codes (they mean nothing under a new scale).  The pages that one call writes must
+ * be different for different sequences.
+ */
+typedef struct DemonKvAppendArgs {
+  DemonKvCache cache;
+  const void* k;
+  int64_t k_seq, k_row, k_head;
+  const void* v;
+  int64_t v_seq, v_row, v_head;
+  const int32_t* table;
+  int64_t ld_table;
+  const int32_t* start; /* [B] */
+  const int32_t* count; /* [B] or NULL */
+  int32_t B, S, W, reserved;
+} DemonKvAppendArgs;
+
+DEMON_API int demon_kv_append(const DemonKvAppendArgs* args, void* stream);
+
+/*
+ * Read back: k_out / v_out [B, max_len, heads, 128] bf16 (sequence and row pitches in elements,
+ * multiples of 8; heads contiguous) = the values of positions 0 .. lens[b] - 1, zeros from there.
+ */
+typedef struct DemonKvReadArgs {
+  DemonKvCache cache;
+  void* k_out;
+  int64_t k_seq, k_row;
+  void* v_out;
+  int64_t v_seq, v_row;
+  const int32_t* table;
+  int64_t ld_table;
+  const int32_t* lens; /* [B] */
+  int32_t B, max_len, W, reserved;
+} DemonKvReadArgs;
+
+DEMON_API int demon_kv_read(const DemonKvReadArgs* args, void* stream);
+
+/*
+ * Attention of queries over the cache: q, o [B, Sq, Hq, 128] bf16 (strides in elements,
+ * multiples of 8), Hq a multiple of the kv heads.  lens[b] keys; q_lens[b] queries (NULL: Sq),
+ * query i at position lens[b] - q_lens[b] + i.  Key j is seen when j < lens[b], j <= position
+ * (causal) and |position - j| <= window (window >= 0).  o = softmax(scale * q . k) v over the
+ * keys seen, zeros for a query that sees none and for rows i >= q_lens[b].  Keys that a query
+ * does not see never reach it, whatever their codes (NaN included).  fp32 scores, sums and
+ * accumulators; the probabilities are rounded to f16.
+ */
+typedef struct DemonKvAttnArgs {
+  DemonKvCache cache;
+  const void* q;
+  int64_t q_seq, q_row, q_head;
+  void* o;
+  int64_t o_seq, o_row, o_head;
+  const int32_t* table;
+  int64_t ld_table;
+  const int32_t* lens;   /* [B] */
+  const int32_t* q_lens; /* [B] or NULL */
+  int32_t B, Sq, Hq, W;
+  int32_t causal, window; /* window -1: no band */
+  float scale;
+  int32_t reserved;
+} DemonKvAttnArgs;
+
+DEMON_API int demon_kv_attention(const DemonKvAttnArgs* args, void* stream);
+
+/* sizeof of the three argument structs as compiled, for binding checks. */
+DEMON_API int demon_kv_struct_sizes(int64_t* append_args, int64_t* read_args, int64_t* attn_args);
+
 #ifdef __cplusplus
 }
 #endif

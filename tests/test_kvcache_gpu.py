@@ -1,0 +1,560 @@
+"""GPU parity of the paged 8-bit K/V cache against its definition in 64 bits (kv_reference.py).
+
+append and read are exact: codes, scales and bf16 values must be equal bit for bit (a scale is a
+power of two and a value has four significant bits).  attention is compared element by element
+with the bound derived in kv_reference.attention: half a step of bf16 for the output, half a step
+of f16 for the probabilities, fp32 sums.
+"""
+import pytest
+import torch
+
+import kv_reference as R
+
+pytestmark = pytest.mark.gpu
+
+BAD_ARG = 0x2
+
+
+def ok():
+    from demon_b200 import _native as nat
+    torch.cuda.synchronize()
+    assert nat.device_status() == (0, 0)
+
+
+def make_table(lens, P, dev, seed, extra=2, width=None):
+    """Random distinct pages for sequences of these capacities: (device table, nested lists, pages)."""
+    need = [-(-n // P) for n in lens]
+    pages = sum(need) + extra
+    order = torch.randperm(pages, generator=torch.Generator().manual_seed(seed)).tolist()
+    W = width or max(1, max(need))
+    rows, at = [], 0
+    for n in need:
+        rows.append(order[at:at + n] + [-1] * (W - n))
+        at += n
+    return torch.tensor(rows, dtype=torch.int32, device=dev), rows, pages
+
+
+def i32(values, dev):
+    return torch.tensor(values, dtype=torch.int32, device=dev)
+
+
+def filled(lens, P, heads, dev, seed, spread=1.0, k_scale_by=None, v_scale_by=None):
+    """A cache holding random values at these lengths, its twin, and the table."""
+    from demon_b200 import kvcache
+    table, rows, pages = make_table(lens, P, dev, seed)
+    cache = kvcache.KVCache.empty(pages, heads, P, dev)
+    ref = R.RefCache(pages, heads, P, dev)
+    g = torch.Generator().manual_seed(seed + 1)
+    S = max(1, max(lens))
+    x = [torch.randn(len(lens), S, heads, 128, generator=g).to(dev) * spread for _ in range(2)]
+    for i, by in enumerate((k_scale_by, v_scale_by)):
+        if by is not None:
+            x[i] = x[i] * by(torch.arange(S, device=dev)).view(1, S, 1, 1)
+    k, v = (t.to(torch.bfloat16) for t in x)
+    kvcache.append(cache, k, v, table, i32([0] * len(lens), dev), i32(lens, dev))
+    ref.append(k, v, rows, [0] * len(lens), lens)
+    return cache, ref, table, rows
+
+
+def same_cache(cache, ref, rows, lens):
+    """Codes of every held position, scales of every held page, bit for bit."""
+    for kv, (c, s) in enumerate(((cache.k, cache.k_scale), (cache.v, cache.v_scale))):
+        P = ref.P
+        for row, n in zip(rows, lens):
+            for i in range(-(-n // P)):
+                m = min(P, n - i * P)
+                got, want = c[row[i], :, :m].double(), ref.codes[kv, row[i], :, :m]
+                assert torch.equal(torch.nan_to_num(got, nan=999.0), torch.nan_to_num(want, nan=999.0))
+                assert torch.equal(s[row[i]].double(), torch.exp2(ref.exp[kv, row[i]].double()))
+
+
+# ------------------------------------------------------------------------------------ append
+
+@pytest.mark.parametrize("P", [16, 32, 64, 128])
+@pytest.mark.parametrize("heads", [1, 3, 8])
+def test_append_matches_definition_over_several_writes(cuda, P, heads):
+    """Prompts, then odd chunks, then single tokens, growing amplitudes: the scales of partly
+    filled pages grow and their codes are rounded again; counts of zero write nothing."""
+    from demon_b200 import kvcache
+    B = 3
+    caps = [2 * P + 5, 7 * P, 3 * P - 1]
+    table, rows, pages = make_table(caps, P, cuda, P + heads)
+    cache, ref = kvcache.KVCache.empty(pages, heads, P, cuda), R.RefCache(pages, heads, P, cuda)
+    g = torch.Generator().manual_seed(P)
+    start = [0, 0, 0]
+    for step, (S, count) in enumerate([(P + 3, [P + 3, 1, P // 2]), (7, [0, 7, 5]), (1, [1, 1, 0]), (1, [1, 1, 1]),
+                                       (P - 3, [P - 3, P - 3, 1])]):
+        k, v = (torch.randn(B, S, heads, 128, generator=g).mul(3.0 ** step * 0.01).to(torch.bfloat16).to(cuda)
+                for _ in range(2))
+        kvcache.append(cache, k, v, table, i32(start, cuda), i32(count, cuda))
+        ref.append(k, v, rows, start, count)
+        start = [a + b for a, b in zip(start, count)]
+        same_cache(cache, ref, rows, start)
+    ok()
+
+
+def test_append_reads_strided_halves_of_one_projection(cuda):
+    """k and v as the two halves of a [B * L, 2 * heads * 128] projection, without count."""
+    from demon_b200 import kvcache
+    B, S, heads, P = 2, 77, 4, 32
+    kv = torch.randn(B * S, 2 * heads * 128, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).to(cuda)
+    ld = kv.stride(0)
+    k = kv.as_strided((B, S, heads, 128), (S * ld, ld, 128, 1))
+    v = kv.as_strided((B, S, heads, 128), (S * ld, ld, 128, 1), heads * 128)
+    table, rows, pages = make_table([S, S], P, cuda, 4)
+    cache, ref = kvcache.KVCache.empty(pages, heads, P, cuda), R.RefCache(pages, heads, P, cuda)
+    kvcache.append(cache, k, v, table, i32([0, 0], cuda))
+    ref.append(k, v, rows, [0, 0], [S, S])
+    same_cache(cache, ref, rows, [S, S])
+    # head-major inputs [B, heads, S, 128], transposed by strides only
+    kt, vt = k.transpose(1, 2).contiguous().transpose(1, 2), v.transpose(1, 2).contiguous().transpose(1, 2)
+    again = kvcache.KVCache.empty(pages, heads, P, cuda)
+    kvcache.append(again, kt, vt, table, i32([0, 0], cuda))
+    assert torch.equal(again.k.view(torch.uint8), cache.k.view(torch.uint8))
+    ok()
+
+
+def test_append_extreme_values(cuda):
+    """Zeros, the smallest and largest magnitudes, infinities and NaN, and every boundary of the
+    scale rule (448 * 2^e and its bf16 neighbours; above 448 * 2^119 values saturate)."""
+    from demon_b200 import kvcache
+    P, heads = 16, 2
+    edge = [0.0, 448.0, 450.0, 446.0, 2.0 ** -133, 3.3895e38, -3.3895e38, 2.0 ** -120, 1.75 * 2.0 ** 100, 1.7578125 * 2.0 ** 100,
+            float("inf"), float("-inf"), float("nan"), -0.0, 1e-30, 65504.0]
+    n = len(edge)
+    x = torch.zeros(1, n * P, heads, 128)
+    for i, a in enumerate(edge):   # one page each: the edge value, small company, and zeros
+        x[0, i * P + 3, 0, 5] = a
+        x[0, i * P:(i + 1) * P, 1, :] = a
+        if a not in (0.0,):
+            x[0, i * P + 4, 0, :64] = torch.randn(64, generator=torch.Generator().manual_seed(i)) * 0.5
+    x = x.to(torch.bfloat16).to(cuda)
+    table, rows, pages = make_table([n * P], P, cuda, 9)
+    cache, ref = kvcache.KVCache.empty(pages, heads, P, cuda), R.RefCache(pages, heads, P, cuda)
+    kvcache.append(cache, x, -x, table, i32([0], cuda))
+    ref.append(x, -x, rows, [0], [n * P])
+    same_cache(cache, ref, rows, [n * P])
+    k, v = kvcache.read(cache, table, i32([n * P], cuda), n * P)
+    for kv, got in enumerate((k, v)):
+        want = ref.values(kv, rows[0], n * P).transpose(0, 1)
+        assert torch.equal(torch.nan_to_num(got[0].double(), nan=123.0), torch.nan_to_num(want, nan=123.0))
+    ok()
+
+
+def test_append_leaves_other_tokens_and_pages_alone(cuda):
+    from demon_b200 import kvcache
+    cache, ref, table, rows = filled([50, 20], 16, 2, cuda, 5)
+    before = cache.k.view(torch.uint8).clone()
+    x = torch.full((2, 4, 2, 128), 1e-3, dtype=torch.bfloat16, device=cuda)     # below the page's scale
+    kvcache.append(cache, x, x, table, i32([30, 0], cuda), i32([2, 0], cuda))
+    after = cache.k.view(torch.uint8)
+    changed = (after != before).flatten(1).any(1).nonzero().flatten().tolist()
+    assert changed in ([], [rows[0][1]])
+    page_b, page_a = before[rows[0][1]], after[rows[0][1]]
+    assert torch.equal(page_b[:, :14], page_a[:, :14])                           # tokens 16 .. 29
+    ref.append(x, x, rows, [30, 0], [2, 0])
+    same_cache(cache, ref, rows, [32, 20])
+    ok()
+
+
+def test_append_again_changes_nothing(cuda):
+    from demon_b200 import kvcache
+    cache, _, table, _ = filled([37], 32, 2, cuda, 6)
+    x = torch.randn(1, 9, 2, 128, generator=torch.Generator().manual_seed(1)).mul(40).to(torch.bfloat16).to(cuda)
+    kvcache.append(cache, x, x, table, i32([20], cuda))
+    one = [t.view(torch.uint8).clone() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale)]
+    kvcache.append(cache, x, x, table, i32([20], cuda))
+    two = [t.view(torch.uint8) for t in (cache.k, cache.v, cache.k_scale, cache.v_scale)]
+    assert all(torch.equal(a, b) for a, b in zip(one, two))
+
+
+# ------------------------------------------------------------------------------------ read
+
+@pytest.mark.parametrize("P,heads", [(16, 1), (32, 8), (64, 3), (128, 2)])
+def test_read_gives_the_values_and_zeros_behind(cuda, P, heads):
+    from demon_b200 import kvcache
+    lens = [0, 1, P, 2 * P + 3, 5 * P - 1]
+    cache, ref, table, rows = filled(lens, P, heads, cuda, P)
+    for max_len in (max(lens), 1, P + 2, max(lens) + 40):
+        held = [min(n, max_len) for n in lens]
+        k, v = kvcache.read(cache, table, i32(lens, cuda), max_len)
+        for kv, got in enumerate((k, v)):
+            for b, n in enumerate(held):
+                assert torch.equal(got[b, :n].double(), ref.values(kv, rows[b], lens[b])[:, :n].transpose(0, 1))
+                assert not bool(got[b, n:].any())
+    ok()
+
+
+def test_read_into_strided_outputs(cuda):
+    from demon_b200 import kvcache
+    lens, heads = [40, 7], 2
+    cache, _, table, _ = filled(lens, 16, heads, cuda, 8)
+    want = kvcache.read(cache, table, i32(lens, cuda), 40)
+    both = torch.full((2, 43, 3, 2, heads, 128), 7.0, dtype=torch.bfloat16, device=cuda)
+    out = (both[:, :40, 0, 0], both[:, :40, 1, 1])
+    got = kvcache.read(cache, table, i32(lens, cuda), 40, out=out)
+    assert got[0].data_ptr() == out[0].data_ptr()
+    assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+    assert bool((both[:, 40:] == 7).all()) and bool((both[:, :, 2] == 7).all())
+    ok()
+
+
+# ------------------------------------------------------------------------------------ attention
+
+def check_attention(cuda, cache, ref, rows, table, lens, q, q_lens=None, causal=False, window=None, scale=None,
+                    label="", **kw):
+    from demon_b200 import kvcache
+    o = kvcache.attention(q, cache, table, i32(lens, cuda), causal=causal, window=window, scale=scale,
+                          q_lens=None if q_lens is None else i32(q_lens, cuda), **kw)
+    sc = 128 ** -0.5 if scale is None else scale
+    for b, n in enumerate(lens):
+        nq = q.shape[1] if q_lens is None else q_lens[b]
+        k, v = ref.values(0, rows[b], n), ref.values(1, rows[b], n)
+        want, own = R.attention(q[b].double(), k, v, nq, causal, window, sc)
+        got = o[b].double()
+        assert torch.equal(torch.isnan(got), torch.isnan(want)), f"{label} b={b}: NaN elsewhere"
+        err = torch.where(torch.isnan(want), torch.zeros_like(want), (got - want).abs())
+        room = torch.where(torch.isnan(want), torch.ones_like(want), R.error_bound(want, own))
+        worst = float((err / room).max()) if err.numel() else 0.0
+        assert worst <= 1.0, f"{label} b={b}: {worst:.3f} of the allowed error"
+        assert not bool(got[nq:].any())
+    ok()
+    return o
+
+
+def queries(B, Sq, Hq, dev, seed, by=1.0):
+    return (torch.randn(B, Sq, Hq, 128, generator=torch.Generator().manual_seed(seed)) * by).to(torch.bfloat16).to(dev)
+
+
+@pytest.mark.parametrize("P", [16, 32, 64, 128])
+@pytest.mark.parametrize("Hq,Hk", [(1, 1), (16, 8), (6, 2), (7, 1), (16, 1), (40, 2)])
+def test_single_tokens(cuda, P, Hq, Hk):
+    lens = [0, 1, 15, P, P + 1, 63, 64, 65, 700]
+    cache, ref, table, rows = filled(lens, P, Hk, cuda, P + Hq)
+    q = queries(len(lens), 1, Hq, cuda, Hq)
+    check_attention(cuda, cache, ref, rows, table, lens, q, causal=True, label=f"P={P} {Hq}/{Hk}")
+
+
+@pytest.mark.parametrize("causal,window", [(True, None), (False, None), (True, 0), (True, 37), (False, 20), (True, 5000)])
+@pytest.mark.parametrize("Sq,Hq,Hk,P", [(2, 16, 8, 64), (5, 8, 1, 16), (17, 6, 2, 32), (40, 4, 4, 128), (130, 4, 2, 64),
+                                        (300, 2, 1, 16), (129, 3, 1, 64), (257, 8, 1, 32)])
+def test_chunks_masks_and_ragged_batches(cuda, causal, window, Sq, Hq, Hk, P):
+    """Fewer keys than queries (rows that see nothing), no keys, ragged queries, odd lengths."""
+    lens = [0, 1, Sq - 1, Sq, 333, 64]
+    q_lens = [Sq, Sq, Sq, 1, max(1, Sq // 2), 0]
+    cache, ref, table, rows = filled(lens, P, Hk, cuda, Sq + P)
+    q = queries(len(lens), Sq, Hq, cuda, Sq)
+    check_attention(cuda, cache, ref, rows, table, lens, q, None, causal, window, label="all rows")
+    check_attention(cuda, cache, ref, rows, table, lens, q, q_lens, causal, window, label="ragged")
+
+
+@pytest.mark.parametrize("Sq,Hq,Hk", [(1, 8, 2), (3, 8, 2), (200, 4, 2)])
+def test_long_caches(cuda, Sq, Hq, Hk):
+    lens = [5000, 4097, 128]
+    cache, ref, table, rows = filled(lens, 64, Hk, cuda, 77)
+    check_attention(cuda, cache, ref, rows, table, lens, queries(3, Sq, Hq, cuda, 5), causal=True)
+    check_attention(cuda, cache, ref, rows, table, lens, queries(3, Sq, Hq, cuda, 5), causal=True, window=1000)
+
+
+@pytest.mark.parametrize("Sq", [1, 9, 150])
+def test_growing_maxima_and_large_scores(cuda, Sq):
+    """Later keys dominate (the running maximum moves in every tile), scores of some hundreds."""
+    cache, ref, table, rows = filled([640], 32, 1, cuda, 3, k_scale_by=lambda t: 0.1 + t / 80.0)
+    check_attention(cuda, cache, ref, rows, table, [640], queries(1, Sq, 4, cuda, 4, 4.0), causal=False)
+
+
+@pytest.mark.parametrize("Sq", [1, 9, 150])
+@pytest.mark.parametrize("step", [3, 11, 40, -3, -11, -40])
+def test_page_scales_far_apart(cuda, Sq, step):
+    """V's scale rises or falls by 2^step from page to page (up to 2^80 in all)."""
+    n_pages = max(2, 80 // abs(step))
+    n = 16 * n_pages
+    by = lambda t: torch.exp2((t // 16).double() * step).float()   # noqa: E731
+    cache, ref, table, rows = filled([n], 16, 1, cuda, 21, v_scale_by=by)
+    check_attention(cuda, cache, ref, rows, table, [n], queries(1, Sq, 2, cuda, 4), causal=True)
+
+
+@pytest.mark.parametrize("Sq", [1, 6, 160])
+@pytest.mark.parametrize("q_by,k_by,v_by", [(1e30, 1e-30, 1e-38), (1e-30, 1e30, 1e37), (1e-38, 1.0, 1.0), (0.0, 1.0, 1.0)])
+def test_extreme_magnitudes(cuda, Sq, q_by, k_by, v_by):
+    cache, ref, table, rows = filled([150], 32, 1, cuda, 31, k_scale_by=lambda t: torch.full_like(t, k_by, dtype=torch.float32),
+                                     v_scale_by=lambda t: torch.full_like(t, v_by, dtype=torch.float32))
+    check_attention(cuda, cache, ref, rows, table, [150], queries(1, Sq, 2, cuda, 4, q_by), causal=True)
+
+
+@pytest.mark.parametrize("Sq", [1, 5, 24, 140])
+def test_nan_reaches_only_the_rows_that_see_it(cuda, Sq):
+    """NaN codes past the length (stale pages), in keys hidden by the causal mask or the band,
+    and in keys that some rows see: V's NaN marks its channel, K's its whole row."""
+    lens = [200, 200 - 7, 64]
+    cache, ref, table, rows = filled([208, 208, 64], 16, 2, cuda, 41)
+    for kv, t in enumerate((cache.k, cache.v)):
+        for row, n in zip(rows, lens):
+            for page in range(len([r for r in row if r >= 0])):
+                for tok in range(16):
+                    if page * 16 + tok >= n:
+                        t.view(torch.uint8)[row[page], :, tok] = 0x7F     # stale: never seen
+    def poison(kv, b, tok, ch):
+        (cache.k, cache.v)[kv].view(torch.uint8)[rows[b][tok // 16], 1, tok % 16, ch] = 0xFF
+        ref.codes[kv, rows[b][tok // 16], 1, tok % 16, ch] = float("nan")
+    poison(1, 0, 199, 77)       # the last key: seen by the last row alone (causal)
+    poison(1, 0, 150, 3)
+    poison(0, 1, 192, 0)        # a key whose score is NaN
+    poison(1, 2, 10, 127)
+    q = queries(3, Sq, 4, cuda, Sq)
+    for causal, window in ((True, None), (True, 30), (False, 25), (False, None)):
+        check_attention(cuda, cache, ref, rows, table, lens, q, None, causal, window, label=f"{causal} {window}")
+
+
+def test_strided_queries_and_outputs(cuda):
+    from demon_b200 import kvcache
+    lens = [90, 33]
+    cache, ref, table, rows = filled(lens, 32, 2, cuda, 51)
+    for Sq in (1, 3, 140):
+        wide = torch.randn(2, Sq + 3, 3, 5, 128, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(cuda)
+        q = wide[:, 1:Sq + 1, 1, :4]
+        buf = torch.full((2, Sq + 2, 2, 6, 128), 9.0, dtype=torch.bfloat16, device=cuda)
+        out = buf[:, 1:Sq + 1, 0, 1:5]
+        want = check_attention(cuda, cache, ref, rows, table, lens, q.contiguous(), causal=True)
+        got = kvcache.attention(q, cache, table, i32(lens, cuda), causal=True, out=out)
+        assert got.data_ptr() == out.data_ptr() and torch.equal(out, want)
+        rest = buf.clone()
+        rest[:, 1:Sq + 1, 0, 1:5] = 9.0
+        assert bool((rest == 9).all())
+        qt = q.contiguous().transpose(1, 2).contiguous().transpose(1, 2)          # head-major
+        assert torch.equal(kvcache.attention(qt, cache, table, i32(lens, cuda), causal=True), want)
+
+
+def test_shared_pages(cuda):
+    """Two sequences over the same condition pages, a third with its own."""
+    cache, ref, table, rows = filled([100, 60], 32, 2, cuda, 61)
+    t3, r3 = torch.stack([table[0], table[0], table[1]]), [rows[0], rows[0], rows[1]]
+    q = queries(3, 20, 4, cuda, 1)
+    check_attention(cuda, cache, ref, r3, t3, [100, 70, 60], q)
+
+
+def test_pages_beyond_32_bit_offsets(cuda):
+    """Codes that lie past 2^32 bytes of the buffers."""
+    from demon_b200 import kvcache
+    P, heads = 128, 8
+    pages = (1 << 32) // (P * heads * 128) + 64
+    codes = [torch.empty(pages, heads, P, 128, dtype=torch.uint8, device=cuda).view(torch.float8_e4m3fn) for _ in range(2)]
+    scales = [torch.full((pages, heads), 2.0 ** -120, device=cuda) for _ in range(2)]
+    cache = kvcache.KVCache(*codes, *scales)
+    small, ref, _, rows = filled([300], P, heads, cuda, 71)
+    moved = [pages - 1 - i for i in range(3)]
+    table = i32([moved], cuda)
+    k, v = kvcache.read(small, i32([rows[0][:3]], cuda), i32([300], cuda), 300)
+    kvcache.append(cache, k, v, table, i32([0], cuda))
+    k2, v2 = kvcache.read(cache, table, i32([300], cuda), 300)
+    assert torch.equal(k, k2) and torch.equal(v, v2)
+    for Sq in (1, 150):
+        q = queries(1, Sq, 16, cuda, 2)
+        o = kvcache.attention(q, cache, table, i32([300], cuda), causal=True)
+        assert torch.equal(o, kvcache.attention(q, small, i32([rows[0][:3]], cuda), i32([300], cuda), causal=True))
+    ok()
+
+
+# ------------------------------------------------------------------------------------ as it is used
+
+def test_a_sequence_grows_token_by_token_and_graphs_replay(cuda):
+    """Prompt, then tokens one at a time through one captured graph (append + attention) whose
+    lengths and inputs change between replays; equal to the eager calls, bit for bit."""
+    from demon_b200 import kvcache
+    heads, Hq, P, B = 2, 4, 16, 2
+    table, rows, pages = make_table([90, 90], P, cuda, 81)
+    g = torch.Generator().manual_seed(5)
+    prompt = [torch.randn(B, 40, heads, 128, generator=g).to(torch.bfloat16).to(cuda) for _ in range(2)]
+    steps = [[torch.randn(B, 1, n, 128, generator=g).mul(1 + t / 5).to(torch.bfloat16).to(cuda) for n in (heads, heads, Hq)]
+             for t in range(40)]
+    out = []
+    for graphed in (False, True):
+        cache, ref = kvcache.KVCache.empty(pages, heads, P, cuda), R.RefCache(pages, heads, P, cuda)
+        start, lens = i32([0, 0], cuda), i32([40, 31], cuda)
+        kvcache.append(cache, *prompt, table, start, lens)
+        ref.append(*prompt, rows, [0, 0], [40, 31])
+        k, v, q = (t.clone() for t in steps[0])
+        pos = lens.clone()
+
+        def step():
+            kvcache.append(cache, k, v, table, pos)
+            return kvcache.attention(q, cache, table, pos + 1, causal=True)
+        got = []
+        if graphed:
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                keep = [t.view(torch.uint8).clone() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale)]
+                step()
+                for t, u in zip((cache.k, cache.v, cache.k_scale, cache.v_scale), keep):
+                    t.view(torch.uint8).copy_(u)
+            torch.cuda.current_stream().wait_stream(side)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                o = step()
+        for t, (kk, vv, qq) in enumerate(steps):
+            k.copy_(kk), v.copy_(vv), q.copy_(qq)
+            if graphed:
+                graph.replay()
+            else:
+                o = step()
+            got.append(o.clone())
+            pos += 1
+        out.append(torch.stack(got))
+        for t, (kk, vv, _) in enumerate(steps):
+            ref.append(kk, vv, rows, [40 + t, 31 + t], [1, 1])
+        same_cache(cache, ref, rows, [80, 71])
+        check_attention(cuda, cache, ref, rows, table, [80, 71], steps[-1][2], causal=True)
+    assert torch.equal(out[0], out[1])
+    ok()
+
+
+def test_calls_on_other_streams(cuda):
+    """An explicit stream, and two streams at once over one cache, equal the plain call."""
+    from demon_b200 import kvcache
+    cache, _, table, _ = filled([3000, 2000], 64, 2, cuda, 91)
+    lens = i32([3000, 2000], cuda)
+    q = queries(2, 1, 4, cuda, 1)
+    q2 = queries(2, 200, 4, cuda, 2)
+    want, want2 = kvcache.attention(q, cache, table, lens, causal=True), kvcache.attention(q2, cache, table, lens, causal=True)
+    kv = kvcache.read(cache, table, lens, 3000)
+    torch.cuda.synchronize()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    got = []
+    for _ in range(10):
+        got.append((kvcache.attention(q, cache, table, lens, causal=True, stream=a),
+                    kvcache.attention(q2, cache, table, lens, causal=True, stream=b),
+                    kvcache.read(cache, table, lens, 3000, stream=a)))
+    torch.cuda.synchronize()
+    for x, y, z in got:
+        assert torch.equal(x, want) and torch.equal(y, want2) and torch.equal(z[0], kv[0]) and torch.equal(z[1], kv[1])
+    ok()
+
+
+def test_repeated_calls_give_equal_bits(cuda):
+    from demon_b200 import kvcache
+    cache, _, table, _ = filled([4000, 100, 999], 32, 2, cuda, 92)
+    lens = i32([4000, 100, 999], cuda)
+    for Sq in (1, 4, 70, 300):
+        q = queries(3, Sq, 8, cuda, Sq)
+        first = kvcache.attention(q, cache, table, lens, causal=True)
+        for _ in range(5):
+            assert torch.equal(kvcache.attention(q, cache, table, lens, causal=True), first)
+
+
+# ------------------------------------------------------------------------------------ refusals
+
+def test_bad_device_values_are_reported_and_harmless(cuda):
+    """Page ids, lengths and starts out of range (checked on the CPU in test_kvcache.py): the
+    status word says so, other sequences are right, nothing else is written."""
+    from demon_b200 import _native as nat
+    from demon_b200 import kvcache
+    lens = [60, 60, 60]
+    cache, ref, table, rows = filled(lens, 16, 2, cuda, 95)
+    before = cache.k.view(torch.uint8).clone()
+    x = torch.randn(3, 4, 2, 128, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).to(cuda)
+    for bad in ([62, -1, 1 << 30], [61, 2147483647, -2147483648]):      # past the table's 64 positions
+        kvcache.append(cache, x, x, table, i32(bad, cuda))
+        torch.cuda.synchronize()
+        assert nat.device_status()[0] == BAD_ARG
+    for count in ([5, -1, 2147483647],):
+        kvcache.append(cache, x, x, table, i32([0, 0, 0], cuda), i32(count, cuda))
+        torch.cuda.synchronize()
+        assert nat.device_status()[0] == BAD_ARG
+    assert torch.equal(cache.k.view(torch.uint8), before)
+    hurt = table.clone()
+    hurt[1, 1], hurt[2, 0] = 1 << 20, -5
+    kvcache.append(cache, x, x, hurt, i32([60, 20, 2], cuda), i32([0, 4, 4], cuda))
+    torch.cuda.synchronize()
+    assert nat.device_status()[0] == BAD_ARG and torch.equal(cache.k.view(torch.uint8), before)
+    k, _ = kvcache.read(cache, hurt, i32([60, 60, 99999], cuda), 60)
+    torch.cuda.synchronize()
+    assert nat.device_status()[0] == BAD_ARG
+    assert torch.equal(k[0].double(), ref.values(0, rows[0], 60).transpose(0, 1))
+    assert not bool(k[1, 16:32].any()) and bool(k[1, :16].any()) and not bool(k[2, :16].any())
+    good = kvcache.attention(queries(3, 1, 4, cuda, 1), cache, table, i32(lens, cuda))
+    for Sq in (1, 140):
+        q = queries(3, Sq, 4, cuda, 1)
+        good = kvcache.attention(q, cache, table, i32(lens, cuda))
+        got = kvcache.attention(q, cache, hurt, i32([60, 60, -3], cuda))
+        torch.cuda.synchronize()
+        assert nat.device_status()[0] == BAD_ARG
+        assert torch.equal(got[0], good[0]) and not bool(got[2].any())
+        # a page that is not there is a page that no query sees
+        left = R.RefCache(1, 2, 16, cuda)
+        k1, v1 = (torch.cat([ref.values(kv, rows[1], 60)[:, :16], ref.values(kv, rows[1], 60)[:, 32:]], 1) for kv in (0, 1))
+        want, own = R.attention(q[1].double(), k1, v1, Sq, False, None, 128 ** -0.5)
+        assert bool(((got[1].double() - want).abs() <= R.error_bound(want, own)).all())
+        del left
+    ok()
+
+
+def test_refusals(cuda):
+    from demon_b200 import _native as nat
+    from demon_b200 import kvcache
+    cache, _, table, _ = filled([40, 40], 16, 2, cuda, 96)
+    lens = i32([40, 40], cuda)
+    q = queries(2, 1, 4, cuda, 1)
+    x = queries(2, 3, 2, cuda, 1)
+    with pytest.raises(nat.DemonError, match="multiple of the kv heads"):
+        kvcache.attention(queries(2, 1, 3, cuda, 1), cache, table, lens)
+    with pytest.raises(nat.DemonError, match="window"):
+        kvcache.attention(q, cache, table, lens, window=-2)
+    with pytest.raises(nat.DemonError, match="scale"):
+        kvcache.attention(q, cache, table, lens, scale=0.0)
+    with pytest.raises(ValueError, match="bf16"):
+        kvcache.attention(q.half(), cache, table, lens)
+    with pytest.raises(ValueError, match="int32"):
+        kvcache.attention(q, cache, table, lens.long())
+    with pytest.raises(ValueError, match="int32"):
+        kvcache.attention(q, cache, table.long(), lens)
+    with pytest.raises(ValueError, match="table"):
+        kvcache.attention(q, cache, table[:1], lens)
+    with pytest.raises(ValueError, match="head_dim"):
+        kvcache.attention(q[..., :64], cache, table, lens)
+    with pytest.raises(ValueError, match="out"):
+        kvcache.attention(q, cache, table, lens, out=q[:, :, :2])
+    with pytest.raises(ValueError, match="cuda"):
+        kvcache.attention(q.cpu(), cache, table, lens)
+    odd = torch.zeros(2, 1, 4, 132, dtype=torch.bfloat16, device=cuda)[..., :128]
+    with pytest.raises(nat.DemonError, match="multiples of 8"):
+        kvcache.attention(odd, cache, table, lens)
+    shifted = torch.zeros(2 * 4 * 128 + 8, dtype=torch.bfloat16, device=cuda)[4:4 + 2 * 4 * 128].view(2, 1, 4, 128)
+    with pytest.raises(nat.DemonError, match="aligned"):
+        kvcache.attention(shifted, cache, table, lens)
+    with pytest.raises(ValueError, match="heads"):
+        kvcache.append(cache, x[:, :, :1], x[:, :, :1], table, lens)
+    with pytest.raises(ValueError, match="start"):
+        kvcache.append(cache, x, x, table, lens[:1])
+    with pytest.raises(ValueError, match="count"):
+        kvcache.append(cache, x, x, table, lens, lens.float())
+    with pytest.raises(ValueError, match="equal"):
+        kvcache.append(cache, x, x[:, :2], table, lens)
+    with pytest.raises(ValueError, match="lens"):
+        kvcache.read(cache, table, lens[:1], 40)
+    with pytest.raises(ValueError, match="out k"):
+        kvcache.read(cache, table, lens, 40, out=(x, x))
+    with pytest.raises(nat.DemonError, match="overlap"):
+        same = torch.empty(1, 40, 2, 128, dtype=torch.bfloat16, device=cuda).expand(2, 40, 2, 128)
+        kvcache.read(cache, table, lens, 40, out=(same, same))
+    ok()
+
+
+def test_empty_calls(cuda):
+    """No sequences, no tokens, no queries, no table columns."""
+    from demon_b200 import kvcache
+    cache, _, table, _ = filled([40, 40], 16, 2, cuda, 97)
+    none = torch.empty(0, table.shape[1], dtype=torch.int32, device=cuda)
+    e = torch.empty(0, dtype=torch.int32, device=cuda)
+    lens = i32([40, 40], cuda)
+    assert kvcache.attention(queries(0, 1, 4, cuda, 1), cache, none, e).shape == (0, 1, 4, 128)
+    assert kvcache.attention(queries(2, 0, 4, cuda, 1), cache, table, lens).shape == (2, 0, 4, 128)
+    kvcache.append(cache, queries(0, 3, 2, cuda, 1), queries(0, 3, 2, cuda, 1), none, e)
+    kvcache.append(cache, queries(2, 0, 2, cuda, 1), queries(2, 0, 2, cuda, 1), table, lens)
+    assert kvcache.read(cache, none, e, 5)[0].shape == (0, 5, 2, 128)
+    assert kvcache.read(cache, table, lens, 0)[0].shape == (2, 0, 2, 128)
+    thin = torch.empty(2, 0, dtype=torch.int32, device=cuda)
+    for Sq in (1, 140):
+        assert not bool(kvcache.attention(queries(2, Sq, 4, cuda, 1), cache, thin, i32([0, 0], cuda)).any())
+    assert not bool(kvcache.read(cache, thin, i32([0, 0], cuda), 9)[0].any())
+    ok()
