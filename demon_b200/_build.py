@@ -24,7 +24,8 @@ CSRC = PKG / "csrc"
 OBJ = PKG / "_build"
 LIB = PKG / "libdemon_b200.so"
 SOURCES = ["capi.cu", "nvfp4_quant.cu", "nvfp4_gemm.cu", "ode_step.cu", "nvfp4_noalloc.cu", "dit_ops.cu",
-           "attention.cu", "kvcache.cu", "kv_attention.cu"]
+           "attention.cu", "kvcache.cu", "kv_attention.cu",
+           "kv_attention_tc.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -33,21 +33,6 @@
 namespace demon {
 namespace kv {
 
-struct AttnParams {
-  Cache c;
-  const __nv_bfloat16* q;
-  int64_t q_seq, q_row, q_head;
-  __nv_bfloat16* o;
-  int64_t o_seq, o_row, o_head;
-  const int32_t *table, *lens, *q_lens;
-  int64_t ld_table;
-  int B, Sq, Hq, G, W;
-  int causal, window;  // window < 0: no band
-  float scale_log2;    // softmax scale * log2(e)
-  int n_rt;            // row tiles per kv head
-  unsigned int* status;
-};
-
 namespace small {
 
 constexpr int kTile = 64;                  // keys per stage
@@ -75,16 +60,6 @@ struct Join {
   static_assert(kEnd <= offScale, "partial results must fit into the ring");
 };
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -97,17 +72,6 @@ __device__ __forceinline__ float quad_max(float x) {
 __device__ __forceinline__ float quad_sum(float x) {
   x += __shfl_xor_sync(0xffffffffu, x, 1);
   return x + __shfl_xor_sync(0xffffffffu, x, 2);
-}
-// 0x80 in every byte of w that is E4M3's NaN.
-__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
-
-__device__ __forceinline__ float ld_shared_f32(uint32_t a) {
-  float v;
-  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
-  return v;
-}
-__device__ __forceinline__ void st_shared_f32x4(uint32_t a, float x, float y, float z, float w) {
-  asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(a), "f"(x), "f"(y), "f"(z), "f"(w) : "memory");
 }
 __device__ __forceinline__ uint32_t map_rank(uint32_t a, uint32_t rank) {
   uint32_t r;
@@ -635,6 +599,7 @@ extern "C" int demon_kv_attention(const DemonKvAttnArgs* a, void* stream) {
     mark_device_done(g_kv_small_attr);
   }
   const int64_t rows = (int64_t)a->Sq * p.G;
+  if (rows > 64) return kv::attention_tc(p, (cudaStream_t)stream);
   const int rt = rows > 16 ? 2 : 1;
   p.n_rt = (int)((rows + 16 * rt - 1) / (16 * rt));
   const int64_t units = (int64_t)a->B * a->cache.heads * p.n_rt;

@@ -45,5 +45,44 @@ __device__ __forceinline__ int scale_exp(float s) {
   return imin(imax((int)((__float_as_uint(s) >> 23) & 255u) - 127, kMinExp), kMaxExp);
 }
 
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// 0x80 in every byte of w that is E4M3's NaN.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
+
+__device__ __forceinline__ float ld_shared_f32(uint32_t a) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ void st_shared_f32x4(uint32_t a, float x, float y, float z, float w) {
+  asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(a), "f"(x), "f"(y), "f"(z), "f"(w) : "memory");
+}
+
+// One attention call, as both attention kernels see it.
+struct AttnParams {
+  Cache c;
+  const __nv_bfloat16* q;
+  int64_t q_seq, q_row, q_head;
+  __nv_bfloat16* o;
+  int64_t o_seq, o_row, o_head;
+  const int32_t *table, *lens, *q_lens;
+  int64_t ld_table;
+  int B, Sq, Hq, G, W;
+  int causal, window;  // window < 0: no band
+  float scale_log2;    // softmax scale * log2(e)
+  int n_rt;            // row tiles (or blocks) per kv head
+  unsigned int* status;
+};
+
 }  // namespace kv
 }  // namespace demon
