@@ -22,11 +22,12 @@
 // Output: O * 2^(M - m - 6) / l.  Both offsets are raised only when exceeded by more than 8.
 //
 // Warp roles (512 threads; setmaxnreg as in attention.cu):
-//   warpgroup 0 / 1   softmax of row half 0 / 1, one query row per thread,
-//   warpgroup 2       Q (cp.async into its slot, converted in place) and the output rows,
+//   warpgroup 0 / 1   row half 0 / 1, one query row per thread: its Q row (copied by cp.async while
+//                     the previous unit's last tile is in work, converted in place), the softmax of
+//                     every key tile, the output row,
+//   warpgroup 2       codes -> f16, swizzled, into a ring of three K / V tiles,
 //   warp 12           MMA issue (one thread) and tensor-memory allocation,
-//   warps 13 - 15     K / V codes: loads of the next half tile stay in flight in registers while
-//                     the ring slot is awaited, then convert, store swizzled, signal.
+//   warp 13           page look-ups, scales, bulk copies of K / V codes into a ring of half tiles.
 // Tensor memory as in attention.cu: S_h at 128 h, P_h over its upper half, O_h at 256 + 128 h.
 //
 // Bound by the exponentials (one per row and key, 16 per clock and SM) and the MMAs, which take
@@ -45,19 +46,19 @@ constexpr int kBlk = 128;                // rows per half, keys per tile
 constexpr int kRows = 2 * kBlk;          // rows per unit
 constexpr int kBox = 128 * 128;          // 64 f16 columns x 128 rows (16 KB)
 constexpr int kTile = 2 * kBox;          // 128 x 128 f16
-constexpr int kSlots = 3;                // K / V ring
-constexpr int kQSlots = 3;               // Q ring (one half of 128 rows each)
+constexpr int kSlots = 3;                // K / V tiles as f16
+constexpr int kRawSlots = 3;             // ring of half tiles (K or V) as codes
+constexpr int kRaw = kBlk * kHeadDim;    // 16 KB
 constexpr int kScSlots = 8;              // tiles whose scales are kept (see the ring comment)
 constexpr int kNanSlots = 4;             // tiles whose NaN maps are kept
-constexpr int kConvWarps = 3;
-constexpr int kItems = 11;               // ceil(32 / kConvWarps) 16-byte loads per lane and half tile
+constexpr int kConvWarps = 4;
 constexpr int kThreads = 512;
 constexpr float kBias = 6.0f;            // P = 2^(.. + 6)
 constexpr float kRaise = 8.0f;           // offsets are raised when exceeded by more than this
 constexpr float kFast = 60.0f;           // |M - m - ev| up to which l comes from P
 
-constexpr int kLaunchRegs = 128, kSoftmaxRegs = 176, kQRegs = 80, kIssueRegs = 80;
-static_assert(256 * kSoftmaxRegs + 128 * kQRegs + 128 * kIssueRegs <= kThreads * kLaunchRegs,
+constexpr int kLaunchRegs = 128, kSoftmaxRegs = 176, kConvRegs = 72, kIssueRegs = 88;
+static_assert(256 * kSoftmaxRegs + 128 * kConvRegs + 128 * kIssueRegs <= kThreads * kLaunchRegs,
               "register split exceeds the launch's registers (setmaxnreg.inc would wait for good)");
 
 // scales of a tile, per 16-key group: K scale, V exponent, 2^(ev_0 - ev_g); then the smallest and
@@ -65,16 +66,16 @@ static_assert(256 * kSoftmaxRegs + 128 * kQRegs + 128 * kIssueRegs <= kThreads *
 constexpr int kScWords = 32;
 constexpr int scK = 0, scEv = 8, scInv = 16, scMin = 24, scMax = 25, scBad = 26;
 
-constexpr int offQ = 0;
-constexpr int offKV = offQ + kQSlots * kTile;
-constexpr int offNan = offKV + kSlots * kTile;                 // [slot][128 keys] 128-bit maps
+constexpr int offQ = 0;                                        // [2 halves]
+constexpr int offKV = offQ + 2 * kTile;
+constexpr int offRaw = offKV + kSlots * kTile;
+constexpr int offNan = offRaw + kRawSlots * kRaw;              // [slot][128 keys] 128-bit maps
 constexpr int offNanRow = offNan + kNanSlots * kBlk * 16;      // [2][128] 128-bit maps
-constexpr int offL = offNanRow + 2 * kBlk * 16;                // [2][128] output factors
-constexpr int offRow = offL + 2 * kBlk * 16;                   // [8][128] rows' powers of two
-constexpr int offSc = offRow + 8 * kBlk * 4;
+constexpr int offSc = offNanRow + 2 * kBlk * 16;
 constexpr int offNanW = offSc + kScSlots * kScWords * 4;       // [slot][warp] any NaN
-constexpr int offBar = offNanW + kScSlots * 4 * 4;
-constexpr int kNumBars = 2 * kQSlots + 2 * kSlots + 14 + 1 + 2 * kScSlots + 8;
+constexpr int offRawMask = offNanW + kScSlots * 4 * 4;         // [slot] 16-key groups copied
+constexpr int offBar = offRawMask + 4 * 4;
+constexpr int kNumBars = 2 + 2 * kSlots + 8 + 1 + 2 * kScSlots + 2 * kRawSlots;
 constexpr int offMisc = offBar + kNumBars * 8;
 constexpr int kSmem = offMisc + 16 + 1024;
 static_assert(kSmem <= 232448, "shared memory exceeds the sm_100 per-block limit");
@@ -173,24 +174,22 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const AttnPar
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + offBar);
-  uint64_t* q_full = bars;                      // [3] Q half converted
-  uint64_t* q_empty = q_full + kQSlots;         // [3] its last S computed
-  uint64_t* kv_full = q_empty + kQSlots;        // [3] K or V tile converted
+  uint64_t* q_full = bars;                      // [2] Q half converted
+  uint64_t* kv_full = q_full + 2;               // [3] K or V tile converted
   uint64_t* kv_empty = kv_full + kSlots;        // [3] its MMAs done
   uint64_t* s_full = kv_empty + kSlots;         // [2] S_h computed
   uint64_t* pa_full = s_full + 2;               // [2] P_h of keys 0-63 in tensor memory
   uint64_t* pb_full = s_full + 4;               // [2] P_h of keys 64-127
   uint64_t* o_full = s_full + 6;                // [2] the unit's last P V done
-  uint64_t* o_empty = s_full + 8;               // [2] O_h read out
-  uint64_t* l_full = s_full + 10;               // [2] output factors written
-  uint64_t* l_empty = s_full + 12;              // [2] output factors read
-  uint64_t* mma_done = s_full + 14;
-  // The scales, NaN maps and row powers have rings longer than any lag between their writers and
-  // readers: K tile t + 2 waits for the slot of a tile whose Q K^T was issued after the softmax of
-  // tile t - 1 published its P, and Q of unit i + 4 for a Q slot of unit i + 2.
+  uint64_t* mma_done = s_full + 8;
+  // The scales and NaN maps have rings longer than any lag between their writers and readers: V of
+  // tile t takes the slot of K of tile t - 1, whose Q K^T were issued after both softmax warpgroups
+  // published P of tile t - 2, and so were done with tile t - 3; the codes of tile t are copied
+  // at most two tiles before that.
   uint64_t* sc_full = mma_done + 1;             // [8] scales of a tile
   uint64_t* nan_full = sc_full + kScSlots;      // [8] NaN map of a tile
-  uint64_t* row_full = nan_full + kScSlots;     // [8] rows' powers of a Q half
+  uint64_t* raw_full = nan_full + kScSlots;     // [3] codes of a half tile copied
+  uint64_t* raw_empty = raw_full + kRawSlots;   // [3] and converted
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + offMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + offMisc + 4);
 
@@ -198,28 +197,25 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const AttnPar
   const uint64_t t0 = globaltimer();
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kQSlots; ++s) {
-      mbar_init(&q_full[s], 4);
-      mbar_init(&q_empty[s], 1);
-    }
     for (int s = 0; s < kSlots; ++s) {
       mbar_init(&kv_full[s], kConvWarps);
       mbar_init(&kv_empty[s], 1);
     }
     for (int h = 0; h < 2; ++h) {
+      mbar_init(&q_full[h], 4);
       mbar_init(&s_full[h], 1);
       mbar_init(&pa_full[h], 4);
       mbar_init(&pb_full[h], 4);
       mbar_init(&o_full[h], 1);
-      mbar_init(&o_empty[h], 4);
-      mbar_init(&l_full[h], 4);
-      mbar_init(&l_empty[h], 4);
     }
     mbar_init(mma_done, 1);
+    for (int s = 0; s < kRawSlots; ++s) {
+      mbar_init(&raw_full[s], 1);
+      mbar_init(&raw_empty[s], kConvWarps);
+    }
     for (int s = 0; s < kScSlots; ++s) {
       mbar_init(&sc_full[s], 1);
       mbar_init(&nan_full[s], kConvWarps);
-      mbar_init(&row_full[s], 4);
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -244,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const AttnPar
         uint32_t g = 0, it = 0, tiles = 0;  // half tiles consumed, units, key tiles (all units)
         bool ok = true;
         auto qk = [&](int h, uint32_t kslot) {
-          const uint32_t qa = sbase + offQ + ((2 * it + h) % kQSlots) * kTile, kb = sbase + offKV + kslot * kTile;
+          const uint32_t qa = sbase + offQ + h * kTile, kb = sbase + offKV + kslot * kTile;
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)
             mma_bf16(tmem + kColS + 128 * h, kmajor_desc(qa, kk), kmajor_desc(kb, kk), idesc_qk, kk > 0);
@@ -272,10 +268,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const AttnPar
           pv(h, vslot, 1, true);
           return true;
         };
-        auto wait_oe = [&](int h) { return wait_on(&o_empty[h], (it & 1u) ^ 1u, 74); };
-        auto wait_q = [&](int h) { return wait_on(&q_full[(2 * it + h) % kQSlots], ((2 * it + h) / kQSlots) & 1u, 75); };
-        auto free_q = [&](int h) { tc_commit(&q_empty[(2 * it + h) % kQSlots]); };
-        // as in attention.cu: a unit's last P_1 V goes after the next unit's first S_0
+        auto wait_q = [&](int h) { return wait_on(&q_full[h], it & 1u, 75); };
+        // As in attention.cu, a unit's last P_1 V goes after the next unit's first S_0.  A unit's first
+        // P_h V may overwrite O_h: its P_h comes from threads that have stored the last unit's rows.
         bool pend = false, pend_acc = false;
         uint32_t pend_v = 0, pend_t = 0;
         auto flush = [&]() {
@@ -293,12 +288,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const AttnPar
           uint32_t gk = g, gv = g + 1;
           if (!wait_q(0) || !wait_kv(gk)) break;
           qk(0, gk % kSlots);
-          if (n == 1) free_q(0);
           if (!flush() || !wait_q(1)) break;
           qk(1, gk % kSlots);
           tc_commit(&kv_empty[gk % kSlots]);
-          if (n == 1) free_q(1);
-          if (!wait_kv(gv) || !wait_oe(0) || !pv_tile(0, gv % kSlots, tiles, false)) break;
+          if (!wait_kv(gv) || !pv_tile(0, gv % kSlots, tiles, false)) break;
           uint32_t prev_v = gv;
           g += 2;
           for (int i = 1; i < n; ++i) {
@@ -306,20 +299,16 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const AttnPar
             gv = g + 1;
             if (!wait_kv(gk)) break;
             qk(0, gk % kSlots);
-            if (i == n - 1) free_q(0);
-            if (i == 1 && !wait_oe(1)) break;
             if (!pv_tile(1, prev_v % kSlots, tiles + i - 1, i - 1 > 0)) break;
             tc_commit(&kv_empty[prev_v % kSlots]);
             qk(1, gk % kSlots);
             tc_commit(&kv_empty[gk % kSlots]);
-            if (i == n - 1) free_q(1);
             if (!wait_kv(gv) || !pv_tile(0, gv % kSlots, tiles + i, true)) break;
             prev_v = gv;
             g += 2;
           }
           if (!ok) break;
           tc_commit(&o_full[0]);
-          if (n == 1 && !wait_oe(1)) break;  // this unit's only P_1 V overwrites O_1
           pend = true;
           pend_v = prev_v;
           pend_t = tiles + n - 1;
@@ -336,23 +325,20 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const AttnPar
         mbar_wait(mma_done, 0, &never, globaltimer(), p.status, 76);
       }
       __syncwarp();
-    } else {
-      // ------------------------------------------------------------------ K / V codes
-      const int cw = warp - 13, c = lane & 3, rl = lane >> 2;
-      uint4 r[kItems];
-      uint32_t g = 0, tiles = 0, j = 0;
-      Unit w, nw;         // the unit being converted, the one of the next tile
-      int tile = 0;       // key tile of w within its range
-      int pid = -1;       // lanes 0 .. 7: page of their 16 keys of the current tile, -1: none seen
-      int npid = -1;      // and of the next tile
-      float sk = 0.0f, sv = 0.0f, nsk = 0.0f, nsv = 0.0f;
-      bool absent = false, nabsent = false;  // a seen group without a page
+    } else if (warp == 13) {
+      // ------------------------------------------------------------------ pages, scales, copies
+      uint32_t n = 0, tiles = 0, j = 0;  // half tiles, tiles
+      Unit w;
+      int tile = 0;
+      int pid = -1;  // lanes 0 .. 7: page of their 16 keys of the tile, -1: none seen
+      float sk = 0.0f, sv = 0.0f;
+      bool absent = false;  // seen keys without a page
+      constexpr int gw = kBlk / NG;  // keys that share a page within a tile
       auto look_up = [&](const Unit& u, int t, int& pg, float& k, float& v, bool& gone) {
         pg = -1;
         k = v = 0.0f;
         gone = false;
-        const int key = (u.tile0 + t) * kBlk + 16 * lane, gw = kBlk / NG;
-        const int gk = key & ~(gw - 1);  // first key of the group that has one scale
+        const int key = (u.tile0 + t) * kBlk + 16 * lane, gk = key & ~(gw - 1);
         if (lane < 8 && gk < u.ks.hi && gk + gw > u.ks.lo) {
           pg = page_id(p.table + u.b * p.ld_table, p.W, key / p.c.P, p.c.pages);
           if (pg >= 0) {
@@ -360,166 +346,286 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const AttnPar
             v = __ldg(p.c.scale[1] + (int64_t)pg * p.c.heads + u.hk);
           } else {
             gone = true;
-            if (cw == 0) report(p.status, DEMON_DEV_BAD_ARG, 64);
+            report(p.status, DEMON_DEV_BAD_ARG, 64);
           }
         }
       };
-      // item n = cw + 3 i: rows 8 (n / 2) .. + 7 of the tile, 64-code half n % 2
-      auto load = [&](const Unit& u, int t, int pg, int kv) {
-        const int k0 = (u.tile0 + t) * kBlk;
-#pragma unroll
-        for (int i = 0; i < kItems; ++i) {
-          const int n = cw + kConvWarps * i;
-          r[i] = make_uint4(0, 0, 0, 0);
-          const int pgi = __shfl_sync(0xffffffffu, pg, (n >> 2) & 7);
-          if (n < 32 && pgi >= 0) {
-            const int key = k0 + 8 * (n >> 1) + rl;
-            const int64_t at = (((int64_t)pgi * p.c.heads + u.hk) * p.c.P + (key & (p.c.P - 1))) * kHeadDim + 64 * (n & 1) + 16 * c;
-            r[i] = __ldg(reinterpret_cast<const uint4*>(p.c.codes[kv] + at));
-          }
-        }
-      };
-      auto store = [&](uint32_t dst, int i, int n) {
-        const int row = 8 * (n >> 1) + rl;
-        uint32_t x[8];
-        e4m3x4_f16(r[i].x, x[0], x[1]);
-        e4m3x4_f16(r[i].y, x[2], x[3]);
-        e4m3x4_f16(r[i].z, x[4], x[5]);
-        e4m3x4_f16(r[i].w, x[6], x[7]);
-        const uint32_t a = dst + (n & 1) * kBox + row * 128;
-        st_shared_v4(a + (((2 * c) ^ rl) << 4), x[0], x[1], x[2], x[3]);
-        st_shared_v4(a + (((2 * c + 1) ^ rl) << 4), x[4], x[5], x[6], x[7]);
-      };
-      bool have = next_unit(p, units, &j, &w);
-      if (have) {
-        look_up(w, 0, pid, sk, sv, absent);
-        load(w, 0, pid, 0);
-      }
-      bool ok = true;
+      bool ok = true, have = next_unit(p, units, &j, &w);
+      if (have) look_up(w, 0, pid, sk, sv, absent);
       while (have && ok) {
-        // the tile after this one
-        bool more = true;
-        int ntile = tile + 1;
-        if (ntile < w.nt) {
-          nw = w;
-        } else {
+        // the next tile's pages and scales are on their way while this one's copies wait for room
+        Unit nw = w;
+        bool more = true, nabsent = false;
+        int ntile = tile + 1, npid = -1;
+        float nsk = 0.0f, nsv = 0.0f;
+        if (ntile >= w.nt) {
           more = next_unit(p, units, &j, &nw);
           ntile = 0;
         }
         if (more) look_up(nw, ntile, npid, nsk, nsv, nabsent);
-        // K
-        if (!(ok = warp_wait(&kv_empty[g % kSlots], ((g / kSlots) & 1u) ^ 1u, abort_flag, t0, p.status, 77))) break;
-        uint32_t dst = sbase + offKV + (g % kSlots) * kTile;
-#pragma unroll
-        for (int i = 0; i < kItems; ++i)
-          if (cw + kConvWarps * i < 32) store(dst, i, cw + kConvWarps * i);
-        if (cw == 0) {
-          const uint32_t sc = sbase + offSc + (tiles % kScSlots) * kScWords * 4;
-          const uint32_t held = __ballot_sync(0xffffffffu, lane < 8 && pid >= 0);
-          const uint32_t gone = __ballot_sync(0xffffffffu, absent);
-          // groups without a page take another group's V exponent: they weigh nothing
-          const int any = held ? __ffs(held) - 1 : 0;
-          int ev = scale_exp(sv);
-          const int ev_any = __shfl_sync(0xffffffffu, ev, any);
-          if (pid < 0) ev = ev_any;
-          const int ev0 = __shfl_sync(0xffffffffu, ev, 0);
-          if (lane >= 8) ev = ev0;
-          const int lo = __reduce_min_sync(0xffffffffu, ev), hi = __reduce_max_sync(0xffffffffu, ev);
-          if (lane < 8) {
-            st_shared_f32(sc + 4 * (scK + lane), fabsf(sk));
-            st_shared_f32(sc + 4 * (scEv + lane), (float)ev);
-            st_shared_f32(sc + 4 * (scInv + lane), exp2i(imin(imax(ev0 - ev, -126), 126)));
-          }
+        const uint32_t held = __ballot_sync(0xffffffffu, pid >= 0), gone = __ballot_sync(0xffffffffu, absent);
+        const uint32_t sc = sbase + offSc + (tiles % kScSlots) * kScWords * 4;
+        // keys without a page take another group's V exponent: they weigh nothing
+        int ev = scale_exp(sv);
+        const int ev_any = __shfl_sync(0xffffffffu, ev, held ? __ffs(held) - 1 : 0);
+        if (pid < 0) ev = ev_any;
+        const int ev0 = __shfl_sync(0xffffffffu, ev, 0);
+        if (lane >= 8) ev = ev0;
+        const int elo = __reduce_min_sync(0xffffffffu, ev), ehi = __reduce_max_sync(0xffffffffu, ev);
+        if (lane < 8) {
+          st_shared_f32(sc + 4 * (scK + lane), fabsf(sk));
+          st_shared_f32(sc + 4 * (scEv + lane), (float)ev);
+          st_shared_f32(sc + 4 * (scInv + lane), exp2i(imin(imax(ev0 - ev, -126), 126)));
+        }
+        if (lane == 0) {
+          st_shared_f32(sc + 4 * scMin, (float)elo);
+          st_shared_f32(sc + 4 * scMax, (float)ehi);
+          st_shared_b32(sc + 4 * scBad, gone);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sc_full[tiles % kScSlots]);
+        const bool copies = pid >= 0 && (16 * lane) % gw == 0;
+        const uint32_t n_copies = __popc(__ballot_sync(0xffffffffu, copies));
+        const int key = (w.tile0 + tile) * kBlk + 16 * lane;
+        const int64_t src = (((int64_t)imax(pid, 0) * p.c.heads + w.hk) * p.c.P + (key & (p.c.P - 1))) * kHeadDim;
+        for (int kv = 0; kv < 2; ++kv, ++n) {
+          const uint32_t s = n % kRawSlots;
+          if (!(ok = warp_wait(&raw_empty[s], ((n / kRawSlots) & 1u) ^ 1u, abort_flag, t0, p.status, 77))) break;
           if (lane == 0) {
-            st_shared_f32(sc + 4 * scMin, (float)lo);
-            st_shared_f32(sc + 4 * scMax, (float)hi);
-            st_shared_b32(sc + 4 * scBad, gone);
+            st_shared_b32(sbase + offRawMask + s * 4, held);
+            mbar_arrive_expect_tx(&raw_full[s], n_copies * gw * kHeadDim);
           }
+          __syncwarp();
+          if (copies) bulk_load(smem + offRaw + s * kRaw + lane * 16 * kHeadDim, p.c.codes[kv] + src, gw * kHeadDim, &raw_full[s]);
         }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&kv_full[g % kSlots]);
-          if (cw == 0) mbar_arrive(&sc_full[tiles % kScSlots]);
-        }
-        ++g;
-        load(w, tile, pid, 1);
-        // V
-        if (!(ok = warp_wait(&kv_empty[g % kSlots], ((g / kSlots) & 1u) ^ 1u, abort_flag, t0, p.status, 78))) break;
-        dst = sbase + offKV + (g % kSlots) * kTile;
-        const int k0 = (w.tile0 + tile) * kBlk;
-        if (k0 < w.ks.lo_all || k0 + kBlk > w.ks.hi_all) {
-          // Some row does not see some key: NaN codes go into a map instead of the product.  (Where
-          // every row sees every key they may run through it.)
-          uint32_t any = 0;
-          const uint32_t map = sbase + offNan + (tiles % kNanSlots) * kBlk * 16;
-#pragma unroll
-          for (int i = 0; i < kItems; ++i) {
-            const int n = cw + kConvWarps * i;
-            if (n >= 32) continue;
-            uint32_t y[4] = {nan_bytes(r[i].x) >> 7, nan_bytes(r[i].y) >> 7, nan_bytes(r[i].z) >> 7, nan_bytes(r[i].w) >> 7};
-            r[i].x &= ~(y[0] * 255u);
-            r[i].y &= ~(y[1] * 255u);
-            r[i].z &= ~(y[2] * 255u);
-            r[i].w &= ~(y[3] * 255u);
-            uint32_t bits = 0;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) bits |= ((y[q] | (y[q] >> 7) | (y[q] >> 14) | (y[q] >> 21)) & 15u) << (4 * q);
-            any |= bits;
-            st_shared_u16(map + (8 * (n >> 1) + rl) * 16 + ((n & 1) * 4 + c) * 2, bits);
-          }
-          any = __reduce_or_sync(0xffffffffu, any);
-          if (lane == 0) st_shared_b32(sbase + offNanW + ((tiles % kScSlots) * 4 + cw) * 4, any);
-        }
-#pragma unroll
-        for (int i = 0; i < kItems; ++i)
-          if (cw + kConvWarps * i < 32) store(dst, i, cw + kConvWarps * i);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&kv_full[g % kSlots]);
-          mbar_arrive(&nan_full[tiles % kScSlots]);
-        }
-        ++g;
-        ++tiles;
+        w = nw;
+        tile = ntile;
+        pid = npid;
+        sk = nsk;
+        sv = nsv;
+        absent = nabsent;
         have = more;
-        if (more) {
-          w = nw;
-          tile = ntile;
-          pid = npid;
-          sk = nsk;
-          sv = nsv;
-          absent = nabsent;
-          load(w, tile, pid, 0);
+        ++tiles;
+      }
+      // no copy may still be in flight when the CTA leaves (immediate on the normal path)
+      volatile int never = 0;
+      for (uint32_t i = n > (uint32_t)kRawSlots ? n - kRawSlots : 0; i < n; ++i)
+        mbar_wait(&raw_full[i % kRawSlots], (i / kRawSlots) & 1u, &never, globaltimer(), p.status, 79);
+      __syncwarp();
+    }
+  } else if (wg == 2) {
+    setmaxnreg_dec<kConvRegs>();
+    // -------------------------------------------------------------------- codes -> f16
+    // Warp cw takes keys 32 cw .. 32 cw + 31: chunk i is 16 codes of row 8 (i / 2) + lane / 4, and
+    // neighbouring rows take opposite halves of their 128 codes (no bank conflicts either way).
+    const int cw = warp & 3, c = lane & 3, rl = lane >> 2;
+    const uint32_t a0 = (uint32_t)rl * 128 + (((2 * c) ^ rl) << 4), a1 = (uint32_t)rl * 128 + (((2 * c + 1) ^ rl) << 4);
+    uint32_t n = 0, tiles = 0, j = 0;
+    bool ok = true;
+    Unit w;
+    while (ok && next_unit(p, units, &j, &w)) {
+      for (int t = 0; ok && t < w.nt; ++t, ++tiles) {
+        const int k0 = (w.tile0 + t) * kBlk;
+        const bool whole = k0 >= w.ks.lo_all && k0 + kBlk <= w.ks.hi_all;
+#pragma unroll 1
+        for (int kv = 0; kv < 2; ++kv, ++n) {
+          const uint32_t s = n % kRawSlots;
+          if (!(ok = warp_wait(&raw_full[s], (n / kRawSlots) & 1u, abort_flag, t0, p.status, 78))) break;
+          const uint32_t held = (ld_shared_b32(sbase + offRawMask + s * 4) >> (2 * cw)) & 3u;
+          const uint32_t src = sbase + offRaw + s * kRaw + (cw * 32 + rl) * kHeadDim + 16 * c;
+          uint4 r[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) r[i] = ld_shared_v4(src + (i >> 1) * 8 * kHeadDim + 64 * ((i & 1) ^ (rl & 1)));
+          if (held != 3u) {  // keys that were not copied: zeros
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (!((held >> (i >> 2)) & 1u)) r[i] = make_uint4(0, 0, 0, 0);
+          }
+          if (!(ok = warp_wait(&kv_empty[n % kSlots], ((n / kSlots) & 1u) ^ 1u, abort_flag, t0, p.status, 86))) break;
+          if (kv && !whole) {
+            // Some row does not see some key: NaN codes go into a map instead of the product.
+            // (Where every row sees every key they may run through it.)
+            const uint32_t map = sbase + offNan + ((tiles % kNanSlots) * kBlk + cw * 32 + rl) * 16;
+            uint32_t any = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const uint32_t y[4] = {nan_bytes(r[i].x) >> 7, nan_bytes(r[i].y) >> 7, nan_bytes(r[i].z) >> 7,
+                                     nan_bytes(r[i].w) >> 7};
+              r[i].x &= ~(y[0] * 255u);
+              r[i].y &= ~(y[1] * 255u);
+              r[i].z &= ~(y[2] * 255u);
+              r[i].w &= ~(y[3] * 255u);
+              uint32_t bits = 0;
+#pragma unroll
+              for (int q = 0; q < 4; ++q) bits |= ((y[q] | (y[q] >> 7) | (y[q] >> 14) | (y[q] >> 21)) & 15u) << (4 * q);
+              any |= bits;
+              st_shared_u16(map + (i >> 1) * 8 * 16 + (((i & 1) ^ (rl & 1)) * 4 + c) * 2, bits);
+            }
+            any = __reduce_or_sync(0xffffffffu, any);
+            if (lane == 0) st_shared_b32(sbase + offNanW + ((tiles % kScSlots) * 4 + cw) * 4, any);
+          }
+          const uint32_t dst = sbase + offKV + (n % kSlots) * kTile + cw * 32 * 128;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            uint32_t x[8];
+            e4m3x4_f16(r[i].x, x[0], x[1]);
+            e4m3x4_f16(r[i].y, x[2], x[3]);
+            e4m3x4_f16(r[i].z, x[4], x[5]);
+            e4m3x4_f16(r[i].w, x[6], x[7]);
+            const uint32_t a = dst + ((i & 1) ^ (rl & 1)) * kBox + (i >> 1) * 8 * 128;
+            st_shared_v4(a + a0, x[0], x[1], x[2], x[3]);
+            st_shared_v4(a + a1, x[4], x[5], x[6], x[7]);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&raw_empty[s]);
+            mbar_arrive(&kv_full[n % kSlots]);
+            if (kv) mbar_arrive(&nan_full[tiles % kScSlots]);
+          }
         }
       }
     }
-  } else if (wg < 2) {
+  } else {
     setmaxnreg_inc<kSoftmaxRegs>();
-    // -------------------------------------------------------------------- softmax
+    // -------------------------------------------------------------------- query rows
     constexpr int GW = kBlk / NG, CH = 8 / NG;  // columns and maximum chains per group
     constexpr int SG = 8 / NG;                  // 16-key scale entries per group
     const int h = wg, quad = warp & 3, rr = quad * 32 + lane;
     const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
     const uint32_t s_addr = tmem + lane_addr + kColS + 128 * h;
     const uint32_t o_addr = tmem + lane_addr + kColO + 128 * h;
-    uint32_t t = 0, it = 0, j = 0;
-    Unit w;
-    while (next_unit(p, units, &j, &w)) {
-      const int64_t row = w.row0 + h * kBlk + rr;
-      const int qi = (int)((uint32_t)row / (uint32_t)p.G);
-      const bool live = row < (int64_t)p.Sq * p.G && qi < w.nq;
-      int jlo = 0, jhi = w.len;  // keys that this row sees: [jlo, jhi)
-      if (live) {
-        const Keys k = visible(qi, qi, w.len, w.nq, p.causal != 0, p.window);
-        jlo = k.lo;
-        jhi = k.hi;
+    const uint32_t q_slot = sbase + offQ + h * kTile;
+    const uint32_t n_rows = (uint32_t)p.Sq * (uint32_t)p.G;
+    // The warp's 32 rows of Q into their slot: rows 2 k + lane / 16, 16 bytes a lane.
+    auto q_load = [&](const Unit& w) {
+      const int sub = lane & 15;
+      uint32_t row = (uint32_t)w.row0 + h * kBlk + quad * 32 + (lane >> 4);
+      int i = (int)(row / (uint32_t)p.G), g = (int)(row - (uint32_t)i * (uint32_t)p.G);
+      const __nv_bfloat16* q = p.q + w.b * p.q_seq + (int64_t)(w.hk * p.G) * p.q_head + sub * 8;
+#pragma unroll 2
+      for (int k = 0; k < 16; ++k) {
+        const int rt = quad * 32 + 2 * k + (lane >> 4);
+        const uint32_t dst = q_slot + (sub >> 3) * kBox + rt * 128 + (((sub & 7) ^ (rt & 7)) << 4);
+        if (row < n_rows && i < w.nq)
+          cp_async_16(dst, q + (int64_t)i * p.q_row + (int64_t)g * p.q_head);
+        else
+          st_shared_v4(dst, 0, 0, 0, 0);
+        row += 2;
+        g += 2;
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          if (g >= p.G) {
+            g -= p.G;
+            ++i;
+          }
       }
-      bool ok = warp_wait(&row_full[(2 * it + h) % 8], ((2 * it + h) / 8) & 1u, abort_flag, t0, p.status, 80);
-      if (!ok) break;
-      const float fr = ld_shared_f32(sbase + offRow + (((2 * it + h) % 8) * kBlk + rr) * 4);
+    };
+    // This thread's row in place: bf16 -> f16 times 2^-e; returns 2^e.
+    auto q_convert = [&]() {
+      cp_async_wait_all();
+      __syncwarp();
+      uint4 x[16];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) x[k] = ld_shared_v4(q_slot + (k >> 3) * kBox + rr * 128 + (((k & 7) ^ (rr & 7)) << 4));
+      uint32_t mx = 0;
+#pragma unroll
+      for (int k = 0; k < 16; ++k)
+        mx = __vmaxu2(mx, __vmaxu2(__vmaxu2(x[k].x & 0x7FFF7FFFu, x[k].y & 0x7FFF7FFFu),
+                                   __vmaxu2(x[k].z & 0x7FFF7FFFu, x[k].w & 0x7FFF7FFFu)));
+      mx = max(mx & 0xFFFFu, mx >> 16);
+      if (mx >= 0x7F80u) {  // infinities and NaN do not count, and pass through
+        mx = 0;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const uint32_t y[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const uint32_t a = y[q] & 0x7FFF7FFFu;
+            mx = __vmaxu2(mx, a & __vcmpltu2(a, 0x7F807F80u));
+          }
+        }
+        mx = max(mx & 0xFFFFu, mx >> 16);
+      }
+      const int e = imax((int)(mx >> 7) - 127 - 13, -126);  // |q| 2^-e < 2^14
+      const float2 mul = make_float2(exp2i(-e), exp2i(-e));
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const float2 f0 = mul_f2(bf2_f2(x[k].x), mul), f1 = mul_f2(bf2_f2(x[k].y), mul), f2 = mul_f2(bf2_f2(x[k].z), mul),
+                     f3 = mul_f2(bf2_f2(x[k].w), mul);
+        st_shared_v4(q_slot + (k >> 3) * kBox + rr * 128 + (((k & 7) ^ (rr & 7)) << 4), pack_f16x2(f0.x, f0.y),
+                     pack_f16x2(f1.x, f1.y), pack_f16x2(f2.x, f2.y), pack_f16x2(f3.x, f3.y));
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full[h]);
+      return exp2i(e) * p.scale_log2;
+    };
+    auto out_row = [&](const Unit& w, bool* inside) {
+      const uint32_t row = (uint32_t)w.row0 + h * kBlk + rr;
+      *inside = row < n_rows;
+      const uint32_t i = row / (uint32_t)p.G, g = row - i * (uint32_t)p.G;
+      return p.o + w.b * p.o_seq + (int64_t)i * p.o_row + (int64_t)(w.hk * p.G + (int)g) * p.o_head;
+    };
+    auto put = [&](__nv_bfloat16* o, const uint32_t (&x)[16]) {  // 32 columns
+      if (wide) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+          asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(o + 16 * q), "r"(x[8 * q]),
+                       "r"(x[8 * q + 1]), "r"(x[8 * q + 2]), "r"(x[8 * q + 3]), "r"(x[8 * q + 4]), "r"(x[8 * q + 5]),
+                       "r"(x[8 * q + 6]), "r"(x[8 * q + 7])
+                       : "memory");
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) st_global_v4(o + 8 * q, make_uint4(x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]));
+      }
+    };
+    // this CTA's next unit; rows of units without keys are zeroed on the way
+    uint32_t j = 0;
+    auto advance = [&](Unit* w) {
+      for (;; ++j) {
+        if ((uint64_t)j * gridDim.x >= units) return false;
+        const uint32_t u = unit_index(j);
+        if (u >= units) continue;
+        bool bad = false;
+        *w = decode(p, u, &bad);
+        if (bad && w->hk == 0 && w->row0 == 0 && threadIdx.x == 0) report(p.status, DEMON_DEV_BAD_ARG, 63);
+        if (w->nt > 0) {
+          ++j;
+          return true;
+        }
+        const uint32_t zero[16] = {};
+        bool inside;
+        __nv_bfloat16* o = out_row(*w, &inside);
+        if (inside)
+          for (int c = 0; c < 4; ++c) put(o + 32 * c, zero);
+      }
+    };
+
+    uint32_t t = 0, it = 0;
+    Unit w, nw;
+    float fr = 0.0f;
+    bool have = advance(&w);
+    if (have) {
+      q_load(w);
+      fr = q_convert();
+    }
+    for (; have; ++it) {
+      int jlo = 0, jhi = w.len;  // keys that this row sees: [jlo, jhi)
+      bool live;
+      {
+        const uint32_t row = (uint32_t)w.row0 + h * kBlk + rr;
+        const int qi = (int)(row / (uint32_t)p.G);
+        live = row < n_rows && qi < w.nq;
+        if (live) {
+          const Keys k = visible(qi, qi, w.len, w.nq, p.causal != 0, p.window);
+          jlo = k.lo;
+          jhi = k.hi;
+        }
+      }
+      const bool more = advance(&nw);
       float M = -INFINITY, m = -INFINITY, l = 0.0f;
-      bool nan_row = false;
+      bool nan_row = false, ok = true;
       for (int i = 0; i < w.nt; ++i, ++t) {
         if (!(ok = warp_wait(&s_full[h], t & 1u, abort_flag, t0, p.status, 81))) break;
         tc_fence_after();
@@ -529,6 +635,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const AttnPar
         tmem_ld_32x32b_x32(s_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(sr + 32));
         tmem_ld_32x32b_x32(s_addr + 64, *reinterpret_cast<uint32_t(*)[32]>(sr + 64));
         tmem_ld_32x32b_x32(s_addr + 96, *reinterpret_cast<uint32_t(*)[32]>(sr + 96));
+        if (i == w.nt - 1 && more) q_load(nw);  // Q of this unit has been used for the last time
         tmem_ld_wait();
         float* s = reinterpret_cast<float*>(sr);
         const uint32_t sc = sbase + offSc + (t % kScSlots) * kScWords * 4;
@@ -562,7 +669,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const AttnPar
 #pragma unroll
           for (int c = 1; c < CH; ++c) gm = fmaxf(gm, mc[c]);
           // kept within 2^+-120: a masked score times 0 would be NaN
-          const float f = fminf(fmaxf(fr * ld_shared_f32(sc + 4 * (scK + gi * SG)) * p.scale_log2, 7.5e-37f), 1.3e36f);
+          const float f = fminf(fmaxf(fr * ld_shared_f32(sc + 4 * (scK + gi * SG)), 7.5e-37f), 1.3e36f);
           const float x = gm * f;
           mt = fmaxf(mt, x);
           Mt = fmaxf(Mt, x + ld_shared_f32(sc + 4 * (scEv + gi * SG)));
@@ -585,7 +692,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const AttnPar
         if (__any_sync(0xffffffffu, far)) {
 #pragma unroll
           for (int c = 0; c < 128; ++c) {
-            const float f = fminf(fmaxf(fr * ld_shared_f32(sc + 4 * (scK + (c / GW) * SG)) * p.scale_log2, 7.5e-37f), 1.3e36f);
+            const float f = fminf(fmaxf(fr * ld_shared_f32(sc + 4 * (scK + (c / GW) * SG)), 7.5e-37f), 1.3e36f);
             l += ex2(fmaf(s[c], f, -ml));
           }
           lw = 0.0f;
@@ -613,7 +720,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const AttnPar
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             const int gi = (32 * c + 16 * half) / GW;
-            const float f = fminf(fmaxf(fr * ld_shared_f32(sc + 4 * (scK + gi * SG)) * p.scale_log2, 7.5e-37f), 1.3e36f);
+            const float f = fminf(fmaxf(fr * ld_shared_f32(sc + 4 * (scK + gi * SG)), 7.5e-37f), 1.3e36f);
             const float n = ld_shared_f32(sc + 4 * (scEv + gi * SG)) - mo + kBias;
             const float2 f2 = make_float2(f, f), n2 = make_float2(n, n);
             float2 acc = make_float2(0.0f, 0.0f);
@@ -635,8 +742,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const AttnPar
         if (lane == 0) mbar_arrive(&pb_full[h]);
         if (k0 < w.ks.lo_all || k0 + kBlk > w.ks.hi_all) {  // the converters left NaN codes of V out
           if (!(ok = warp_wait(&nan_full[t % kScSlots], (t / kScSlots) & 1u, abort_flag, t0, p.status, 83))) break;
-          const uint32_t nw = sbase + offNanW + (t % kScSlots) * 16;
-          if (ld_shared_b32(nw) | ld_shared_b32(nw + 4) | ld_shared_b32(nw + 8)) {
+          const uint32_t nwd = sbase + offNanW + (t % kScSlots) * 16;
+          if (ld_shared_b32(nwd) | ld_shared_b32(nwd + 4) | ld_shared_b32(nwd + 8) | ld_shared_b32(nwd + 12)) {
             uint4 seen = make_uint4(0, 0, 0, 0);
             const uint32_t map = sbase + offNan + (t % kNanSlots) * kBlk * 16;
             for (int c = imax(lo, 0); c <= imin(hi, kBlk - 1); ++c) {
@@ -646,8 +753,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const AttnPar
               seen.z |= x.z;
               seen.w |= x.w;
             }
-            // the row's map is handed over with its output factors: the last unit's must be read
-            if (!(ok = warp_wait(&l_empty[h], (it & 1u) ^ 1u, abort_flag, t0, p.status, 84))) break;
             const uint32_t a = sbase + offNanRow + (h * kBlk + rr) * 16;
             if (nan_row) {
               const uint4 x = ld_shared_v4(a);
@@ -662,184 +767,53 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const AttnPar
         }
       }
       if (!ok) break;
-      if (!warp_wait(&l_empty[h], (it & 1u) ^ 1u, abort_flag, t0, p.status, 85)) break;
-      // output factor 2^(M - m - 6) / l, in two parts that both stay normal
-      float fa = 0.0f, fb = 0.0f;
+      if (more) fr = q_convert();
+      // the output row: O 2^(M - m - 6) / l, the factor in two parts where it is not normal
+      float fa = 1.0f, fb = 0.0f;
       if (live && l != 0.0f) {
-        fa = ex2(0.5f * (M - m - kBias));
-        fb = fa / l;
-      }
-      st_shared_f32x4(sbase + offL + (h * kBlk + rr) * 16, fa, fb, nan_row ? 1.0f : 0.0f, 0.0f);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&l_full[h]);
-      ++it;
-    }
-  } else {
-    setmaxnreg_dec<kQRegs>();
-    // -------------------------------------------------------------------- Q in, output rows out
-    const int quad = warp & 3, rr = quad * 32 + lane, sub = lane & 15;
-    const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
-    const uint32_t n_rows = (uint32_t)p.Sq * (uint32_t)p.G;
-    // rows quad * 32 + 2 k + (lane / 16) of half h: 16 bytes per lane
-    auto q_load = [&](const Unit& w, uint32_t slot, int h) {
-      uint32_t row = (uint32_t)w.row0 + h * kBlk + quad * 32 + (lane >> 4);
-      int i = (int)(row / (uint32_t)p.G), g = (int)(row - (uint32_t)i * (uint32_t)p.G);
-      const __nv_bfloat16* q = p.q + w.b * p.q_seq + (int64_t)(w.hk * p.G) * p.q_head + sub * 8;
-#pragma unroll 4
-      for (int k = 0; k < 16; ++k) {
-        const int rt = quad * 32 + 2 * k + (lane >> 4);
-        const uint32_t dst = sbase + offQ + slot * kTile + (sub >> 3) * kBox + rt * 128 + (((sub & 7) ^ (rt & 7)) << 4);
-        if (row < n_rows && i < w.nq)
-          cp_async_16(dst, q + (int64_t)i * p.q_row + (int64_t)g * p.q_head);
-        else
-          st_shared_v4(dst, 0, 0, 0, 0);
-        row += 2;
-        g += 2;
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-          if (g >= p.G) {
-            g -= p.G;
-            ++i;
-          }
-      }
-    };
-    auto q_convert = [&](uint32_t qi, int h) {
-      cp_async_wait_all();
-      const uint32_t slot = qi % kQSlots;
-#pragma unroll 4
-      for (int k = 0; k < 16; ++k) {
-        const int rt = quad * 32 + 2 * k + (lane >> 4);
-        const uint32_t a = sbase + offQ + slot * kTile + (sub >> 3) * kBox + rt * 128 + (((sub & 7) ^ (rt & 7)) << 4);
-        const uint4 x = ld_shared_v4(a);
-        uint32_t mx = __vmaxu2(__vmaxu2(x.x & 0x7FFF7FFFu, x.y & 0x7FFF7FFFu), __vmaxu2(x.z & 0x7FFF7FFFu, x.w & 0x7FFF7FFFu));
-        mx = max(mx & 0xFFFFu, mx >> 16);
-        if (mx >= 0x7F80u) mx = 0;  // infinities and NaN pass through at any power
-#pragma unroll
-        for (int o = 1; o < 16; o <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        const int e = imax((int)(mx >> 7) - 127 - 13, -126);  // |q| 2^-e < 2^14
-        const float2 mul = make_float2(exp2i(-e), exp2i(-e));
-        const float2 f0 = mul_f2(bf2_f2(x.x), mul), f1 = mul_f2(bf2_f2(x.y), mul), f2 = mul_f2(bf2_f2(x.z), mul),
-                     f3 = mul_f2(bf2_f2(x.w), mul);
-        st_shared_v4(a, pack_f16x2(f0.x, f0.y), pack_f16x2(f1.x, f1.y), pack_f16x2(f2.x, f2.y), pack_f16x2(f3.x, f3.y));
-        if (sub == 0) st_shared_f32(sbase + offRow + ((qi % 8) * kBlk + rt) * 4, exp2i(e));
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&q_full[slot]);
-        mbar_arrive(&row_full[qi % 8]);
-      }
-      (void)h;
-    };
-    auto wait_slot = [&](uint32_t qi) {
-      return warp_wait(&q_empty[qi % kQSlots], ((qi / kQSlots) & 1u) ^ 1u, abort_flag, t0, p.status, 90);
-    };
-    auto out_row = [&](const Unit& w, int h, bool* inside) {
-      const uint32_t row = (uint32_t)w.row0 + h * kBlk + rr;
-      *inside = row < n_rows;
-      const uint32_t i = row / (uint32_t)p.G, g = row - i * (uint32_t)p.G;
-      return p.o + w.b * p.o_seq + (int64_t)i * p.o_row + (int64_t)(w.hk * p.G + (int)g) * p.o_head;
-    };
-    auto put = [&](__nv_bfloat16* o, const uint32_t (&x)[16]) {  // 32 columns
-      if (wide) {
-#pragma unroll
-        for (int q = 0; q < 2; ++q)
-          asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(o + 16 * q), "r"(x[8 * q]),
-                       "r"(x[8 * q + 1]), "r"(x[8 * q + 2]), "r"(x[8 * q + 3]), "r"(x[8 * q + 4]), "r"(x[8 * q + 5]),
-                       "r"(x[8 * q + 6]), "r"(x[8 * q + 7])
-                       : "memory");
-      } else {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) st_global_v4(o + 8 * q, make_uint4(x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]));
-      }
-    };
-    // this CTA's next unit; rows of units without keys are zeroed on the way
-    uint32_t j = 0;
-    auto advance = [&](Unit* w) {
-      for (;; ++j) {
-        if ((uint64_t)j * gridDim.x >= units) return false;
-        const uint32_t u = unit_index(j);
-        if (u >= units) continue;
-        bool bad = false;
-        *w = decode(p, u, &bad);
-        if (bad && w->hk == 0 && w->row0 == 0 && threadIdx.x == 256) report(p.status, DEMON_DEV_BAD_ARG, 63);
-        if (w->nt > 0) {
-          ++j;
-          return true;
-        }
-        const uint32_t zero[16] = {};
-        for (int h = 0; h < 2; ++h) {
-          bool inside;
-          __nv_bfloat16* o = out_row(*w, h, &inside);
-          if (inside)
-            for (int c = 0; c < 4; ++c) put(o + 32 * c, zero);
+        const float x = M - m - kBias;
+        if (fabsf(x) > 100.0f) {
+          fa = ex2(0.5f * x);
+          fb = fa / l;
+        } else {
+          fb = ex2(x) / l;
         }
       }
-    };
-    auto epilogue = [&](const Unit& w, uint32_t it, int h) {
-      if (!warp_wait(&l_full[h], it & 1u, abort_flag, t0, p.status, 91)) return false;
-      const float4 f = ld_shared_f32x4(sbase + offL + (h * kBlk + rr) * 16);
-      uint4 nan = make_uint4(0, 0, 0, 0);
-      if (f.z != 0.0f) nan = ld_shared_v4(sbase + offNanRow + (h * kBlk + rr) * 16);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&l_empty[h]);
       bool inside;
-      __nv_bfloat16* out = out_row(w, h, &inside);
-      if (!warp_wait(&o_full[h], it & 1u, abort_flag, t0, p.status, 92)) return false;
+      __nv_bfloat16* out = out_row(w, &inside);
+      uint4 nan = make_uint4(0, 0, 0, 0);
+      if (nan_row) nan = ld_shared_v4(sbase + offNanRow + (h * kBlk + rr) * 16);
+      const bool odd = __any_sync(0xffffffffu, fa != 1.0f || nan_row);
+      if (!warp_wait(&o_full[h], it & 1u, abort_flag, t0, p.status, 92)) break;
       tc_fence_after();
-      const float2 fa = make_float2(f.x, f.x), fb = make_float2(f.y, f.y);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t o[32];
-        tmem_ld_32x32b_x32(tmem + lane_addr + kColO + 128 * h + 32 * c, o);
+      for (int part = 0; part < 2; ++part) {
+        uint32_t o[64];
+        tmem_ld_32x32b_x32(o_addr + 64 * part, *reinterpret_cast<uint32_t(*)[32]>(o));
+        tmem_ld_32x32b_x32(o_addr + 64 * part + 32, *reinterpret_cast<uint32_t(*)[32]>(o + 32));
         tmem_ld_wait();
-        if (c == 3) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&o_empty[h]);
-        }
-        if (f.z != 0.0f) {
-          const uint32_t bits = c == 0 ? nan.x : c == 1 ? nan.y : c == 2 ? nan.z : nan.w;
+        if (odd) {
 #pragma unroll
-          for (int q = 0; q < 32; ++q)
-            if ((bits >> q) & 1u) o[q] = 0x7FFFFFFFu;
+          for (int q = 0; q < 64; ++q) {
+            const uint32_t bits = part == 0 ? (q < 32 ? nan.x : nan.y) : (q < 32 ? nan.z : nan.w);
+            o[q] = (bits >> (q & 31)) & 1u ? 0x7FFFFFFFu : __float_as_uint(__uint_as_float(o[q]) * fa);
+          }
         }
-        uint32_t x[16];
+        const float2 f2 = make_float2(fb, fb);
 #pragma unroll
-        for (int q = 0; q < 16; ++q) {
-          const float2 v = mul_f2(mul_f2(make_float2(__uint_as_float(o[2 * q]), __uint_as_float(o[2 * q + 1])), fa), fb);
-          x[q] = f.y == 0.0f ? 0u : pack_bf16x2(v.x, v.y);  // rows that see nothing: zeros, never 0 * NaN
+        for (int c = 0; c < 2; ++c) {
+          uint32_t x[16];
+#pragma unroll
+          for (int q = 0; q < 16; ++q) {
+            const float2 v = mul_f2(make_float2(__uint_as_float(o[32 * c + 2 * q]), __uint_as_float(o[32 * c + 2 * q + 1])), f2);
+            x[q] = fb == 0.0f ? 0u : pack_bf16x2(v.x, v.y);  // rows that see nothing: zeros, never 0 * NaN
+          }
+          if (inside) put(out + 64 * part + 32 * c, x);
         }
-        if (inside) put(out + 32 * c, x);
       }
-      return true;
-    };
-
-    Unit w, nw;
-    uint32_t it = 0;
-    bool have = advance(&w);
-    if (have) {
-      q_load(w, 0, 0);
-      q_load(w, 1, 1);
-      q_convert(0, 0);
-      q_convert(1, 1);
-    }
-    while (have) {
-      const bool more = advance(&nw);
-      const uint32_t n0 = 2 * it + 2, n1 = 2 * it + 3;
-      if (more) {
-        if (!wait_slot(n0)) break;
-        q_load(nw, n0 % kQSlots, 0);
-        q_convert(n0, 0);
-        if (!wait_slot(n1)) break;
-        q_load(nw, n1 % kQSlots, 1);
-      }
-      if (!epilogue(w, it, 0)) break;
-      if (more) q_convert(n1, 1);
-      if (!epilogue(w, it, 1)) break;
+      tc_fence_before();  // O_h is read before this warp publishes the next unit's P_h
       w = nw;
       have = more;
-      ++it;
     }
     cp_async_wait_all();  // no copy in flight when the CTA leaves
   }
