@@ -61,10 +61,10 @@ constexpr int kLaunchRegs = 128, kSoftmaxRegs = 176, kConvRegs = 72, kIssueRegs 
 static_assert(256 * kSoftmaxRegs + 128 * kConvRegs + 128 * kIssueRegs <= kThreads * kLaunchRegs,
               "register split exceeds the launch's registers (setmaxnreg.inc would wait for good)");
 
-// scales of a tile, per 16-key group: K scale, V exponent, 2^(ev_0 - ev_g); then the smallest and
-// largest V exponent and the groups without a page
-constexpr int kScWords = 32;
-constexpr int scK = 0, scEv = 8, scInv = 16, scMin = 24, scMax = 25, scBad = 26;
+// Scales of a tile: per 16 keys {K scale, V exponent ev, 2^(ev_0 - ev), 0}, then {smallest ev,
+// largest ev, 16-key groups without a page, 0}.
+constexpr int kScWords = 36;
+constexpr int kScTail = 32;
 
 constexpr int offQ = 0;                                        // [2 halves]
 constexpr int offKV = offQ + 2 * kTile;
@@ -123,6 +123,15 @@ __device__ __forceinline__ uint32_t ld_shared_b32(uint32_t a) {
   return v;
 }
 __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// 32 lanes x 16 consecutive 32-bit columns -> 16 registers per thread.
+__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
 
 struct Unit {
   int b, hk, len, nq;
@@ -372,16 +381,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const AttnPar
         const int ev0 = __shfl_sync(0xffffffffu, ev, 0);
         if (lane >= 8) ev = ev0;
         const int elo = __reduce_min_sync(0xffffffffu, ev), ehi = __reduce_max_sync(0xffffffffu, ev);
-        if (lane < 8) {
-          st_shared_f32(sc + 4 * (scK + lane), fabsf(sk));
-          st_shared_f32(sc + 4 * (scEv + lane), (float)ev);
-          st_shared_f32(sc + 4 * (scInv + lane), exp2i(imin(imax(ev0 - ev, -126), 126)));
-        }
-        if (lane == 0) {
-          st_shared_f32(sc + 4 * scMin, (float)elo);
-          st_shared_f32(sc + 4 * scMax, (float)ehi);
-          st_shared_b32(sc + 4 * scBad, gone);
-        }
+        if (lane < 8) st_shared_f32x4(sc + 16 * lane, fabsf(sk), (float)ev, exp2i(imin(imax(ev0 - ev, -126), 126)), 0.0f);
+        if (lane == 8) st_shared_f32x4(sc + 4 * kScTail, (float)elo, (float)ehi, __uint_as_float(gone), 0.0f);
         __syncwarp();
         if (lane == 0) mbar_arrive(&sc_full[tiles % kScSlots]);
         const bool copies = pid >= 0 && (16 * lane) % gw == 0;
@@ -639,21 +640,17 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const AttnPar
         tmem_ld_wait();
         float* s = reinterpret_cast<float*>(sr);
         const uint32_t sc = sbase + offSc + (t % kScSlots) * kScWords * 4;
+        const float4 tail = ld_shared_f32x4(sc + 4 * kScTail);
+        const uint32_t gone = __float_as_uint(tail.z);
         const int k0 = (w.tile0 + i) * kBlk;
         const int lo = jlo - k0, hi = jhi - 1 - k0;
-        if (__any_sync(0xffffffffu, lo > 0)) {
+        if (__any_sync(0xffffffffu, lo > 0 || hi < kBlk - 1 || gone != 0)) {
+          // keys that this row does not see, and pages that do not exist
 #pragma unroll
-          for (int c = 0; c < 128; ++c) s[c] = c < lo ? -INFINITY : s[c];
+          for (int c = 0; c < 128; ++c) s[c] = (c < lo || c > hi || ((gone >> (c >> 4)) & 1u)) ? -INFINITY : s[c];
         }
-        if (__any_sync(0xffffffffu, hi < kBlk - 1)) {
-#pragma unroll
-          for (int c = 0; c < 128; ++c) s[c] = c > hi ? -INFINITY : s[c];
-        }
-        const uint32_t gone = ld_shared_b32(sc + 4 * scBad);
-        if (gone) {  // pages that do not exist: seen by no row
-#pragma unroll
-          for (int c = 0; c < 128; ++c) s[c] = (gone >> (c >> 4)) & 1u ? -INFINITY : s[c];
-        }
+        // score factor of a group, kept within 2^+-120: a masked score times 0 would be NaN
+        const auto factor_of = [&](float k) { return fminf(fmaxf(fr * k, 7.5e-37f), 1.3e36f); };
         // maxima per group, in score units and with V's exponent
         float mt = -INFINITY, Mt = -INFINITY;
 #pragma unroll
@@ -668,49 +665,45 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const AttnPar
           float gm = mc[0];
 #pragma unroll
           for (int c = 1; c < CH; ++c) gm = fmaxf(gm, mc[c]);
-          // kept within 2^+-120: a masked score times 0 would be NaN
-          const float f = fminf(fmaxf(fr * ld_shared_f32(sc + 4 * (scK + gi * SG)), 7.5e-37f), 1.3e36f);
-          const float x = gm * f;
+          const float4 g4 = ld_shared_f32x4(sc + 16 * gi * SG);
+          const float x = gm * factor_of(g4.x);
           mt = fmaxf(mt, x);
-          Mt = fmaxf(Mt, x + ld_shared_f32(sc + 4 * (scEv + gi * SG)));
+          Mt = fmaxf(Mt, x + g4.y);
         }
-        if (mt > m + kRaise || (m == -INFINITY && mt > -INFINITY)) {
-          l *= ex2(m - mt);
-          m = mt;
-        }
-        float factor = 1.0f;
-        bool rescale = false;
-        if (Mt > M + kRaise || (M == -INFINITY && Mt > -INFINITY)) {
-          factor = ex2(M - Mt);
-          rescale = i > 0;
-          M = Mt;
-        }
-        const float mo = M == -INFINITY ? 0.0f : M, ml = m == -INFINITY ? 0.0f : m;
+        const bool up = mt > m + kRaise || (m == -INFINITY && mt > -INFINITY);
+        const bool UP = Mt > M + kRaise || (M == -INFINITY && Mt > -INFINITY);
+        const float m1 = up ? mt : m, M1 = UP ? Mt : M;
+        const float mo = M1 == -INFINITY ? 0.0f : M1, ml = m1 == -INFINITY ? 0.0f : m1;
         const float D = mo - ml;
-        const bool far = D - ld_shared_f32(sc + 4 * scMin) > kFast || ld_shared_f32(sc + 4 * scMax) - D > kFast;
-        float lw = ex2(D - kBias - ld_shared_f32(sc + 4 * scEv));  // weight of group 0's sum in l
-        if (__any_sync(0xffffffffu, far)) {
+        const bool far = D - tail.x > kFast || tail.y - D > kFast;
+        float lw = D;
+        if (__any_sync(0xffffffffu, up || UP || far)) {
+          if (up) l *= ex2(m - m1);
+          if (__any_sync(0xffffffffu, UP && i > 0)) {
+            // O_h *= 2^(M - M1): O_h is idle until this tile's P is published
+            const float f = UP ? ex2(M - M1) : 1.0f;
+#pragma unroll 1
+            for (int oc = 0; oc < 8; ++oc) {
+              uint32_t o[16];
+              tmem_ld_32x32b_x16(o_addr + 16 * oc, o);
+              tmem_ld_wait();
 #pragma unroll
-          for (int c = 0; c < 128; ++c) {
-            const float f = fminf(fmaxf(fr * ld_shared_f32(sc + 4 * (scK + (c / GW) * SG)), 7.5e-37f), 1.3e36f);
-            l += ex2(fmaf(s[c], f, -ml));
+              for (int q = 0; q < 16; ++q) o[q] = __float_as_uint(__uint_as_float(o[q]) * f);
+              tmem_st_32x32b_x16(o_addr + 16 * oc, o);
+            }
           }
-          lw = 0.0f;
+          if (__any_sync(0xffffffffu, far)) {  // l's terms by an exponential of their own
+#pragma unroll
+            for (int c = 0; c < 128; ++c) l += ex2(fmaf(s[c], factor_of(ld_shared_f32(sc + 16 * (c / GW) * SG)), -ml));
+            lw = -INFINITY;
+          }
+          m = m1;
+          M = M1;
         }
+        float gf = 0.0f, gn = 0.0f, gl = 0.0f;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           if (c == 2) {
-            if (__any_sync(0xffffffffu, rescale)) {
-#pragma unroll
-              for (int oc = 0; oc < 4; ++oc) {
-                uint32_t o[32];
-                tmem_ld_32x32b_x32(o_addr + 32 * oc, o);
-                tmem_ld_wait();
-#pragma unroll
-                for (int q = 0; q < 32; ++q) o[q] = __float_as_uint(__uint_as_float(o[q]) * factor);
-                tmem_st_32x32b_x32(o_addr + 32 * oc, o);
-              }
-            }
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
@@ -719,10 +712,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const AttnPar
           uint32_t pk[16];
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            const int gi = (32 * c + 16 * half) / GW;
-            const float f = fminf(fmaxf(fr * ld_shared_f32(sc + 4 * (scK + gi * SG)), 7.5e-37f), 1.3e36f);
-            const float n = ld_shared_f32(sc + 4 * (scEv + gi * SG)) - mo + kBias;
-            const float2 f2 = make_float2(f, f), n2 = make_float2(n, n);
+            if ((32 * c + 16 * half) % GW == 0) {  // the next group
+              const float4 g4 = ld_shared_f32x4(sc + 16 * ((32 * c + 16 * half) / GW) * SG);
+              gf = factor_of(g4.x);
+              gn = g4.y - mo + kBias;
+              if (c == 0 && half == 0) lw = ex2(lw - kBias - g4.y);  // weight of group 0's sum in l
+              gl = lw * g4.z;
+            }
+            const float2 f2 = make_float2(gf, gf), n2 = make_float2(gn, gn);
             float2 acc = make_float2(0.0f, 0.0f);
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
@@ -732,7 +729,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const AttnPar
               acc = add_f2(acc, e);
               pk[8 * half + q] = pack_f16x2(e.x, e.y);
             }
-            l = fmaf(lw * ld_shared_f32(sc + 4 * (scInv + gi * SG)), acc.x + acc.y, l);
+            l = fmaf(gl, acc.x + acc.y, l);
           }
           tmem_st_32x32b_x16(s_addr + kColP + 16 * c, pk);
         }
