@@ -148,6 +148,32 @@ int make_tmap_3d_bf16(CUtensorMap* map, const void* base, uint64_t cols, uint64_
   return DEMON_OK;
 }
 
+int make_tmap_4d_bf16(CUtensorMap* map, const void* base, const uint64_t (&dims)[4], const uint64_t (&pitch)[3],
+                      const uint32_t (&box)[4]) {
+  if (!encoder()) {
+    set_error("cuTensorMapEncodeTiled is unavailable from the driver");
+    return DEMON_ERR_CUDA;
+  }
+  cuuint64_t d[4], st[3];
+  cuuint32_t b[4];
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  for (int i = 0; i < 4; ++i) {
+    d[i] = dims[i];
+    b[i] = box[i];
+  }
+  for (int i = 0; i < 3; ++i) st[i] = dims[i + 1] > 1 ? pitch[i] : 16;  // unused along an extent of 1
+  const CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), d, st, b, estr,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled failed (%d): dims %llu x %llu x %llu x %llu pitches %llu/%llu/%llu", (int)r,
+              (unsigned long long)d[0], (unsigned long long)d[1], (unsigned long long)d[2], (unsigned long long)d[3],
+              (unsigned long long)st[0], (unsigned long long)st[1], (unsigned long long)st[2]);
+    return DEMON_ERR_INVALID;
+  }
+  return DEMON_OK;
+}
+
 }  // namespace demon
 
 extern "C" int demon_abi_version(void) { return DEMON_ABI_VERSION; }

@@ -33,6 +33,11 @@ int make_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, 
 int make_tmap_3d_bf16(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows, uint64_t depth,
                       uint64_t ld_bytes, uint64_t depth_bytes, uint32_t box_cols, uint32_t box_rows);
 
+// 4-D bf16 tiled tensor map with 128-byte swizzle: extents, pitches of dimensions 1 .. 3 in bytes,
+// box.  Pitches of dimensions of extent 1 may be anything.
+int make_tmap_4d_bf16(CUtensorMap* map, const void* base, const uint64_t (&dims)[4], const uint64_t (&pitch)[3],
+                      const uint32_t (&box)[4]);
+
 // Host-only argument checks of demon_nvfp4_quantize / demon_nvfp4_gemm (no CUDA call, no
 // launch): DEMON_OK, or DEMON_ERR_INVALID with the message set.  The entry points run them
 // first; callers that chain both kernels run both before launching either.

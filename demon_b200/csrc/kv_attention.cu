@@ -599,7 +599,7 @@ extern "C" int demon_kv_attention(const DemonKvAttnArgs* a, void* stream) {
     mark_device_done(g_kv_small_attr);
   }
   const int64_t rows = (int64_t)a->Sq * p.G;
-  if (rows > 64) return kv::attention_tc(p, (cudaStream_t)stream);
+  if (rows > 64 && p.G <= 128) return kv::attention_tc(p, (cudaStream_t)stream);
   const int rt = rows > 16 ? 2 : 1;
   p.n_rt = (int)((rows + 16 * rt - 1) / (16 * rt));
   const int64_t units = (int64_t)a->B * a->cache.heads * p.n_rt;

@@ -2,10 +2,10 @@
 // chunks, the DiT's cross attention) on the 5th-generation tensor cores.
 //
 // The same function as the small kernel in kv_attention.cu (rows, masks, empty rows, NaN).  Work
-// unit: one (sequence, kv head, block of 256 query rows), a row being (token, query head) with
-// the G query heads of the kv head next to each other, so that any G fills the tiles.  The two
-// halves of 128 rows share every K / V tile of 128 keys.  Persistent CTAs (one per SM), blocks
-// with the most keys (the last of a causal prompt) first.
+// unit: one (sequence, kv head, block of 2 Tt query tokens), Tt = floor(128 / G): each half of the
+// block is Tt tokens times the G query heads of the kv head, up to 128 rows of a tile.  The two
+// halves share every K / V tile of 128 keys.  Persistent CTAs (one per SM), blocks with the most
+// keys (the last of a causal prompt) first.
 //
 // Operands.  The codes go from their pages through registers into shared memory as f16, which
 // holds every E4M3 value: one conversion instruction per two codes, so that the scales stay out
@@ -22,12 +22,12 @@
 // Output: O * 2^(M - m - 6) / l.  Both offsets are raised only when exceeded by more than 8.
 //
 // Warp roles (512 threads; setmaxnreg as in attention.cu):
-//   warpgroup 0 / 1   row half 0 / 1, one query row per thread: its Q row (copied by cp.async while
-//                     the previous unit's last tile is in work, converted in place), the softmax of
-//                     every key tile, the output row,
-//   warpgroup 2       codes -> f16, swizzled, into a ring of three K / V tiles,
+//   warpgroup 0 / 1   row half 0 / 1, one query row per thread: the softmax of every key tile, the
+//                     output row,
+//   warpgroup 2       codes -> f16, swizzled, into a ring of three K / V tiles; the Q rows in place,
 //   warp 12           MMA issue (one thread) and tensor-memory allocation,
-//   warp 13           page look-ups, scales, bulk copies of K / V codes into a ring of half tiles.
+//   warp 13           page look-ups, scales, bulk copies of K / V codes into a ring of half tiles,
+//   warp 14           the next unit's Q by TMA, each half as soon as the last Q K^T has read the slot.
 // Tensor memory as in attention.cu: S_h at 128 h, P_h over its upper half, O_h at 256 + 128 h.
 //
 // Bound by the exponentials (one per row and key, 16 per clock and SM) and the MMAs, which take
@@ -43,7 +43,6 @@ namespace kv {
 namespace tc {
 
 constexpr int kBlk = 128;                // rows per half, keys per tile
-constexpr int kRows = 2 * kBlk;          // rows per unit
 constexpr int kBox = 128 * 128;          // 64 f16 columns x 128 rows (16 KB)
 constexpr int kTile = 2 * kBox;          // 128 x 128 f16
 constexpr int kSlots = 3;                // K / V tiles as f16
@@ -71,11 +70,12 @@ constexpr int offKV = offQ + 2 * kTile;
 constexpr int offRaw = offKV + kSlots * kTile;
 constexpr int offNan = offRaw + kRawSlots * kRaw;              // [slot][128 keys] 128-bit maps
 constexpr int offNanRow = offNan + kNanSlots * kBlk * 16;      // [2][128] 128-bit maps
-constexpr int offSc = offNanRow + 2 * kBlk * 16;
+constexpr int offRow = offNanRow + 2 * kBlk * 16;              // [2 units][2 halves][128] powers of two
+constexpr int offSc = offRow + 4 * kBlk * 4;
 constexpr int offNanW = offSc + kScSlots * kScWords * 4;       // [slot][warp] any NaN
 constexpr int offRawMask = offNanW + kScSlots * 4 * 4;         // [slot] 16-key groups copied
 constexpr int offBar = offRawMask + 4 * 4;
-constexpr int kNumBars = 2 + 2 * kSlots + 8 + 1 + 2 * kScSlots + 2 * kRawSlots;
+constexpr int kNumBars = 4 + 2 * kSlots + 8 + 1 + 2 * kScSlots + 2 * kRawSlots + 6;
 constexpr int offMisc = offBar + kNumBars * 8;
 constexpr int kSmem = offMisc + 16 + 1024;
 static_assert(kSmem <= 232448, "shared memory exceeds the sm_100 per-block limit");
@@ -87,12 +87,15 @@ constexpr uint32_t kColS = 0, kColP = 64, kColO = 256;
 constexpr uint32_t idesc_f16(int M, int N) {
   return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
-__device__ __forceinline__ uint64_t kmajor_desc(uint32_t tile, int kk) {
-  return smem_desc(tile + (uint32_t)(kk >> 2) * kBox + (uint32_t)(kk & 3) * 32, 16, 1024, 2);
-}
-__device__ __forceinline__ uint64_t mnmajor_desc(uint32_t tile, int kk) {
-  return smem_desc(tile + (uint32_t)kk * 2048, kBox, 1024, 2);
-}
+// Shared-memory descriptors of 128-byte-swizzled tiles (see attention.cu): the low word holds the
+// address (>> 4) and the leading byte offset, the high word the stride and layout, so a k-step is an
+// addition to the low word.
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);  // stride 1024 B, version 1, swizzle 128 B
+__device__ __forceinline__ uint32_t kmajor_lo(uint32_t tile) { return (tile >> 4) | ((16u >> 4) << 16); }
+__device__ __forceinline__ uint32_t mnmajor_lo(uint32_t tile) { return (tile >> 4) | ((uint32_t)(kBox >> 4) << 16); }
+__host__ __device__ constexpr uint32_t kmajor_step(int kk) { return (uint32_t)((kk >> 2) * kBox + (kk & 3) * 32) >> 4; }
+__host__ __device__ constexpr uint32_t mnmajor_step(int kk) { return (uint32_t)(kk * 2048) >> 4; }
+__device__ __forceinline__ uint64_t desc_of(uint32_t lo) { return (uint64_t)lo | ((uint64_t)kDescHi << 32); }
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -122,7 +125,15 @@ __device__ __forceinline__ uint32_t ld_shared_b32(uint32_t a) {
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
   return v;
 }
-__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+// 4-D tiled load.
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tmap, uint64_t* bar, int32_t x, int32_t y, int32_t z,
+                                            int32_t u) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(tmap), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(u)
+      : "memory");
+}
 
 // 32 lanes x 16 consecutive 32-bit columns -> 16 registers per thread.
 __device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
@@ -135,7 +146,7 @@ __device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)
 
 struct Unit {
   int b, hk, len, nq;
-  int64_t row0;     // first row (token * G + head) of the block
+  int i0;           // first token of the block
   Keys ks;          // keys that some / every row of the block sees
   int tile0, nt;    // key tiles
 };
@@ -151,13 +162,12 @@ __device__ __forceinline__ Unit decode(const AttnParams& p, uint32_t u, bool* ba
   const uint32_t q = u / bh, r = u - q * bh;
   w.b = (int)(r / (uint32_t)p.c.heads);
   w.hk = (int)(r - (uint32_t)w.b * (uint32_t)p.c.heads);
-  w.row0 = (int64_t)(p.n_rt - 1 - (int)q) * kRows;
+  w.i0 = (p.n_rt - 1 - (int)q) * 2 * p.Tt;
   w.len = clamp_len(__ldg(p.lens + w.b), p.W * p.c.P, bad);
   w.nq = p.q_lens ? clamp_len(__ldg(p.q_lens + w.b), p.Sq, bad) : p.Sq;
-  const int i0 = (int)((uint32_t)w.row0 / (uint32_t)p.G);
-  const int i1 = imin((int)((uint32_t)(w.row0 + kRows - 1) / (uint32_t)p.G), w.nq - 1);
+  const int i1 = imin(w.i0 + 2 * p.Tt, w.nq) - 1;
   w.ks.lo = w.ks.hi = w.ks.lo_all = w.ks.hi_all = 0;
-  if (i0 <= i1) w.ks = visible(i0, i1, w.len, w.nq, p.causal != 0, p.window);
+  if (w.i0 <= i1) w.ks = visible(w.i0, i1, w.len, w.nq, p.causal != 0, p.window);
   w.tile0 = w.ks.lo / kBlk;
   w.nt = w.ks.hi > w.ks.lo ? (w.ks.hi + kBlk - 1) / kBlk - w.tile0 : 0;
   return w;
@@ -178,13 +188,15 @@ __device__ __forceinline__ bool next_unit(const AttnParams& p, uint32_t units, u
 }
 
 template <int NG>  // 16-key-or-larger groups of a tile with a scale of their own: 128 / min(P, 128)
-__global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const AttnParams p, const uint32_t units, const int wide) {
+__global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const AttnParams p,
+                                                                    const uint32_t units, const int wide) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + offBar);
   uint64_t* q_full = bars;                      // [2] Q half converted
-  uint64_t* kv_full = q_full + 2;               // [3] K or V tile converted
+  uint64_t* q_empty = q_full + 2;               // [2] the unit's last Q K^T done
+  uint64_t* kv_full = q_empty + 2;              // [3] K or V tile converted
   uint64_t* kv_empty = kv_full + kSlots;        // [3] its MMAs done
   uint64_t* s_full = kv_empty + kSlots;         // [2] S_h computed
   uint64_t* pa_full = s_full + 2;               // [2] P_h of keys 0-63 in tensor memory
@@ -199,6 +211,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const AttnPar
   uint64_t* nan_full = sc_full + kScSlots;      // [8] NaN map of a tile
   uint64_t* raw_full = nan_full + kScSlots;     // [3] codes of a half tile copied
   uint64_t* raw_empty = raw_full + kRawSlots;   // [3] and converted
+  uint64_t* row_full = raw_empty + kRawSlots;   // [2 units][2 halves] rows' powers of two
+  uint64_t* q_raw = row_full + 4;               // [2] Q half copied
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + offMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + offMisc + 4);
 
@@ -211,7 +225,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const AttnPar
       mbar_init(&kv_empty[s], 1);
     }
     for (int h = 0; h < 2; ++h) {
-      mbar_init(&q_full[h], 4);
+      mbar_init(&q_full[h], kConvWarps);
+      mbar_init(&q_empty[h], 1);
+      mbar_init(&q_raw[h], 1);
+      mbar_init(&row_full[h], kConvWarps);
+      mbar_init(&row_full[2 + h], kConvWarps);
       mbar_init(&s_full[h], 1);
       mbar_init(&pa_full[h], 4);
       mbar_init(&pb_full[h], 4);
@@ -249,19 +267,19 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const AttnPar
         uint32_t g = 0, it = 0, tiles = 0;  // half tiles consumed, units, key tiles (all units)
         bool ok = true;
         auto qk = [&](int h, uint32_t kslot) {
-          const uint32_t qa = sbase + offQ + h * kTile, kb = sbase + offKV + kslot * kTile;
+          const uint32_t qa = kmajor_lo(sbase + offQ + h * kTile), kb = kmajor_lo(sbase + offKV + kslot * kTile);
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)
-            mma_bf16(tmem + kColS + 128 * h, kmajor_desc(qa, kk), kmajor_desc(kb, kk), idesc_qk, kk > 0);
+            mma_bf16(tmem + kColS + 128 * h, desc_of(qa + kmajor_step(kk)), desc_of(kb + kmajor_step(kk)), idesc_qk, kk > 0);
           tc_commit(&s_full[h]);
         };
         auto pv = [&](int h, uint32_t vslot, int half, bool acc) {
-          const uint32_t vb = sbase + offKV + vslot * kTile;
+          const uint32_t vb = mnmajor_lo(sbase + offKV + vslot * kTile);
 #pragma unroll
           for (int k4 = 0; k4 < 4; ++k4) {
             const int kk = 4 * half + k4;
-            mma_bf16_ts(tmem + kColO + 128 * h, tmem + kColS + 128 * h + kColP + 8 * kk, mnmajor_desc(vb, kk), idesc_pv,
-                        (acc || kk > 0) ? 1u : 0u);
+            mma_bf16_ts(tmem + kColO + 128 * h, tmem + kColS + 128 * h + kColP + 8 * kk, desc_of(vb + mnmajor_step(kk)),
+                        idesc_pv, (acc || kk > 0) ? 1u : 0u);
           }
         };
         auto wait_on = [&](uint64_t* bar, uint32_t parity, unsigned int where) {
@@ -297,9 +315,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const AttnPar
           uint32_t gk = g, gv = g + 1;
           if (!wait_q(0) || !wait_kv(gk)) break;
           qk(0, gk % kSlots);
+          if (n == 1) tc_commit(&q_empty[0]);
           if (!flush() || !wait_q(1)) break;
           qk(1, gk % kSlots);
           tc_commit(&kv_empty[gk % kSlots]);
+          if (n == 1) tc_commit(&q_empty[1]);
           if (!wait_kv(gv) || !pv_tile(0, gv % kSlots, tiles, false)) break;
           uint32_t prev_v = gv;
           g += 2;
@@ -308,10 +328,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const AttnPar
             gv = g + 1;
             if (!wait_kv(gk)) break;
             qk(0, gk % kSlots);
+            if (i == n - 1) tc_commit(&q_empty[0]);
             if (!pv_tile(1, prev_v % kSlots, tiles + i - 1, i - 1 > 0)) break;
             tc_commit(&kv_empty[prev_v % kSlots]);
             qk(1, gk % kSlots);
             tc_commit(&kv_empty[gk % kSlots]);
+            if (i == n - 1) tc_commit(&q_empty[1]);
             if (!wait_kv(gv) || !pv_tile(0, gv % kSlots, tiles + i, true)) break;
             prev_v = gv;
             g += 2;
@@ -413,6 +435,27 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const AttnPar
       for (uint32_t i = n > (uint32_t)kRawSlots ? n - kRawSlots : 0; i < n; ++i)
         mbar_wait(&raw_full[i % kRawSlots], (i / kRawSlots) & 1u, &never, globaltimer(), p.status, 79);
       __syncwarp();
+    } else if (warp == 14) {
+      // ------------------------------------------------------------------ Q
+      if (elect_one()) {
+        uint32_t j = 0, it = 0;
+        uint32_t issued = 0;  // halves
+        Unit w;
+        bool ok = true;
+        const uint32_t bytes = (uint32_t)(p.Tt * p.G) * kHeadDim * 2;
+        for (; ok && next_unit(p, units, &j, &w); ++it)
+          for (int h = 0; h < 2; ++h, ++issued) {
+            if (!(ok = mbar_wait(&q_empty[h], (it & 1u) ^ 1u, abort_flag, t0, p.status, 91))) break;
+            mbar_arrive_expect_tx(&q_raw[h], bytes);
+            for (int box = 0; box < 2; ++box)
+              tma_load_4d(sbase + offQ + h * kTile + box * kBox, &tmQ, &q_raw[h], 64 * box, w.hk * p.G, w.i0 + h * p.Tt, w.b);
+          }
+        // no copy may still be in flight when the CTA leaves (immediate on the normal path)
+        volatile int never = 0;
+        for (uint32_t i = issued > 2 ? issued - 2 : 0; i < issued; ++i)
+          mbar_wait(&q_raw[i & 1], (i >> 1) & 1u, &never, globaltimer(), p.status, 93);
+      }
+      __syncwarp();
     }
   } else if (wg == 2) {
     setmaxnreg_dec<kConvRegs>();
@@ -421,10 +464,57 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const AttnPar
     // neighbouring rows take opposite halves of their 128 codes (no bank conflicts either way).
     const int cw = warp & 3, c = lane & 3, rl = lane >> 2;
     const uint32_t a0 = (uint32_t)rl * 128 + (((2 * c) ^ rl) << 4), a1 = (uint32_t)rl * 128 + (((2 * c + 1) ^ rl) << 4);
-    uint32_t n = 0, tiles = 0, j = 0;
+    // One row per thread in place (row 32 cw + lane): bf16 -> f16 times 2^-e
+    auto q_convert = [&](int h, uint32_t unit) {
+      const int rr = cw * 32 + lane;
+      const uint32_t base = sbase + offQ + h * kTile + rr * 128;
+      uint32_t mx = 0, all = 0;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const uint4 x = ld_shared_v4(base + (k >> 3) * kBox + (((k & 7) ^ (rr & 7)) << 4));
+        const uint32_t y[4] = {x.x & 0x7FFF7FFFu, x.y & 0x7FFF7FFFu, x.z & 0x7FFF7FFFu, x.w & 0x7FFF7FFFu};
+        all = __vmaxu2(all, __vmaxu2(__vmaxu2(y[0], y[1]), __vmaxu2(y[2], y[3])));
+      }
+      all = max(all & 0xFFFFu, all >> 16);
+      mx = all;
+      if (all >= 0x7F80u) {  // infinities and NaN do not count, and pass through
+        mx = 0;
+        for (int k = 0; k < 16; ++k) {
+          const uint4 x = ld_shared_v4(base + (k >> 3) * kBox + (((k & 7) ^ (rr & 7)) << 4));
+          const uint32_t y[4] = {x.x & 0x7FFF7FFFu, x.y & 0x7FFF7FFFu, x.z & 0x7FFF7FFFu, x.w & 0x7FFF7FFFu};
+          for (int q = 0; q < 4; ++q) mx = __vmaxu2(mx, y[q] & __vcmpltu2(y[q], 0x7F807F80u));
+        }
+        mx = max(mx & 0xFFFFu, mx >> 16);
+      }
+      const int e = imax((int)(mx >> 7) - 127 - 13, -126);  // |q| 2^-e < 2^14
+      const float2 mul = make_float2(exp2i(-e), exp2i(-e));
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
+        uint4 x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = ld_shared_v4(base + part * kBox + ((k ^ (rr & 7)) << 4));
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float2 f0 = mul_f2(bf2_f2(x[k].x), mul), f1 = mul_f2(bf2_f2(x[k].y), mul), f2 = mul_f2(bf2_f2(x[k].z), mul),
+                       f3 = mul_f2(bf2_f2(x[k].w), mul);
+          st_shared_v4(base + part * kBox + ((k ^ (rr & 7)) << 4), pack_f16x2(f0.x, f0.y), pack_f16x2(f1.x, f1.y),
+                       pack_f16x2(f2.x, f2.y), pack_f16x2(f3.x, f3.y));
+        }
+      }
+      const uint32_t rs = (unit & 1) * 2 + h;
+      st_shared_f32(sbase + offRow + (rs * kBlk + rr) * 4, exp2i(e));
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&q_full[h]);
+        mbar_arrive(&row_full[rs]);
+      }
+    };
+
+    uint32_t n = 0, tiles = 0, j = 0, it = 0;
     bool ok = true;
     Unit w;
-    while (ok && next_unit(p, units, &j, &w)) {
+    for (; ok && next_unit(p, units, &j, &w); ++it) {
       for (int t = 0; ok && t < w.nt; ++t, ++tiles) {
         const int k0 = (w.tile0 + t) * kBlk;
         const bool whole = k0 >= w.ks.lo_all && k0 + kBlk <= w.ks.hi_all;
@@ -485,6 +575,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const AttnPar
             if (kv) mbar_arrive(&nan_full[tiles % kScSlots]);
           }
         }
+        if (t == 0 && ok) {
+          for (int h = 0; ok && h < 2; ++h) {
+            ok = warp_wait(&q_raw[h], it & 1u, abort_flag, t0, p.status, 90);
+            if (ok) q_convert(h, it);
+          }
+        }
       }
     }
   } else {
@@ -496,77 +592,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const AttnPar
     const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
     const uint32_t s_addr = tmem + lane_addr + kColS + 128 * h;
     const uint32_t o_addr = tmem + lane_addr + kColO + 128 * h;
-    const uint32_t q_slot = sbase + offQ + h * kTile;
-    const uint32_t n_rows = (uint32_t)p.Sq * (uint32_t)p.G;
-    // The warp's 32 rows of Q into their slot: rows 2 k + lane / 16, 16 bytes a lane.
-    auto q_load = [&](const Unit& w) {
-      const int sub = lane & 15;
-      uint32_t row = (uint32_t)w.row0 + h * kBlk + quad * 32 + (lane >> 4);
-      int i = (int)(row / (uint32_t)p.G), g = (int)(row - (uint32_t)i * (uint32_t)p.G);
-      const __nv_bfloat16* q = p.q + w.b * p.q_seq + (int64_t)(w.hk * p.G) * p.q_head + sub * 8;
-#pragma unroll 2
-      for (int k = 0; k < 16; ++k) {
-        const int rt = quad * 32 + 2 * k + (lane >> 4);
-        const uint32_t dst = q_slot + (sub >> 3) * kBox + rt * 128 + (((sub & 7) ^ (rt & 7)) << 4);
-        if (row < n_rows && i < w.nq)
-          cp_async_16(dst, q + (int64_t)i * p.q_row + (int64_t)g * p.q_head);
-        else
-          st_shared_v4(dst, 0, 0, 0, 0);
-        row += 2;
-        g += 2;
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-          if (g >= p.G) {
-            g -= p.G;
-            ++i;
-          }
-      }
-    };
-    // This thread's row in place: bf16 -> f16 times 2^-e; returns 2^e.
-    auto q_convert = [&]() {
-      cp_async_wait_all();
-      __syncwarp();
-      uint4 x[16];
-#pragma unroll
-      for (int k = 0; k < 16; ++k) x[k] = ld_shared_v4(q_slot + (k >> 3) * kBox + rr * 128 + (((k & 7) ^ (rr & 7)) << 4));
-      uint32_t mx = 0;
-#pragma unroll
-      for (int k = 0; k < 16; ++k)
-        mx = __vmaxu2(mx, __vmaxu2(__vmaxu2(x[k].x & 0x7FFF7FFFu, x[k].y & 0x7FFF7FFFu),
-                                   __vmaxu2(x[k].z & 0x7FFF7FFFu, x[k].w & 0x7FFF7FFFu)));
-      mx = max(mx & 0xFFFFu, mx >> 16);
-      if (mx >= 0x7F80u) {  // infinities and NaN do not count, and pass through
-        mx = 0;
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          const uint32_t y[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const uint32_t a = y[q] & 0x7FFF7FFFu;
-            mx = __vmaxu2(mx, a & __vcmpltu2(a, 0x7F807F80u));
-          }
-        }
-        mx = max(mx & 0xFFFFu, mx >> 16);
-      }
-      const int e = imax((int)(mx >> 7) - 127 - 13, -126);  // |q| 2^-e < 2^14
-      const float2 mul = make_float2(exp2i(-e), exp2i(-e));
-#pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        const float2 f0 = mul_f2(bf2_f2(x[k].x), mul), f1 = mul_f2(bf2_f2(x[k].y), mul), f2 = mul_f2(bf2_f2(x[k].z), mul),
-                     f3 = mul_f2(bf2_f2(x[k].w), mul);
-        st_shared_v4(q_slot + (k >> 3) * kBox + rr * 128 + (((k & 7) ^ (rr & 7)) << 4), pack_f16x2(f0.x, f0.y),
-                     pack_f16x2(f1.x, f1.y), pack_f16x2(f2.x, f2.y), pack_f16x2(f3.x, f3.y));
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&q_full[h]);
-      return exp2i(e) * p.scale_log2;
-    };
+    const int ri = rr / p.G, rg = rr - ri * p.G;  // token and head of this row within the half
+    auto token_of = [&](const Unit& w) { return w.i0 + h * p.Tt + ri; };
     auto out_row = [&](const Unit& w, bool* inside) {
-      const uint32_t row = (uint32_t)w.row0 + h * kBlk + rr;
-      *inside = row < n_rows;
-      const uint32_t i = row / (uint32_t)p.G, g = row - i * (uint32_t)p.G;
-      return p.o + w.b * p.o_seq + (int64_t)i * p.o_row + (int64_t)(w.hk * p.G + (int)g) * p.o_head;
+      const int i = token_of(w);
+      *inside = ri < p.Tt && i < p.Sq;
+      return p.o + w.b * p.o_seq + (int64_t)i * p.o_row + (int64_t)(w.hk * p.G + rg) * p.o_head;
     };
     auto put = [&](__nv_bfloat16* o, const uint32_t (&x)[16]) {  // 32 columns
       if (wide) {
@@ -590,7 +621,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const AttnPar
         if (u >= units) continue;
         bool bad = false;
         *w = decode(p, u, &bad);
-        if (bad && w->hk == 0 && w->row0 == 0 && threadIdx.x == 0) report(p.status, DEMON_DEV_BAD_ARG, 63);
+        if (bad && w->hk == 0 && w->i0 == 0 && threadIdx.x == 0) report(p.status, DEMON_DEV_BAD_ARG, 63);
         if (w->nt > 0) {
           ++j;
           return true;
@@ -605,19 +636,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const AttnPar
 
     uint32_t t = 0, it = 0;
     Unit w, nw;
-    float fr = 0.0f;
+    const uint32_t nan_at = sbase + offNanRow + (h * kBlk + rr) * 16;
     bool have = advance(&w);
-    if (have) {
-      q_load(w);
-      fr = q_convert();
-    }
     for (; have; ++it) {
       int jlo = 0, jhi = w.len;  // keys that this row sees: [jlo, jhi)
       bool live;
       {
-        const uint32_t row = (uint32_t)w.row0 + h * kBlk + rr;
-        const int qi = (int)(row / (uint32_t)p.G);
-        live = row < n_rows && qi < w.nq;
+        const int qi = token_of(w);
+        live = ri < p.Tt && qi < w.nq;
         if (live) {
           const Keys k = visible(qi, qi, w.len, w.nq, p.causal != 0, p.window);
           jlo = k.lo;
@@ -626,25 +652,29 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const AttnPar
       }
       const bool more = advance(&nw);
       float M = -INFINITY, m = -INFINITY, l = 0.0f;
-      bool nan_row = false, ok = true;
+      st_shared_v4(nan_at, 0, 0, 0, 0);
+      const uint32_t rs = (it & 1) * 2 + h;
+      bool ok = warp_wait(&row_full[rs], (it >> 1) & 1u, abort_flag, t0, p.status, 80);
+      if (!ok) break;
+      const float fr = ld_shared_f32(sbase + offRow + (rs * kBlk + rr) * 4) * p.scale_log2;
       for (int i = 0; i < w.nt; ++i, ++t) {
-        if (!(ok = warp_wait(&s_full[h], t & 1u, abort_flag, t0, p.status, 81))) break;
-        tc_fence_after();
         if (!(ok = warp_wait(&sc_full[t % kScSlots], (t / kScSlots) & 1u, abort_flag, t0, p.status, 82))) break;
-        uint32_t sr[128];
-        tmem_ld_32x32b_x32(s_addr + 0, *reinterpret_cast<uint32_t(*)[32]>(sr + 0));
-        tmem_ld_32x32b_x32(s_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(sr + 32));
-        tmem_ld_32x32b_x32(s_addr + 64, *reinterpret_cast<uint32_t(*)[32]>(sr + 64));
-        tmem_ld_32x32b_x32(s_addr + 96, *reinterpret_cast<uint32_t(*)[32]>(sr + 96));
-        if (i == w.nt - 1 && more) q_load(nw);  // Q of this unit has been used for the last time
-        tmem_ld_wait();
-        float* s = reinterpret_cast<float*>(sr);
         const uint32_t sc = sbase + offSc + (t % kScSlots) * kScWords * 4;
         const float4 tail = ld_shared_f32x4(sc + 4 * kScTail);
         const uint32_t gone = __float_as_uint(tail.z);
         const int k0 = (w.tile0 + i) * kBlk;
         const int lo = jlo - k0, hi = jhi - 1 - k0;
-        if (__any_sync(0xffffffffu, lo > 0 || hi < kBlk - 1 || gone != 0)) {
+        const bool partly = __any_sync(0xffffffffu, lo > 0 || hi < kBlk - 1 || gone != 0);
+        if (!(ok = warp_wait(&s_full[h], t & 1u, abort_flag, t0, p.status, 81))) break;
+        tc_fence_after();
+        uint32_t sr[128];
+        tmem_ld_32x32b_x32(s_addr + 0, *reinterpret_cast<uint32_t(*)[32]>(sr + 0));
+        tmem_ld_32x32b_x32(s_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(sr + 32));
+        tmem_ld_32x32b_x32(s_addr + 64, *reinterpret_cast<uint32_t(*)[32]>(sr + 64));
+        tmem_ld_32x32b_x32(s_addr + 96, *reinterpret_cast<uint32_t(*)[32]>(sr + 96));
+        tmem_ld_wait();
+        float* s = reinterpret_cast<float*>(sr);
+        if (partly) {
           // keys that this row does not see, and pages that do not exist
 #pragma unroll
           for (int c = 0; c < 128; ++c) s[c] = (c < lo || c > hi || ((gone >> (c >> 4)) & 1u)) ? -INFINITY : s[c];
@@ -739,9 +769,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const AttnPar
         if (lane == 0) mbar_arrive(&pb_full[h]);
         if (k0 < w.ks.lo_all || k0 + kBlk > w.ks.hi_all) {  // the converters left NaN codes of V out
           if (!(ok = warp_wait(&nan_full[t % kScSlots], (t / kScSlots) & 1u, abort_flag, t0, p.status, 83))) break;
-          const uint32_t nwd = sbase + offNanW + (t % kScSlots) * 16;
-          if (ld_shared_b32(nwd) | ld_shared_b32(nwd + 4) | ld_shared_b32(nwd + 8) | ld_shared_b32(nwd + 12)) {
-            uint4 seen = make_uint4(0, 0, 0, 0);
+          const uint4 any = ld_shared_v4(sbase + offNanW + (t % kScSlots) * 16);
+          if (any.x | any.y | any.z | any.w) {
+            uint4 seen = ld_shared_v4(nan_at);
             const uint32_t map = sbase + offNan + (t % kNanSlots) * kBlk * 16;
             for (int c = imax(lo, 0); c <= imin(hi, kBlk - 1); ++c) {
               const uint4 x = ld_shared_v4(map + c * 16);
@@ -750,21 +780,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const AttnPar
               seen.z |= x.z;
               seen.w |= x.w;
             }
-            const uint32_t a = sbase + offNanRow + (h * kBlk + rr) * 16;
-            if (nan_row) {
-              const uint4 x = ld_shared_v4(a);
-              seen.x |= x.x;
-              seen.y |= x.y;
-              seen.z |= x.z;
-              seen.w |= x.w;
-            }
-            st_shared_v4(a, seen.x, seen.y, seen.z, seen.w);
-            nan_row = true;
+            st_shared_v4(nan_at, seen.x, seen.y, seen.z, seen.w);
           }
         }
       }
       if (!ok) break;
-      if (more) fr = q_convert();
       // the output row: O 2^(M - m - 6) / l, the factor in two parts where it is not normal
       float fa = 1.0f, fb = 0.0f;
       if (live && l != 0.0f) {
@@ -778,9 +798,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const AttnPar
       }
       bool inside;
       __nv_bfloat16* out = out_row(w, &inside);
-      uint4 nan = make_uint4(0, 0, 0, 0);
-      if (nan_row) nan = ld_shared_v4(sbase + offNanRow + (h * kBlk + rr) * 16);
-      const bool odd = __any_sync(0xffffffffu, fa != 1.0f || nan_row);
+      const uint4 nan = ld_shared_v4(nan_at);
+      const bool odd = __any_sync(0xffffffffu, fa != 1.0f || (nan.x | nan.y | nan.z | nan.w) != 0);
       if (!warp_wait(&o_full[h], it & 1u, abort_flag, t0, p.status, 92)) break;
       tc_fence_after();
 #pragma unroll
@@ -812,7 +831,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const AttnPar
       w = nw;
       have = more;
     }
-    cp_async_wait_all();  // no copy in flight when the CTA leaves
   }
 
   tc_fence_before();
@@ -839,11 +857,15 @@ int prepare() {
 
 int attention_tc(AttnParams p, cudaStream_t st) {
   using namespace tc;
-  const int64_t rows = (int64_t)p.Sq * p.G;
-  p.n_rt = (int)((rows + kRows - 1) / kRows);
+  p.Tt = kBlk / p.G;
+  p.n_rt = (p.Sq + 2 * p.Tt - 1) / (2 * p.Tt);
   const int64_t units = (int64_t)p.n_rt * p.B * p.c.heads;
-  DEMON_CHECK_ARG(rows < ((int64_t)1 << 31) - kRows && units < ((int64_t)1 << 31), "kv_attention: too many query rows (%lld)",
-                  (long long)rows);
+  DEMON_CHECK_ARG(units < ((int64_t)1 << 31), "kv_attention: too many work units (%lld)", (long long)units);
+  CUtensorMap tq;
+  const int rc0 = make_tmap_4d_bf16(&tq, p.q, {kHeadDim, (uint64_t)p.Hq, (uint64_t)p.Sq, (uint64_t)p.B},
+                                    {(uint64_t)p.q_head * 2, (uint64_t)p.q_row * 2, (uint64_t)p.q_seq * 2},
+                                    {64, (uint32_t)p.G, (uint32_t)p.Tt, 1});
+  if (rc0 != DEMON_OK) return rc0;
   if (device_pending(g_attr)) {
     int rc = prepare<1>();
     if (rc == DEMON_OK) rc = prepare<2>();
@@ -858,10 +880,10 @@ int attention_tc(AttnParams p, cudaStream_t st) {
   const unsigned grid = (unsigned)std::min<int64_t>(units, sms);
   const int wide = ((uintptr_t)p.o & 31) == 0 && p.o_seq % 16 == 0 && p.o_row % 16 == 0 && p.o_head % 16 == 0;
   switch (p.c.P) {
-    case 16: attention_tc_kernel<8><<<grid, kThreads, kSmem, st>>>(p, (uint32_t)units, wide); break;
-    case 32: attention_tc_kernel<4><<<grid, kThreads, kSmem, st>>>(p, (uint32_t)units, wide); break;
-    case 64: attention_tc_kernel<2><<<grid, kThreads, kSmem, st>>>(p, (uint32_t)units, wide); break;
-    default: attention_tc_kernel<1><<<grid, kThreads, kSmem, st>>>(p, (uint32_t)units, wide); break;
+    case 16: attention_tc_kernel<8><<<grid, kThreads, kSmem, st>>>(tq, p, (uint32_t)units, wide); break;
+    case 32: attention_tc_kernel<4><<<grid, kThreads, kSmem, st>>>(tq, p, (uint32_t)units, wide); break;
+    case 64: attention_tc_kernel<2><<<grid, kThreads, kSmem, st>>>(tq, p, (uint32_t)units, wide); break;
+    default: attention_tc_kernel<1><<<grid, kThreads, kSmem, st>>>(tq, p, (uint32_t)units, wide); break;
   }
   DEMON_CUDA(cudaGetLastError());
   return DEMON_OK;

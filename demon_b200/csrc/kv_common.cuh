@@ -81,6 +81,7 @@ struct AttnParams {
   int causal, window;  // window < 0: no band
   float scale_log2;    // softmax scale * log2(e)
   int n_rt;            // row tiles (or blocks) per kv head
+  int Tt;              // tokens per half block (tensor-core kernel)
   unsigned int* status;
 };
 

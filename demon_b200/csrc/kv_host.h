@@ -6,7 +6,7 @@ namespace demon {
 namespace kv {
 struct Cache;
 struct AttnParams;
-// kv_attention_tc.cu: the call's rows in blocks of 256 on the tensor cores.
+// kv_attention_tc.cu: the call's rows in blocks on the tensor cores; at most 128 query heads per kv head.
 int attention_tc(AttnParams p, cudaStream_t st);
 }  // namespace kv
 // DEMON_OK, or DEMON_ERR_INVALID with the message set (`who`: the entry point's name).
