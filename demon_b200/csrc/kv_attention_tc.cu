@@ -21,14 +21,18 @@
 // where 2^(t_j - m) does not; the tile's sum then takes a second exponential per key.
 // Output: O * 2^(M - m - 6) / l.  Both offsets are raised only when exceeded by more than 8.
 //
-// Warp roles (512 threads; setmaxnreg as in attention.cu):
-//   warpgroup 0 / 1   row half 0 / 1, one query row per thread: the softmax of every key tile, the
+// Warp roles (512 threads):
+//   warpgroup 0 / 1   row half 0 / 1, one query row per thread: the softmax in steps of 64 keys, the
 //                     output row,
 //   warpgroup 2       codes -> f16, swizzled, into a ring of three K / V tiles; the Q rows in place,
 //   warp 12           MMA issue (one thread) and tensor-memory allocation,
 //   warp 13           page look-ups, scales, bulk copies of K / V codes into a ring of half tiles,
-//   warp 14           the next unit's Q by TMA, each half as soon as the last Q K^T has read the slot.
-// Tensor memory as in attention.cu: S_h at 128 h, P_h over its upper half, O_h at 256 + 128 h.
+//   warp 14           the next unit's Q by TMA, each half as soon as the last Q K^T has read the slot,
+//   warp 15           the list of units: lengths and masks into a ring of records that every role reads.
+// Tensor memory (512 columns): two score buffers of 64 keys per half, S_h at 128 h + 64 (step % 2), the
+// f16 probabilities over their upper halves, and O_h at 256 + 128 h.  Q K^T of step u + 1 is issued
+// before P V of step u, so that a softmax warp finds its next scores ready; with one buffer of 128
+// keys it waited some 1,600 of 4,400 clocks per 128 keys for P V and Q K^T to pass through.
 //
 // Bound by the exponentials (one per row and key, 16 per clock and SM) and the MMAs, which take
 // as long; short key ranges (256 keys of a condition are two tiles) by the units' Q and output.
@@ -51,17 +55,17 @@ constexpr int kRaw = kBlk * kHeadDim;    // 16 KB
 constexpr int kScSlots = 8;              // tiles whose scales are kept (see the ring comment)
 constexpr int kNanSlots = 4;             // tiles whose NaN maps are kept
 constexpr int kConvWarps = 4;
+constexpr int kUnitSlots = 4;            // unit records in flight
+constexpr int kUnitReaders = 8 + kConvWarps + 3;  // warps that read each record
 constexpr int kThreads = 512;
 constexpr float kBias = 6.0f;            // P = 2^(.. + 6)
 constexpr float kRaise = 8.0f;           // offsets are raised when exceeded by more than this
 constexpr float kFast = 60.0f;           // |M - m - ev| up to which l comes from P
 
-constexpr int kLaunchRegs = 128, kSoftmaxRegs = 176, kConvRegs = 72, kIssueRegs = 88;
-static_assert(256 * kSoftmaxRegs + 128 * kConvRegs + 128 * kIssueRegs <= kThreads * kLaunchRegs,
-              "register split exceeds the launch's registers (setmaxnreg.inc would wait for good)");
+constexpr int kStep = 64;                // keys per softmax step
 
-// Scales of a tile: per 16 keys {K scale, V exponent ev, 2^(ev_0 - ev), 0}, then {smallest ev,
-// largest ev, 16-key groups without a page, 0}.
+// Scales of a tile: per 16 keys {K scale, V exponent ev, 2^(ev_0 - ev), 0}, and {., -inf, ., -inf}
+// for keys without a page, which so weigh nothing; then {smallest ev, largest ev, ev_0, 0}.
 constexpr int kScWords = 36;
 constexpr int kScTail = 32;
 
@@ -73,15 +77,16 @@ constexpr int offNanRow = offNan + kNanSlots * kBlk * 16;      // [2][128] 128-b
 constexpr int offRow = offNanRow + 2 * kBlk * 16;              // [2 units][2 halves][128] powers of two
 constexpr int offSc = offRow + 4 * kBlk * 4;
 constexpr int offNanW = offSc + kScSlots * kScWords * 4;       // [slot][warp] any NaN
-constexpr int offRawMask = offNanW + kScSlots * 4 * 4;         // [slot] 16-key groups copied
+constexpr int offUnit = offNanW + kScSlots * 4 * 4;            // [slot] 12 words
+constexpr int offRawMask = offUnit + kUnitSlots * 48;          // [slot] 16-key groups copied
 constexpr int offBar = offRawMask + 4 * 4;
-constexpr int kNumBars = 4 + 2 * kSlots + 8 + 1 + 2 * kScSlots + 2 * kRawSlots + 6;
+constexpr int kNumBars = 4 + 2 * kSlots + 12 + 1 + 2 * kScSlots + 2 * kRawSlots + 6 + 2 * kUnitSlots;
 constexpr int offMisc = offBar + kNumBars * 8;
 constexpr int kSmem = offMisc + 16 + 1024;
 static_assert(kSmem <= 232448, "shared memory exceeds the sm_100 per-block limit");
 
 constexpr uint32_t kTmemCols = 512;
-constexpr uint32_t kColS = 0, kColP = 64, kColO = 256;
+constexpr uint32_t kColS = 0, kColP = 32, kColO = 256;  // P within its score buffer
 
 // kind::f16, F16 x F16 -> F32, K-major A and B
 constexpr uint32_t idesc_f16(int M, int N) {
@@ -101,18 +106,13 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
+// A warp-uniform bounded wait.  Most find their phase complete, and the cost of a completed wait
+// counts on the MMA warp's path (175 clocks each with the abort flag read every time: 439 us against
+// 402 us for 16 heads over 6,016 queries and keys), so only a wait that goes on looks at the flag.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, uint64_t t0,
                                           unsigned int* status, unsigned int where) {
-  const bool ok = mbar_wait(bar, parity, abort, t0, status, where);
-  return __all_sync(0xffffffffu, ok && *abort == 0);
-}
-template <int N>
-__device__ __forceinline__ void setmaxnreg_inc() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void setmaxnreg_dec() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+  if (__all_sync(0xffffffffu, mbar_try_wait(smem_u32(bar), parity))) return true;
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, t0, status, where));
 }
 __device__ __forceinline__ void st_shared_u16(uint32_t a, uint32_t x) {
   asm volatile("st.shared.u16 [%0], %1;" ::"r"(a), "h"((unsigned short)x) : "memory");
@@ -148,7 +148,8 @@ struct Unit {
   int b, hk, len, nq;
   int i0;           // first token of the block
   Keys ks;          // keys that some / every row of the block sees
-  int tile0, nt;    // key tiles
+  int tile0, nt;    // key tiles; nt 0: no keys (its rows are zeros), nt -1: no more units
+  int ns;           // steps of 64 keys
 };
 
 // The j-th unit of this CTA: rounds go over the CTAs in turn, back and forth, since the units
@@ -169,22 +170,23 @@ __device__ __forceinline__ Unit decode(const AttnParams& p, uint32_t u, bool* ba
   w.ks.lo = w.ks.hi = w.ks.lo_all = w.ks.hi_all = 0;
   if (w.i0 <= i1) w.ks = visible(w.i0, i1, w.len, w.nq, p.causal != 0, p.window);
   w.tile0 = w.ks.lo / kBlk;
-  w.nt = w.ks.hi > w.ks.lo ? (w.ks.hi + kBlk - 1) / kBlk - w.tile0 : 0;
+  w.ns = w.ks.hi > w.ks.lo ? (w.ks.hi - w.tile0 * kBlk + kStep - 1) / kStep : 0;
+  w.nt = (w.ns + 1) / 2;
   return w;
 }
-// Advances *j to the next unit with keys; false when there is none.
-__device__ __forceinline__ bool next_unit(const AttnParams& p, uint32_t units, uint32_t* j, Unit* w) {
-  bool bad = false;
-  for (;; ++*j) {
-    if ((uint64_t)*j * gridDim.x >= units) return false;
-    const uint32_t u = unit_index(*j);
-    if (u >= units) continue;
-    *w = decode(p, u, &bad);
-    if (w->nt > 0) {
-      ++*j;
-      return true;
-    }
-  }
+// A unit's record in shared memory.
+__device__ __forceinline__ void put_unit(uint32_t a, const Unit& w) {
+  st_shared_v4(a, w.b, w.hk, w.len, w.nq);
+  st_shared_v4(a + 16, w.i0, w.ks.lo, w.ks.hi, w.ks.lo_all);
+  st_shared_v4(a + 32, w.ks.hi_all, w.tile0, w.nt, w.ns);
+}
+__device__ __forceinline__ Unit get_unit(uint32_t a) {
+  const uint4 x = ld_shared_v4(a), y = ld_shared_v4(a + 16), z = ld_shared_v4(a + 32);
+  Unit w;
+  w.b = (int)x.x, w.hk = (int)x.y, w.len = (int)x.z, w.nq = (int)x.w;
+  w.i0 = (int)y.x, w.ks.lo = (int)y.y, w.ks.hi = (int)y.z, w.ks.lo_all = (int)y.w;
+  w.ks.hi_all = (int)z.x, w.tile0 = (int)z.y, w.nt = (int)z.z, w.ns = (int)z.w;
+  return w;
 }
 
 template <int NG>  // 16-key-or-larger groups of a tile with a scale of their own: 128 / min(P, 128)
@@ -198,21 +200,23 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
   uint64_t* q_empty = q_full + 2;               // [2] the unit's last Q K^T done
   uint64_t* kv_full = q_empty + 2;              // [3] K or V tile converted
   uint64_t* kv_empty = kv_full + kSlots;        // [3] its MMAs done
-  uint64_t* s_full = kv_empty + kSlots;         // [2] S_h computed
-  uint64_t* pa_full = s_full + 2;               // [2] P_h of keys 0-63 in tensor memory
-  uint64_t* pb_full = s_full + 4;               // [2] P_h of keys 64-127
-  uint64_t* o_full = s_full + 6;                // [2] the unit's last P V done
-  uint64_t* mma_done = s_full + 8;
+  uint64_t* s_full = kv_empty + kSlots;         // [2 halves][2 buffers] S computed
+  uint64_t* p_full = s_full + 4;                // [2 halves][2 buffers] P in tensor memory
+  uint64_t* pv_done = p_full + 4;               // [2] P_h V of a step done
+  uint64_t* o_full = pv_done + 2;               // [2] the unit's last P_h V done
+  uint64_t* mma_done = o_full + 2;
   // The scales and NaN maps have rings longer than any lag between their writers and readers: V of
-  // tile t takes the slot of K of tile t - 1, whose Q K^T were issued after both softmax warpgroups
-  // published P of tile t - 2, and so were done with tile t - 3; the codes of tile t are copied
-  // at most two tiles before that.
+  // tile t takes the slot of K of tile t - 1, whose last Q K^T was issued after both softmax
+  // warpgroups had published, and so were done with, tile t - 2; the codes of tile t are copied at
+  // most two tiles before that.
   uint64_t* sc_full = mma_done + 1;             // [8] scales of a tile
   uint64_t* nan_full = sc_full + kScSlots;      // [8] NaN map of a tile
   uint64_t* raw_full = nan_full + kScSlots;     // [3] codes of a half tile copied
   uint64_t* raw_empty = raw_full + kRawSlots;   // [3] and converted
   uint64_t* row_full = raw_empty + kRawSlots;   // [2 units][2 halves] rows' powers of two
   uint64_t* q_raw = row_full + 4;               // [2] Q half copied
+  uint64_t* unit_full = q_raw + 2;              // [4] unit record written
+  uint64_t* unit_empty = unit_full + kUnitSlots;  // [4] and read by every role
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + offMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + offMisc + 4);
 
@@ -230,12 +234,18 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       mbar_init(&q_raw[h], 1);
       mbar_init(&row_full[h], kConvWarps);
       mbar_init(&row_full[2 + h], kConvWarps);
-      mbar_init(&s_full[h], 1);
-      mbar_init(&pa_full[h], 4);
-      mbar_init(&pb_full[h], 4);
+      mbar_init(&pv_done[h], 1);
       mbar_init(&o_full[h], 1);
+      for (int buf = 0; buf < 2; ++buf) {
+        mbar_init(&s_full[2 * h + buf], 1);
+        mbar_init(&p_full[2 * h + buf], 4);
+      }
     }
     mbar_init(mma_done, 1);
+    for (int s = 0; s < kUnitSlots; ++s) {
+      mbar_init(&unit_full[s], 1);
+      mbar_init(&unit_empty[s], kUnitReaders);
+    }
     for (int s = 0; s < kRawSlots; ++s) {
       mbar_init(&raw_full[s], 1);
       mbar_init(&raw_empty[s], kConvWarps);
@@ -256,98 +266,97 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
   const int wg = warp >> 2;
+  // The next unit for this warp (*j counts records); false at the end.  Units without keys only
+  // matter to the warps that write rows.
+  auto next_record = [&](uint32_t* j, Unit* w) {
+    const uint32_t s = *j % kUnitSlots;
+    if (!warp_wait(&unit_full[s], (*j / kUnitSlots) & 1u, abort_flag, t0, p.status, 70)) return false;
+    *w = get_unit(sbase + offUnit + s * 48);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&unit_empty[s]);
+    ++*j;
+    return w->nt >= 0;
+  };
+  auto next_unit = [&](uint32_t* j, Unit* w) {
+    do {
+      if (!next_record(j, w)) return false;
+    } while (w->nt == 0);
+    return true;
+  };
 
   if (wg == 3) {
-    setmaxnreg_dec<kIssueRegs>();
     if (warp == 12) {
-      // ------------------------------------------------------------------ MMA issue
+      // ------------------------------------------------------------------ MMA issue (one thread)
       if (elect_one()) {
-        const uint32_t idesc_qk = idesc_f16(kBlk, kBlk);
+        const uint32_t idesc_qk = idesc_f16(kBlk, kStep);
         const uint32_t idesc_pv = idesc_f16(kBlk, kHeadDim) | (1u << 16);  // B (V) MN-major
-        uint32_t g = 0, it = 0, tiles = 0;  // half tiles consumed, units, key tiles (all units)
-        bool ok = true;
-        auto qk = [&](int h, uint32_t kslot) {
-          const uint32_t qa = kmajor_lo(sbase + offQ + h * kTile), kb = kmajor_lo(sbase + offKV + kslot * kTile);
+        uint32_t g = 0, it = 0, step = 0;  // half tiles, units, steps (all units)
+        // S_h of a step: keys 64 part .. of the K tile in a slot
+        auto qk = [&](int h, uint32_t kslot, uint32_t part, uint32_t at) {
+          const uint32_t qa = kmajor_lo(sbase + offQ + h * kTile);
+          const uint32_t kb = kmajor_lo(sbase + offKV + kslot * kTile + part * kStep * 128);
+          const uint32_t d = tmem + kColS + 128 * h + kStep * (at & 1);
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)
-            mma_bf16(tmem + kColS + 128 * h, desc_of(qa + kmajor_step(kk)), desc_of(kb + kmajor_step(kk)), idesc_qk, kk > 0);
-          tc_commit(&s_full[h]);
+            mma_bf16(d, desc_of(qa + kmajor_step(kk)), desc_of(kb + kmajor_step(kk)), idesc_qk, kk > 0);
+          tc_commit(&s_full[2 * h + (at & 1)]);
         };
-        auto pv = [&](int h, uint32_t vslot, int half, bool acc) {
-          const uint32_t vb = mnmajor_lo(sbase + offKV + vslot * kTile);
+        auto pv = [&](int h, uint32_t vslot, uint32_t part, uint32_t at, bool acc) {
+          const uint32_t vb = mnmajor_lo(sbase + offKV + vslot * kTile + part * 4 * 2048);
+          const uint32_t pa = tmem + kColS + 128 * h + kStep * (at & 1) + kColP;
 #pragma unroll
-          for (int k4 = 0; k4 < 4; ++k4) {
-            const int kk = 4 * half + k4;
-            mma_bf16_ts(tmem + kColO + 128 * h, tmem + kColS + 128 * h + kColP + 8 * kk, desc_of(vb + mnmajor_step(kk)),
-                        idesc_pv, (acc || kk > 0) ? 1u : 0u);
-          }
+          for (int kk = 0; kk < 4; ++kk)
+            mma_bf16_ts(tmem + kColO + 128 * h, pa + 8 * kk, desc_of(vb + mnmajor_step(kk)), idesc_pv, (acc || kk > 0) ? 1u : 0u);
+          tc_commit(&pv_done[h]);
         };
         auto wait_on = [&](uint64_t* bar, uint32_t parity, unsigned int where) {
-          ok = mbar_wait(bar, parity, abort_flag, t0, p.status, where);
-          if (ok) tc_fence_after();
+          const bool ok = mbar_wait(bar, parity, abort_flag, t0, p.status, where);
+          tc_fence_after();
           return ok;
         };
-        auto wait_kv = [&](uint32_t gi) { return wait_on(&kv_full[gi % kSlots], (gi / kSlots) & 1u, 71); };
-        auto pv_tile = [&](int h, uint32_t vslot, uint32_t t, bool acc) {
-          if (!wait_on(&pa_full[h], t & 1u, 72)) return false;
-          pv(h, vslot, 0, acc);
-          if (!wait_on(&pb_full[h], t & 1u, 73)) return false;
-          pv(h, vslot, 1, true);
-          return true;
-        };
-        auto wait_q = [&](int h) { return wait_on(&q_full[h], it & 1u, 75); };
-        // As in attention.cu, a unit's last P_1 V goes after the next unit's first S_0.  A unit's first
-        // P_h V may overwrite O_h: its P_h comes from threads that have stored the last unit's rows.
-        bool pend = false, pend_acc = false;
-        uint32_t pend_v = 0, pend_t = 0;
-        auto flush = [&]() {
-          if (!pend) return true;
-          if (!pv_tile(1, pend_v % kSlots, pend_t, pend_acc)) return false;
-          tc_commit(&kv_empty[pend_v % kSlots]);
-          tc_commit(&o_full[1]);
-          pend = false;
-          return true;
-        };
-        uint32_t j = 0;
-        Unit w;
-        while (ok && next_unit(p, units, &j, &w)) {
-          const int n = w.nt;
-          uint32_t gk = g, gv = g + 1;
-          if (!wait_q(0) || !wait_kv(gk)) break;
-          qk(0, gk % kSlots);
-          if (n == 1) tc_commit(&q_empty[0]);
-          if (!flush() || !wait_q(1)) break;
-          qk(1, gk % kSlots);
-          tc_commit(&kv_empty[gk % kSlots]);
-          if (n == 1) tc_commit(&q_empty[1]);
-          if (!wait_kv(gv) || !pv_tile(0, gv % kSlots, tiles, false)) break;
-          uint32_t prev_v = gv;
-          g += 2;
-          for (int i = 1; i < n; ++i) {
-            gk = g;
-            gv = g + 1;
-            if (!wait_kv(gk)) break;
-            qk(0, gk % kSlots);
-            if (i == n - 1) tc_commit(&q_empty[0]);
-            if (!pv_tile(1, prev_v % kSlots, tiles + i - 1, i - 1 > 0)) break;
-            tc_commit(&kv_empty[prev_v % kSlots]);
-            qk(1, gk % kSlots);
-            tc_commit(&kv_empty[gk % kSlots]);
-            if (i == n - 1) tc_commit(&q_empty[1]);
-            if (!wait_kv(gv) || !pv_tile(0, gv % kSlots, tiles + i, true)) break;
-            prev_v = gv;
-            g += 2;
+        // Per step: Q K^T of the next step for both halves, then P V of this one.  A unit's first P_h V
+        // may overwrite O_h: its P_h comes from threads that have stored the last unit's rows.
+        bool ok = true;
+        for (uint32_t j = 0; ok; ++j) {
+          const uint32_t us = j % kUnitSlots;
+          if (!wait_on(&unit_full[us], (j / kUnitSlots) & 1u, 70)) break;
+          const int ns = (int)ld_shared_b32(sbase + offUnit + us * 48 + 44);
+          mbar_arrive(&unit_empty[us]);
+          if (ns < 0) break;
+          uint32_t ks = g % kSlots, kp = (g / kSlots) & 1u;  // slot and phase of the K tile to come
+#pragma unroll 1
+          for (int v = 0; v <= ns; ++v) {  // v: the step whose scores are issued; v - 1: whose product is
+            if (v < ns) {
+              ks = (g + (uint32_t)(v & ~1)) % kSlots;
+              kp = ((g + (uint32_t)(v & ~1)) / kSlots) & 1u;
+              if (!(v & 1) && !(ok = wait_on(&kv_full[ks], kp, 71))) break;
+              const uint32_t at = step + (uint32_t)v;
+              if (v == 0 && !(ok = wait_on(&q_full[0], it & 1u, 75))) break;
+              qk(0, ks, v & 1, at);
+              if (v == ns - 1) tc_commit(&q_empty[0]);
+              if (v == 0 && !(ok = wait_on(&q_full[1], it & 1u, 75))) break;
+              qk(1, ks, v & 1, at);
+              if (v == ns - 1) tc_commit(&q_empty[1]);
+              if ((v & 1) || v == ns - 1) tc_commit(&kv_empty[ks]);
+            }
+            if (v == 0) continue;
+            const uint32_t u = (uint32_t)v - 1, at = step + u, buf = at & 1u, ph = (at >> 1) & 1u;
+            const uint32_t vg = g + (u & ~1u) + 1, vs = vg % kSlots;
+            if (!(u & 1) && !(ok = wait_on(&kv_full[vs], (vg / kSlots) & 1u, 71))) break;
+            if (!(ok = wait_on(&p_full[buf], ph, 72))) break;
+            pv(0, vs, u & 1, at, u > 0);
+            if (v == ns) tc_commit(&o_full[0]);
+            if (!(ok = wait_on(&p_full[2 + buf], ph, 73))) break;
+            pv(1, vs, u & 1, at, u > 0);
+            if (v == ns) tc_commit(&o_full[1]);
+            if ((u & 1) || v == ns) tc_commit(&kv_empty[vs]);
           }
-          if (!ok) break;
-          tc_commit(&o_full[0]);
-          pend = true;
-          pend_v = prev_v;
-          pend_t = tiles + n - 1;
-          pend_acc = n > 1;
-          tiles += n;
-          ++it;
+          if (ns > 0) {
+            step += (uint32_t)ns;
+            g += 2 * (uint32_t)((ns + 1) / 2);
+            ++it;
+          }
         }
-        if (ok) flush();
         tc_commit(mma_done);
       }
       __syncwarp();
@@ -381,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
           }
         }
       };
-      bool ok = true, have = next_unit(p, units, &j, &w);
+      bool ok = true, have = next_unit(&j, &w);
       if (have) look_up(w, 0, pid, sk, sv, absent);
       while (have && ok) {
         // the next tile's pages and scales are on their way while this one's copies wait for room
@@ -390,11 +399,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         int ntile = tile + 1, npid = -1;
         float nsk = 0.0f, nsv = 0.0f;
         if (ntile >= w.nt) {
-          more = next_unit(p, units, &j, &nw);
+          more = next_unit(&j, &nw);
           ntile = 0;
         }
         if (more) look_up(nw, ntile, npid, nsk, nsv, nabsent);
-        const uint32_t held = __ballot_sync(0xffffffffu, pid >= 0), gone = __ballot_sync(0xffffffffu, absent);
+        const uint32_t held = __ballot_sync(0xffffffffu, pid >= 0);
         const uint32_t sc = sbase + offSc + (tiles % kScSlots) * kScWords * 4;
         // keys without a page take another group's V exponent: they weigh nothing
         int ev = scale_exp(sv);
@@ -403,8 +412,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         const int ev0 = __shfl_sync(0xffffffffu, ev, 0);
         if (lane >= 8) ev = ev0;
         const int elo = __reduce_min_sync(0xffffffffu, ev), ehi = __reduce_max_sync(0xffffffffu, ev);
-        if (lane < 8) st_shared_f32x4(sc + 16 * lane, fabsf(sk), (float)ev, exp2i(imin(imax(ev0 - ev, -126), 126)), 0.0f);
-        if (lane == 8) st_shared_f32x4(sc + 4 * kScTail, (float)elo, (float)ehi, __uint_as_float(gone), 0.0f);
+        if (lane < 8)
+          st_shared_f32x4(sc + 16 * lane, fabsf(sk), absent ? -INFINITY : (float)ev, exp2i(imin(imax(ev0 - ev, -126), 126)),
+                          absent ? -INFINITY : 0.0f);
+        if (lane == 8) st_shared_f32x4(sc + 4 * kScTail, (float)elo, (float)ehi, (float)ev0, 0.0f);
         __syncwarp();
         if (lane == 0) mbar_arrive(&sc_full[tiles % kScSlots]);
         const bool copies = pid >= 0 && (16 * lane) % gw == 0;
@@ -437,28 +448,51 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       __syncwarp();
     } else if (warp == 14) {
       // ------------------------------------------------------------------ Q
-      if (elect_one()) {
-        uint32_t j = 0, it = 0;
-        uint32_t issued = 0;  // halves
-        Unit w;
-        bool ok = true;
-        const uint32_t bytes = (uint32_t)(p.Tt * p.G) * kHeadDim * 2;
-        for (; ok && next_unit(p, units, &j, &w); ++it)
-          for (int h = 0; h < 2; ++h, ++issued) {
-            if (!(ok = mbar_wait(&q_empty[h], (it & 1u) ^ 1u, abort_flag, t0, p.status, 91))) break;
+      uint32_t j = 0, it = 0;
+      uint32_t issued = 0;  // halves
+      Unit w;
+      bool ok = true;
+      const uint32_t bytes = (uint32_t)(p.Tt * p.G) * kHeadDim * 2;
+      for (; ok && next_unit(&j, &w); ++it)
+        for (int h = 0; h < 2; ++h) {
+          if (!(ok = warp_wait(&q_empty[h], (it & 1u) ^ 1u, abort_flag, t0, p.status, 91))) break;
+          if (lane == 0) {
             mbar_arrive_expect_tx(&q_raw[h], bytes);
             for (int box = 0; box < 2; ++box)
               tma_load_4d(sbase + offQ + h * kTile + box * kBox, &tmQ, &q_raw[h], 64 * box, w.hk * p.G, w.i0 + h * p.Tt, w.b);
           }
-        // no copy may still be in flight when the CTA leaves (immediate on the normal path)
-        volatile int never = 0;
-        for (uint32_t i = issued > 2 ? issued - 2 : 0; i < issued; ++i)
-          mbar_wait(&q_raw[i & 1], (i >> 1) & 1u, &never, globaltimer(), p.status, 93);
-      }
+          __syncwarp();
+          ++issued;
+        }
+      // no copy may still be in flight when the CTA leaves (immediate on the normal path)
+      volatile int never = 0;
+      for (uint32_t i = issued > 2 ? issued - 2 : 0; i < issued; ++i)
+        mbar_wait(&q_raw[i & 1], (i >> 1) & 1u, &never, globaltimer(), p.status, 93);
       __syncwarp();
+    } else {
+      // ------------------------------------------------------------------ units
+      for (uint32_t j = 0, n = 0;; ++j) {
+        bool bad = false;
+        Unit w;
+        w.nt = w.ns = -1;
+        if ((uint64_t)j * gridDim.x < units) {
+          const uint32_t u = unit_index(j);
+          if (u >= units) continue;
+          w = decode(p, u, &bad);
+          if (bad && w.hk == 0 && w.i0 == 0 && lane == 0) report(p.status, DEMON_DEV_BAD_ARG, 63);
+        }
+        const uint32_t s = n % kUnitSlots;
+        if (!warp_wait(&unit_empty[s], ((n / kUnitSlots) & 1u) ^ 1u, abort_flag, t0, p.status, 69)) break;
+        if (lane == 0) {
+          put_unit(sbase + offUnit + s * 48, w);
+          mbar_arrive(&unit_full[s]);
+        }
+        __syncwarp();
+        ++n;
+        if (w.nt < 0) break;
+      }
     }
   } else if (wg == 2) {
-    setmaxnreg_dec<kConvRegs>();
     // -------------------------------------------------------------------- codes -> f16
     // Warp cw takes keys 32 cw .. 32 cw + 31: chunk i is 16 codes of row 8 (i / 2) + lane / 4, and
     // neighbouring rows take opposite halves of their 128 codes (no bank conflicts either way).
@@ -468,38 +502,25 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
     auto q_convert = [&](int h, uint32_t unit) {
       const int rr = cw * 32 + lane;
       const uint32_t base = sbase + offQ + h * kTile + rr * 128;
-      uint32_t mx = 0, all = 0;
-#pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        const uint4 x = ld_shared_v4(base + (k >> 3) * kBox + (((k & 7) ^ (rr & 7)) << 4));
+      const uint32_t flip = (rr & 7) << 4;
+      uint32_t mx = 0;
+#pragma unroll 4
+      for (int k = 0; k < 16; ++k) {  // infinities and NaN do not count, and pass through
+        const uint4 x = ld_shared_v4(base + (k >> 3) * kBox + ((k & 7) << 4 ^ flip));
         const uint32_t y[4] = {x.x & 0x7FFF7FFFu, x.y & 0x7FFF7FFFu, x.z & 0x7FFF7FFFu, x.w & 0x7FFF7FFFu};
-        all = __vmaxu2(all, __vmaxu2(__vmaxu2(y[0], y[1]), __vmaxu2(y[2], y[3])));
+#pragma unroll
+        for (int q = 0; q < 4; ++q) mx = __vmaxu2(mx, y[q] & __vcmpltu2(y[q], 0x7F807F80u));
       }
-      all = max(all & 0xFFFFu, all >> 16);
-      mx = all;
-      if (all >= 0x7F80u) {  // infinities and NaN do not count, and pass through
-        mx = 0;
-        for (int k = 0; k < 16; ++k) {
-          const uint4 x = ld_shared_v4(base + (k >> 3) * kBox + (((k & 7) ^ (rr & 7)) << 4));
-          const uint32_t y[4] = {x.x & 0x7FFF7FFFu, x.y & 0x7FFF7FFFu, x.z & 0x7FFF7FFFu, x.w & 0x7FFF7FFFu};
-          for (int q = 0; q < 4; ++q) mx = __vmaxu2(mx, y[q] & __vcmpltu2(y[q], 0x7F807F80u));
-        }
-        mx = max(mx & 0xFFFFu, mx >> 16);
-      }
+      mx = max(mx & 0xFFFFu, mx >> 16);
       const int e = imax((int)(mx >> 7) - 127 - 13, -126);  // |q| 2^-e < 2^14
       const float2 mul = make_float2(exp2i(-e), exp2i(-e));
-#pragma unroll
-      for (int part = 0; part < 2; ++part) {
-        uint4 x[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) x[k] = ld_shared_v4(base + part * kBox + ((k ^ (rr & 7)) << 4));
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float2 f0 = mul_f2(bf2_f2(x[k].x), mul), f1 = mul_f2(bf2_f2(x[k].y), mul), f2 = mul_f2(bf2_f2(x[k].z), mul),
-                       f3 = mul_f2(bf2_f2(x[k].w), mul);
-          st_shared_v4(base + part * kBox + ((k ^ (rr & 7)) << 4), pack_f16x2(f0.x, f0.y), pack_f16x2(f1.x, f1.y),
-                       pack_f16x2(f2.x, f2.y), pack_f16x2(f3.x, f3.y));
-        }
+#pragma unroll 4
+      for (int k = 0; k < 16; ++k) {
+        const uint32_t a = base + (k >> 3) * kBox + ((k & 7) << 4 ^ flip);
+        const uint4 x = ld_shared_v4(a);
+        const float2 f0 = mul_f2(bf2_f2(x.x), mul), f1 = mul_f2(bf2_f2(x.y), mul), f2 = mul_f2(bf2_f2(x.z), mul),
+                     f3 = mul_f2(bf2_f2(x.w), mul);
+        st_shared_v4(a, pack_f16x2(f0.x, f0.y), pack_f16x2(f1.x, f1.y), pack_f16x2(f2.x, f2.y), pack_f16x2(f3.x, f3.y));
       }
       const uint32_t rs = (unit & 1) * 2 + h;
       st_shared_f32(sbase + offRow + (rs * kBlk + rr) * 4, exp2i(e));
@@ -514,7 +535,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
     uint32_t n = 0, tiles = 0, j = 0, it = 0;
     bool ok = true;
     Unit w;
-    for (; ok && next_unit(p, units, &j, &w); ++it) {
+    for (; ok && next_unit(&j, &w); ++it) {
       for (int t = 0; ok && t < w.nt; ++t, ++tiles) {
         const int k0 = (w.tile0 + t) * kBlk;
         const bool whole = k0 >= w.ks.lo_all && k0 + kBlk <= w.ks.hi_all;
@@ -536,24 +557,28 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
           if (kv && !whole) {
             // Some row does not see some key: NaN codes go into a map instead of the product.
             // (Where every row sees every key they may run through it.)
-            const uint32_t map = sbase + offNan + ((tiles % kNanSlots) * kBlk + cw * 32 + rl) * 16;
             uint32_t any = 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const uint32_t y[4] = {nan_bytes(r[i].x) >> 7, nan_bytes(r[i].y) >> 7, nan_bytes(r[i].z) >> 7,
-                                     nan_bytes(r[i].w) >> 7};
-              r[i].x &= ~(y[0] * 255u);
-              r[i].y &= ~(y[1] * 255u);
-              r[i].z &= ~(y[2] * 255u);
-              r[i].w &= ~(y[3] * 255u);
-              uint32_t bits = 0;
-#pragma unroll
-              for (int q = 0; q < 4; ++q) bits |= ((y[q] | (y[q] >> 7) | (y[q] >> 14) | (y[q] >> 21)) & 15u) << (4 * q);
-              any |= bits;
-              st_shared_u16(map + (i >> 1) * 8 * 16 + (((i & 1) ^ (rl & 1)) * 4 + c) * 2, bits);
-            }
+            for (int i = 0; i < 8; ++i) any |= nan_bytes(r[i].x) | nan_bytes(r[i].y) | nan_bytes(r[i].z) | nan_bytes(r[i].w);
             any = __reduce_or_sync(0xffffffffu, any);
             if (lane == 0) st_shared_b32(sbase + offNanW + ((tiles % kScSlots) * 4 + cw) * 4, any);
+            const uint32_t map = sbase + offNan + ((tiles % kNanSlots) * kBlk + cw * 32 + rl) * 16;
+            if (any) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                uint32_t y[4] = {r[i].x, r[i].y, r[i].z, r[i].w}, bits = 0;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                  const uint32_t x = nan_bytes(y[q]) >> 7;
+                  y[q] &= ~(x * 255u);
+                  bits |= ((x | (x >> 7) | (x >> 14) | (x >> 21)) & 15u) << (4 * q);
+                }
+                r[i] = make_uint4(y[0], y[1], y[2], y[3]);
+                st_shared_u16(map + (i >> 1) * 8 * 16 + (((i & 1) ^ (rl & 1)) * 4 + c) * 2, bits);
+              }
+            } else {
+              st_shared_v4(sbase + offNan + ((tiles % kNanSlots) * kBlk + cw * 32 + lane) * 16, 0, 0, 0, 0);
+            }
           }
           const uint32_t dst = sbase + offKV + (n % kSlots) * kTile + cw * 32 * 128;
 #pragma unroll
@@ -576,6 +601,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
           }
         }
         if (t == 0 && ok) {
+#pragma unroll 1
           for (int h = 0; ok && h < 2; ++h) {
             ok = warp_wait(&q_raw[h], it & 1u, abort_flag, t0, p.status, 90);
             if (ok) q_convert(h, it);
@@ -584,13 +610,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       }
     }
   } else {
-    setmaxnreg_inc<kSoftmaxRegs>();
     // -------------------------------------------------------------------- query rows
-    constexpr int GW = kBlk / NG, CH = 8 / NG;  // columns and maximum chains per group
-    constexpr int SG = 8 / NG;                  // 16-key scale entries per group
+    constexpr int NS = NG > 1 ? NG / 2 : 1;      // scale groups of a step
+    constexpr int GW = kStep / NS, CH = 4 / NS;  // their columns and maximum chains
+    constexpr int SG = 4 / NS;                   // 16-key scale entries per group
     const int h = wg, quad = warp & 3, rr = quad * 32 + lane;
     const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
-    const uint32_t s_addr = tmem + lane_addr + kColS + 128 * h;
     const uint32_t o_addr = tmem + lane_addr + kColO + 128 * h;
     const int ri = rr / p.G, rg = rr - ri * p.G;  // token and head of this row within the half
     auto token_of = [&](const Unit& w) { return w.i0 + h * p.Tt + ri; };
@@ -612,33 +637,26 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         for (int q = 0; q < 4; ++q) st_global_v4(o + 8 * q, make_uint4(x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]));
       }
     };
-    // this CTA's next unit; rows of units without keys are zeroed on the way
+    // the next unit; rows of units without keys are zeroed on the way
     uint32_t j = 0;
     auto advance = [&](Unit* w) {
-      for (;; ++j) {
-        if ((uint64_t)j * gridDim.x >= units) return false;
-        const uint32_t u = unit_index(j);
-        if (u >= units) continue;
-        bool bad = false;
-        *w = decode(p, u, &bad);
-        if (bad && w->hk == 0 && w->i0 == 0 && threadIdx.x == 0) report(p.status, DEMON_DEV_BAD_ARG, 63);
-        if (w->nt > 0) {
-          ++j;
-          return true;
-        }
+      while (next_record(&j, w)) {
+        if (w->nt > 0) return true;
         const uint32_t zero[16] = {};
         bool inside;
         __nv_bfloat16* o = out_row(*w, &inside);
-        if (inside)
+        if (inside) {
+#pragma unroll 1
           for (int c = 0; c < 4; ++c) put(o + 32 * c, zero);
+        }
       }
+      return false;
     };
 
-    uint32_t t = 0, it = 0;
-    Unit w, nw;
+    uint32_t t = 0, it = 0, step = 0;  // tiles, units, steps (all units)
+    Unit w;
     const uint32_t nan_at = sbase + offNanRow + (h * kBlk + rr) * 16;
-    bool have = advance(&w);
-    for (; have; ++it) {
+    for (; advance(&w); ++it) {
       int jlo = 0, jhi = w.len;  // keys that this row sees: [jlo, jhi)
       bool live;
       {
@@ -650,41 +668,41 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
           jhi = k.hi;
         }
       }
-      const bool more = advance(&nw);
       float M = -INFINITY, m = -INFINITY, l = 0.0f;
       st_shared_v4(nan_at, 0, 0, 0, 0);
       const uint32_t rs = (it & 1) * 2 + h;
       bool ok = warp_wait(&row_full[rs], (it >> 1) & 1u, abort_flag, t0, p.status, 80);
       if (!ok) break;
       const float fr = ld_shared_f32(sbase + offRow + (rs * kBlk + rr) * 4) * p.scale_log2;
-      for (int i = 0; i < w.nt; ++i, ++t) {
-        if (!(ok = warp_wait(&sc_full[t % kScSlots], (t / kScSlots) & 1u, abort_flag, t0, p.status, 82))) break;
-        const uint32_t sc = sbase + offSc + (t % kScSlots) * kScWords * 4;
+      for (int i = 0; i < w.ns; ++i, ++step) {
+        const uint32_t tt = t + (uint32_t)(i >> 1);  // key tile
+        if (!(i & 1) && !(ok = warp_wait(&sc_full[tt % kScSlots], (tt / kScSlots) & 1u, abort_flag, t0, p.status, 82))) break;
+        const uint32_t sc = sbase + offSc + (tt % kScSlots) * kScWords * 4;
         const float4 tail = ld_shared_f32x4(sc + 4 * kScTail);
-        const uint32_t gone = __float_as_uint(tail.z);
-        const int k0 = (w.tile0 + i) * kBlk;
+        const uint32_t sg = sc + 64 * (i & 1);  // this step's scale entries
+        const int k0 = (w.tile0 + (i >> 1)) * kBlk + kStep * (i & 1);
         const int lo = jlo - k0, hi = jhi - 1 - k0;
-        const bool partly = __any_sync(0xffffffffu, lo > 0 || hi < kBlk - 1 || gone != 0);
-        if (!(ok = warp_wait(&s_full[h], t & 1u, abort_flag, t0, p.status, 81))) break;
+        const bool partly = __any_sync(0xffffffffu, lo > 0 || hi < kStep - 1);
+        const uint32_t buf = step & 1u;
+        const uint32_t s_addr = tmem + lane_addr + kColS + 128 * h + kStep * buf;
+        if (!(ok = warp_wait(&s_full[2 * h + buf], (step >> 1) & 1u, abort_flag, t0, p.status, 81))) break;
         tc_fence_after();
-        uint32_t sr[128];
+        uint32_t sr[kStep];
         tmem_ld_32x32b_x32(s_addr + 0, *reinterpret_cast<uint32_t(*)[32]>(sr + 0));
         tmem_ld_32x32b_x32(s_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(sr + 32));
-        tmem_ld_32x32b_x32(s_addr + 64, *reinterpret_cast<uint32_t(*)[32]>(sr + 64));
-        tmem_ld_32x32b_x32(s_addr + 96, *reinterpret_cast<uint32_t(*)[32]>(sr + 96));
         tmem_ld_wait();
         float* s = reinterpret_cast<float*>(sr);
         if (partly) {
-          // keys that this row does not see, and pages that do not exist
+          // keys that this row does not see
 #pragma unroll
-          for (int c = 0; c < 128; ++c) s[c] = (c < lo || c > hi || ((gone >> (c >> 4)) & 1u)) ? -INFINITY : s[c];
+          for (int c = 0; c < kStep; ++c) s[c] = (c < lo || c > hi) ? -INFINITY : s[c];
         }
         // score factor of a group, kept within 2^+-120: a masked score times 0 would be NaN
         const auto factor_of = [&](float k) { return fminf(fmaxf(fr * k, 7.5e-37f), 1.3e36f); };
         // maxima per group, in score units and with V's exponent
         float mt = -INFINITY, Mt = -INFINITY;
 #pragma unroll
-        for (int gi = 0; gi < NG; ++gi) {
+        for (int gi = 0; gi < NS; ++gi) {
           float mc[CH];
 #pragma unroll
           for (int c = 0; c < CH; ++c) {
@@ -695,9 +713,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
           float gm = mc[0];
 #pragma unroll
           for (int c = 1; c < CH; ++c) gm = fmaxf(gm, mc[c]);
-          const float4 g4 = ld_shared_f32x4(sc + 16 * gi * SG);
+          const float4 g4 = ld_shared_f32x4(sg + 16 * gi * SG);
           const float x = gm * factor_of(g4.x);
-          mt = fmaxf(mt, x);
+          mt = fmaxf(mt, x + g4.w);
           Mt = fmaxf(Mt, x + g4.y);
         }
         const bool up = mt > m + kRaise || (m == -INFINITY && mt > -INFINITY);
@@ -710,7 +728,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         if (__any_sync(0xffffffffu, up || UP || far)) {
           if (up) l *= ex2(m - m1);
           if (__any_sync(0xffffffffu, UP && i > 0)) {
-            // O_h *= 2^(M - M1): O_h is idle until this tile's P is published
+            // O_h *= 2^(M - M1): once the last step's P V is done O_h is idle until P is published (the
+            // one before it is: it went ahead of this step's Q K^T, so the parity is unambiguous)
+            if (!(ok = warp_wait(&pv_done[h], (step - 1) & 1u, abort_flag, t0, p.status, 84))) break;
+            tc_fence_after();
             const float f = UP ? ex2(M - M1) : 1.0f;
 #pragma unroll 1
             for (int oc = 0; oc < 8; ++oc) {
@@ -723,30 +744,33 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             }
           }
           if (__any_sync(0xffffffffu, far)) {  // l's terms by an exponential of their own
+#pragma unroll 1
+            for (int c = 0; c < kStep; c += 16) {
+              uint32_t x[16];
+              tmem_ld_32x32b_x16(s_addr + c, x);
+              tmem_ld_wait();
+              const float4 g4 = ld_shared_f32x4(sg + c);
+              const float f = factor_of(g4.x);
 #pragma unroll
-            for (int c = 0; c < 128; ++c) l += ex2(fmaf(s[c], factor_of(ld_shared_f32(sc + 16 * (c / GW) * SG)), -ml));
+              for (int q = 0; q < 16; ++q)
+                l += c + q < lo || c + q > hi ? 0.0f : ex2(fmaf(__uint_as_float(x[q]), f, g4.w - ml));
+            }
             lw = -INFINITY;
           }
           m = m1;
           M = M1;
         }
+        lw = ex2(lw - kBias - tail.z);  // weight of a sum at ev_0 in l
         float gf = 0.0f, gn = 0.0f, gl = 0.0f;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          if (c == 2) {
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&pa_full[h]);
-          }
+        for (int c = 0; c < 2; ++c) {
           uint32_t pk[16];
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             if ((32 * c + 16 * half) % GW == 0) {  // the next group
-              const float4 g4 = ld_shared_f32x4(sc + 16 * ((32 * c + 16 * half) / GW) * SG);
+              const float4 g4 = ld_shared_f32x4(sg + 16 * ((32 * c + 16 * half) / GW) * SG);
               gf = factor_of(g4.x);
               gn = g4.y - mo + kBias;
-              if (c == 0 && half == 0) lw = ex2(lw - kBias - g4.y);  // weight of group 0's sum in l
               gl = lw * g4.z;
             }
             const float2 f2 = make_float2(gf, gf), n2 = make_float2(gn, gn);
@@ -763,17 +787,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
           }
           tmem_st_32x32b_x16(s_addr + kColP + 16 * c, pk);
         }
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&pb_full[h]);
-        if (k0 < w.ks.lo_all || k0 + kBlk > w.ks.hi_all) {  // the converters left NaN codes of V out
-          if (!(ok = warp_wait(&nan_full[t % kScSlots], (t / kScSlots) & 1u, abort_flag, t0, p.status, 83))) break;
-          const uint4 any = ld_shared_v4(sbase + offNanW + (t % kScSlots) * 16);
+        const int kt = (w.tile0 + (i >> 1)) * kBlk;
+        if (kt < w.ks.lo_all || kt + kBlk > w.ks.hi_all) {  // the converters leave NaN codes of V out of such tiles
+          if (!(ok = warp_wait(&nan_full[tt % kScSlots], (tt / kScSlots) & 1u, abort_flag, t0, p.status, 83))) break;
+          const uint4 any = ld_shared_v4(sbase + offNanW + (tt % kScSlots) * 16);
           if (any.x | any.y | any.z | any.w) {
             uint4 seen = ld_shared_v4(nan_at);
-            const uint32_t map = sbase + offNan + (t % kNanSlots) * kBlk * 16;
-            for (int c = imax(lo, 0); c <= imin(hi, kBlk - 1); ++c) {
+            const uint32_t map = sbase + offNan + ((tt % kNanSlots) * kBlk + kStep * (i & 1)) * 16;
+            for (int c = imax(lo, 0); c <= imin(hi, kStep - 1); ++c) {
               const uint4 x = ld_shared_v4(map + c * 16);
               seen.x |= x.x;
               seen.y |= x.y;
@@ -783,53 +804,45 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             st_shared_v4(nan_at, seen.x, seen.y, seen.z, seen.w);
           }
         }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[2 * h + buf]);
       }
+      t += w.nt;
       if (!ok) break;
-      // the output row: O 2^(M - m - 6) / l, the factor in two parts where it is not normal
-      float fa = 1.0f, fb = 0.0f;
+      // the output row: O 2^(M - m - 6) / l, the factor in two parts that stay normal
+      float fa = 0.0f, fb = 0.0f;
       if (live && l != 0.0f) {
-        const float x = M - m - kBias;
-        if (fabsf(x) > 100.0f) {
-          fa = ex2(0.5f * x);
-          fb = fa / l;
-        } else {
-          fb = ex2(x) / l;
-        }
+        fa = ex2(0.5f * (M - m - kBias));
+        fb = fa / l;
       }
       bool inside;
       __nv_bfloat16* out = out_row(w, &inside);
-      const uint4 nan = ld_shared_v4(nan_at);
-      const bool odd = __any_sync(0xffffffffu, fa != 1.0f || (nan.x | nan.y | nan.z | nan.w) != 0);
       if (!warp_wait(&o_full[h], it & 1u, abort_flag, t0, p.status, 92)) break;
       tc_fence_after();
-#pragma unroll
-      for (int part = 0; part < 2; ++part) {
-        uint32_t o[64];
-        tmem_ld_32x32b_x32(o_addr + 64 * part, *reinterpret_cast<uint32_t(*)[32]>(o));
-        tmem_ld_32x32b_x32(o_addr + 64 * part + 32, *reinterpret_cast<uint32_t(*)[32]>(o + 32));
+      const float2 a2 = make_float2(fa, fa), b2 = make_float2(fb, fb);
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        uint32_t o[32], x[16];
+        tmem_ld_32x32b_x32(o_addr + 32 * c, o);
         tmem_ld_wait();
-        if (odd) {
 #pragma unroll
-          for (int q = 0; q < 64; ++q) {
-            const uint32_t bits = part == 0 ? (q < 32 ? nan.x : nan.y) : (q < 32 ? nan.z : nan.w);
-            o[q] = (bits >> (q & 31)) & 1u ? 0x7FFFFFFFu : __float_as_uint(__uint_as_float(o[q]) * fa);
-          }
+        for (int q = 0; q < 16; ++q) {
+          const float2 v = mul_f2(mul_f2(make_float2(__uint_as_float(o[2 * q]), __uint_as_float(o[2 * q + 1])), a2), b2);
+          x[q] = fb == 0.0f ? 0u : pack_bf16x2(v.x, v.y);  // rows that see nothing: zeros, never 0 * NaN
         }
-        const float2 f2 = make_float2(fb, fb);
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t x[16];
-#pragma unroll
-          for (int q = 0; q < 16; ++q) {
-            const float2 v = mul_f2(make_float2(__uint_as_float(o[32 * c + 2 * q]), __uint_as_float(o[32 * c + 2 * q + 1])), f2);
-            x[q] = fb == 0.0f ? 0u : pack_bf16x2(v.x, v.y);  // rows that see nothing: zeros, never 0 * NaN
-          }
-          if (inside) put(out + 64 * part + 32 * c, x);
+        if (inside) put(out + 32 * c, x);
+      }
+      const uint4 nan = ld_shared_v4(nan_at);
+      if ((nan.x | nan.y | nan.z | nan.w) && live) {  // channels that met a NaN of V
+#pragma unroll 1
+        for (int d = 0; d < kHeadDim; ++d) {
+          const uint32_t bits = d < 32 ? nan.x : d < 64 ? nan.y : d < 96 ? nan.z : nan.w;
+          if ((bits >> (d & 31)) & 1u) reinterpret_cast<unsigned short*>(out)[d] = 0x7FFF;
         }
       }
       tc_fence_before();  // O_h is read before this warp publishes the next unit's P_h
-      w = nw;
-      have = more;
     }
   }
 
@@ -843,12 +856,6 @@ std::atomic<uint64_t> g_attr{0};
 
 template <int NG>
 int prepare() {
-  cudaFuncAttributes fa;
-  DEMON_CUDA(cudaFuncGetAttributes(&fa, attention_tc_kernel<NG>));
-  if (fa.numRegs != kLaunchRegs) {
-    set_error("kv_attention: kernel built with %d registers per thread, the register split needs %d", fa.numRegs, kLaunchRegs);
-    return DEMON_ERR_CUDA;
-  }
   DEMON_CUDA(cudaFuncSetAttribute(attention_tc_kernel<NG>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
   return DEMON_OK;
 }
