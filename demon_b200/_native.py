@@ -182,9 +182,8 @@ def load() -> ctypes.CDLL:
         L.demon_silu_mul_quantize.argtypes = [_vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp]
         L.demon_head_norm_rope.argtypes = [_vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _f32, _vp]
         L.demon_attention.argtypes = [ctypes.POINTER(DemonAttnArgs), _vp]
-        L.demon_kv_append.argtypes = [ctypes.POINTER(DemonKvAppendArgs), _vp]
-        L.demon_kv_read.argtypes = [ctypes.POINTER(DemonKvReadArgs), _vp]
-        L.demon_kv_attention.argtypes = [ctypes.POINTER(DemonKvAttnArgs), _vp]
+        # argument blocks packed by kvcache.py (the structures above give their layout)
+        L.demon_kv_append.argtypes = L.demon_kv_read.argtypes = L.demon_kv_attention.argtypes = [ctypes.c_char_p, _vp]
         L.demon_kv_struct_sizes.argtypes = [ctypes.POINTER(_i64)] * 3
         for name in EXPORTED:
             getattr(L, name).restype = (_i64 if name in ("demon_nvfp4_sf_bytes", "demon_nvfp4_noalloc_scratch_bytes",
@@ -227,6 +226,12 @@ def stream_ptr(stream=None) -> int:
     import torch
     s = stream if stream is not None else torch.cuda.current_stream()
     return int(s.cuda_stream)
+
+
+def raw_stream(index: int) -> int:
+    """cudaStream_t of the current torch stream of device `index`, without a Stream object."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def device_status(stream=None) -> tuple[int, int]:

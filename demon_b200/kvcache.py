@@ -26,7 +26,7 @@ PyTorch fallback: every call goes to libdemon_b200.so.
 from __future__ import annotations
 
 import contextlib
-import ctypes
+import struct
 from dataclasses import dataclass
 
 import torch
@@ -58,8 +58,11 @@ class KVCache:
                 raise ValueError(f"cache {n} must be a contiguous float32 tensor [pages, heads]")
         if not k.is_cuda or any(t.device != k.device for t in (v, self.k_scale, self.v_scale)):
             raise ValueError("the cache's tensors must be on one CUDA device (demon_b200 has no CPU path)")
-        self._c = nat.DemonKvCache(nat.ptr(k), nat.ptr(v), nat.ptr(self.k_scale), nat.ptr(self.v_scale), k.shape[0],
-                                   k.shape[1], k.shape[2], HEAD_DIM, 0)
+        self._device = k.device
+        self._index = k.get_device()
+        self._heads = k.shape[1]
+        self._c = (k.data_ptr(), v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(), k.shape[0], k.shape[1],
+                   k.shape[2], HEAD_DIM, 0)
 
     @classmethod
     def empty(cls, pages: int, heads: int, page_size: int = 64, device="cuda") -> "KVCache":
@@ -82,38 +85,55 @@ class KVCache:
         return self.k.shape[2]
 
 
-def _launch(device: torch.device, stream):
+# The argument blocks of include/demon_b200.h as struct formats (native sizes, no implicit padding:
+# every 8-byte field lies at a multiple of 8).  Packing one takes a fraction of a microsecond where a
+# ctypes structure of as many fields takes several, and a call for one token is bound by the host.
+_CACHE = "4Pq4i"
+_APPEND = struct.Struct("@" + _CACHE + "P3qP3qPqPP4i")
+_READ = struct.Struct("@" + _CACHE + "P2qP2qPqP4i")
+_ATTN = struct.Struct("@" + _CACHE + "P3qP3qPqPP4i2ifi")
+for _s, _c in ((_APPEND, nat.DemonKvAppendArgs), (_READ, nat.DemonKvReadArgs), (_ATTN, nat.DemonKvAttnArgs)):
+    assert _s.size == nat.ctypes.sizeof(_c)
+
+_NO_CONTEXT = contextlib.nullcontext()
+_DEFAULT_SCALE = HEAD_DIM ** -0.5
+
+
+def _launch(index: int, stream):
     """The context a call launches in: the tensors' device current, and, when the caller names a
     stream, that stream current too (so that outputs are allocated for it)."""
     if stream is not None:
         return torch.cuda.stream(stream)
-    if device.index != torch.cuda.current_device():
-        return torch.cuda.device(device)
-    return contextlib.nullcontext()
+    if index != torch._C._cuda_getDevice():
+        return torch.cuda.device(index)
+    return _NO_CONTEXT
 
 
-def _bf16_rows(t: torch.Tensor, name: str, device: torch.device) -> None:
-    if t.dtype != torch.bfloat16 or t.dim() != 4 or t.device != device:
-        raise ValueError(f"{name} must be a 4-D bf16 tensor [B, rows, heads, 128] on {device}")
-    if t.shape[3] != HEAD_DIM or (t.stride(3) != 1 and t.numel()):
-        raise ValueError(f"{name}: head_dim must be 128 with unit stride (shape {tuple(t.shape)}, strides {t.stride()})")
+def _bf16_rows(t: torch.Tensor, name: str, index: int) -> tuple:
+    """Checks a [B, rows, heads, 128] bf16 tensor; its shape and (sequence, row, head) strides, 0
+    along dimensions of one entry (where a stride means nothing)."""
+    shape = t.shape
+    if t.dtype is not torch.bfloat16 or len(shape) != 4 or t.get_device() != index:
+        raise ValueError(f"{name} must be a 4-D bf16 tensor [B, rows, heads, 128] on cuda:{index}")
+    st = t.stride()
+    if shape[3] != HEAD_DIM or (st[3] != 1 and t.numel()):
+        raise ValueError(f"{name}: head_dim must be 128 with unit stride (shape {tuple(shape)}, strides {st})")
+    return shape, (0 if shape[0] == 1 else st[0], 0 if shape[1] == 1 else st[1], 0 if shape[2] == 1 else st[2])
 
 
-def _strides(t: torch.Tensor) -> tuple:
-    """(sequence, row, head) strides, 0 along dimensions of one entry (where a stride means nothing)."""
-    return tuple(0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride()[:3]))
+def _int32(t: torch.Tensor, name: str, B: int, index: int) -> int:
+    if t.dtype is not torch.int32 or t.shape != (B,) or t.get_device() != index or (B > 1 and t.stride(0) != 1):
+        raise ValueError(f"{name} must be a contiguous int32 tensor [{B}] on cuda:{index}")
+    return t.data_ptr()
 
 
-def _int32(t: torch.Tensor, name: str, B: int, device: torch.device) -> None:
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != B or t.device != device or (B > 1 and t.stride(0) != 1):
-        raise ValueError(f"{name} must be a contiguous int32 tensor [{B}] on {device}")
-
-
-def _table(t: torch.Tensor, B: int, device: torch.device) -> int:
-    if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != B or t.device != device or \
+def _table(t: torch.Tensor, B: int, index: int) -> tuple:
+    """(pointer, row pitch, width) of a page table."""
+    if t.dtype is not torch.int32 or t.dim() != 2 or t.shape[0] != B or t.get_device() != index or \
             (t.shape[1] > 1 and t.stride(1) != 1):
-        raise ValueError(f"table must be an int32 tensor [{B}, W] with unit column stride on {device}")
-    return t.stride(0) if B > 1 else t.shape[1]
+        raise ValueError(f"table must be an int32 tensor [{B}, W] with unit column stride on cuda:{index}")
+    W = t.shape[1]
+    return t.data_ptr(), t.stride(0) if B > 1 else W, W
 
 
 def append(cache: KVCache, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, start: torch.Tensor,
@@ -126,45 +146,43 @@ def append(cache: KVCache, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor
     through their strides (multiples of 8 elements; columns of a fused projection work as they
     are).  The pages a call writes must belong to one sequence each.
     """
-    dev = cache.k.device
-    _bf16_rows(k, "k", dev)
-    _bf16_rows(v, "v", dev)
-    B, S, H, _ = k.shape
-    if v.shape != k.shape or H != cache.heads:
-        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must be equal, with the cache's {cache.heads} heads")
-    ld = _table(table, B, dev)
-    _int32(start, "start", B, dev)
-    if count is not None:
-        _int32(count, "count", B, dev)
-    a = nat.DemonKvAppendArgs(cache._c, nat.ptr(k), *_strides(k), nat.ptr(v), *_strides(v), nat.ptr(table), ld,
-                              nat.ptr(start), nat.ptr(count), B, S, table.shape[1], 0)
+    dev = cache._index
+    shape, ks = _bf16_rows(k, "k", dev)
+    vshape, vs = _bf16_rows(v, "v", dev)
+    B, S = shape[0], shape[1]
+    if vshape != shape or shape[2] != cache._heads:
+        raise ValueError(f"k {tuple(shape)} and v {tuple(vshape)} must be equal, with the cache's {cache._heads} heads")
+    tp, ld, W = _table(table, B, dev)
+    args = _APPEND.pack(*cache._c, k.data_ptr(), *ks, v.data_ptr(), *vs, tp, ld, _int32(start, "start", B, dev),
+                        0 if count is None else _int32(count, "count", B, dev), B, S, W, 0)
     with _launch(dev, stream):
-        nat.check(nat.load().demon_kv_append(ctypes.byref(a), nat.stream_ptr(stream)))
+        nat.check(nat.load().demon_kv_append(args, nat.raw_stream(dev)))
 
 
 def read(cache: KVCache, table: torch.Tensor, lens: torch.Tensor, max_len: int, out=None, stream=None):
     """The cached values back in bf16: (k, v), each [B, max_len, heads, 128], positions
     0 .. ``lens[b]`` - 1 of sequence b and zeros from there.  ``out``: a (k, v) pair to write
     into (heads contiguous within a row)."""
-    dev = cache.k.device
+    dev, H, max_len = cache._index, cache._heads, int(max_len)
     B = table.shape[0]
-    ld = _table(table, B, dev)
-    _int32(lens, "lens", B, dev)
-    shape = (B, int(max_len), cache.heads, HEAD_DIM)
+    tp, ld, W = _table(table, B, dev)
+    lp = _int32(lens, "lens", B, dev)
     with _launch(dev, stream):
         if out is None:
-            out = tuple(torch.empty(shape, dtype=torch.bfloat16, device=dev) for _ in range(2))
+            out = torch.empty((2, B, max_len, H, HEAD_DIM), dtype=torch.bfloat16, device=cache._device).unbind(0)
+            row = H * HEAD_DIM
+            pitch = ((max_len * row, row),) * 2
         else:
+            pitch = []
             for t, n in zip(out, ("out k", "out v")):
-                _bf16_rows(t, n, dev)
-                if tuple(t.shape) != shape or (cache.heads > 1 and t.stride(2) != HEAD_DIM):
-                    raise ValueError(f"{n} must be {list(shape)} with contiguous heads, got {tuple(t.shape)}, "
-                                     f"strides {t.stride()}")
+                shape, st = _bf16_rows(t, n, dev)
+                if tuple(shape) != (B, max_len, H, HEAD_DIM) or (H > 1 and st[2] != HEAD_DIM):
+                    raise ValueError(f"{n} must be {[B, max_len, H, HEAD_DIM]} with contiguous heads, got "
+                                     f"{tuple(shape)}, strides {t.stride()}")
+                pitch.append((st[0], st[1] if max_len > 1 else H * HEAD_DIM))
         ko, vo = out
-        pitch = [(t.stride(0), t.stride(1) if max_len > 1 else cache.heads * HEAD_DIM) for t in out]
-        a = nat.DemonKvReadArgs(cache._c, nat.ptr(ko), *pitch[0], nat.ptr(vo), *pitch[1], nat.ptr(table), ld,
-                                nat.ptr(lens), B, int(max_len), table.shape[1], 0)
-        nat.check(nat.load().demon_kv_read(ctypes.byref(a), nat.stream_ptr(stream)))
+        args = _READ.pack(*cache._c, ko.data_ptr(), *pitch[0], vo.data_ptr(), *pitch[1], tp, ld, lp, B, max_len, W, 0)
+        nat.check(nat.load().demon_kv_read(args, nat.raw_stream(dev)))
     return ko, vo
 
 
@@ -178,23 +196,25 @@ def attention(q: torch.Tensor, cache: KVCache, table: torch.Tensor, lens: torch.
     hides the keys after that position, ``window`` those farther than ``window`` from it.  Rows
     that see no key, and rows i >= ``q_lens[b]``, are zero.  ``scale`` defaults to 1 / sqrt(128).
     """
-    dev = cache.k.device
-    _bf16_rows(q, "q", dev)
-    B, Sq, Hq, _ = q.shape
-    ld = _table(table, B, dev)
-    _int32(lens, "lens", B, dev)
-    if q_lens is not None:
-        _int32(q_lens, "q_lens", B, dev)
+    dev = cache._index
+    shape, qs = _bf16_rows(q, "q", dev)
+    if 0 in qs and any(n > 1 and st == 0 for n, st in zip(shape, qs)):
+        q = q.contiguous()  # broadcast queries
+        qs = _bf16_rows(q, "q", dev)[1]
+    B, Sq, Hq, _ = shape
+    tp, ld, W = _table(table, B, dev)
+    lp = _int32(lens, "lens", B, dev)
+    qp = 0 if q_lens is None else _int32(q_lens, "q_lens", B, dev)
     with _launch(dev, stream):
         if out is None:
-            out = torch.empty(B, Sq, Hq, HEAD_DIM, dtype=torch.bfloat16, device=dev)
+            out = torch.empty(shape, dtype=torch.bfloat16, device=cache._device)
+            os = (Sq * Hq * HEAD_DIM, Hq * HEAD_DIM, HEAD_DIM)
         else:
-            _bf16_rows(out, "out", dev)
-            if out.shape != q.shape:
-                raise ValueError(f"out must be {tuple(q.shape)}, got {tuple(out.shape)}")
-        a = nat.DemonKvAttnArgs(cache._c, nat.ptr(q), *_strides(q), nat.ptr(out), *_strides(out), nat.ptr(table), ld,
-                                nat.ptr(lens), nat.ptr(q_lens), B, Sq, Hq, table.shape[1], 1 if causal else 0,
-                                -1 if window is None else int(window),
-                                float(HEAD_DIM ** -0.5 if scale is None else scale), 0)
-        nat.check(nat.load().demon_kv_attention(ctypes.byref(a), nat.stream_ptr(stream)))
+            oshape, os = _bf16_rows(out, "out", dev)
+            if oshape != shape or any(n > 1 and st == 0 for n, st in zip(shape, os)):
+                raise ValueError(f"out must be {tuple(shape)} without overlap, got {tuple(oshape)}, strides {out.stride()}")
+        args = _ATTN.pack(*cache._c, q.data_ptr(), *qs, out.data_ptr(), *os, tp, ld, lp, qp, B, Sq, Hq, W,
+                          1 if causal else 0, -1 if window is None else min(int(window), 1 << 30),
+                          _DEFAULT_SCALE if scale is None else float(scale), 0)
+        nat.check(nat.load().demon_kv_attention(args, nat.raw_stream(dev)))
     return out

@@ -174,4 +174,4 @@ def test_struct_layouts_match_and_entry_points_refuse_without_a_gpu():
         pytest.skip("a GPU is present")
     for fn, args in ((lib.demon_kv_append, nat.DemonKvAppendArgs()), (lib.demon_kv_read, nat.DemonKvReadArgs()),
                      (lib.demon_kv_attention, nat.DemonKvAttnArgs())):
-        assert fn(ctypes.byref(args), None) != nat.DEMON_OK and nat.last_error()
+        assert fn(bytes(args), None) != nat.DEMON_OK and nat.last_error()

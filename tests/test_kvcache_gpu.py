@@ -321,6 +321,8 @@ def test_strided_queries_and_outputs(cuda):
         rest = buf.clone()
         rest[:, 1:Sq + 1, 0, 1:5] = 9.0
         assert bool((rest == 9).all())
+        same = kvcache.attention(q[:1].expand(2, -1, -1, -1), cache, table, i32(lens, cuda), causal=True)   # broadcast
+        assert torch.equal(same, kvcache.attention(q[:1].repeat(2, 1, 1, 1), cache, table, i32(lens, cuda), causal=True))
         qt = q.contiguous().transpose(1, 2).contiguous().transpose(1, 2)          # head-major
         assert torch.equal(kvcache.attention(qt, cache, table, i32(lens, cuda), causal=True), want)
 
@@ -520,6 +522,8 @@ def test_refusals(cuda):
         kvcache.attention(q, cache, table, lens, out=q[:, :, :2])
     with pytest.raises(ValueError, match="cuda"):
         kvcache.attention(q.cpu(), cache, table, lens)
+    with pytest.raises(ValueError, match="overlap"):
+        kvcache.attention(q, cache, table, lens, out=q[:1].clone().expand(2, -1, -1, -1))
     odd = torch.zeros(2, 1, 4, 132, dtype=torch.bfloat16, device=cuda)[..., :128]
     with pytest.raises(nat.DemonError, match="multiples of 8"):
         kvcache.attention(odd, cache, table, lens)
