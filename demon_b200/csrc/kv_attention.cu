@@ -3,27 +3,30 @@
 // (j < length, causal and band limits; a query that sees no key gives zeros).
 //
 // Small kernel (few query rows per kv head: single tokens, short chunks).  Bound by reading the
-// codes, 256 bytes per key and kv head.  All G = Hq / Hk query heads of a kv head and up to 16
-// query tokens share one pass over its keys: a row is (token, query head), row r = i * G + g.
-// A CTA takes 16 * RT rows and a range of keys in tiles of 64; one warp copies the tiles of K
-// and V codes, as they lie in the pages, into a ring in shared memory (bulk copies of a page's
-// 2 to 8 KB, mbarriers); four warps per 16 rows each take 16 keys of a tile.  The keys of a row
-// tile are split over a thread-block cluster, which joins its partial results through
-// distributed shared memory: one launch, no workspace.
+// codes, 256 bytes per key and kv head.  All G = Hq / Hk query heads of a kv head share one pass
+// over its keys: a row is (token, query head), r = i * G + g.  A CTA takes 8 NR * RT rows and a
+// range of keys in tiles of 64; one warp copies the tiles of K and V codes, as they lie in the
+// pages, into a ring in shared memory (bulk copies of a page's 2 to 8 KB, mbarriers); four warps
+// per row group each take 32 keys of every second tile.  The keys of a row tile are split over a
+// thread-block cluster, which joins its partial results through distributed shared memory: one
+// launch, no workspace.
 //
-// A warp's step on 16 keys, all in registers (mma.sync m16n8k16, fp32 accumulators):
-//   S = Q K^T: E4M3 codes become f16 exactly; Q is f16 too, each row times a power of two that
+// A warp's step on 32 keys, all in registers (mma.sync m16n8k16, fp32 accumulators), with the keys
+// and V's channels on the 16-wide side of the MMAs and the query rows on the 8-wide one, so that a
+// few rows waste little:
+//   S^T = K Q^T: E4M3 codes become f16 exactly; Q is f16 too, each row times a power of two that
 //     brings its largest value to [2^13, 2^14) (exact down to 2^-28 of that value).  The page's
 //     K scale, the row's power and the softmax scale are one fp32 factor of the score.
 //   softmax: running maximum m and sum l per row; p = 2^(t - m + 14), so that f16 keeps p's full
-//     precision down to 2^-28 of the row's largest; l sums the unrounded p.
-//   O += P V: the codes of V go in unscaled; O is held in units of 2^e_ref, the largest V scale
-//     met so far.  A page with a smaller scale 2^e has P multiplied by 2^(e - e_ref), exactly;
-//     if that is below 2^-8, its product goes through accumulators of its own, so that P's
-//     precision never depends on the scales.
-// The f16 conversions take one instruction per two codes, and only a byte permute stands
-// between V's rows and the operand layout (the keys and channels of a step may be taken in any
-// order as long as both operands agree).
+//     precision down to 2^-28 of the row's largest; l sums the unrounded p.  P^T's 8 x 8 blocks
+//     are transposed across the warp (movmatrix) from accumulator to operand layout.
+//   O^T += V^T P^T: the codes of V go in unscaled; O is held in units of 2^e_ref, the largest V
+//     scale met so far.  Keys of a page with a smaller scale 2^e have P multiplied by
+//     2^(e - e_ref), exactly; if that is below 2^-8, their product goes through accumulators of
+//     its own, so that P's precision never depends on the scales.
+// The f16 conversions take one instruction per two codes (and one more for the upper half of a
+// word), and only a byte permute stands between V's rows and the operand layout: the keys and
+// channels of a step may be taken in any order as long as both operands agree.
 #include <algorithm>
 
 #include "demon_host.h"
@@ -36,28 +39,34 @@ namespace kv {
 namespace small {
 
 constexpr int kTile = 64;                  // keys per stage
-constexpr int kWarpKeys = 16;              // keys per warp and stage
+constexpr int kWarpKeys = 32;              // keys per warp and step
 constexpr int kHalf = kTile * kHeadDim;    // one stage's K (or V) codes, 8 KB
-constexpr int kStages = 6;
-constexpr int kKeyWarps = kTile / kWarpKeys;
+constexpr int kKeyWarps = 4;               // per row group: two per tile, on alternating tiles
 constexpr float kPBias = 14.0f;            // p is scaled by 2^14 (see above)
 constexpr int kFoldMin = -8;               // smallest V scale, relative to e_ref, folded into P
 
-constexpr int offScale = kStages * 2 * kHalf;           // [stage][piece][K, V] fp32
-constexpr int offBar = offScale + kStages * 4 * 2 * 4;  // full[stage], empty[stage]
-constexpr int offMisc = offBar + 2 * kStages * 8;       // abort flag
-constexpr int kSmem = offMisc + 16;
-
-// After the key loop the ring holds the partial results: per warp O [16][128] fp32, then the
-// CTA's sum [16 RT][128], and the rows' statistics.
-constexpr int kWarpO = 16 * kHeadDim * 4;
-template <int RT>
-struct Join {
+// NR: 8-row MMA tiles per warp; RT: row groups (of four warps) per CTA.
+template <int NR, int RT>
+struct Cfg {
+  static constexpr int kRows = 8 * NR;                    // rows of a group
+  static constexpr int kThreads = (kKeyWarps * RT + 1) * 32;
+  // ring: what keeps the memory busy with the CTAs that registers allow on an SM (NR 1: three)
+  static constexpr int kStages = NR == 1 ? 4 : 6;
+  // The two warps of a tile see every second one: with an even number of stages they meet every
+  // phase of the stages they use.  (With three, a warp one phase ahead took the phase before as its own.)
+  static_assert(kStages % 2 == 0, "a stage must always belong to the same warps");
+  static constexpr int kMinCtas = NR == 1 ? 3 : 2 / RT;
+  static constexpr int offScale = kStages * 2 * kHalf;    // [stage][piece][K, V] fp32
+  static constexpr int offBar = offScale + kStages * 4 * 2 * 4;  // full[stage], empty[stage]
+  static constexpr int offMisc = offBar + kStages * 2 * 8;       // abort flag
+  static constexpr int kSmem = offMisc + 16;
+  // After the key loop the ring holds the partial results: per warp O [rows][128] fp32, then the
+  // CTA's sum, and the rows' statistics.
+  static constexpr int kWarpO = kRows * kHeadDim * 4;
   static constexpr int offSum = kKeyWarps * RT * kWarpO;
-  static constexpr int offStat = offSum + RT * kWarpO;               // per warp and row: m, l, e
-  static constexpr int offRow = offStat + kKeyWarps * RT * 16 * 12;  // CTA, per row: M, L, E
-  static constexpr int kEnd = offRow + RT * 16 * 12;
-  static_assert(kEnd <= offScale, "partial results must fit into the ring");
+  static constexpr int offStat = offSum + RT * kWarpO;                  // per warp and row: m, l, e
+  static constexpr int offRow = offStat + kKeyWarps * RT * kRows * 12;  // CTA, per row: M, L, E
+  static_assert(offRow + RT * kRows * 12 <= offScale, "partial results must fit into the ring");
 };
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -65,13 +74,21 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float quad_max(float x) {
-  x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-  return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
-__device__ __forceinline__ float quad_sum(float x) {
-  x += __shfl_xor_sync(0xffffffffu, x, 1);
-  return x + __shfl_xor_sync(0xffffffffu, x, 2);
+// over the eight lanes that share lane % 4
+__device__ __forceinline__ float oct_max(float x) {
+  x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+  x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+  return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+}
+__device__ __forceinline__ float oct_sum(float x) {
+  x += __shfl_xor_sync(0xffffffffu, x, 4);
+  x += __shfl_xor_sync(0xffffffffu, x, 8);
+  return x + __shfl_xor_sync(0xffffffffu, x, 16);
 }
 __device__ __forceinline__ uint32_t map_rank(uint32_t a, uint32_t rank) {
   uint32_t r;
@@ -96,24 +113,30 @@ __device__ __forceinline__ void bulk_load_s(uint32_t dst, const void* src, uint3
       : "memory");
 }
 
+// Cluster barrier in the form that counts threads (the .aligned one needs every warp whole at it).
+__device__ __forceinline__ void cluster_join() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+
 // Factor that brings a partial result with maximum m (and V unit 2^e) to maximum M (unit 2^E).
 __device__ __forceinline__ float join_factor(float m, float M) {
   return m == -INFINITY ? 0.0f : ex2(m - M);
 }
 __device__ __forceinline__ float unit_factor(int e, int E) { return e - E < -126 ? 0.0f : exp2i(imin(e - E, 0)); }
 
-template <int RT>
-__global__ void __launch_bounds__(kKeyWarps* RT * 32 + 32, 2 / RT) attention_small_kernel(const AttnParams p) {
+template <int NR, int RT>
+__global__ void __launch_bounds__(Cfg<NR, RT>::kThreads, Cfg<NR, RT>::kMinCtas) attention_small_kernel(const AttnParams p) {
+  using C = Cfg<NR, RT>;
+  constexpr int kStages = C::kStages;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sbase = smem_u32(smem);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + offBar);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::offBar);
   uint64_t* empty = full + kStages;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + offMisc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::offMisc);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint64_t t0 = globaltimer();
-  uint32_t rank, csize;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
-  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(csize));
+  const uint32_t csize = (uint32_t)p.cluster, rank = blockIdx.x % csize;  // clusters lie along x
 
   // unit: row tile fastest, then kv head, then sequence
   const uint32_t unit = blockIdx.x / csize;
@@ -125,8 +148,8 @@ __global__ void __launch_bounds__(kKeyWarps* RT * 32 + 32, 2 / RT) attention_sma
   const int len = clamp_len(p.lens[b], p.W * p.c.P, &bad);
   const int nq = p.q_lens ? clamp_len(p.q_lens[b], p.Sq, &bad) : p.Sq;
   if (bad && threadIdx.x == 0 && rank == 0 && rt == 0 && hk == 0) report(p.status, DEMON_DEV_BAD_ARG, 63);
-  const int64_t n_rows = (int64_t)p.Sq * p.G, row0 = (int64_t)rt * 16 * RT;
-  const int i0 = (int)(row0 / p.G), i1 = imin((int)((row0 + 16 * RT - 1) / p.G), nq - 1);
+  const int n_rows = p.Sq * p.G, row0 = rt * C::kRows * RT;  // below 2^31 (checked on the host)
+  const int i0 = row0 / p.G, i1 = imin((row0 + C::kRows * RT - 1) / p.G, nq - 1);
   Keys ks;
   ks.lo = ks.hi = ks.lo_all = ks.hi_all = 0;
   if (i0 <= i1) ks = visible(i0, i1, len, nq, p.causal != 0, p.window);
@@ -138,7 +161,7 @@ __global__ void __launch_bounds__(kKeyWarps* RT * 32 + 32, 2 / RT) attention_sma
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], kKeyWarps * RT);
+      mbar_init(&empty[s], 2 * RT);
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -148,13 +171,19 @@ __global__ void __launch_bounds__(kKeyWarps* RT * 32 + 32, 2 / RT) attention_sma
   const int step = imin(p.c.P, kTile);  // keys per piece: what of a page lies in a tile
   const int pieces = kTile / step;
 
-  // per-warp partial results (warps of the key loop)
-  float o[16][4];
-  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+  // per-warp partial results: accumulator j of row tile r holds channels 16 g + 2 j (+ 1) of rows
+  // 2 c, 2 c + 1 of the tile
+  float o[NR][8][4];
+  float m[NR][2], l[NR][2];
   int e_ref = kMinExp;
   const int g = lane >> 2, c = lane & 3;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+  for (int r = 0; r < NR; ++r) {
+    m[r][0] = m[r][1] = -INFINITY;
+    l[r][0] = l[r][1] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[r][j][0] = o[r][j][1] = o[r][j][2] = o[r][j][3] = 0.0f;
+  }
 
   if (warp == kKeyWarps * RT) {
     // ------------------------------------------------------------------------ copies
@@ -188,7 +217,7 @@ __global__ void __launch_bounds__(kKeyWarps* RT * 32 + 32, 2 / RT) attention_sma
         const bool mine = lane >= t && lane < t + pieces;
         const uint32_t here = __ballot_sync(0xffffffffu, mine && pid >= 0);
         if (mine) {
-          const uint32_t sc = sbase + offScale + (s * 4 + lane - t) * 8;
+          const uint32_t sc = sbase + C::offScale + (s * 4 + lane - t) * 8;
           st_shared_f32(sc, sk);
           st_shared_f32(sc + 4, sv);
         }
@@ -213,26 +242,25 @@ __global__ void __launch_bounds__(kKeyWarps* RT * 32 + 32, 2 / RT) attention_sma
     }
   } else {
     // ------------------------------------------------------------------------ key loop
-    const int kw = warp % kKeyWarps, wt = warp / kKeyWarps;  // 16-key part of a tile, row tile
-    // this lane's two rows of Q: rows g and g + 8 of the warp's sixteen
-    uint32_t qf[8][4];
-    float fac[2];
-    int pos[2];
+    const int kw = warp % kKeyWarps, wt = warp / kKeyWarps;  // part of the keys, row group
+    // Q^T: row g of each row tile, k-step s, lane c: channels 16 c + 64 (s / 4) + 4 (s % 4) + 0..3, as
+    // K's codes lie
+    uint32_t qf[NR][8][2];
+    float fac[NR][2];  // score factors and positions of rows 2 c, 2 c + 1
+    int pos[NR][2];
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int64_t r = row0 + wt * 16 + g + 8 * half;
-      const int i = (int)(r / p.G), gq = (int)(r - (int64_t)i * p.G);
-      const bool valid = r < n_rows && i < nq;
-      pos[half] = len - nq + i;
+    for (int r = 0; r < NR; ++r) {
+      const int grow = row0 + wt * C::kRows + 8 * r + g;
+      const int i = grow / p.G, gq = grow - i * p.G;
       uint4 w[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) w[j] = make_uint4(0, 0, 0, 0);
-      if (valid) {
+      if (grow < n_rows && i < nq) {
         const __nv_bfloat16* q = p.q + b * p.q_seq + (int64_t)i * p.q_row + (int64_t)(hk * p.G + gq) * p.q_head;
 #pragma unroll
         for (int j = 0; j < 4; ++j) w[j] = __ldg(reinterpret_cast<const uint4*>(q + 16 * c + 64 * (j >> 1) + 8 * (j & 1)));
       }
-      uint32_t mx = 0;
+      uint32_t mx = 0;  // infinities and NaN do not count, and pass through
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const uint32_t x[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
@@ -247,178 +275,227 @@ __global__ void __launch_bounds__(kKeyWarps* RT * 32 + 32, 2 / RT) attention_sma
       mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
       const int k = imax((int)(mx >> 7) - 127 - 13, -126);  // |q| 2^-k < 2^14
       const float2 mul = make_float2(exp2i(-k), exp2i(-k));
-      fac[half] = exp2i(k);
-      // k-step s, lane c: channels 16 c + 64 (s / 4) + 4 (s % 4) + 0..3, as K's codes lie
 #pragma unroll
       for (int s = 0; s < 8; ++s) {
         const uint4& ww = w[2 * (s >> 2) + ((s & 3) >> 1)];
-        const uint32_t x0 = (s & 1) ? ww.z : ww.x, x1 = (s & 1) ? ww.w : ww.y;
-        const float2 f0 = mul_f2(bf2_f2(x0), mul), f1 = mul_f2(bf2_f2(x1), mul);
-        qf[s][half] = pack_f16x2(f0.x, f0.y);
-        qf[s][2 + half] = pack_f16x2(f1.x, f1.y);
+        const float2 f0 = mul_f2(bf2_f2((s & 1) ? ww.z : ww.x), mul), f1 = mul_f2(bf2_f2((s & 1) ? ww.w : ww.y), mul);
+        qf[r][s][0] = pack_f16x2(f0.x, f0.y);
+        qf[r][s][1] = pack_f16x2(f1.x, f1.y);
+      }
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        fac[r][x] = exp2i(__shfl_sync(0xffffffffu, k, 4 * (2 * c + x))) * p.scale_log2;
+        pos[r][x] = len - nq + __shfl_sync(0xffffffffu, i, 4 * (2 * c + x));
       }
     }
-    // keys of a step: S column n of 8-column tile nt is key 4 (n / 2) + 2 nt + n % 2, so that the
-    // P operand's columns of lane c are keys 4 c .. 4 c + 3
+    // keys of a 16-key block: A row x is key 4 (x % 8 / 2) + 2 (x / 8) + x % 2, so that the P operand's
+    // columns of lane c are keys 4 c .. 4 c + 3
     const int kkey = 4 * (g >> 1) + (g & 1);
-    const uint32_t k_off = (uint32_t)(kw * kWarpKeys + kkey) * kHeadDim + 16 * c;
-    const uint32_t v_off = (uint32_t)kHalf + (uint32_t)(kw * kWarpKeys + 4 * c) * kHeadDim + 16 * g;
-    const int piece = kw * kWarpKeys / step;
+    const uint32_t k_off = (uint32_t)((kw & 1) * kWarpKeys + kkey) * kHeadDim + 16 * c;
+    const uint32_t v_off = (uint32_t)kHalf + (uint32_t)((kw & 1) * kWarpKeys + 4 * c) * kHeadDim + 16 * g;
 
     bool ok = true;
-    for (int t = 0; t < n_tiles; ++t) {
+    for (int t = kw >> 1; t < n_tiles; t += 2) {
       const int s = t % kStages;
       ok = mbar_wait(&full[s], (uint32_t)(t / kStages) & 1u, abort_flag, t0, p.status, 67);
-      ok = __all_sync(0xffffffffu, ok && *abort_flag == 0);
+      ok = __all_sync(0xffffffffu, ok);
+      __syncwarp();  // together for the MMAs
       if (!ok) break;
-      const int j0 = (first + t) * kTile + kw * kWarpKeys;
-      const uint32_t sc = sbase + offScale + (s * 4 + piece) * 8;
-      const float sk = ld_shared_f32(sc), sv = ld_shared_f32(sc + 4);
-      if (!(sk < 0.0f) && j0 < ks.hi && j0 + kWarpKeys > ks.lo) {
+      const int j0 = (first + t) * kTile + (kw & 1) * kWarpKeys;
+      if (j0 < ks.hi && j0 + kWarpKeys > ks.lo) {
         const uint32_t st = sbase + s * 2 * kHalf;
-        float sa[2][4];
+        float sk[2];
+        int ev[2];
+        bool there[2];  // keys 16 z .. of the step: a page, and some row that sees them
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
-          sa[nt][0] = sa[nt][1] = sa[nt][2] = sa[nt][3] = 0.0f;
+        for (int z = 0; z < 2; ++z) {
+          const uint32_t sc = sbase + C::offScale + (s * 4 + ((kw & 1) * kWarpKeys + 16 * z) / step) * 8;
+          sk[z] = ld_shared_f32(sc);
+          ev[z] = scale_exp(ld_shared_f32(sc + 4));
+          there[z] = !(sk[z] < 0.0f) && j0 + 16 * z < ks.hi && j0 + 16 * z + 16 > ks.lo;
+        }
+        float sa[2][NR][4];
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+#pragma unroll
+          for (int r = 0; r < NR; ++r) sa[z][r][0] = sa[z][r][1] = sa[z][r][2] = sa[z][r][3] = 0.0f;
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            const uint4 w = ld_shared_v4(st + k_off + nt * 2 * kHeadDim + 64 * half);
-            uint32_t x0, x1;
-            e4m3x4_f16(w.x, x0, x1);
-            mma_f16(sa[nt], qf[4 * half + 0], x0, x1);
-            e4m3x4_f16(w.y, x0, x1);
-            mma_f16(sa[nt], qf[4 * half + 1], x0, x1);
-            e4m3x4_f16(w.z, x0, x1);
-            mma_f16(sa[nt], qf[4 * half + 2], x0, x1);
-            e4m3x4_f16(w.w, x0, x1);
-            mma_f16(sa[nt], qf[4 * half + 3], x0, x1);
+            const uint4 x = ld_shared_v4(st + k_off + 16 * z * kHeadDim + 64 * half);
+            const uint4 y = ld_shared_v4(st + k_off + (16 * z + 2) * kHeadDim + 64 * half);
+            const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) {
+              uint32_t a[4];  // keys (x, y), channels 0, 1 and 2, 3 of the word
+              e4m3x4_f16(xs[q4], a[0], a[2]);
+              e4m3x4_f16(ys[q4], a[1], a[3]);
+#pragma unroll
+              for (int r = 0; r < NR; ++r) mma_f16(sa[z][r], a, qf[r][4 * half + q4][0], qf[r][4 * half + q4][1]);
+            }
           }
         }
-        const float f0 = fac[0] * sk * p.scale_log2, f1 = fac[1] * sk * p.scale_log2;
+        // scores; accumulator i of block z is key kkey + 2 (i / 2) + 16 z of row 2 c + i % 2
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
-          sa[nt][0] *= f0;
-          sa[nt][1] *= f0;
-          sa[nt][2] *= f1;
-          sa[nt][3] *= f1;
-        }
-        uint4 w[4];  // V: channels 16 g .. 16 g + 15 of keys 4 c .. 4 c + 3
+        for (int z = 0; z < 2; ++z)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = ld_shared_v4(st + v_off + i * kHeadDim);
-        const bool whole = j0 >= ks.lo_all && j0 + kWarpKeys <= ks.hi_all;
-        uint32_t see = 0xFFu;  // bit 4 half + i: row `half` sees key 4 c + i
+          for (int r = 0; r < NR; ++r) {
+            const float f0 = fac[r][0] * sk[z], f1 = fac[r][1] * sk[z];
+            sa[z][r][0] *= f0;
+            sa[z][r][1] *= f1;
+            sa[z][r][2] *= f0;
+            sa[z][r][3] *= f1;
+          }
+        const bool whole = there[0] && there[1] && j0 >= ks.lo_all && j0 + kWarpKeys <= ks.hi_all;
         if (!whole) {
-          see = 0;
 #pragma unroll
-          for (int half = 0; half < 2; ++half)
+          for (int z = 0; z < 2; ++z)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int j = j0 + 4 * c + i;
-              const bool v = j < len && (!p.causal || j <= pos[half]) &&
-                             (p.window < 0 || (j <= pos[half] + p.window && j >= pos[half] - p.window));
-              see |= (uint32_t)v << (4 * half + i);
-            }
-#pragma unroll
-          for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (!((see >> (4 * (i >> 1) + 2 * nt + (i & 1))) & 1u)) sa[nt][i] = -INFINITY;
-          // a NaN of V in a key that some row does not see: it must not reach that row as 0 * NaN
-          uint32_t nn = 0;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) nn |= nan_bytes(w[i].x) | nan_bytes(w[i].y) | nan_bytes(w[i].z) | nan_bytes(w[i].w);
-          if (__any_sync(0xffffffffu, nn != 0)) {
-            uint32_t a[4];  // who sees what, as a 0 / 1 operand
-            const uint32_t one = 0x3C00u;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {  // a[0]: row g, keys 4c, 4c+1; a[1]: row g+8; a[2], a[3]: keys 4c+2, 4c+3
-              const uint32_t bits = see >> (4 * (r & 1) + 2 * (r >> 1));
-              a[r] = ((bits & 1u) ? one : 0u) | ((bits & 2u) ? one << 16 : 0u);
-            }
-            uint32_t x[4][4] = {{w[0].x, w[0].y, w[0].z, w[0].w}, {w[1].x, w[1].y, w[1].z, w[1].w},
-                                {w[2].x, w[2].y, w[2].z, w[2].w}, {w[3].x, w[3].y, w[3].z, w[3].w}};
-#pragma unroll
-            for (int nt = 0; nt < 16; ++nt) {
-              const int sh = 8 * (nt & 3);
-              const uint32_t n0 = (nan_bytes(x[0][nt >> 2]) >> sh) & 0x80u, n1 = (nan_bytes(x[1][nt >> 2]) >> sh) & 0x80u;
-              const uint32_t n2 = (nan_bytes(x[2][nt >> 2]) >> sh) & 0x80u, n3 = (nan_bytes(x[3][nt >> 2]) >> sh) & 0x80u;
-              float cnt[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-              mma_f16(cnt, a, (n0 ? one : 0u) | (n1 ? one << 16 : 0u), (n2 ? one : 0u) | (n3 ? one << 16 : 0u));
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (cnt[i] > 0.0f) o[nt][i] = __int_as_float(0x7FFFFFFF);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {  // and out of the product
-              w[i].x &= ~((nan_bytes(w[i].x) >> 7) * 255u);
-              w[i].y &= ~((nan_bytes(w[i].y) >> 7) * 255u);
-              w[i].z &= ~((nan_bytes(w[i].z) >> 7) * 255u);
-              w[i].w &= ~((nan_bytes(w[i].w) >> 7) * 255u);
-            }
-          }
-        }
-        // running maximum
-        const float x0 = quad_max(fmaxf(fmaxf(sa[0][0], sa[0][1]), fmaxf(sa[1][0], sa[1][1])));
-        const float x1 = quad_max(fmaxf(fmaxf(sa[0][2], sa[0][3]), fmaxf(sa[1][2], sa[1][3])));
-        const int ev = scale_exp(sv);
-        const int eu = imax(e_ref, ev);  // O's unit from here on
-        if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1) || eu != e_ref) {
-          const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
-          const float a0 = n0 == -INFINITY ? 1.0f : ex2(m0 - n0), a1 = n1 == -INFINITY ? 1.0f : ex2(m1 - n1);
-          l0 *= a0;
-          l1 *= a1;
-          const float uf = unit_factor(e_ref, eu);
-          const float b0 = a0 * uf, b1 = a1 * uf;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            o[i][0] *= b0;
-            o[i][1] *= b0;
-            o[i][2] *= b1;
-            o[i][3] *= b1;
-          }
-          m0 = n0;
-          m1 = n1;
-          e_ref = eu;
-        }
-        const float d0 = kPBias - (m0 == -INFINITY ? 0.0f : m0), d1 = kPBias - (m1 == -INFINITY ? 0.0f : m1);
-#pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
-          sa[nt][0] = ex2(sa[nt][0] + d0);
-          sa[nt][1] = ex2(sa[nt][1] + d0);
-          sa[nt][2] = ex2(sa[nt][2] + d1);
-          sa[nt][3] = ex2(sa[nt][3] + d1);
-          l0 += sa[nt][0] + sa[nt][1];
-          l1 += sa[nt][2] + sa[nt][3];
-        }
-        const int de = ev - eu;  // <= 0
-        const bool apart = de < kFoldMin;
-        const float fold = apart ? 1.0f : exp2i(de);
-        const uint32_t pa[4] = {pack_f16x2(sa[0][0] * fold, sa[0][1] * fold), pack_f16x2(sa[0][2] * fold, sa[0][3] * fold),
-                                pack_f16x2(sa[1][0] * fold, sa[1][1] * fold), pack_f16x2(sa[1][2] * fold, sa[1][3] * fold)};
-        const uint32_t x[4][4] = {{w[0].x, w[0].y, w[0].z, w[0].w}, {w[1].x, w[1].y, w[1].z, w[1].w},
-                                  {w[2].x, w[2].y, w[2].z, w[2].w}, {w[3].x, w[3].y, w[3].z, w[3].w}};
-        const float back = unit_factor(ev, eu);
-#pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) {
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            // bytes (key 4c, key 4c+1) of two channels, and of the other two keys
-            const uint32_t sel = hf ? 0x7362u : 0x5140u;
-            uint32_t b00, b01, b10, b11;
-            e4m3x4_f16(__byte_perm(x[0][q4], x[1][q4], sel), b00, b01);
-            e4m3x4_f16(__byte_perm(x[2][q4], x[3][q4], sel), b10, b11);
-            const int nt = 4 * q4 + 2 * hf;
-            if (!apart) {
-              mma_f16(o[nt], pa, b00, b10);
-              mma_f16(o[nt + 1], pa, b01, b11);
-            } else {
-              float y0[4] = {0.0f, 0.0f, 0.0f, 0.0f}, y1[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-              mma_f16(y0, pa, b00, b10);
-              mma_f16(y1, pa, b01, b11);
+            for (int r = 0; r < NR; ++r)
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                o[nt][i] = fmaf(y0[i], back, o[nt][i]);
-                o[nt + 1][i] = fmaf(y1[i], back, o[nt + 1][i]);
+                const int j = j0 + 16 * z + kkey + 2 * (i >> 1), at = pos[r][i & 1];
+                const bool sees = there[z] && j < len && (!p.causal || j <= at) &&
+                                  (p.window < 0 || (j <= at + p.window && j >= at - p.window));
+                if (!sees) sa[z][r][i] = -INFINITY;
+              }
+        }
+        // running maximum and unit
+        const int eu = imax(e_ref, imax(there[0] ? ev[0] : kMinExp, there[1] ? ev[1] : kMinExp));
+        float mx[NR][2];
+        bool up = eu != e_ref;
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            mx[r][x] = oct_max(fmaxf(fmaxf(sa[0][r][x], sa[0][r][2 + x]), fmaxf(sa[1][r][x], sa[1][r][2 + x])));
+            up = up || mx[r][x] > m[r][x];
+          }
+        if (__any_sync(0xffffffffu, up)) {
+          const float uf = unit_factor(e_ref, eu);
+#pragma unroll
+          for (int r = 0; r < NR; ++r) {
+            float f[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const float n = fmaxf(m[r][x], mx[r][x]);
+              const float a = n == -INFINITY ? 1.0f : ex2(m[r][x] - n);
+              l[r][x] *= a;
+              m[r][x] = n;
+              f[x] = a * uf;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              o[r][j][0] *= f[0];
+              o[r][j][1] *= f[1];
+              o[r][j][2] *= f[0];
+              o[r][j][3] *= f[1];
+            }
+          }
+          e_ref = eu;
+        }
+        uint32_t pb[2][NR][2];  // P^T operands
+        bool apart = false;
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          const int de = there[z] ? ev[z] - eu : 0;  // <= 0
+          apart = apart || de < kFoldMin;
+          const float fold = de < kFoldMin ? 1.0f : exp2i(de);
+#pragma unroll
+          for (int r = 0; r < NR; ++r) {
+            float e[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float mm = m[r][i & 1];
+              e[i] = ex2(sa[z][r][i] + (kPBias - (mm == -INFINITY ? 0.0f : mm)));
+              l[r][i & 1] += e[i];
+              e[i] *= fold;
+            }
+            pb[z][r][0] = transpose_8x8(pack_f16x2(e[0], e[1]));
+            pb[z][r][1] = transpose_8x8(pack_f16x2(e[2], e[3]));
+          }
+        }
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          uint4 w[4];  // V: channels 16 g .. 16 g + 15 of keys 4 c .. 4 c + 3
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = ld_shared_v4(st + v_off + (16 * z + i) * kHeadDim);
+          if (!whole) {
+            if (!there[z]) continue;  // (uniform) nothing of the block counts, and it may not have been copied
+            // a NaN of V in a key that some row does not see: it must not reach that row as 0 * NaN
+            uint32_t nn = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) nn |= nan_bytes(w[i].x) | nan_bytes(w[i].y) | nan_bytes(w[i].z) | nan_bytes(w[i].w);
+            if (__any_sync(0xffffffffu, nn != 0)) {
+              uint32_t x[4][4] = {{w[0].x, w[0].y, w[0].z, w[0].w}, {w[1].x, w[1].y, w[1].z, w[1].w},
+                                  {w[2].x, w[2].y, w[2].z, w[2].w}, {w[3].x, w[3].y, w[3].z, w[3].w}};
+#pragma unroll
+              for (int r = 0; r < NR; ++r) {
+                uint32_t see = 0;  // bit i: row g of the tile sees key 4 c + i
+                const int at = len - nq + (row0 + wt * C::kRows + 8 * r + g) / p.G;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const int j = j0 + 16 * z + 4 * c + i;
+                  see |= (uint32_t)(j < len && (!p.causal || j <= at) &&
+                                    (p.window < 0 || (j <= at + p.window && j >= at - p.window)))
+                         << i;
+                }
+                const uint32_t one = 0x3C00u;
+                const uint32_t b0 = ((see & 1u) ? one : 0u) | ((see & 2u) ? one << 16 : 0u);
+                const uint32_t b1 = ((see & 4u) ? one : 0u) | ((see & 8u) ? one << 16 : 0u);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                  uint32_t a[4];
+#pragma unroll
+                  for (int q = 0; q < 4; ++q) {  // channel 2 j + q % 2, keys 2 (q / 2) and the next
+                    const int sh = 8 * ((2 * j + (q & 1)) & 3);
+                    const uint32_t n0 = (nan_bytes(x[2 * (q >> 1)][j >> 1]) >> sh) & 0x80u;
+                    const uint32_t n1 = (nan_bytes(x[2 * (q >> 1) + 1][j >> 1]) >> sh) & 0x80u;
+                    a[q] = (n0 ? one : 0u) | (n1 ? one << 16 : 0u);
+                  }
+                  float cnt[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                  mma_f16(cnt, a, b0, b1);
+#pragma unroll
+                  for (int i = 0; i < 4; ++i)
+                    if (cnt[i] > 0.0f) o[r][j][i] = __int_as_float(0x7FFFFFFF);
+                }
+              }
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {  // and out of the product
+                w[i].x &= ~((nan_bytes(w[i].x) >> 7) * 255u);
+                w[i].y &= ~((nan_bytes(w[i].y) >> 7) * 255u);
+                w[i].z &= ~((nan_bytes(w[i].z) >> 7) * 255u);
+                w[i].w &= ~((nan_bytes(w[i].w) >> 7) * 255u);
+              }
+            }
+          }
+          const uint32_t x[4][4] = {{w[0].x, w[0].y, w[0].z, w[0].w}, {w[1].x, w[1].y, w[1].z, w[1].w},
+                                    {w[2].x, w[2].y, w[2].z, w[2].w}, {w[3].x, w[3].y, w[3].z, w[3].w}};
+          // bytes (key 4c, key 4c+1) of channels 2 j, 2 j + 1, and of the other two keys
+          auto v_operand = [&](int j, uint32_t (&a)[4]) {
+            const uint32_t sel = (j & 1) ? 0x7362u : 0x5140u;
+            e4m3x4_f16(__byte_perm(x[0][j >> 1], x[1][j >> 1], sel), a[0], a[1]);
+            e4m3x4_f16(__byte_perm(x[2][j >> 1], x[3][j >> 1], sel), a[2], a[3]);
+          };
+          if (!__any_sync(0xffffffffu, apart && ev[z] - eu < kFoldMin)) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              uint32_t a[4];
+              v_operand(j, a);
+#pragma unroll
+              for (int r = 0; r < NR; ++r) mma_f16(o[r][j], a, pb[z][r][0], pb[z][r][1]);
+            }
+          } else {  // (a block of its own: as a choice inside the loop it was predicated, twice the instructions)
+            const float back = unit_factor(ev[z], eu);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              uint32_t a[4];
+              v_operand(j, a);
+#pragma unroll
+              for (int r = 0; r < NR; ++r) {
+                float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                mma_f16(y, a, pb[z][r][0], pb[z][r][1]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[r][j][i] = fmaf(y[i], back, o[r][j][i]);
               }
             }
           }
@@ -427,42 +504,43 @@ __global__ void __launch_bounds__(kKeyWarps* RT * 32 + 32, 2 / RT) attention_sma
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[s]);
     }
-    l0 = quad_sum(l0);
-    l1 = quad_sum(l1);
+#pragma unroll
+    for (int r = 0; r < NR; ++r)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) l[r][x] = oct_sum(l[r][x]);
   }
 
   // -------------------------------------------------------------------------- join
-  using J = Join<RT>;
   __syncthreads();  // every tile consumed: the ring is free (every copy was waited for)
   if (warp < kKeyWarps * RT) {
-    const uint32_t wo = sbase + warp * kWarpO, ws = sbase + J::offStat + warp * 16 * 12;
-    if (c == 0) {
-      st_shared_f32(ws + g * 12, m0);
-      st_shared_f32(ws + g * 12 + 4, l0);
-      st_shared_f32(ws + g * 12 + 8, __int_as_float(e_ref));
-      st_shared_f32(ws + (g + 8) * 12, m1);
-      st_shared_f32(ws + (g + 8) * 12 + 4, l1);
-      st_shared_f32(ws + (g + 8) * 12 + 8, __int_as_float(e_ref));
-    }
-    // O column n of 8-column tile nt is channel 16 n + nt
+    const uint32_t wo = sbase + warp * C::kWarpO, ws = sbase + C::offStat + warp * C::kRows * 12;
 #pragma unroll
-    for (int q4 = 0; q4 < 4; ++q4) {
-      st_shared_f32x4(wo + (g * kHeadDim + 32 * c + 4 * q4) * 4, o[4 * q4][0], o[4 * q4 + 1][0], o[4 * q4 + 2][0], o[4 * q4 + 3][0]);
-      st_shared_f32x4(wo + (g * kHeadDim + 32 * c + 16 + 4 * q4) * 4, o[4 * q4][1], o[4 * q4 + 1][1], o[4 * q4 + 2][1], o[4 * q4 + 3][1]);
-      st_shared_f32x4(wo + ((g + 8) * kHeadDim + 32 * c + 4 * q4) * 4, o[4 * q4][2], o[4 * q4 + 1][2], o[4 * q4 + 2][2], o[4 * q4 + 3][2]);
-      st_shared_f32x4(wo + ((g + 8) * kHeadDim + 32 * c + 16 + 4 * q4) * 4, o[4 * q4][3], o[4 * q4 + 1][3], o[4 * q4 + 2][3], o[4 * q4 + 3][3]);
-    }
+    for (int r = 0; r < NR; ++r)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int row = 8 * r + 2 * c + x;
+        if (g == 0) {
+          st_shared_f32(ws + row * 12, m[r][x]);
+          st_shared_f32(ws + row * 12 + 4, l[r][x]);
+          st_shared_f32(ws + row * 12 + 8, __int_as_float(e_ref));
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          st_shared_f32x4(wo + (row * kHeadDim + 16 * g + 4 * q) * 4, o[r][2 * q][x], o[r][2 * q][2 + x], o[r][2 * q + 1][x],
+                          o[r][2 * q + 1][2 + x]);
+      }
   }
   __syncthreads();
   // the CTA's four partial results of each row into one: a warp per row, four channels a lane
-  const int n_warps = kKeyWarps * RT + 1;
-  for (int r = warp; r < 16 * RT; r += n_warps) {
-    const int wt = r >> 4, rr = r & 15;
+  constexpr int n_warps = kKeyWarps * RT + 1;
+  const int rows_here = imin(C::kRows * RT, n_rows - row0);
+  for (int r = warp; r < rows_here; r += n_warps) {
+    const int wt = r / C::kRows, rr = r % C::kRows;
     float mm[kKeyWarps], M = -INFINITY, L = 0.0f;
     int ee[kKeyWarps], E = kMinExp;
 #pragma unroll
     for (int k = 0; k < kKeyWarps; ++k) {
-      const uint32_t ws = sbase + J::offStat + ((wt * kKeyWarps + k) * 16 + rr) * 12;
+      const uint32_t ws = sbase + C::offStat + ((wt * kKeyWarps + k) * C::kRows + rr) * 12;
       mm[k] = ld_shared_f32(ws);
       ee[k] = __float_as_int(ld_shared_f32(ws + 8));
       M = fmaxf(M, mm[k]);
@@ -471,49 +549,51 @@ __global__ void __launch_bounds__(kKeyWarps* RT * 32 + 32, 2 / RT) attention_sma
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
     for (int k = 0; k < kKeyWarps; ++k) {
-      const uint32_t ws = sbase + J::offStat + ((wt * kKeyWarps + k) * 16 + rr) * 12;
+      const uint32_t ws = sbase + C::offStat + ((wt * kKeyWarps + k) * C::kRows + rr) * 12;
       const float f = join_factor(mm[k], M);
       L = fmaf(ld_shared_f32(ws + 4), f, L);
       const float fo = f * unit_factor(ee[k], E);
-      const float4 v = ld_shared_f32x4(sbase + (wt * kKeyWarps + k) * kWarpO + (rr * kHeadDim + 4 * lane) * 4);
+      const float4 v = ld_shared_f32x4(sbase + (wt * kKeyWarps + k) * C::kWarpO + (rr * kHeadDim + 4 * lane) * 4);
       acc.x = fmaf(v.x, fo, acc.x);
       acc.y = fmaf(v.y, fo, acc.y);
       acc.z = fmaf(v.z, fo, acc.z);
       acc.w = fmaf(v.w, fo, acc.w);
     }
-    st_shared_f32x4(sbase + J::offSum + (r * kHeadDim + 4 * lane) * 4, acc.x, acc.y, acc.z, acc.w);
+    st_shared_f32x4(sbase + C::offSum + (r * kHeadDim + 4 * lane) * 4, acc.x, acc.y, acc.z, acc.w);
     if (lane == 0) {
-      const uint32_t wr = sbase + J::offRow + r * 12;
+      const uint32_t wr = sbase + C::offRow + r * 12;
       st_shared_f32(wr, M);
       st_shared_f32(wr + 4, L);
       st_shared_f32(wr + 8, __int_as_float(E));
     }
   }
-  cluster_sync();
+  if (csize > 1)
+    cluster_join();
+  else
+    __syncwarp();  // a row's result is read by the warp that wrote it
   // rows of the cluster's results shared out over its CTAs
-  for (int r = (int)rank * n_warps + warp; r < 16 * RT; r += (int)csize * n_warps) {
-    const int64_t grow = row0 + r;
-    if (grow >= n_rows) continue;
+  for (int r = (int)rank * n_warps + warp; r < rows_here; r += (int)csize * n_warps) {
+    const int grow = row0 + r;
     float M = -INFINITY, L = 0.0f;
     int E = kMinExp;
     for (uint32_t k = 0; k < csize; ++k) {
-      const uint32_t wr = map_rank(sbase + J::offRow + r * 12, k);
+      const uint32_t wr = map_rank(sbase + C::offRow + r * 12, k);
       M = fmaxf(M, ld_cluster_f32(wr));
       E = imax(E, __float_as_int(ld_cluster_f32(wr + 8)));
     }
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (uint32_t k = 0; k < csize; ++k) {
-      const uint32_t wr = map_rank(sbase + J::offRow + r * 12, k);
+      const uint32_t wr = map_rank(sbase + C::offRow + r * 12, k);
       const float f = join_factor(ld_cluster_f32(wr), M);
       L = fmaf(ld_cluster_f32(wr + 4), f, L);
       const float fo = f * unit_factor(__float_as_int(ld_cluster_f32(wr + 8)), E);
-      const float4 v = ld_cluster_f32x4(map_rank(sbase + J::offSum + (r * kHeadDim + 4 * lane) * 4, k));
+      const float4 v = ld_cluster_f32x4(map_rank(sbase + C::offSum + (r * kHeadDim + 4 * lane) * 4, k));
       acc.x = fmaf(v.x, fo, acc.x);
       acc.y = fmaf(v.y, fo, acc.y);
       acc.z = fmaf(v.z, fo, acc.z);
       acc.w = fmaf(v.w, fo, acc.w);
     }
-    const int i = (int)(grow / p.G), gq = (int)(grow - (int64_t)i * p.G);
+    const int i = grow / p.G, gq = grow - i * p.G;
     // L == 0: the row sees no key (a NaN score makes L NaN, and stays)
     const float inv = (i < nq && L != 0.0f) ? 1.0f / L : 0.0f;
     const float un = exp2i(E);
@@ -522,15 +602,13 @@ __global__ void __launch_bounds__(kKeyWarps* RT * 32 + 32, 2 / RT) attention_sma
       out = make_uint2(pack_bf16x2(acc.x * inv * un, acc.y * inv * un), pack_bf16x2(acc.z * inv * un, acc.w * inv * un));
     *reinterpret_cast<uint2*>(p.o + b * p.o_seq + (int64_t)i * p.o_row + (int64_t)(hk * p.G + gq) * p.o_head + 4 * lane) = out;
   }
-  cluster_sync();  // no CTA leaves while another still reads its results
+  if (csize > 1) cluster_join();  // no CTA leaves while another still reads its results
 }
 
 }  // namespace small
 }  // namespace kv
 
 namespace {
-
-std::atomic<uint64_t> g_kv_small_attr{0};
 
 int kv_attn_check(const DemonKvAttnArgs* a) {
   DEMON_CHECK_ARG(a != nullptr, "kv_attention: null argument block");
@@ -552,12 +630,30 @@ int kv_attn_check(const DemonKvAttnArgs* a) {
   return DEMON_OK;
 }
 
-template <int RT>
-int launch_small(const kv::AttnParams& p, int64_t units, int cluster, cudaStream_t st) {
+template <int NR, int RT>
+int launch_small(kv::AttnParams p, const DemonKvAttnArgs* a, cudaStream_t st) {
+  using C = kv::small::Cfg<NR, RT>;
+  static std::atomic<uint64_t> attr_done{0};
+  const auto kernel = kv::small::attention_small_kernel<NR, RT>;
+  if (device_pending(attr_done)) {
+    DEMON_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+    DEMON_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    mark_device_done(attr_done);
+  }
+  const int64_t rows = (int64_t)a->Sq * p.G;
+  DEMON_CHECK_ARG(rows < ((int64_t)1 << 31) - 64, "kv_attention: too many query rows (%lld)", (long long)rows);
+  p.n_rt = (int)((rows + C::kRows * RT - 1) / (C::kRows * RT));
+  const int64_t units = (int64_t)a->B * a->cache.heads * p.n_rt;
+  // Keys split over a cluster until some four waves of CTAs exist, at least two tiles per CTA.
+  const int64_t tiles = ((int64_t)a->W * a->cache.page_size + kv::small::kTile - 1) / kv::small::kTile;
+  int cluster = 1;
+  while (cluster < 16 && units * cluster < 148 * C::kMinCtas && tiles >= 4 * cluster) cluster *= 2;
+  DEMON_CHECK_ARG(units * cluster < ((int64_t)1 << 31), "kv_attention: too many work units (%lld)", (long long)units);
+  p.cluster = cluster;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(units * cluster), 1, 1);
-  cfg.blockDim = dim3(kv::small::kKeyWarps * RT * 32 + 32, 1, 1);
-  cfg.dynamicSmemBytes = kv::small::kSmem;
+  cfg.blockDim = dim3(C::kThreads, 1, 1);
+  cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -565,8 +661,8 @@ int launch_small(const kv::AttnParams& p, int64_t units, int cluster, cudaStream
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  DEMON_CUDA(cudaLaunchKernelEx(&cfg, kv::small::attention_small_kernel<RT>, p));
+  cfg.numAttrs = cluster > 1 ? 1 : 0;
+  DEMON_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
   return DEMON_OK;
 }
 
@@ -591,23 +687,9 @@ extern "C" int demon_kv_attention(const DemonKvAttnArgs* a, void* stream) {
   p.causal = a->causal != 0, p.window = std::min(a->window, kv::kMaxTokens - 2);
   p.scale_log2 = (float)((double)a->scale * 1.4426950408889634);
   p.status = status_word();
-  if (device_pending(g_kv_small_attr)) {
-    DEMON_CUDA(cudaFuncSetAttribute(kv::small::attention_small_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, kv::small::kSmem));
-    DEMON_CUDA(cudaFuncSetAttribute(kv::small::attention_small_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, kv::small::kSmem));
-    DEMON_CUDA(cudaFuncSetAttribute(kv::small::attention_small_kernel<1>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    DEMON_CUDA(cudaFuncSetAttribute(kv::small::attention_small_kernel<2>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    mark_device_done(g_kv_small_attr);
-  }
   const int64_t rows = (int64_t)a->Sq * p.G;
   if (rows > 64 && p.G <= 128) return kv::attention_tc(p, (cudaStream_t)stream);
-  const int rt = rows > 16 ? 2 : 1;
-  p.n_rt = (int)((rows + 16 * rt - 1) / (16 * rt));
-  const int64_t units = (int64_t)a->B * a->cache.heads * p.n_rt;
-  // Keys split over a cluster until some four waves of CTAs exist, at least two tiles per CTA.
-  const int64_t tiles = ((int64_t)a->W * a->cache.page_size + kv::small::kTile - 1) / kv::small::kTile;
-  int cluster = 1;
-  while (cluster < 16 && units * cluster < 4 * 148 * (rt == 1 ? 2 : 1) && tiles >= 4 * cluster) cluster *= 2;
-  DEMON_CHECK_ARG(units * cluster < ((int64_t)1 << 31), "kv_attention: too many work units (%lld)", (long long)units);
-  return rt == 1 ? launch_small<1>(p, units, cluster, (cudaStream_t)stream)
-                 : launch_small<2>(p, units, cluster, (cudaStream_t)stream);
+  if (rows <= 8) return launch_small<1, 1>(p, a, (cudaStream_t)stream);
+  if (rows <= 16) return launch_small<2, 1>(p, a, (cudaStream_t)stream);
+  return launch_small<2, 2>(p, a, (cudaStream_t)stream);
 }

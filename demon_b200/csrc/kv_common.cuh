@@ -82,6 +82,7 @@ struct AttnParams {
   float scale_log2;    // softmax scale * log2(e)
   int n_rt;            // row tiles (or blocks) per kv head
   int Tt;              // tokens per half block (tensor-core kernel)
+  int cluster;         // CTAs per cluster (small kernel)
   unsigned int* status;
 };
 
