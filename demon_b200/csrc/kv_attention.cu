@@ -28,6 +28,7 @@
 // word), and only a byte permute stands between V's rows and the operand layout: the keys and
 // channels of a step may be taken in any order as long as both operands agree.
 #include <algorithm>
+#include <cmath>
 
 #include "demon_host.h"
 #include "kv_common.cuh"
@@ -50,23 +51,28 @@ template <int NR, int RT>
 struct Cfg {
   static constexpr int kRows = 8 * NR;                    // rows of a group
   static constexpr int kThreads = (kKeyWarps * RT + 1) * 32;
-  // ring: what keeps the memory busy with the CTAs that registers allow on an SM (NR 1: three)
-  static constexpr int kStages = NR == 1 ? 4 : 6;
+  // ring: what keeps the memory busy with the CTAs that registers allow on an SM
+  static constexpr int kStages = RT == 1 ? 4 : 6;
   // The two warps of a tile see every second one: with an even number of stages they meet every
   // phase of the stages they use.  (With three, a warp one phase ahead took the phase before as its own.)
   static_assert(kStages % 2 == 0, "a stage must always belong to the same warps");
-  static constexpr int kMinCtas = NR == 1 ? 3 : 2 / RT;
+  static constexpr int kMinCtas = RT == 1 ? 3 : 1;
+  // Registers: a scheduler's quarter of the file holds whole warps, so 128 let three CTAs of five
+  // warps in (200 would leave one), 168 one of nine.
+  static constexpr int kRegs = RT == 1 ? 128 : 168;
+  static constexpr bool kQShared = NR > 1;                // Q operands in shared memory, for those registers
   static constexpr int offScale = kStages * 2 * kHalf;    // [stage][piece][K, V] fp32
   static constexpr int offBar = offScale + kStages * 4 * 2 * 4;  // full[stage], empty[stage]
   static constexpr int offMisc = offBar + kStages * 2 * 8;       // abort flag
-  static constexpr int kSmem = offMisc + 16;
+  static constexpr int offQ = offMisc + 16;               // [row group][k-step][lane] Q operands
+  static constexpr int kSmem = offQ + (kQShared ? RT * 8 * 32 * 16 : 0);
   // After the key loop the ring holds the partial results: per warp O [rows][128] fp32, then the
   // CTA's sum, and the rows' statistics.
   static constexpr int kWarpO = kRows * kHeadDim * 4;
   static constexpr int offSum = kKeyWarps * RT * kWarpO;
   static constexpr int offStat = offSum + RT * kWarpO;                  // per warp and row: m, l, e
   static constexpr int offRow = offStat + kKeyWarps * RT * kRows * 12;  // CTA, per row: M, L, E
-  static_assert(offRow + RT * kRows * 12 <= offScale, "partial results must fit into the ring");
+  static_assert(offRow + RT * kRows * 12 <= offScale && offQ % 16 == 0, "partial results must fit into the ring");
 };
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -126,7 +132,7 @@ __device__ __forceinline__ float join_factor(float m, float M) {
 __device__ __forceinline__ float unit_factor(int e, int E) { return e - E < -126 ? 0.0f : exp2i(imin(e - E, 0)); }
 
 template <int NR, int RT>
-__global__ void __launch_bounds__(Cfg<NR, RT>::kThreads, Cfg<NR, RT>::kMinCtas) attention_small_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(Cfg<NR, RT>::kThreads) __maxnreg__((Cfg<NR, RT>::kRegs)) attention_small_kernel(const AttnParams p) {
   using C = Cfg<NR, RT>;
   constexpr int kStages = C::kStages;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -245,7 +251,7 @@ __global__ void __launch_bounds__(Cfg<NR, RT>::kThreads, Cfg<NR, RT>::kMinCtas) 
     const int kw = warp % kKeyWarps, wt = warp / kKeyWarps;  // part of the keys, row group
     // Q^T: row g of each row tile, k-step s, lane c: channels 16 c + 64 (s / 4) + 4 (s % 4) + 0..3, as
     // K's codes lie
-    uint32_t qf[NR][8][2];
+    uint32_t qf[NR][8][2];  // (NR 2: read again from shared memory for every step)
     float fac[NR][2];  // score factors and positions of rows 2 c, 2 c + 1
     int pos[NR][2];
 #pragma unroll
@@ -288,6 +294,15 @@ __global__ void __launch_bounds__(Cfg<NR, RT>::kThreads, Cfg<NR, RT>::kMinCtas) 
         pos[r][x] = len - nq + __shfl_sync(0xffffffffu, i, 4 * (2 * c + x));
       }
     }
+    if (C::kQShared) {
+      if (kw == 0) {
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+          st_shared_v4(sbase + C::offQ + ((wt * 8 + s) * 32 + lane) * 16, qf[0][s][0], qf[0][s][1], qf[NR - 1][s][0],
+                       qf[NR - 1][s][1]);
+      }
+      asm volatile("bar.sync 1, %0;" ::"n"(kKeyWarps * RT * 32) : "memory");  // the key warps
+    }
     // keys of a 16-key block: A row x is key 4 (x % 8 / 2) + 2 (x / 8) + x % 2, so that the P operand's
     // columns of lane c are keys 4 c .. 4 c + 3
     const int kkey = 4 * (g >> 1) + (g & 1);
@@ -316,21 +331,38 @@ __global__ void __launch_bounds__(Cfg<NR, RT>::kThreads, Cfg<NR, RT>::kMinCtas) 
         }
         float sa[2][NR][4];
 #pragma unroll
-        for (int z = 0; z < 2; ++z) {
+        for (int z = 0; z < 2; ++z)
 #pragma unroll
           for (int r = 0; r < NR; ++r) sa[z][r][0] = sa[z][r][1] = sa[z][r][2] = sa[z][r][3] = 0.0f;
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const uint4 x = ld_shared_v4(st + k_off + 16 * z * kHeadDim + 64 * half);
-            const uint4 y = ld_shared_v4(st + k_off + (16 * z + 2) * kHeadDim + 64 * half);
-            const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+        for (int half = 0; half < 2; ++half) {
+          uint4 kx[2], ky[2];
 #pragma unroll
-            for (int q4 = 0; q4 < 4; ++q4) {
+          for (int z = 0; z < 2; ++z) {
+            kx[z] = ld_shared_v4(st + k_off + 16 * z * kHeadDim + 64 * half);
+            ky[z] = ld_shared_v4(st + k_off + (16 * z + 2) * kHeadDim + 64 * half);
+          }
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4) {
+            uint32_t qb[NR][2];
+            if (C::kQShared) {
+              const uint4 q = ld_shared_v4(sbase + C::offQ + ((wt * 8 + 4 * half + q4) * 32 + lane) * 16);
+              qb[0][0] = q.x;
+              qb[0][1] = q.y;
+              qb[NR - 1][0] = q.z;
+              qb[NR - 1][1] = q.w;
+            } else {
+              qb[0][0] = qf[0][4 * half + q4][0];
+              qb[0][1] = qf[0][4 * half + q4][1];
+            }
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+              const uint32_t xs[4] = {kx[z].x, kx[z].y, kx[z].z, kx[z].w}, ys[4] = {ky[z].x, ky[z].y, ky[z].z, ky[z].w};
               uint32_t a[4];  // keys (x, y), channels 0, 1 and 2, 3 of the word
               e4m3x4_f16(xs[q4], a[0], a[2]);
               e4m3x4_f16(ys[q4], a[1], a[3]);
 #pragma unroll
-              for (int r = 0; r < NR; ++r) mma_f16(sa[z][r], a, qf[r][4 * half + q4][0], qf[r][4 * half + q4][1]);
+              for (int r = 0; r < NR; ++r) mma_f16(sa[z][r], a, qb[r][0], qb[r][1]);
             }
           }
         }
@@ -688,8 +720,21 @@ extern "C" int demon_kv_attention(const DemonKvAttnArgs* a, void* stream) {
   p.scale_log2 = (float)((double)a->scale * 1.4426950408889634);
   p.status = status_word();
   const int64_t rows = (int64_t)a->Sq * p.G;
-  if (rows > 64 && p.G <= 128) return kv::attention_tc(p, (cudaStream_t)stream);
   if (rows <= 8) return launch_small<1, 1>(p, a, (cudaStream_t)stream);
   if (rows <= 16) return launch_small<2, 1>(p, a, (cudaStream_t)stream);
+  // More rows: the small kernel reads the keys once per 32 rows, at about 2 TB/s (60 rows, 4 x 20,000
+  // keys: 129 us; the other kernel 428 us for 80 rows of the same); the tensor-core kernel takes
+  // 2.7 us per tile of 128 keys for 256 rows on one SM (16 x 1,500 rows, 256 keys: 68 us; the small
+  // kernel 597 us).  The lesser estimate is taken, with the keys that the table covers, or those of
+  // the window.
+  if (p.G <= 128) {
+    const int tokens = 2 * (128 / p.G);
+    double keys = (double)a->W * a->cache.page_size;
+    if (p.window >= 0) keys = std::min(keys, (double)tokens + p.window * (p.causal ? 1.0 : 2.0));
+    const double units = (double)a->B * a->cache.heads * ((a->Sq + tokens - 1) / tokens);
+    const double us_tc = std::ceil(units / 148.0) * std::ceil(keys / 128.0) * 2.7;
+    const double us_small = (double)a->B * a->cache.heads * (double)((rows + 31) / 32) * keys * 256.0 / 2.0e6;
+    if (us_tc < us_small) return kv::attention_tc(p, (cudaStream_t)stream);
+  }
   return launch_small<2, 2>(p, a, (cudaStream_t)stream);
 }
