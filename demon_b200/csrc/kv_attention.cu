@@ -29,6 +29,8 @@
 // channels of a step may be taken in any order as long as both operands agree.
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
+#include <cstring>
 
 #include "demon_host.h"
 #include "kv_common.cuh"
@@ -720,6 +722,10 @@ extern "C" int demon_kv_attention(const DemonKvAttnArgs* a, void* stream) {
   p.scale_log2 = (float)((double)a->scale * 1.4426950408889634);
   p.status = status_word();
   const int64_t rows = (int64_t)a->Sq * p.G;
+  // DEMON_KV_ATTENTION=small / tc takes one of the two kernels for every call (tests, measurements)
+  const char* force = std::getenv("DEMON_KV_ATTENTION");
+  const bool small_only = force && std::strcmp(force, "small") == 0;
+  if (force && std::strcmp(force, "tc") == 0 && p.G <= 128) return kv::attention_tc(p, (cudaStream_t)stream);
   if (rows <= 8) return launch_small<1, 1>(p, a, (cudaStream_t)stream);
   if (rows <= 16) return launch_small<2, 1>(p, a, (cudaStream_t)stream);
   // More rows: the small kernel reads the keys once per 32 rows, at about 2 TB/s (60 rows, 4 x 20,000
@@ -727,7 +733,7 @@ extern "C" int demon_kv_attention(const DemonKvAttnArgs* a, void* stream) {
   // 2.7 us per tile of 128 keys for 256 rows on one SM (16 x 1,500 rows, 256 keys: 68 us; the small
   // kernel 597 us).  The lesser estimate is taken, with the keys that the table covers, or those of
   // the window.
-  if (p.G <= 128) {
+  if (p.G <= 128 && !small_only) {
     const int tokens = 2 * (128 / p.G);
     double keys = (double)a->W * a->cache.page_size;
     if (p.window >= 0) keys = std::min(keys, (double)tokens + p.window * (p.causal ? 1.0 : 2.0));

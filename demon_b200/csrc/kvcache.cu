@@ -12,9 +12,14 @@
 // One pass: 16 tokens of a page and head are one warp's, 16 lanes x 16 bytes per token, all
 // eight of a lane's loads in flight and kept in registers between the maximum and the
 // rounding; P / 16 warps of a CTA share a page and join their maxima through shared memory.
+// Bound by memory for prompts (22,000 tokens of 8 heads: 134 MB in 25.9 us, 5.2 TB/s; 36.9 us with
+// 64-bit unit arithmetic, a finite mask on every word and the page looked up before the loads),
+// by the launch for single tokens (3 us).  Four CTAs per SM: 28.2 us with three, 27.5 with five.
 //
 // Read.  Eight lanes take one token and head (128 codes, 16 per lane) and write its 256 bytes;
-// consecutive rows are the heads of one token, so a warp's stores are contiguous.
+// consecutive rows are the heads of one token, so a warp's stores are contiguous.  Bound by memory,
+// the writes above all: 32-byte stores and two rows per lane took 135.6 us to 106.5 us for 691 MB
+// (6.5 TB/s, the measured copy rate; four rows or 16-byte stores keep fewer requests in flight).
 #include "demon_host.h"
 #include "kv_common.cuh"
 #include "kv_host.h"
@@ -33,48 +38,38 @@ struct AppendParams {
   int64_t ld_table;
   int B, S, W, T;     // T: pages an append can touch
   int groups;         // page-head groups per CTA: 128 / P
-  int64_t units;      // B * T * 2 * heads groups in all
+  uint32_t units;     // B * T * 2 * heads groups in all
   unsigned int* status;
 };
 
-// max over the finite halves of packed bf16 magnitudes
+// max of packed bf16 magnitudes, and the same over the finite ones
+__device__ __forceinline__ uint32_t mag_max(uint32_t m, uint32_t v) { return __vmaxu2(m, v & 0x7FFF7FFFu); }
 __device__ __forceinline__ uint32_t finite_max(uint32_t m, uint32_t v) {
   const uint32_t a = v & 0x7FFF7FFFu;
-  const uint32_t fin = __vcmpltu2(a, 0x7F807F80u);
-  return __vmaxu2(m, a & fin);
+  return __vmaxu2(m, a & __vcmpltu2(a, 0x7F807F80u));
 }
 
-__global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kAppendThreads, 4) append_kernel(const AppendParams p) {
   __shared__ uint32_t warp_max[kAppendThreads / 32];
   const int P = p.c.P, nw = P / kTokWarp;  // warps per page
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int grp = warp / nw, wip = warp - grp * nw;
   // unit order: heads fastest, then K / V, then the page, then the sequence, so that a CTA's
   // neighbours read the same token rows
-  const int64_t u = (int64_t)blockIdx.x * p.groups + grp;
+  const uint32_t u = blockIdx.x * (uint32_t)p.groups + grp;  // below 2^31 (checked on the host)
   bool active = u < p.units;
-  const int64_t uu = active ? u : 0;
-  const int h = (int)(uu % p.c.heads);
-  const int64_t r1 = uu / p.c.heads;
-  const int kv = (int)(r1 & 1);
-  const int64_t r2 = r1 >> 1;
-  const int t = (int)(r2 % p.T), b = (int)(r2 / p.T);
+  const uint32_t uu = active ? u : 0, heads = (uint32_t)p.c.heads;
+  const uint32_t r1 = uu / heads, r2 = r1 >> 1;
+  const int h = (int)(uu - r1 * heads), kv = (int)(r1 & 1);
+  const int b = (int)(r2 / (uint32_t)p.T), t = (int)(r2 - (uint32_t)b * (uint32_t)p.T);
 
   const Span sp = append_span(p.start[b], p.count ? p.count[b] : p.S, p.S, p.W * P);
   if (sp.bad && active && t == 0 && h == 0 && lane == 0 && wip == 0) report(p.status, DEMON_DEV_BAD_ARG, 60);
   const int end = sp.start + sp.count;
   const int page = sp.start / P + t, tok0 = page * P;
   active = active && sp.count > 0 && tok0 < end;
-  int pid = -1;
-  if (active) {
-    pid = page_id(p.table + b * p.ld_table, p.W, page, p.c.pages);
-    if (pid < 0 && h == 0 && lane == 0 && wip == 0) report(p.status, DEMON_DEV_BAD_ARG, 61);
-    active = pid >= 0;
-  }
-  const int64_t ph = active ? (int64_t)pid * p.c.heads + h : 0;
-  const int n_old = imin(imax(sp.start - tok0, 0), P);
-  const float s_old = active && n_old > 0 ? p.c.scale[kv][ph] : 0.0f;
 
+  // the new tokens' loads first: their addresses do not wait for the page
   const int sub = lane & 15;
   uint4 v[8];
   bool mine[8];
@@ -88,9 +83,23 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
       v[j] = __ldg(reinterpret_cast<const uint4*>(p.x[kv] + b * p.seq[kv] + (int64_t)(pos - sp.start) * p.row[kv] +
                                                   h * p.head[kv] + sub * 8));
   }
+  int pid = -1;
+  if (active) {
+    pid = page_id(p.table + b * p.ld_table, p.W, page, p.c.pages);
+    if (pid < 0 && h == 0 && lane == 0 && wip == 0) report(p.status, DEMON_DEV_BAD_ARG, 61);
+    active = pid >= 0;
+  }
+  const int64_t ph = active ? (int64_t)pid * p.c.heads + h : 0;
+  const int n_old = imin(imax(sp.start - tok0, 0), P);
+  const float s_old = active && n_old > 0 ? p.c.scale[kv][ph] : 0.0f;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) mx = finite_max(finite_max(finite_max(finite_max(mx, v[j].x), v[j].y), v[j].z), v[j].w);
-  uint32_t am = mx > 0 ? (((mx & 0xFFFFu) > (mx >> 16)) ? (mx & 0xFFFFu) : (mx >> 16)) : 0u;
+  for (int j = 0; j < 8; ++j) mx = mag_max(mag_max(mag_max(mag_max(mx, v[j].x), v[j].y), v[j].z), v[j].w);
+  if (__vcmpgeu2(mx, 0x7F807F80u)) {  // infinities or NaN: they do not count
+    mx = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) mx = finite_max(finite_max(finite_max(finite_max(mx, v[j].x), v[j].y), v[j].z), v[j].w);
+  }
+  uint32_t am = max(mx & 0xFFFFu, mx >> 16);
   am = __reduce_max_sync(0xffffffffu, am);
   if (nw > 1) {
     if (lane == 0) warp_max[warp] = am;
@@ -138,15 +147,17 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
 // ---------------------------------------------------------------------------------- read
 
 constexpr int kReadThreads = 256;
-constexpr int kReadRows = 4;  // rows (token, head) per eight lanes
+constexpr int kReadRows = 2;  // rows (token, head) per eight lanes
 
 struct ReadParams {
   Cache c;
   __nv_bfloat16* out[2];
   int64_t seq[2], row[2];  // element strides of out; heads contiguous
   const int32_t *table, *lens;
-  int64_t ld_table, rows;  // rows of a sequence: max_len * heads
+  int64_t ld_table;
+  uint32_t rows;  // rows of a sequence: max_len * heads
   int W;
+  int wide;  // 32-byte stores: outputs and pitches aligned to 32 bytes
   unsigned int* status;
 };
 
@@ -155,16 +166,16 @@ __global__ void __launch_bounds__(kReadThreads) read_kernel(const ReadParams p) 
   const int sub = threadIdx.x & 7;
   bool bad = false;
   const int len = clamp_len(p.lens[b], p.W * P, &bad);
-  const int64_t r0 = ((int64_t)blockIdx.x * kReadRows) * (kReadThreads / 8) + (threadIdx.x >> 3);
+  const uint32_t r0 = (blockIdx.x * kReadRows) * (kReadThreads / 8) + (threadIdx.x >> 3), heads = (uint32_t)p.c.heads;
   const int32_t* row = p.table + b * p.ld_table;
   uint4 w[kReadRows];
   float s[kReadRows];
   int tok[kReadRows], h[kReadRows];
 #pragma unroll
   for (int j = 0; j < kReadRows; ++j) {
-    const int64_t r = r0 + j * (kReadThreads / 8);
-    tok[j] = r < p.rows ? (int)(r / p.c.heads) : -1;
-    h[j] = (int)(r - (int64_t)tok[j] * p.c.heads);
+    const uint32_t r = r0 + j * (kReadThreads / 8);
+    tok[j] = r < p.rows ? (int)(r / heads) : -1;
+    h[j] = (int)(r - (uint32_t)tok[j] * heads);
     w[j] = make_uint4(0, 0, 0, 0);
     s[j] = 0.0f;
     if (tok[j] >= 0 && tok[j] < len) {
@@ -192,8 +203,14 @@ __global__ void __launch_bounds__(kReadThreads) read_kernel(const ReadParams p) 
       r[2 * i] = pack_bf16x2(a.x * s[j], a.y * s[j]);
       r[2 * i + 1] = pack_bf16x2(c.x * s[j], c.y * s[j]);
     }
-    st_global_v4(o, make_uint4(r[0], r[1], r[2], r[3]));
-    st_global_v4(o + 8, make_uint4(r[4], r[5], r[6], r[7]));
+    if (p.wide) {
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(o), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+                   "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                   : "memory");
+    } else {
+      st_global_v4(o, make_uint4(r[0], r[1], r[2], r[3]));
+      st_global_v4(o + 8, make_uint4(r[4], r[5], r[6], r[7]));
+    }
   }
   if (bad) report(p.status, DEMON_DEV_BAD_ARG, 62);
 }
@@ -262,10 +279,11 @@ extern "C" int demon_kv_append(const DemonKvAppendArgs* a, void* stream) {
   p.B = a->B, p.S = a->S, p.W = a->W;
   p.T = kv::append_pages(a->S, a->cache.page_size);
   p.groups = kv::kAppendThreads / 32 / (a->cache.page_size / kv::kTokWarp);
-  p.units = (int64_t)a->B * p.T * 2 * a->cache.heads;
+  const int64_t units = (int64_t)a->B * p.T * 2 * a->cache.heads;
+  DEMON_CHECK_ARG(units < ((int64_t)1 << 31) - 8, "kv_append: too many pages (%lld)", (long long)units);
+  p.units = (uint32_t)units;
   p.status = status_word();
-  const int64_t grid = (p.units + p.groups - 1) / p.groups;
-  DEMON_CHECK_ARG(grid < ((int64_t)1 << 31), "kv_append: too many pages (%lld)", (long long)p.units);
+  const int64_t grid = (units + p.groups - 1) / p.groups;
   kv::append_kernel<<<(unsigned)grid, kv::kAppendThreads, 0, (cudaStream_t)stream>>>(p);
   DEMON_CUDA(cudaGetLastError());
   return DEMON_OK;
@@ -295,12 +313,15 @@ extern "C" int demon_kv_read(const DemonKvReadArgs* a, void* stream) {
   p.out[1] = (__nv_bfloat16*)a->v_out;
   p.seq[0] = a->k_seq, p.row[0] = a->k_row, p.seq[1] = a->v_seq, p.row[1] = a->v_row;
   p.table = a->table, p.lens = a->lens, p.ld_table = a->ld_table;
-  p.rows = (int64_t)a->max_len * a->cache.heads;
+  const int64_t rows = (int64_t)a->max_len * a->cache.heads;
+  DEMON_CHECK_ARG(rows < ((int64_t)1 << 31) - 256, "kv_read: too many rows a sequence (%lld)", (long long)rows);
+  p.rows = (uint32_t)rows;
   p.W = a->W;
+  p.wide = (((uintptr_t)a->k_out | (uintptr_t)a->v_out) & 31) == 0 && a->k_seq % 16 == 0 && a->k_row % 16 == 0 &&
+           a->v_seq % 16 == 0 && a->v_row % 16 == 0;
   p.status = status_word();
   const int64_t per = (int64_t)kv::kReadRows * (kv::kReadThreads / 8);
-  const int64_t grid = (p.rows + per - 1) / per;
-  DEMON_CHECK_ARG(grid < ((int64_t)1 << 31), "kv_read: output too long");
+  const int64_t grid = (rows + per - 1) / per;
   kv::read_kernel<<<dim3((unsigned)grid, (unsigned)a->B, 2), kv::kReadThreads, 0, (cudaStream_t)stream>>>(p);
   DEMON_CUDA(cudaGetLastError());
   return DEMON_OK;

@@ -5,6 +5,8 @@ power of two and a value has four significant bits).  attention is compared elem
 with the bound derived in kv_reference.attention: half a step of bf16 for the output, half a step
 of f16 for the probabilities, fp32 sums.
 """
+import os
+
 import pytest
 import torch
 
@@ -203,6 +205,28 @@ def test_read_into_strided_outputs(cuda):
 
 def check_attention(cuda, cache, ref, rows, table, lens, q, q_lens=None, causal=False, window=None, scale=None,
                     label="", **kw):
+    """The call as it is, then through each of the two kernels (few rows, tensor cores)."""
+    chosen = os.environ.get("DEMON_KV_ATTENTION", "")
+    for name in [n for n in ("small", "tc", "") if n != chosen] + [chosen]:
+        os.environ["DEMON_KV_ATTENTION"] = name
+        o = check_one(cuda, cache, ref, rows, table, lens, q, q_lens, causal, window, scale, f"{name} {label}", **kw)
+    return o
+
+
+@pytest.fixture(autouse=True)
+def _no_choice_left():
+    yield
+    os.environ.pop("DEMON_KV_ATTENTION", None)
+
+
+@pytest.fixture(params=["", "small", "tc"])
+def which(request):
+    """The attention kernel as the call chooses it, and each of the two."""
+    os.environ["DEMON_KV_ATTENTION"] = request.param
+    return request.param
+
+
+def check_one(cuda, cache, ref, rows, table, lens, q, q_lens, causal, window, scale, label, **kw):
     from demon_b200 import kvcache
     o = kvcache.attention(q, cache, table, i32(lens, cuda), causal=causal, window=window, scale=scale,
                           q_lens=None if q_lens is None else i32(q_lens, cuda), **kw)
@@ -306,7 +330,7 @@ def test_nan_reaches_only_the_rows_that_see_it(cuda, Sq):
         check_attention(cuda, cache, ref, rows, table, lens, q, None, causal, window, label=f"{causal} {window}")
 
 
-def test_strided_queries_and_outputs(cuda):
+def test_strided_queries_and_outputs(cuda, which):
     from demon_b200 import kvcache
     lens = [90, 33]
     cache, ref, table, rows = filled(lens, 32, 2, cuda, 51)
@@ -335,7 +359,7 @@ def test_shared_pages(cuda):
     check_attention(cuda, cache, ref, r3, t3, [100, 70, 60], q)
 
 
-def test_pages_beyond_32_bit_offsets(cuda):
+def test_pages_beyond_32_bit_offsets(cuda, which):
     """Codes that lie past 2^32 bytes of the buffers."""
     from demon_b200 import kvcache
     P, heads = 128, 8
@@ -415,7 +439,7 @@ def test_a_sequence_grows_token_by_token_and_graphs_replay(cuda):
     ok()
 
 
-def test_calls_on_other_streams(cuda):
+def test_calls_on_other_streams(cuda, which):
     """An explicit stream, and two streams at once over one cache, equal the plain call."""
     from demon_b200 import kvcache
     cache, _, table, _ = filled([3000, 2000], 64, 2, cuda, 91)
@@ -437,7 +461,7 @@ def test_calls_on_other_streams(cuda):
     ok()
 
 
-def test_repeated_calls_give_equal_bits(cuda):
+def test_repeated_calls_give_equal_bits(cuda, which):
     from demon_b200 import kvcache
     cache, _, table, _ = filled([4000, 100, 999], 32, 2, cuda, 92)
     lens = i32([4000, 100, 999], cuda)
@@ -450,7 +474,7 @@ def test_repeated_calls_give_equal_bits(cuda):
 
 # ------------------------------------------------------------------------------------ refusals
 
-def test_bad_device_values_are_reported_and_harmless(cuda):
+def test_bad_device_values_are_reported_and_harmless(cuda, which):
     """Page ids, lengths and starts out of range (checked on the CPU in test_kvcache.py): the
     status word says so, other sequences are right, nothing else is written."""
     from demon_b200 import _native as nat
@@ -548,7 +572,7 @@ def test_refusals(cuda):
     ok()
 
 
-def test_empty_calls(cuda):
+def test_empty_calls(cuda, which):
     """No sequences, no tokens, no queries, no table columns."""
     from demon_b200 import kvcache
     cache, _, table, _ = filled([40, 40], 16, 2, cuda, 97)
