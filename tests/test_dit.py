@@ -226,3 +226,44 @@ def test_dit_hot_lora_strength_sweep_and_remove(cuda):
     for name in lora:
         m.get_submodule(name).lora.remove("cfg4")
     assert torch.equal(_run(g, d, cuda), base)
+
+
+@pytest.mark.gpu
+def test_cross_attention_from_the_8_bit_cache(cuda):
+    """encoder_kv(cache="e4m3"): the forward over cached conditions against the forward over the
+    same values read back into bf16 (the two attention kernels round probabilities to f16 and to
+    bf16: one-ulp differences, hence the whole-forward bar), conditions shared by rows(), and the
+    values themselves against the bf16 K / V (half a step of E4M3 is 2^-4 of a value, or 2^-10 of
+    the page's largest where codes are subnormal)."""
+    from demon_b200 import kvcache
+    d = _fixture()
+    m = _model(d, cuda)
+    t, enc = d["t"].to(cuda), d["enc"].to(cuda)
+    B, L = enc.shape[:2]
+    cfg = m.cfg
+    width = cfg.num_key_value_heads * 128
+
+    def run(kv, x=d["x"].to(cuda), tt=t, ctx=d["ctx"].to(cuda)):
+        return m(hidden_states=x, timestep=tt, timestep_r=tt, context_latents=ctx, encoder_kv=kv)[0]
+
+    with torch.no_grad():
+        plain, _ = m.encoder_kv(enc)
+        cached, n = m.encoder_kv(enc, cache="e4m3", page_size=16)
+        assert n == L and len(cached) == len(m.layers)
+        back = []
+        for c, kv in zip(cached, plain):
+            k, v = kvcache.read(c.cache, c.table, c.lens, L)
+            both = torch.cat([k.reshape(B * L, width), v.reshape(B * L, width)], 1)
+            back.append(both)
+            err, ref = (both.float() - kv.float()).abs(), kv.float()
+            assert bool((err <= torch.maximum(ref.abs() * 2.0 ** -4, ref.abs().max() * 2.0 ** -10)).all())
+        got, want = run((cached, L)), run((back, L))
+        assert torch.isfinite(got.float()).all()
+        assert _rel(got, want) <= 0.15
+        assert torch.equal(got, run((cached, L)))
+        # every sequence over the first condition, by page numbers alone
+        same = run(([c.rows([0] * B) for c in cached], L))
+        first, _ = m.encoder_kv(enc[:1].expand(B, -1, -1), cache="e4m3", page_size=16)
+        assert torch.equal(same, run((first, L)))
+    with pytest.raises(ValueError, match="e4m3"):
+        m.encoder_kv(enc, cache="int8")
