@@ -22,20 +22,22 @@
 // Output: O * 2^(M - m - 6) / l.  Both offsets are raised only when exceeded by more than 8.
 //
 // Warp roles (512 threads):
-//   warpgroup 0 / 1   row half 0 / 1, one query row per thread: the softmax in steps of 64 keys, the
+//   warpgroup 0 / 1   row half 0 / 1, one query row per thread: the softmax of every key tile, the
 //                     output row,
 //   warpgroup 2       codes -> f16, swizzled, into a ring of three K / V tiles; the Q rows in place,
 //   warp 12           MMA issue (one thread) and tensor-memory allocation,
 //   warp 13           page look-ups, scales, bulk copies of K / V codes into a ring of half tiles,
 //   warp 14           the next unit's Q by TMA, each half as soon as the last Q K^T has read the slot,
 //   warp 15           the list of units: lengths and masks into a ring of records that every role reads.
-// Tensor memory (512 columns): two score buffers of 64 keys per half, S_h at 128 h + 64 (step % 2), the
-// f16 probabilities over their upper halves, and O_h at 256 + 128 h.  Q K^T of step u + 1 is issued
-// before P V of step u, so that a softmax warp finds its next scores ready; with one buffer of 128
-// keys it waited some 1,600 of 4,400 clocks per 128 keys for P V and Q K^T to pass through.
+// Tensor memory as in attention.cu: S_h at 128 h, P_h over its upper half, O_h at 256 + 128 h.
 //
-// Bound by the exponentials (one per row and key, 16 per clock and SM) and the MMAs, which take
-// as long; short key ranges (256 keys of a condition are two tiles) by the units' Q and output.
+// Bound by the softmax warps' path from S to P (some 3,000 clocks per tile and half, of which the
+// exponentials' rate asks for 1,024) and, for short key ranges (256 keys of a condition are two
+// tiles), by the units' Q conversion and output.  Measured, 16 query heads over 8: 6,016 x 6,016
+// 362 us (0.82 PFLOP/s; the bf16 kernel of attention.cu 266 us), 16 x 750 over 256 keys 69 us (bf16
+// 34 us), 6,001 causal 186 us.  Slower, not kept: steps of 64 keys with two score buffers (Q K^T 64
+// wide takes the tensor core longer, and the overheads of a step double: 396 us); two threads per row
+// (466 us); the next scores loaded ahead of the exponentials (509 us, they come late).
 #include <algorithm>
 
 #include "demon_host.h"
@@ -62,7 +64,11 @@ constexpr float kBias = 6.0f;            // P = 2^(.. + 6)
 constexpr float kRaise = 8.0f;           // offsets are raised when exceeded by more than this
 constexpr float kFast = 60.0f;           // |M - m - ev| up to which l comes from P
 
-constexpr int kStep = 64;                // keys per softmax step
+
+// Registers per thread after the split (setmaxnreg): the launch gives 512 x 128.
+constexpr int kLaunchRegs = 128, kSoftmaxRegs = 176, kConvRegs = 80, kIssueRegs = 80;
+static_assert(256 * kSoftmaxRegs + 128 * kConvRegs + 128 * kIssueRegs <= kThreads * kLaunchRegs,
+              "register split exceeds the launch's registers (setmaxnreg.inc would wait for good)");
 
 // Scales of a tile: per 16 keys {K scale, V exponent ev, 2^(ev_0 - ev), 0}, and {., -inf, ., -inf}
 // for keys without a page, which so weigh nothing; then {smallest ev, largest ev, ev_0, 0}.
@@ -80,13 +86,13 @@ constexpr int offNanW = offSc + kScSlots * kScWords * 4;       // [slot][warp] a
 constexpr int offUnit = offNanW + kScSlots * 4 * 4;            // [slot] 12 words
 constexpr int offRawMask = offUnit + kUnitSlots * 48;          // [slot] 16-key groups copied
 constexpr int offBar = offRawMask + 4 * 4;
-constexpr int kNumBars = 4 + 2 * kSlots + 12 + 1 + 2 * kScSlots + 2 * kRawSlots + 6 + 2 * kUnitSlots;
+constexpr int kNumBars = 4 + 2 * kSlots + 8 + 1 + 2 * kScSlots + 2 * kRawSlots + 6 + 2 * kUnitSlots;
 constexpr int offMisc = offBar + kNumBars * 8;
 constexpr int kSmem = offMisc + 16 + 1024;
 static_assert(kSmem <= 232448, "shared memory exceeds the sm_100 per-block limit");
 
 constexpr uint32_t kTmemCols = 512;
-constexpr uint32_t kColS = 0, kColP = 32, kColO = 256;  // P within its score buffer
+constexpr uint32_t kColS = 0, kColP = 64, kColO = 256;  // P over the upper half of S
 
 // kind::f16, F16 x F16 -> F32, K-major A and B
 constexpr uint32_t idesc_f16(int M, int N) {
@@ -113,6 +119,14 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
                                           unsigned int* status, unsigned int where) {
   if (__all_sync(0xffffffffu, mbar_try_wait(smem_u32(bar), parity))) return true;
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, t0, status, where));
+}
+template <int N>
+__device__ __forceinline__ void setmaxnreg_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void setmaxnreg_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 __device__ __forceinline__ void st_shared_u16(uint32_t a, uint32_t x) {
   asm volatile("st.shared.u16 [%0], %1;" ::"r"(a), "h"((unsigned short)x) : "memory");
@@ -149,7 +163,6 @@ struct Unit {
   int i0;           // first token of the block
   Keys ks;          // keys that some / every row of the block sees
   int tile0, nt;    // key tiles; nt 0: no keys (its rows are zeros), nt -1: no more units
-  int ns;           // steps of 64 keys
 };
 
 // The j-th unit of this CTA: rounds go over the CTAs in turn, back and forth, since the units
@@ -170,22 +183,21 @@ __device__ __forceinline__ Unit decode(const AttnParams& p, uint32_t u, bool* ba
   w.ks.lo = w.ks.hi = w.ks.lo_all = w.ks.hi_all = 0;
   if (w.i0 <= i1) w.ks = visible(w.i0, i1, w.len, w.nq, p.causal != 0, p.window);
   w.tile0 = w.ks.lo / kBlk;
-  w.ns = w.ks.hi > w.ks.lo ? (w.ks.hi - w.tile0 * kBlk + kStep - 1) / kStep : 0;
-  w.nt = (w.ns + 1) / 2;
+  w.nt = w.ks.hi > w.ks.lo ? (w.ks.hi + kBlk - 1) / kBlk - w.tile0 : 0;
   return w;
 }
 // A unit's record in shared memory.
 __device__ __forceinline__ void put_unit(uint32_t a, const Unit& w) {
   st_shared_v4(a, w.b, w.hk, w.len, w.nq);
   st_shared_v4(a + 16, w.i0, w.ks.lo, w.ks.hi, w.ks.lo_all);
-  st_shared_v4(a + 32, w.ks.hi_all, w.tile0, w.nt, w.ns);
+  st_shared_v4(a + 32, w.ks.hi_all, w.tile0, w.nt, 0);
 }
 __device__ __forceinline__ Unit get_unit(uint32_t a) {
   const uint4 x = ld_shared_v4(a), y = ld_shared_v4(a + 16), z = ld_shared_v4(a + 32);
   Unit w;
   w.b = (int)x.x, w.hk = (int)x.y, w.len = (int)x.z, w.nq = (int)x.w;
   w.i0 = (int)y.x, w.ks.lo = (int)y.y, w.ks.hi = (int)y.z, w.ks.lo_all = (int)y.w;
-  w.ks.hi_all = (int)z.x, w.tile0 = (int)z.y, w.nt = (int)z.z, w.ns = (int)z.w;
+  w.ks.hi_all = (int)z.x, w.tile0 = (int)z.y, w.nt = (int)z.z;
   return w;
 }
 
@@ -200,11 +212,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
   uint64_t* q_empty = q_full + 2;               // [2] the unit's last Q K^T done
   uint64_t* kv_full = q_empty + 2;              // [3] K or V tile converted
   uint64_t* kv_empty = kv_full + kSlots;        // [3] its MMAs done
-  uint64_t* s_full = kv_empty + kSlots;         // [2 halves][2 buffers] S computed
-  uint64_t* p_full = s_full + 4;                // [2 halves][2 buffers] P in tensor memory
-  uint64_t* pv_done = p_full + 4;               // [2] P_h V of a step done
-  uint64_t* o_full = pv_done + 2;               // [2] the unit's last P_h V done
-  uint64_t* mma_done = o_full + 2;
+  uint64_t* s_full = kv_empty + kSlots;         // [2] S_h computed
+  uint64_t* pa_full = s_full + 2;               // [2] P_h of keys 0-63 in tensor memory
+  uint64_t* pb_full = s_full + 4;               // [2] P_h of keys 64-127
+  uint64_t* o_full = s_full + 6;                // [2] the unit's last P_h V done
+  uint64_t* mma_done = s_full + 8;
   // The scales and NaN maps have rings longer than any lag between their writers and readers: V of
   // tile t takes the slot of K of tile t - 1, whose last Q K^T was issued after both softmax
   // warpgroups had published, and so were done with, tile t - 2; the codes of tile t are copied at
@@ -234,12 +246,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       mbar_init(&q_raw[h], 1);
       mbar_init(&row_full[h], kConvWarps);
       mbar_init(&row_full[2 + h], kConvWarps);
-      mbar_init(&pv_done[h], 1);
+      mbar_init(&s_full[h], 1);
+      mbar_init(&pa_full[h], 4);
+      mbar_init(&pb_full[h], 4);
       mbar_init(&o_full[h], 1);
-      for (int buf = 0; buf < 2; ++buf) {
-        mbar_init(&s_full[2 * h + buf], 1);
-        mbar_init(&p_full[2 * h + buf], 4);
-      }
     }
     mbar_init(mma_done, 1);
     for (int s = 0; s < kUnitSlots; ++s) {
@@ -285,77 +295,86 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
   };
 
   if (wg == 3) {
+    setmaxnreg_dec<kIssueRegs>();
     if (warp == 12) {
       // ------------------------------------------------------------------ MMA issue (one thread)
       if (elect_one()) {
-        const uint32_t idesc_qk = idesc_f16(kBlk, kStep);
+        const uint32_t idesc_qk = idesc_f16(kBlk, kBlk);
         const uint32_t idesc_pv = idesc_f16(kBlk, kHeadDim) | (1u << 16);  // B (V) MN-major
-        uint32_t g = 0, it = 0, step = 0;  // half tiles, units, steps (all units)
-        // S_h of a step: keys 64 part .. of the K tile in a slot
-        auto qk = [&](int h, uint32_t kslot, uint32_t part, uint32_t at) {
-          const uint32_t qa = kmajor_lo(sbase + offQ + h * kTile);
-          const uint32_t kb = kmajor_lo(sbase + offKV + kslot * kTile + part * kStep * 128);
-          const uint32_t d = tmem + kColS + 128 * h + kStep * (at & 1);
+        uint32_t g = 0, it = 0, tiles = 0;  // half tiles, units, key tiles (all units)
+        auto qk = [&](int h, uint32_t kslot) {
+          const uint32_t qa = kmajor_lo(sbase + offQ + h * kTile), kb = kmajor_lo(sbase + offKV + kslot * kTile);
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)
-            mma_bf16(d, desc_of(qa + kmajor_step(kk)), desc_of(kb + kmajor_step(kk)), idesc_qk, kk > 0);
-          tc_commit(&s_full[2 * h + (at & 1)]);
+            mma_bf16(tmem + kColS + 128 * h, desc_of(qa + kmajor_step(kk)), desc_of(kb + kmajor_step(kk)), idesc_qk, kk > 0);
+          tc_commit(&s_full[h]);
         };
-        auto pv = [&](int h, uint32_t vslot, uint32_t part, uint32_t at, bool acc) {
-          const uint32_t vb = mnmajor_lo(sbase + offKV + vslot * kTile + part * 4 * 2048);
-          const uint32_t pa = tmem + kColS + 128 * h + kStep * (at & 1) + kColP;
+        auto pv = [&](int h, uint32_t vslot, int half, bool acc) {
+          const uint32_t vb = mnmajor_lo(sbase + offKV + vslot * kTile);
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            mma_bf16_ts(tmem + kColO + 128 * h, pa + 8 * kk, desc_of(vb + mnmajor_step(kk)), idesc_pv, (acc || kk > 0) ? 1u : 0u);
-          tc_commit(&pv_done[h]);
+          for (int k4 = 0; k4 < 4; ++k4) {
+            const int kk = 4 * half + k4;
+            mma_bf16_ts(tmem + kColO + 128 * h, tmem + kColS + 128 * h + kColP + 8 * kk, desc_of(vb + mnmajor_step(kk)),
+                        idesc_pv, (acc || kk > 0) ? 1u : 0u);
+          }
         };
         auto wait_on = [&](uint64_t* bar, uint32_t parity, unsigned int where) {
           const bool ok = mbar_wait(bar, parity, abort_flag, t0, p.status, where);
           tc_fence_after();
           return ok;
         };
-        // Per step: Q K^T of the next step for both halves, then P V of this one.  A unit's first P_h V
-        // may overwrite O_h: its P_h comes from threads that have stored the last unit's rows.
-        bool ok = true;
+        // The key tiles of all units form one stream; per tile: S_0, the last tile's P_1 V, S_1, P_0 V
+        // (one half's softmax runs while the other half's products do, across units too).  A unit's
+        // first P_h V may overwrite O_h: its P_h comes from threads that have stored the last unit's rows.
+        bool ok = true, pend = false, pend_acc = false, pend_last = false;
+        uint32_t pend_v = 0;
+        auto flush = [&]() {  // P_1 V of the last tile
+          if (!pend) return true;
+          if (!wait_on(&pa_full[1], (tiles - 1) & 1u, 72)) return false;
+          pv(1, pend_v, 0, pend_acc);
+          if (!wait_on(&pb_full[1], (tiles - 1) & 1u, 73)) return false;
+          pv(1, pend_v, 1, true);
+          tc_commit(&kv_empty[pend_v]);
+          if (pend_last) tc_commit(&o_full[1]);
+          pend = false;
+          return true;
+        };
         for (uint32_t j = 0; ok; ++j) {
           const uint32_t us = j % kUnitSlots;
           if (!wait_on(&unit_full[us], (j / kUnitSlots) & 1u, 70)) break;
-          const int ns = (int)ld_shared_b32(sbase + offUnit + us * 48 + 44);
+          const int nt = (int)ld_shared_b32(sbase + offUnit + us * 48 + 40);
           mbar_arrive(&unit_empty[us]);
-          if (ns < 0) break;
-          uint32_t ks = g % kSlots, kp = (g / kSlots) & 1u;  // slot and phase of the K tile to come
+          if (nt < 0) {
+            flush();
+            break;
+          }
+          if (nt == 0) continue;
+          if (!(ok = wait_on(&q_full[0], it & 1u, 75) && wait_on(&kv_full[g % kSlots], (g / kSlots) & 1u, 71))) break;
 #pragma unroll 1
-          for (int v = 0; v <= ns; ++v) {  // v: the step whose scores are issued; v - 1: whose product is
-            if (v < ns) {
-              ks = (g + (uint32_t)(v & ~1)) % kSlots;
-              kp = ((g + (uint32_t)(v & ~1)) / kSlots) & 1u;
-              if (!(v & 1) && !(ok = wait_on(&kv_full[ks], kp, 71))) break;
-              const uint32_t at = step + (uint32_t)v;
-              if (v == 0 && !(ok = wait_on(&q_full[0], it & 1u, 75))) break;
-              qk(0, ks, v & 1, at);
-              if (v == ns - 1) tc_commit(&q_empty[0]);
-              if (v == 0 && !(ok = wait_on(&q_full[1], it & 1u, 75))) break;
-              qk(1, ks, v & 1, at);
-              if (v == ns - 1) tc_commit(&q_empty[1]);
-              if ((v & 1) || v == ns - 1) tc_commit(&kv_empty[ks]);
-            }
-            if (v == 0) continue;
-            const uint32_t u = (uint32_t)v - 1, at = step + u, buf = at & 1u, ph = (at >> 1) & 1u;
-            const uint32_t vg = g + (u & ~1u) + 1, vs = vg % kSlots;
-            if (!(u & 1) && !(ok = wait_on(&kv_full[vs], (vg / kSlots) & 1u, 71))) break;
-            if (!(ok = wait_on(&p_full[buf], ph, 72))) break;
-            pv(0, vs, u & 1, at, u > 0);
-            if (v == ns) tc_commit(&o_full[0]);
-            if (!(ok = wait_on(&p_full[2 + buf], ph, 73))) break;
-            pv(1, vs, u & 1, at, u > 0);
-            if (v == ns) tc_commit(&o_full[1]);
-            if ((u & 1) || v == ns) tc_commit(&kv_empty[vs]);
+          for (int i = 0; i < nt; ++i) {
+            const uint32_t ks = g % kSlots, vs = (g + 1) % kSlots, vp = ((g + 1) / kSlots) & 1u;  // K has been waited for
+            g += 2;
+            const bool last = i == nt - 1;
+            qk(0, ks);
+            if (last) tc_commit(&q_empty[0]);
+            if (!(ok = flush() && (i > 0 || wait_on(&q_full[1], it & 1u, 75)))) break;
+            qk(1, ks);
+            tc_commit(&kv_empty[ks]);
+            if (last) tc_commit(&q_empty[1]);
+            if (!(ok = wait_on(&kv_full[vs], vp, 71) && wait_on(&pa_full[0], tiles & 1u, 72))) break;
+            pv(0, vs, 0, i > 0);
+            // the next K before the last wait of this tile
+            if (!last && !(ok = wait_on(&kv_full[g % kSlots], (g / kSlots) & 1u, 71))) break;
+            if (!(ok = wait_on(&pb_full[0], tiles & 1u, 73))) break;
+            pv(0, vs, 1, true);
+            if (last) tc_commit(&o_full[0]);
+            pend = true;
+            pend_v = vs;
+            pend_acc = i > 0;
+            pend_last = last;
+            ++tiles;
           }
-          if (ns > 0) {
-            step += (uint32_t)ns;
-            g += 2 * (uint32_t)((ns + 1) / 2);
-            ++it;
-          }
+          ++it;
         }
         tc_commit(mma_done);
       }
@@ -474,7 +493,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       for (uint32_t j = 0, n = 0;; ++j) {
         bool bad = false;
         Unit w;
-        w.nt = w.ns = -1;
+        w.nt = -1;
         if ((uint64_t)j * gridDim.x < units) {
           const uint32_t u = unit_index(j);
           if (u >= units) continue;
@@ -493,6 +512,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       }
     }
   } else if (wg == 2) {
+    setmaxnreg_dec<kConvRegs>();
     // -------------------------------------------------------------------- codes -> f16
     // Warp cw takes keys 32 cw .. 32 cw + 31: chunk i is 16 codes of row 8 (i / 2) + lane / 4, and
     // neighbouring rows take opposite halves of their 128 codes (no bank conflicts either way).
@@ -504,12 +524,20 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       const uint32_t base = sbase + offQ + h * kTile + rr * 128;
       const uint32_t flip = (rr & 7) << 4;
       uint32_t mx = 0;
-#pragma unroll 4
-      for (int k = 0; k < 16; ++k) {  // infinities and NaN do not count, and pass through
+#pragma unroll 8
+      for (int k = 0; k < 16; ++k) {
         const uint4 x = ld_shared_v4(base + (k >> 3) * kBox + ((k & 7) << 4 ^ flip));
-        const uint32_t y[4] = {x.x & 0x7FFF7FFFu, x.y & 0x7FFF7FFFu, x.z & 0x7FFF7FFFu, x.w & 0x7FFF7FFFu};
+        mx = __vmaxu2(mx, __vmaxu2(__vmaxu2(x.x & 0x7FFF7FFFu, x.y & 0x7FFF7FFFu), __vmaxu2(x.z & 0x7FFF7FFFu, x.w & 0x7FFF7FFFu)));
+      }
+      if (__vcmpgeu2(mx, 0x7F807F80u)) {  // infinities and NaN do not count, and pass through
+        mx = 0;
+#pragma unroll 1
+        for (int k = 0; k < 16; ++k) {
+          const uint4 x = ld_shared_v4(base + (k >> 3) * kBox + ((k & 7) << 4 ^ flip));
+          const uint32_t y[4] = {x.x & 0x7FFF7FFFu, x.y & 0x7FFF7FFFu, x.z & 0x7FFF7FFFu, x.w & 0x7FFF7FFFu};
 #pragma unroll
-        for (int q = 0; q < 4; ++q) mx = __vmaxu2(mx, y[q] & __vcmpltu2(y[q], 0x7F807F80u));
+          for (int q = 0; q < 4; ++q) mx = __vmaxu2(mx, y[q] & __vcmpltu2(y[q], 0x7F807F80u));
+        }
       }
       mx = max(mx & 0xFFFFu, mx >> 16);
       const int e = imax((int)(mx >> 7) - 127 - 13, -126);  // |q| 2^-e < 2^14
@@ -600,7 +628,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             if (kv) mbar_arrive(&nan_full[tiles % kScSlots]);
           }
         }
-        if (t == 0 && ok) {
+        if (t == 0 && ok) {  // (between K and V no faster: 70 against 69 us for two tiles a unit)
 #pragma unroll 1
           for (int h = 0; ok && h < 2; ++h) {
             ok = warp_wait(&q_raw[h], it & 1u, abort_flag, t0, p.status, 90);
@@ -610,10 +638,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       }
     }
   } else {
+    setmaxnreg_inc<kSoftmaxRegs>();
     // -------------------------------------------------------------------- query rows
-    constexpr int NS = NG > 1 ? NG / 2 : 1;      // scale groups of a step
-    constexpr int GW = kStep / NS, CH = 4 / NS;  // their columns and maximum chains
-    constexpr int SG = 4 / NS;                   // 16-key scale entries per group
+    constexpr int GW = kBlk / NG, CH = 8 / NG;  // columns and maximum chains per scale group
+    constexpr int SG = 8 / NG;                  // 16-key scale entries per group
     const int h = wg, quad = warp & 3, rr = quad * 32 + lane;
     const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
     const uint32_t o_addr = tmem + lane_addr + kColO + 128 * h;
@@ -653,7 +681,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       return false;
     };
 
-    uint32_t t = 0, it = 0, step = 0;  // tiles, units, steps (all units)
+    const uint32_t s_addr = tmem + lane_addr + kColS + 128 * h;
+    uint32_t t = 0, it = 0;  // tiles, units
     Unit w;
     const uint32_t nan_at = sbase + offNanRow + (h * kBlk + rr) * 16;
     for (; advance(&w); ++it) {
@@ -674,35 +703,44 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       bool ok = warp_wait(&row_full[rs], (it >> 1) & 1u, abort_flag, t0, p.status, 80);
       if (!ok) break;
       const float fr = ld_shared_f32(sbase + offRow + (rs * kBlk + rr) * 4) * p.scale_log2;
-      for (int i = 0; i < w.ns; ++i, ++step) {
-        const uint32_t tt = t + (uint32_t)(i >> 1);  // key tile
-        if (!(i & 1) && !(ok = warp_wait(&sc_full[tt % kScSlots], (tt / kScSlots) & 1u, abort_flag, t0, p.status, 82))) break;
-        const uint32_t sc = sbase + offSc + (tt % kScSlots) * kScWords * 4;
+      // the keys that every row of the warp sees: tiles within them need no mask
+      const int all_lo = __reduce_max_sync(0xffffffffu, jlo), all_hi = __reduce_min_sync(0xffffffffu, jhi);
+#pragma unroll 1
+      for (int i = 0; i < w.nt; ++i, ++t) {
+        if (!(ok = warp_wait(&sc_full[t % kScSlots], (t / kScSlots) & 1u, abort_flag, t0, p.status, 82))) break;
+        const uint32_t sc = sbase + offSc + (t % kScSlots) * kScWords * 4;
         const float4 tail = ld_shared_f32x4(sc + 4 * kScTail);
-        const uint32_t sg = sc + 64 * (i & 1);  // this step's scale entries
-        const int k0 = (w.tile0 + (i >> 1)) * kBlk + kStep * (i & 1);
-        const int lo = jlo - k0, hi = jhi - 1 - k0;
-        const bool partly = __any_sync(0xffffffffu, lo > 0 || hi < kStep - 1);
-        const uint32_t buf = step & 1u;
-        const uint32_t s_addr = tmem + lane_addr + kColS + 128 * h + kStep * buf;
-        if (!(ok = warp_wait(&s_full[2 * h + buf], (step >> 1) & 1u, abort_flag, t0, p.status, 81))) break;
+        const int k0 = (w.tile0 + i) * kBlk;
+        if (!(ok = warp_wait(&s_full[h], t & 1u, abort_flag, t0, p.status, 81))) break;
         tc_fence_after();
-        uint32_t sr[kStep];
+        if (k0 < all_lo || k0 + kBlk > all_hi) {
+          // Keys that some row does not see: -inf into its scores where they lie.  (On the loaded
+          // registers the same choice cost every tile, 382 us against 337 for 16 heads, 6,016 x 6,016.)
+          const int lo = jlo - k0, hi = jhi - 1 - k0;
+#pragma unroll 1
+          for (int c = 0; c < kBlk; c += 16) {
+            uint32_t x[16];
+            tmem_ld_32x32b_x16(s_addr + c, x);
+            tmem_ld_wait();
+#pragma unroll
+            for (int q = 0; q < 16; ++q) x[q] = (c + q < lo || c + q > hi) ? 0xFF800000u : x[q];
+            tmem_st_32x32b_x16(s_addr + c, x);
+          }
+          tmem_st_wait();
+        }
+        uint32_t sr[kBlk];
         tmem_ld_32x32b_x32(s_addr + 0, *reinterpret_cast<uint32_t(*)[32]>(sr + 0));
         tmem_ld_32x32b_x32(s_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(sr + 32));
+        tmem_ld_32x32b_x32(s_addr + 64, *reinterpret_cast<uint32_t(*)[32]>(sr + 64));
+        tmem_ld_32x32b_x32(s_addr + 96, *reinterpret_cast<uint32_t(*)[32]>(sr + 96));
         tmem_ld_wait();
         float* s = reinterpret_cast<float*>(sr);
-        if (partly) {
-          // keys that this row does not see
-#pragma unroll
-          for (int c = 0; c < kStep; ++c) s[c] = (c < lo || c > hi) ? -INFINITY : s[c];
-        }
         // score factor of a group, kept within 2^+-120: a masked score times 0 would be NaN
         const auto factor_of = [&](float k) { return fminf(fmaxf(fr * k, 7.5e-37f), 1.3e36f); };
         // maxima per group, in score units and with V's exponent
         float mt = -INFINITY, Mt = -INFINITY;
 #pragma unroll
-        for (int gi = 0; gi < NS; ++gi) {
+        for (int gi = 0; gi < NG; ++gi) {
           float mc[CH];
 #pragma unroll
           for (int c = 0; c < CH; ++c) {
@@ -713,7 +751,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
           float gm = mc[0];
 #pragma unroll
           for (int c = 1; c < CH; ++c) gm = fmaxf(gm, mc[c]);
-          const float4 g4 = ld_shared_f32x4(sg + 16 * gi * SG);
+          const float4 g4 = ld_shared_f32x4(sc + 16 * gi * SG);
           const float x = gm * factor_of(g4.x);
           mt = fmaxf(mt, x + g4.w);
           Mt = fmaxf(Mt, x + g4.y);
@@ -728,10 +766,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         if (__any_sync(0xffffffffu, up || UP || far)) {
           if (up) l *= ex2(m - m1);
           if (__any_sync(0xffffffffu, UP && i > 0)) {
-            // O_h *= 2^(M - M1): once the last step's P V is done O_h is idle until P is published (the
-            // one before it is: it went ahead of this step's Q K^T, so the parity is unambiguous)
-            if (!(ok = warp_wait(&pv_done[h], (step - 1) & 1u, abort_flag, t0, p.status, 84))) break;
-            tc_fence_after();
+            // O_h *= 2^(M - M1): O_h is idle until this tile's P is published
             const float f = UP ? ex2(M - M1) : 1.0f;
 #pragma unroll 1
             for (int oc = 0; oc < 8; ++oc) {
@@ -745,15 +780,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
           }
           if (__any_sync(0xffffffffu, far)) {  // l's terms by an exponential of their own
 #pragma unroll 1
-            for (int c = 0; c < kStep; c += 16) {
+            for (int c = 0; c < kBlk; c += 16) {
               uint32_t x[16];
               tmem_ld_32x32b_x16(s_addr + c, x);
               tmem_ld_wait();
-              const float4 g4 = ld_shared_f32x4(sg + c);
+              const float4 g4 = ld_shared_f32x4(sc + c);
               const float f = factor_of(g4.x);
 #pragma unroll
-              for (int q = 0; q < 16; ++q)
-                l += c + q < lo || c + q > hi ? 0.0f : ex2(fmaf(__uint_as_float(x[q]), f, g4.w - ml));
+              for (int q = 0; q < 16; ++q) l += ex2(fmaf(__uint_as_float(x[q]), f, g4.w - ml));
             }
             lw = -INFINITY;
           }
@@ -763,12 +797,18 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         lw = ex2(lw - kBias - tail.z);  // weight of a sum at ev_0 in l
         float gf = 0.0f, gn = 0.0f, gl = 0.0f;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+        for (int c = 0; c < 4; ++c) {
+          if (c == 2) {
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&pa_full[h]);
+          }
           uint32_t pk[16];
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             if ((32 * c + 16 * half) % GW == 0) {  // the next group
-              const float4 g4 = ld_shared_f32x4(sg + 16 * ((32 * c + 16 * half) / GW) * SG);
+              const float4 g4 = ld_shared_f32x4(sc + 16 * ((32 * c + 16 * half) / GW) * SG);
               gf = factor_of(g4.x);
               gn = g4.y - mo + kBias;
               gl = lw * g4.z;
@@ -787,14 +827,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
           }
           tmem_st_32x32b_x16(s_addr + kColP + 16 * c, pk);
         }
-        const int kt = (w.tile0 + (i >> 1)) * kBlk;
-        if (kt < w.ks.lo_all || kt + kBlk > w.ks.hi_all) {  // the converters leave NaN codes of V out of such tiles
-          if (!(ok = warp_wait(&nan_full[tt % kScSlots], (tt / kScSlots) & 1u, abort_flag, t0, p.status, 83))) break;
-          const uint4 any = ld_shared_v4(sbase + offNanW + (tt % kScSlots) * 16);
+        if (k0 < w.ks.lo_all || k0 + kBlk > w.ks.hi_all) {  // the converters leave NaN codes of V out of such tiles
+          if (!(ok = warp_wait(&nan_full[t % kScSlots], (t / kScSlots) & 1u, abort_flag, t0, p.status, 83))) break;
+          const uint4 any = ld_shared_v4(sbase + offNanW + (t % kScSlots) * 16);
           if (any.x | any.y | any.z | any.w) {
             uint4 seen = ld_shared_v4(nan_at);
-            const uint32_t map = sbase + offNan + ((tt % kNanSlots) * kBlk + kStep * (i & 1)) * 16;
-            for (int c = imax(lo, 0); c <= imin(hi, kStep - 1); ++c) {
+            const uint32_t map = sbase + offNan + (t % kNanSlots) * kBlk * 16;
+#pragma unroll 1
+            for (int c = imax(jlo - k0, 0); c <= imin(jhi - 1 - k0, kBlk - 1); ++c) {
               const uint4 x = ld_shared_v4(map + c * 16);
               seen.x |= x.x;
               seen.y |= x.y;
@@ -807,9 +847,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[2 * h + buf]);
+        if (lane == 0) mbar_arrive(&pb_full[h]);
       }
-      t += w.nt;
       if (!ok) break;
       // the output row: O 2^(M - m - 6) / l, the factor in two parts that stay normal
       float fa = 0.0f, fb = 0.0f;
@@ -823,16 +862,22 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       tc_fence_after();
       const float2 a2 = make_float2(fa, fa), b2 = make_float2(fb, fb);
 #pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
-        uint32_t o[32], x[16];
-        tmem_ld_32x32b_x32(o_addr + 32 * c, o);
+      for (int c = 0; c < 2; ++c) {
+        uint32_t o[64];
+        tmem_ld_32x32b_x32(o_addr + 64 * c, *reinterpret_cast<uint32_t(*)[32]>(o));
+        tmem_ld_32x32b_x32(o_addr + 64 * c + 32, *reinterpret_cast<uint32_t(*)[32]>(o + 32));
         tmem_ld_wait();
 #pragma unroll
-        for (int q = 0; q < 16; ++q) {
-          const float2 v = mul_f2(mul_f2(make_float2(__uint_as_float(o[2 * q]), __uint_as_float(o[2 * q + 1])), a2), b2);
-          x[q] = fb == 0.0f ? 0u : pack_bf16x2(v.x, v.y);  // rows that see nothing: zeros, never 0 * NaN
+        for (int d = 0; d < 2; ++d) {
+          uint32_t x[16];
+#pragma unroll
+          for (int q = 0; q < 16; ++q) {
+            const float2 v = mul_f2(
+                mul_f2(make_float2(__uint_as_float(o[32 * d + 2 * q]), __uint_as_float(o[32 * d + 2 * q + 1])), a2), b2);
+            x[q] = fb == 0.0f ? 0u : pack_bf16x2(v.x, v.y);  // rows that see nothing: zeros, never 0 * NaN
+          }
+          if (inside) put(out + 64 * c + 32 * d, x);
         }
-        if (inside) put(out + 32 * c, x);
       }
       const uint4 nan = ld_shared_v4(nan_at);
       if ((nan.x | nan.y | nan.z | nan.w) && live) {  // channels that met a NaN of V
@@ -856,6 +901,12 @@ std::atomic<uint64_t> g_attr{0};
 
 template <int NG>
 int prepare() {
+  cudaFuncAttributes fa;
+  DEMON_CUDA(cudaFuncGetAttributes(&fa, attention_tc_kernel<NG>));
+  if (fa.numRegs != kLaunchRegs) {  // with fewer at launch the setmaxnreg.inc would never return
+    set_error("kv_attention: kernel built with %d registers per thread, the register split needs %d", fa.numRegs, kLaunchRegs);
+    return DEMON_ERR_CUDA;
+  }
   DEMON_CUDA(cudaFuncSetAttribute(attention_tc_kernel<NG>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
   return DEMON_OK;
 }
