@@ -22,9 +22,10 @@
 // Output: O * 2^(M - m - 6) / l.  Both offsets are raised only when exceeded by more than 8.
 //
 // Warp roles (512 threads):
-//   warpgroup 0 / 1   row half 0 / 1, one query row per thread: the softmax of every key tile, the
+//   warpgroup 0 / 1   row half 0 / 1, one query row per thread: its Q row in place (before the last
+//                     unit's output, so that Q K^T runs meanwhile), the softmax of every key tile, the
 //                     output row,
-//   warpgroup 2       codes -> f16, swizzled, into a ring of three K / V tiles; the Q rows in place,
+//   warpgroup 2       codes -> f16, swizzled, into a ring of three K / V tiles,
 //   warp 12           MMA issue (one thread) and tensor-memory allocation,
 //   warp 13           page look-ups, scales, bulk copies of K / V codes into a ring of half tiles,
 //   warp 14           the next unit's Q by TMA, each half as soon as the last Q K^T has read the slot,
@@ -33,9 +34,10 @@
 //
 // Bound by the softmax warps' path from S to P (some 3,000 clocks per tile and half, of which the
 // exponentials' rate asks for 1,024) and, for short key ranges (256 keys of a condition are two
-// tiles), by the units' Q conversion and output.  Measured, 16 query heads over 8: 6,016 x 6,016
-// 362 us (0.82 PFLOP/s; the bf16 kernel of attention.cu 266 us), 16 x 750 over 256 keys 69 us (bf16
-// 34 us), 6,001 causal 186 us.  Slower, not kept: steps of 64 keys with two score buffers (Q K^T 64
+// tiles), by the units' Q conversion and output (Q converted by warpgroup 2 after the unit's first
+// tile: 69 us for 16 x 750 over 256 keys against 65).  Measured, 16 query heads over 8: 6,016 x 6,016
+// 358 us (0.83 PFLOP/s; the bf16 kernel of attention.cu 264 us), 16 x 750 over 256 keys 65 us (bf16
+// 34 us), 6,001 causal 184 us.  Slower, not kept: steps of 64 keys with two score buffers (Q K^T 64
 // wide takes the tensor core longer, and the overheads of a step double: 396 us); two threads per row
 // (466 us); the next scores loaded ahead of the exponentials (509 us, they come late).
 #include <algorithm>
@@ -64,7 +66,6 @@ constexpr float kBias = 6.0f;            // P = 2^(.. + 6)
 constexpr float kRaise = 8.0f;           // offsets are raised when exceeded by more than this
 constexpr float kFast = 60.0f;           // |M - m - ev| up to which l comes from P
 
-
 // Registers per thread after the split (setmaxnreg): the launch gives 512 x 128.
 constexpr int kLaunchRegs = 128, kSoftmaxRegs = 176, kConvRegs = 80, kIssueRegs = 80;
 static_assert(256 * kSoftmaxRegs + 128 * kConvRegs + 128 * kIssueRegs <= kThreads * kLaunchRegs,
@@ -80,13 +81,12 @@ constexpr int offKV = offQ + 2 * kTile;
 constexpr int offRaw = offKV + kSlots * kTile;
 constexpr int offNan = offRaw + kRawSlots * kRaw;              // [slot][128 keys] 128-bit maps
 constexpr int offNanRow = offNan + kNanSlots * kBlk * 16;      // [2][128] 128-bit maps
-constexpr int offRow = offNanRow + 2 * kBlk * 16;              // [2 units][2 halves][128] powers of two
-constexpr int offSc = offRow + 4 * kBlk * 4;
+constexpr int offSc = offNanRow + 2 * kBlk * 16;
 constexpr int offNanW = offSc + kScSlots * kScWords * 4;       // [slot][warp] any NaN
 constexpr int offUnit = offNanW + kScSlots * 4 * 4;            // [slot] 12 words
 constexpr int offRawMask = offUnit + kUnitSlots * 48;          // [slot] 16-key groups copied
 constexpr int offBar = offRawMask + 4 * 4;
-constexpr int kNumBars = 4 + 2 * kSlots + 8 + 1 + 2 * kScSlots + 2 * kRawSlots + 6 + 2 * kUnitSlots;
+constexpr int kNumBars = 4 + 2 * kSlots + 8 + 1 + 2 * kScSlots + 2 * kRawSlots + 2 + 2 * kUnitSlots;
 constexpr int offMisc = offBar + kNumBars * 8;
 constexpr int kSmem = offMisc + 16 + 1024;
 static_assert(kSmem <= 232448, "shared memory exceeds the sm_100 per-block limit");
@@ -225,8 +225,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
   uint64_t* nan_full = sc_full + kScSlots;      // [8] NaN map of a tile
   uint64_t* raw_full = nan_full + kScSlots;     // [3] codes of a half tile copied
   uint64_t* raw_empty = raw_full + kRawSlots;   // [3] and converted
-  uint64_t* row_full = raw_empty + kRawSlots;   // [2 units][2 halves] rows' powers of two
-  uint64_t* q_raw = row_full + 4;               // [2] Q half copied
+  uint64_t* q_raw = raw_empty + kRawSlots;      // [2] Q half copied
   uint64_t* unit_full = q_raw + 2;              // [4] unit record written
   uint64_t* unit_empty = unit_full + kUnitSlots;  // [4] and read by every role
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + offMisc);
@@ -241,11 +240,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       mbar_init(&kv_empty[s], 1);
     }
     for (int h = 0; h < 2; ++h) {
-      mbar_init(&q_full[h], kConvWarps);
+      mbar_init(&q_full[h], 4);
       mbar_init(&q_empty[h], 1);
       mbar_init(&q_raw[h], 1);
-      mbar_init(&row_full[h], kConvWarps);
-      mbar_init(&row_full[2 + h], kConvWarps);
       mbar_init(&s_full[h], 1);
       mbar_init(&pa_full[h], 4);
       mbar_init(&pb_full[h], 4);
@@ -518,52 +515,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
     // neighbouring rows take opposite halves of their 128 codes (no bank conflicts either way).
     const int cw = warp & 3, c = lane & 3, rl = lane >> 2;
     const uint32_t a0 = (uint32_t)rl * 128 + (((2 * c) ^ rl) << 4), a1 = (uint32_t)rl * 128 + (((2 * c + 1) ^ rl) << 4);
-    // One row per thread in place (row 32 cw + lane): bf16 -> f16 times 2^-e
-    auto q_convert = [&](int h, uint32_t unit) {
-      const int rr = cw * 32 + lane;
-      const uint32_t base = sbase + offQ + h * kTile + rr * 128;
-      const uint32_t flip = (rr & 7) << 4;
-      uint32_t mx = 0;
-#pragma unroll 8
-      for (int k = 0; k < 16; ++k) {
-        const uint4 x = ld_shared_v4(base + (k >> 3) * kBox + ((k & 7) << 4 ^ flip));
-        mx = __vmaxu2(mx, __vmaxu2(__vmaxu2(x.x & 0x7FFF7FFFu, x.y & 0x7FFF7FFFu), __vmaxu2(x.z & 0x7FFF7FFFu, x.w & 0x7FFF7FFFu)));
-      }
-      if (__vcmpgeu2(mx, 0x7F807F80u)) {  // infinities and NaN do not count, and pass through
-        mx = 0;
-#pragma unroll 1
-        for (int k = 0; k < 16; ++k) {
-          const uint4 x = ld_shared_v4(base + (k >> 3) * kBox + ((k & 7) << 4 ^ flip));
-          const uint32_t y[4] = {x.x & 0x7FFF7FFFu, x.y & 0x7FFF7FFFu, x.z & 0x7FFF7FFFu, x.w & 0x7FFF7FFFu};
-#pragma unroll
-          for (int q = 0; q < 4; ++q) mx = __vmaxu2(mx, y[q] & __vcmpltu2(y[q], 0x7F807F80u));
-        }
-      }
-      mx = max(mx & 0xFFFFu, mx >> 16);
-      const int e = imax((int)(mx >> 7) - 127 - 13, -126);  // |q| 2^-e < 2^14
-      const float2 mul = make_float2(exp2i(-e), exp2i(-e));
-#pragma unroll 4
-      for (int k = 0; k < 16; ++k) {
-        const uint32_t a = base + (k >> 3) * kBox + ((k & 7) << 4 ^ flip);
-        const uint4 x = ld_shared_v4(a);
-        const float2 f0 = mul_f2(bf2_f2(x.x), mul), f1 = mul_f2(bf2_f2(x.y), mul), f2 = mul_f2(bf2_f2(x.z), mul),
-                     f3 = mul_f2(bf2_f2(x.w), mul);
-        st_shared_v4(a, pack_f16x2(f0.x, f0.y), pack_f16x2(f1.x, f1.y), pack_f16x2(f2.x, f2.y), pack_f16x2(f3.x, f3.y));
-      }
-      const uint32_t rs = (unit & 1) * 2 + h;
-      st_shared_f32(sbase + offRow + (rs * kBlk + rr) * 4, exp2i(e));
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&q_full[h]);
-        mbar_arrive(&row_full[rs]);
-      }
-    };
-
-    uint32_t n = 0, tiles = 0, j = 0, it = 0;
+    uint32_t n = 0, tiles = 0, j = 0;
     bool ok = true;
     Unit w;
-    for (; ok && next_unit(&j, &w); ++it) {
+    while (ok && next_unit(&j, &w)) {
       for (int t = 0; ok && t < w.nt; ++t, ++tiles) {
         const int k0 = (w.tile0 + t) * kBlk;
         const bool whole = k0 >= w.ks.lo_all && k0 + kBlk <= w.ks.hi_all;
@@ -628,13 +583,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             if (kv) mbar_arrive(&nan_full[tiles % kScSlots]);
           }
         }
-        if (t == 0 && ok) {  // (between K and V no faster: 70 against 69 us for two tiles a unit)
-#pragma unroll 1
-          for (int h = 0; ok && h < 2; ++h) {
-            ok = warp_wait(&q_raw[h], it & 1u, abort_flag, t0, p.status, 90);
-            if (ok) q_convert(h, it);
-          }
-        }
       }
     }
   } else {
@@ -682,10 +630,52 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
     };
 
     const uint32_t s_addr = tmem + lane_addr + kColS + 128 * h;
+    // This thread's row of the unit's Q in place, bf16 -> f16 times 2^-e, once the copy has landed;
+    // the score factor of the row in *f
+    auto q_convert = [&](uint32_t unit, float* f) {
+      if (!warp_wait(&q_raw[h], unit & 1u, abort_flag, t0, p.status, 90)) return false;
+      const uint32_t base = sbase + offQ + h * kTile + rr * 128;
+      const uint32_t flip = (rr & 7) << 4;
+      uint32_t mx = 0;
+#pragma unroll 8
+      for (int k = 0; k < 16; ++k) {
+        const uint4 x = ld_shared_v4(base + (k >> 3) * kBox + ((k & 7) << 4 ^ flip));
+        mx = __vmaxu2(mx, __vmaxu2(__vmaxu2(x.x & 0x7FFF7FFFu, x.y & 0x7FFF7FFFu), __vmaxu2(x.z & 0x7FFF7FFFu, x.w & 0x7FFF7FFFu)));
+      }
+      if (__vcmpgeu2(mx, 0x7F807F80u)) {  // infinities and NaN do not count, and pass through
+        mx = 0;
+#pragma unroll 1
+        for (int k = 0; k < 16; ++k) {
+          const uint4 x = ld_shared_v4(base + (k >> 3) * kBox + ((k & 7) << 4 ^ flip));
+          const uint32_t y[4] = {x.x & 0x7FFF7FFFu, x.y & 0x7FFF7FFFu, x.z & 0x7FFF7FFFu, x.w & 0x7FFF7FFFu};
+#pragma unroll
+          for (int q = 0; q < 4; ++q) mx = __vmaxu2(mx, y[q] & __vcmpltu2(y[q], 0x7F807F80u));
+        }
+      }
+      mx = max(mx & 0xFFFFu, mx >> 16);
+      const int e = imax((int)(mx >> 7) - 127 - 13, -126);  // |q| 2^-e < 2^14
+      const float2 mul = make_float2(exp2i(-e), exp2i(-e));
+#pragma unroll 4
+      for (int k = 0; k < 16; ++k) {
+        const uint32_t a = base + (k >> 3) * kBox + ((k & 7) << 4 ^ flip);
+        const uint4 x = ld_shared_v4(a);
+        const float2 f0 = mul_f2(bf2_f2(x.x), mul), f1 = mul_f2(bf2_f2(x.y), mul), f2 = mul_f2(bf2_f2(x.z), mul),
+                     f3 = mul_f2(bf2_f2(x.w), mul);
+        st_shared_v4(a, pack_f16x2(f0.x, f0.y), pack_f16x2(f1.x, f1.y), pack_f16x2(f2.x, f2.y), pack_f16x2(f3.x, f3.y));
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full[h]);
+      *f = exp2i(e) * p.scale_log2;
+      return true;
+    };
+
     uint32_t t = 0, it = 0;  // tiles, units
-    Unit w;
+    Unit w, nw;
+    float fr = 0.0f, next_fr = 0.0f;
     const uint32_t nan_at = sbase + offNanRow + (h * kBlk + rr) * 16;
-    for (; advance(&w); ++it) {
+    bool have = advance(&w) && q_convert(0, &fr);
+    for (; have; ++it) {
       int jlo = 0, jhi = w.len;  // keys that this row sees: [jlo, jhi)
       bool live;
       {
@@ -699,10 +689,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       }
       float M = -INFINITY, m = -INFINITY, l = 0.0f;
       st_shared_v4(nan_at, 0, 0, 0, 0);
-      const uint32_t rs = (it & 1) * 2 + h;
-      bool ok = warp_wait(&row_full[rs], (it >> 1) & 1u, abort_flag, t0, p.status, 80);
-      if (!ok) break;
-      const float fr = ld_shared_f32(sbase + offRow + (rs * kBlk + rr) * 4) * p.scale_log2;
+      bool ok = true;
       // the keys that every row of the warp sees: tiles within them need no mask
       const int all_lo = __reduce_max_sync(0xffffffffu, jlo), all_hi = __reduce_min_sync(0xffffffffu, jhi);
 #pragma unroll 1
@@ -850,6 +837,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         if (lane == 0) mbar_arrive(&pb_full[h]);
       }
       if (!ok) break;
+      // the next unit's Q, so that its Q K^T runs during this one's output
+      const bool more = advance(&nw);
+      if (more && !q_convert(it + 1, &next_fr)) break;
       // the output row: O 2^(M - m - 6) / l, the factor in two parts that stay normal
       float fa = 0.0f, fb = 0.0f;
       if (live && l != 0.0f) {
@@ -888,6 +878,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         }
       }
       tc_fence_before();  // O_h is read before this warp publishes the next unit's P_h
+      w = nw;
+      fr = next_fr;
+      have = more;
     }
   }
 
