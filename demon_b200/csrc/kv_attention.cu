@@ -143,7 +143,6 @@ __global__ void __launch_bounds__(Cfg<NR, RT>::kThreads) __maxnreg__((Cfg<NR, RT
   uint64_t* empty = full + kStages;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::offMisc);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint64_t t0 = globaltimer();
   const uint32_t csize = (uint32_t)p.cluster, rank = blockIdx.x % csize;  // clusters lie along x
 
   // unit: row tile fastest, then kv head, then sequence
@@ -219,7 +218,7 @@ __global__ void __launch_bounds__(Cfg<NR, RT>::kThreads) __maxnreg__((Cfg<NR, RT
       const int n_here = imin(32, n_pieces - base);
       for (int t = 0; t < n_here && ok; t += pieces) {
         const int tile = (base + t) / pieces, s = tile % kStages;
-        ok = mbar_wait(&empty[s], ((uint32_t)(tile / kStages) & 1u) ^ 1u, abort_flag, t0, p.status, 65);
+        ok = bounded_wait(&empty[s], ((uint32_t)(tile / kStages) & 1u) ^ 1u, abort_flag, p, 65);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         const bool mine = lane >= t && lane < t + pieces;
@@ -314,7 +313,7 @@ __global__ void __launch_bounds__(Cfg<NR, RT>::kThreads) __maxnreg__((Cfg<NR, RT
     bool ok = true;
     for (int t = kw >> 1; t < n_tiles; t += 2) {
       const int s = t % kStages;
-      ok = mbar_wait(&full[s], (uint32_t)(t / kStages) & 1u, abort_flag, t0, p.status, 67);
+      ok = bounded_wait(&full[s], (uint32_t)(t / kStages) & 1u, abort_flag, p, 67);
       ok = __all_sync(0xffffffffu, ok);
       __syncwarp();  // together for the MMAs
       if (!ok) break;

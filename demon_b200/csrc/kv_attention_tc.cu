@@ -115,10 +115,10 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // A warp-uniform bounded wait.  Most find their phase complete, and the cost of a completed wait
 // counts on the MMA warp's path (175 clocks each with the abort flag read every time: 439 us against
 // 402 us for 16 heads over 6,016 queries and keys), so only a wait that goes on looks at the flag.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, uint64_t t0,
-                                          unsigned int* status, unsigned int where) {
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, const AttnParams& p,
+                                          unsigned int where) {
   if (__all_sync(0xffffffffu, mbar_try_wait(smem_u32(bar), parity))) return true;
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, t0, status, where));
+  return __all_sync(0xffffffffu, bounded_wait(bar, parity, abort, p, where));
 }
 template <int N>
 __device__ __forceinline__ void setmaxnreg_inc() {
@@ -232,7 +232,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + offMisc + 4);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint64_t t0 = globaltimer();
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kSlots; ++s) {
@@ -277,7 +276,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
   // matter to the warps that write rows.
   auto next_record = [&](uint32_t* j, Unit* w) {
     const uint32_t s = *j % kUnitSlots;
-    if (!warp_wait(&unit_full[s], (*j / kUnitSlots) & 1u, abort_flag, t0, p.status, 70)) return false;
+    if (!warp_wait(&unit_full[s], (*j / kUnitSlots) & 1u, abort_flag, p, 70)) return false;
     *w = get_unit(sbase + offUnit + s * 48);
     __syncwarp();
     if (lane == 0) mbar_arrive(&unit_empty[s]);
@@ -316,7 +315,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
           }
         };
         auto wait_on = [&](uint64_t* bar, uint32_t parity, unsigned int where) {
-          const bool ok = mbar_wait(bar, parity, abort_flag, t0, p.status, where);
+          const bool ok = bounded_wait(bar, parity, abort_flag, p, where);
           tc_fence_after();
           return ok;
         };
@@ -440,7 +439,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         const int64_t src = (((int64_t)imax(pid, 0) * p.c.heads + w.hk) * p.c.P + (key & (p.c.P - 1))) * kHeadDim;
         for (int kv = 0; kv < 2; ++kv, ++n) {
           const uint32_t s = n % kRawSlots;
-          if (!(ok = warp_wait(&raw_empty[s], ((n / kRawSlots) & 1u) ^ 1u, abort_flag, t0, p.status, 77))) break;
+          if (!(ok = warp_wait(&raw_empty[s], ((n / kRawSlots) & 1u) ^ 1u, abort_flag, p, 77))) break;
           if (lane == 0) {
             st_shared_b32(sbase + offRawMask + s * 4, held);
             mbar_arrive_expect_tx(&raw_full[s], n_copies * gw * kHeadDim);
@@ -471,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       const uint32_t bytes = (uint32_t)(p.Tt * p.G) * kHeadDim * 2;
       for (; ok && next_unit(&j, &w); ++it)
         for (int h = 0; h < 2; ++h) {
-          if (!(ok = warp_wait(&q_empty[h], (it & 1u) ^ 1u, abort_flag, t0, p.status, 91))) break;
+          if (!(ok = warp_wait(&q_empty[h], (it & 1u) ^ 1u, abort_flag, p, 91))) break;
           if (lane == 0) {
             mbar_arrive_expect_tx(&q_raw[h], bytes);
             for (int box = 0; box < 2; ++box)
@@ -498,7 +497,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
           if (bad && w.hk == 0 && w.i0 == 0 && lane == 0) report(p.status, DEMON_DEV_BAD_ARG, 63);
         }
         const uint32_t s = n % kUnitSlots;
-        if (!warp_wait(&unit_empty[s], ((n / kUnitSlots) & 1u) ^ 1u, abort_flag, t0, p.status, 69)) break;
+        if (!warp_wait(&unit_empty[s], ((n / kUnitSlots) & 1u) ^ 1u, abort_flag, p, 69)) break;
         if (lane == 0) {
           put_unit(sbase + offUnit + s * 48, w);
           mbar_arrive(&unit_full[s]);
@@ -525,7 +524,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
 #pragma unroll 1
         for (int kv = 0; kv < 2; ++kv, ++n) {
           const uint32_t s = n % kRawSlots;
-          if (!(ok = warp_wait(&raw_full[s], (n / kRawSlots) & 1u, abort_flag, t0, p.status, 78))) break;
+          if (!(ok = warp_wait(&raw_full[s], (n / kRawSlots) & 1u, abort_flag, p, 78))) break;
           const uint32_t held = (ld_shared_b32(sbase + offRawMask + s * 4) >> (2 * cw)) & 3u;
           const uint32_t src = sbase + offRaw + s * kRaw + (cw * 32 + rl) * kHeadDim + 16 * c;
           uint4 r[8];
@@ -536,7 +535,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             for (int i = 0; i < 8; ++i)
               if (!((held >> (i >> 2)) & 1u)) r[i] = make_uint4(0, 0, 0, 0);
           }
-          if (!(ok = warp_wait(&kv_empty[n % kSlots], ((n / kSlots) & 1u) ^ 1u, abort_flag, t0, p.status, 86))) break;
+          if (!(ok = warp_wait(&kv_empty[n % kSlots], ((n / kSlots) & 1u) ^ 1u, abort_flag, p, 86))) break;
           if (kv && !whole) {
             // Some row does not see some key: NaN codes go into a map instead of the product.
             // (Where every row sees every key they may run through it.)
@@ -633,7 +632,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
     // This thread's row of the unit's Q in place, bf16 -> f16 times 2^-e, once the copy has landed;
     // the score factor of the row in *f
     auto q_convert = [&](uint32_t unit, float* f) {
-      if (!warp_wait(&q_raw[h], unit & 1u, abort_flag, t0, p.status, 90)) return false;
+      if (!warp_wait(&q_raw[h], unit & 1u, abort_flag, p, 90)) return false;
       const uint32_t base = sbase + offQ + h * kTile + rr * 128;
       const uint32_t flip = (rr & 7) << 4;
       uint32_t mx = 0;
@@ -694,11 +693,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       const int all_lo = __reduce_max_sync(0xffffffffu, jlo), all_hi = __reduce_min_sync(0xffffffffu, jhi);
 #pragma unroll 1
       for (int i = 0; i < w.nt; ++i, ++t) {
-        if (!(ok = warp_wait(&sc_full[t % kScSlots], (t / kScSlots) & 1u, abort_flag, t0, p.status, 82))) break;
+        if (!(ok = warp_wait(&sc_full[t % kScSlots], (t / kScSlots) & 1u, abort_flag, p, 82))) break;
         const uint32_t sc = sbase + offSc + (t % kScSlots) * kScWords * 4;
         const float4 tail = ld_shared_f32x4(sc + 4 * kScTail);
         const int k0 = (w.tile0 + i) * kBlk;
-        if (!(ok = warp_wait(&s_full[h], t & 1u, abort_flag, t0, p.status, 81))) break;
+        if (!(ok = warp_wait(&s_full[h], t & 1u, abort_flag, p, 81))) break;
         tc_fence_after();
         if (k0 < all_lo || k0 + kBlk > all_hi) {
           // Keys that some row does not see: -inf into its scores where they lie.  (On the loaded
@@ -815,7 +814,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
           tmem_st_32x32b_x16(s_addr + kColP + 16 * c, pk);
         }
         if (k0 < w.ks.lo_all || k0 + kBlk > w.ks.hi_all) {  // the converters leave NaN codes of V out of such tiles
-          if (!(ok = warp_wait(&nan_full[t % kScSlots], (t / kScSlots) & 1u, abort_flag, t0, p.status, 83))) break;
+          if (!(ok = warp_wait(&nan_full[t % kScSlots], (t / kScSlots) & 1u, abort_flag, p, 83))) break;
           const uint4 any = ld_shared_v4(sbase + offNanW + (t % kScSlots) * 16);
           if (any.x | any.y | any.z | any.w) {
             uint4 seen = ld_shared_v4(nan_at);
@@ -848,7 +847,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       }
       bool inside;
       __nv_bfloat16* out = out_row(w, &inside);
-      if (!warp_wait(&o_full[h], it & 1u, abort_flag, t0, p.status, 92)) break;
+      if (!warp_wait(&o_full[h], it & 1u, abort_flag, p, 92)) break;
       tc_fence_after();
       const float2 a2 = make_float2(fa, fa), b2 = make_float2(fb, fb);
 #pragma unroll 1

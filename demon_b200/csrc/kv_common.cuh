@@ -94,5 +94,31 @@ struct AttnParams {
   unsigned int* status;
 };
 
+// What a wait of a call may take: 2 s, and 1 us for every key of the table, some ten times what the
+// attention kernels need for the units that a warp may wait for (a cache may hold 2^30 keys).
+__device__ __forceinline__ uint64_t wait_limit(const AttnParams& p) {
+  return DEMON_WAIT_LIMIT_NS + (uint64_t)(uint32_t)p.W * (uint32_t)p.c.P * 1000u;
+}
+// mbar_wait with the time counted from this wait's own start, not the kernel's: a long call (half a
+// million tokens over as many keys take seconds) is no failure.
+__device__ __forceinline__ bool bounded_wait(uint64_t* bar, uint32_t parity, volatile int* abort, const AttnParams& p,
+                                             unsigned int where) {
+  const uint32_t a = smem_u32(bar);
+  uint64_t since = 0;
+  for (uint32_t i = 0;; ++i) {
+    if (mbar_try_wait(a, parity)) return true;
+    if ((i & 255u) == 255u) {
+      if (*abort) return false;
+      const uint64_t now = globaltimer();
+      if (since == 0) since = now;
+      if (now - since > wait_limit(p)) {
+        *abort = 1;
+        report(p.status, DEMON_DEV_TIMEOUT, where);
+        return false;
+      }
+    }
+  }
+}
+
 }  // namespace kv
 }  // namespace demon

@@ -307,6 +307,7 @@ extern "C" int demon_kv_read(const DemonKvReadArgs* a, void* stream) {
   DEMON_CHECK_ARG(a->B == 1 || (a->k_seq >= (a->max_len - 1) * a->k_row + width &&
                                 a->v_seq >= (a->max_len - 1) * a->v_row + width),
                   "kv_read: output sequences overlap");
+  DEMON_CHECK_ARG(a->k_out != a->v_out, "kv_read: k_out and v_out overlap");
   kv::ReadParams p{};
   p.c = kv_cache(&a->cache);
   p.out[0] = (__nv_bfloat16*)a->k_out;

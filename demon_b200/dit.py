@@ -103,7 +103,17 @@ class CrossCache:
     def rows(self, index) -> "CrossCache":
         """The same pages for another batch: entry i is condition ``index[i]`` (a condition may
         stand in several sequences; nothing is copied but its page numbers)."""
-        index = torch.as_tensor(index, device=self.table.device)
+        index = torch.as_tensor(index)
+        if index.dtype == torch.bool or index.dtype.is_floating_point or index.dim() != 1:
+            raise ValueError("rows: index must be a list or 1-D tensor of integers")
+        n = self.table.shape[0]
+        if index.is_cuda:  # no look at its values from here: an index out of range sees no page
+            inside = (index >= 0) & (index < n)
+            index = torch.where(inside, index, 0)
+            return CrossCache(self.cache, torch.where(inside[:, None], self.table[index], -1), self.lens[index])
+        if index.numel() and not (0 <= int(index.min()) and int(index.max()) < n):
+            raise IndexError(f"rows: index out of range for {n} conditions")
+        index = index.to(self.table.device)
         return CrossCache(self.cache, self.table[index].contiguous(), self.lens[index].contiguous())
 
 

@@ -37,9 +37,12 @@ HEAD_DIM = 128
 PAGE_SIZES = (16, 32, 64, 128)
 
 
-@dataclass
+@dataclass(frozen=True, eq=False)
 class KVCache:
-    """E4M3 codes ``k`` / ``v`` [pages, heads, page_size, 128] and scales [pages, heads]."""
+    """E4M3 codes ``k`` / ``v`` [pages, heads, page_size, 128] and scales [pages, heads].
+
+    The tensors are checked once and cannot be replaced (their contents are what append changes).
+    """
     k: torch.Tensor        # float8_e4m3fn [pages, heads, page_size, 128], contiguous
     v: torch.Tensor
     k_scale: torch.Tensor  # float32 [pages, heads], powers of two
@@ -58,11 +61,11 @@ class KVCache:
                 raise ValueError(f"cache {n} must be a contiguous float32 tensor [pages, heads]")
         if not k.is_cuda or any(t.device != k.device for t in (v, self.k_scale, self.v_scale)):
             raise ValueError("the cache's tensors must be on one CUDA device (demon_b200 has no CPU path)")
-        self._device = k.device
-        self._index = k.get_device()
-        self._heads = k.shape[1]
-        self._c = (k.data_ptr(), v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(), k.shape[0], k.shape[1],
-                   k.shape[2], HEAD_DIM, 0)
+        # what every call needs of them (frozen: set past the dataclass)
+        self.__dict__.update(
+            _device=k.device, _index=k.get_device(), _heads=k.shape[1],
+            _c=(k.data_ptr(), v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(), k.shape[0], k.shape[1],
+                k.shape[2], HEAD_DIM, 0))
 
     @classmethod
     def empty(cls, pages: int, heads: int, page_size: int = 64, device="cuda") -> "KVCache":
@@ -103,6 +106,8 @@ def _launch(index: int, stream):
     """The context a call launches in: the tensors' device current, and, when the caller names a
     stream, that stream current too (so that outputs are allocated for it)."""
     if stream is not None:
+        if stream.device_index != index:
+            raise ValueError(f"stream is on cuda:{stream.device_index}, the tensors on cuda:{index}")
         return torch.cuda.stream(stream)
     if index != torch._C._cuda_getDevice():
         return torch.cuda.device(index)
@@ -195,17 +200,18 @@ def attention(q: torch.Tensor, cache: KVCache, table: torch.Tensor, lens: torch.
     its ``q_lens[b]`` (default Sq) stands at position ``lens[b] - q_lens[b] + i``; ``causal``
     hides the keys after that position, ``window`` those farther than ``window`` from it.  Rows
     that see no key, and rows i >= ``q_lens[b]``, are zero.  ``scale`` defaults to 1 / sqrt(128).
+    ``out`` may be ``q`` itself; it must not overlap other rows of it.
     """
     dev = cache._index
     shape, qs = _bf16_rows(q, "q", dev)
-    if 0 in qs and any(n > 1 and st == 0 for n, st in zip(shape, qs)):
-        q = q.contiguous()  # broadcast queries
-        qs = _bf16_rows(q, "q", dev)[1]
     B, Sq, Hq, _ = shape
     tp, ld, W = _table(table, B, dev)
     lp = _int32(lens, "lens", B, dev)
     qp = 0 if q_lens is None else _int32(q_lens, "q_lens", B, dev)
     with _launch(dev, stream):
+        if 0 in qs and any(n > 1 and st == 0 for n, st in zip(shape, qs)):
+            q = q.contiguous()  # broadcast queries, copied on the call's own stream
+            qs = _bf16_rows(q, "q", dev)[1]
         if out is None:
             out = torch.empty(shape, dtype=torch.bfloat16, device=cache._device)
             os = (Sq * Hq * HEAD_DIM, Hq * HEAD_DIM, HEAD_DIM)

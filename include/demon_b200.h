@@ -420,7 +420,7 @@ DEMON_API int demon_kv_append(const DemonKvAppendArgs* args, void* stream);
 
 /*
  * Read back: k_out / v_out [B, max_len, heads, 128] bf16 (sequence and row pitches in elements,
- * multiples of 8; heads contiguous) = the values of positions 0 .. lens[b] - 1, zeros from there.
+ * multiples of 8; heads contiguous; not overlapping) = the values of positions 0 .. lens[b] - 1, zeros from there.
  */
 typedef struct DemonKvReadArgs {
   DemonKvCache cache;
@@ -443,7 +443,11 @@ DEMON_API int demon_kv_read(const DemonKvReadArgs* args, void* stream);
  * (causal) and |position - j| <= window (window >= 0).  o = softmax(scale * q . k) v over the
  * keys seen, zeros for a query that sees none and for rows i >= q_lens[b].  Keys that a query
  * does not see never reach it, whatever their codes (NaN included).  fp32 scores, sums and
- * accumulators; the probabilities are rounded to f16.
+ * accumulators; the probabilities are rounded to f16.  o may be q, with the same strides; it must
+ * not overlap q in another way.  Which of two kernels runs (few rows: keys split over a cluster;
+ * many: tensor cores) depends on the size of the whole call, so a sequence's result can differ in
+ * rounding with the batch; DEMON_KV_ATTENTION=small or =tc in the environment takes one of them
+ * for every call (tc up to 128 query heads per kv head).
  */
 typedef struct DemonKvAttnArgs {
   DemonKvCache cache;

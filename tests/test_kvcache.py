@@ -175,3 +175,27 @@ def test_struct_layouts_match_and_entry_points_refuse_without_a_gpu():
     for fn, args in ((lib.demon_kv_append, nat.DemonKvAppendArgs()), (lib.demon_kv_read, nat.DemonKvReadArgs()),
                      (lib.demon_kv_attention, nat.DemonKvAttnArgs())):
         assert fn(bytes(args), None) != nat.DEMON_OK and nat.last_error()
+
+
+def test_a_stream_of_another_device_is_refused():
+    from types import SimpleNamespace
+
+    from demon_b200.kvcache import _launch
+    with pytest.raises(ValueError, match="stream is on cuda:1"):
+        _launch(0, SimpleNamespace(device_index=1))
+
+
+def test_rows_of_a_condition_cache_refuses_what_is_not_a_condition():
+    from demon_b200.dit import CrossCache
+    kv = CrossCache(None, torch.arange(6, dtype=torch.int32).view(3, 2), torch.tensor([5, 6, 7], dtype=torch.int32))
+    got = kv.rows([2, 0, 0, 2])
+    assert got.table.tolist() == [[4, 5], [0, 1], [0, 1], [4, 5]] and got.lens.tolist() == [7, 5, 5, 7]
+    assert got.table.is_contiguous() and got.table.dtype == got.lens.dtype == torch.int32
+    assert kv.rows(torch.tensor([1])).lens.tolist() == [6]
+    assert kv.rows(torch.zeros(0, dtype=torch.int64)).table.shape == (0, 2)
+    for bad in ([3], [0, -1], torch.tensor([0, 7])):
+        with pytest.raises(IndexError, match="out of range"):
+            kv.rows(bad)
+    for bad in (1, [[0]], [0.5], torch.tensor([True, False, True])):
+        with pytest.raises(ValueError, match="index"):
+            kv.rows(bad)

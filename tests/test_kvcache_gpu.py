@@ -590,3 +590,93 @@ def test_empty_calls(cuda, which):
         assert not bool(kvcache.attention(queries(2, Sq, 4, cuda, 1), cache, thin, i32([0, 0], cuda)).any())
     assert not bool(kvcache.read(cache, thin, i32([0, 0], cuda), 9)[0].any())
     ok()
+
+
+def test_the_cache_keeps_the_tensors_it_checked(cuda):
+    import dataclasses
+    cache, _, _, _ = filled([40], 16, 2, cuda, 98)
+    for name in ("k", "v", "k_scale", "v_scale"):
+        with pytest.raises(dataclasses.FrozenInstanceError):
+            setattr(cache, name, getattr(cache, name).clone())
+
+
+def test_read_refuses_one_output_for_both(cuda):
+    from demon_b200 import _native as nat
+    from demon_b200 import kvcache
+    cache, _, table, _ = filled([40], 16, 2, cuda, 99)
+    x = torch.empty(1, 40, 2, 128, dtype=torch.bfloat16, device=cuda)
+    with pytest.raises(nat.DemonError, match="overlap"):
+        kvcache.read(cache, table, i32([40], cuda), 40, out=(x, x))
+
+
+def test_output_in_place_of_the_queries(cuda, which):
+    from demon_b200 import kvcache
+    lens, nq = [700, 90, 0], [1.0, 0.5, 1.0]
+    cache, _, table, _ = filled(lens, 32, 2, cuda, 100)
+    for Sq in (1, 3, 40, 300):
+        q = queries(3, Sq, 6, cuda, Sq)
+        n = i32([max(1, int(Sq * f)) for f in nq], cuda)
+        want = kvcache.attention(q, cache, table, i32(lens, cuda), causal=True, q_lens=n)
+        kvcache.attention(q, cache, table, i32(lens, cuda), causal=True, q_lens=n, out=q)
+        assert torch.equal(q, want)
+    ok()
+
+
+def test_broadcast_queries_on_another_stream(cuda, which):
+    """The copy of broadcast queries belongs to the call's stream, whatever the current one does."""
+    from demon_b200 import kvcache
+    cache, _, table, _ = filled([300, 200], 64, 2, cuda, 101)
+    lens, s = i32([300, 200], cuda), torch.cuda.Stream()
+    for Sq in (2, 200):
+        q = queries(1, Sq, 4, cuda, Sq)
+        want = kvcache.attention(q.repeat(2, 1, 1, 1), cache, table, lens)
+        torch.cuda.synchronize()
+        torch.cuda._sleep(100_000_000)   # some 50 ms
+        got = kvcache.attention(q.expand(2, -1, -1, -1), cache, table, lens, stream=s)
+        s.synchronize()
+        assert torch.equal(got, want)
+        torch.cuda.synchronize()
+    ok()
+
+
+def test_condition_rows_by_a_device_index(cuda):
+    """An index held on the device is not looked at from the host; out of range it names no page."""
+    from demon_b200 import _native as nat
+    from demon_b200 import kvcache
+    from demon_b200.dit import CrossCache
+    cache, _, table, _ = filled([60, 50], 16, 2, cuda, 102)
+    kv = CrossCache(cache, table, i32([60, 50], cuda))
+    q = queries(4, 2, 4, cuda, 1)
+    for index in ([1, 0, 0, 1], [1, 2, -1, 0]):
+        r = kv.rows(torch.tensor(index, device=cuda))
+        o = kvcache.attention(q, r.cache, r.table, r.lens)
+        bits, _ = nat.device_status()
+        assert (bits != 0) == any(i not in (0, 1) for i in index)
+        for b, i in enumerate(index):
+            if i in (0, 1):
+                one = kvcache.attention(q[b:b + 1], cache, table[i:i + 1], kv.lens[i:i + 1])
+                assert torch.equal(o[b:b + 1], one)
+            else:
+                assert not bool(o[b].any())
+    ok()
+
+
+def test_a_call_of_several_seconds(cuda):
+    """300,000 queries of 16 heads over 2^20 keys (some 3 s): no wait gives up on a long call.
+
+    The table names 8 pages again and again, so that every row equals the row over these 8 pages.
+    Tolerance: two bf16 outputs (2^-9 each, relative); the long call adds 2^16 matrix instructions
+    of 16 keys into an fp32 accumulator, each dropping at most 2^-23 of sum p |v|, and 2^13 tile
+    sums of 2^-24 into the softmax sum.
+    """
+    from demon_b200 import kvcache
+    cache, ref, table, rows = filled([1024], 128, 1, cuda, 103)
+    q = queries(1, 500, 16, cuda, 5).repeat(1, 600, 1, 1)
+    long = table[:, :8].repeat(1, 1024).contiguous()
+    o = kvcache.attention(q, cache, long, i32([1 << 20], cuda))
+    want = kvcache.attention(q[:, :500], cache, table, i32([1024], cuda)).double()
+    ok()
+    own = float(ref.values(1, rows[0], 1024).double().abs().max())
+    for i in (0, 77_500, 299_500):
+        err = (o[:, i:i + 500].double() - want).abs()
+        assert bool((err <= (2.0 ** -8 + 2.0 ** -11) * want.abs() + 2.0 ** -7 * own).all())
