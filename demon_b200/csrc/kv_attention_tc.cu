@@ -35,9 +35,9 @@
 // Bound by the softmax warps' path from S to P (some 3,000 clocks per tile and half, of which the
 // exponentials' rate asks for 1,024) and, for short key ranges (256 keys of a condition are two
 // tiles), by the units' Q conversion and output (Q converted by warpgroup 2 after the unit's first
-// tile: 69 us for 16 x 750 over 256 keys against 65).  Measured, 16 query heads over 8: 6,016 x 6,016
-// 358 us (0.83 PFLOP/s; the bf16 kernel of attention.cu 264 us), 16 x 750 over 256 keys 65 us (bf16
-// 34 us), 6,001 causal 184 us.  Slower, not kept: steps of 64 keys with two score buffers (Q K^T 64
+// tile: 69 us for 16 x 750 over 256 keys against 64).  Measured, 16 query heads over 8: 6,016 x 6,016
+// 328 to 357 us with the box (0.83 to 0.90 PFLOP/s; the bf16 kernel of attention.cu 264 us), 16 x 750 over 256 keys 64 us (bf16
+// 34 us), 6,001 causal 176 us.  Slower, not kept: steps of 64 keys with two score buffers (Q K^T 64
 // wide takes the tensor core longer, and the overheads of a step double: 396 us); two threads per row
 // (466 us); the next scores loaded ahead of the exponentials (509 us, they come late).
 #include <algorithm>
@@ -320,8 +320,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
           return ok;
         };
         // The key tiles of all units form one stream; per tile: S_0, the last tile's P_1 V, S_1, P_0 V
-        // (one half's softmax runs while the other half's products do, across units too).  A unit's
-        // first P_h V may overwrite O_h: its P_h comes from threads that have stored the last unit's rows.
+        // (one half's softmax runs while the other half's products do, across units too; P_1 V of a
+        // unit's last tile before the next unit's Q: 66.8 us against 64 for 16 x 750 over 256 keys, the
+        // halves then store their rows at the same time).  A unit's first P_h V may overwrite O_h: its
+        // P_h comes from threads that have stored the last unit's rows.
         bool ok = true, pend = false, pend_acc = false, pend_last = false;
         uint32_t pend_v = 0;
         auto flush = [&]() {  // P_1 V of the last tile
@@ -635,18 +637,19 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       if (!warp_wait(&q_raw[h], unit & 1u, abort_flag, p, 90)) return false;
       const uint32_t base = sbase + offQ + h * kTile + rr * 128;
       const uint32_t flip = (rr & 7) << 4;
+      // read once and kept: the shared memory's bandwidth is what this costs
+      uint4 x[16];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) x[k] = ld_shared_v4(base + (k >> 3) * kBox + ((k & 7) << 4 ^ flip));
       uint32_t mx = 0;
-#pragma unroll 8
-      for (int k = 0; k < 16; ++k) {
-        const uint4 x = ld_shared_v4(base + (k >> 3) * kBox + ((k & 7) << 4 ^ flip));
-        mx = __vmaxu2(mx, __vmaxu2(__vmaxu2(x.x & 0x7FFF7FFFu, x.y & 0x7FFF7FFFu), __vmaxu2(x.z & 0x7FFF7FFFu, x.w & 0x7FFF7FFFu)));
-      }
+#pragma unroll
+      for (int k = 0; k < 16; ++k)
+        mx = __vmaxu2(mx, __vmaxu2(__vmaxu2(x[k].x & 0x7FFF7FFFu, x[k].y & 0x7FFF7FFFu), __vmaxu2(x[k].z & 0x7FFF7FFFu, x[k].w & 0x7FFF7FFFu)));
       if (__vcmpgeu2(mx, 0x7F807F80u)) {  // infinities and NaN do not count, and pass through
         mx = 0;
-#pragma unroll 1
+#pragma unroll
         for (int k = 0; k < 16; ++k) {
-          const uint4 x = ld_shared_v4(base + (k >> 3) * kBox + ((k & 7) << 4 ^ flip));
-          const uint32_t y[4] = {x.x & 0x7FFF7FFFu, x.y & 0x7FFF7FFFu, x.z & 0x7FFF7FFFu, x.w & 0x7FFF7FFFu};
+          const uint32_t y[4] = {x[k].x & 0x7FFF7FFFu, x[k].y & 0x7FFF7FFFu, x[k].z & 0x7FFF7FFFu, x[k].w & 0x7FFF7FFFu};
 #pragma unroll
           for (int q = 0; q < 4; ++q) mx = __vmaxu2(mx, y[q] & __vcmpltu2(y[q], 0x7F807F80u));
         }
@@ -654,13 +657,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       mx = max(mx & 0xFFFFu, mx >> 16);
       const int e = imax((int)(mx >> 7) - 127 - 13, -126);  // |q| 2^-e < 2^14
       const float2 mul = make_float2(exp2i(-e), exp2i(-e));
-#pragma unroll 4
+#pragma unroll
       for (int k = 0; k < 16; ++k) {
-        const uint32_t a = base + (k >> 3) * kBox + ((k & 7) << 4 ^ flip);
-        const uint4 x = ld_shared_v4(a);
-        const float2 f0 = mul_f2(bf2_f2(x.x), mul), f1 = mul_f2(bf2_f2(x.y), mul), f2 = mul_f2(bf2_f2(x.z), mul),
-                     f3 = mul_f2(bf2_f2(x.w), mul);
-        st_shared_v4(a, pack_f16x2(f0.x, f0.y), pack_f16x2(f1.x, f1.y), pack_f16x2(f2.x, f2.y), pack_f16x2(f3.x, f3.y));
+        const float2 f0 = mul_f2(bf2_f2(x[k].x), mul), f1 = mul_f2(bf2_f2(x[k].y), mul), f2 = mul_f2(bf2_f2(x[k].z), mul),
+                     f3 = mul_f2(bf2_f2(x[k].w), mul);
+        st_shared_v4(base + (k >> 3) * kBox + ((k & 7) << 4 ^ flip), pack_f16x2(f0.x, f0.y), pack_f16x2(f1.x, f1.y),
+                     pack_f16x2(f2.x, f2.y), pack_f16x2(f3.x, f3.y));
       }
       fence_proxy_async_smem();
       __syncwarp();
