@@ -43,7 +43,7 @@ EXPORTED = (
     "demon_nvfp4_linear_noalloc", "demon_test_arm_gemm_stall",
     "demon_bf16_linear", "demon_adanorm_quantize", "demon_silu_mul_quantize", "demon_head_norm_rope",
     "demon_attention", "demon_attention_args_size",
-    "demon_kv_append", "demon_kv_read", "demon_kv_attention", "demon_kv_struct_sizes",
+    "demon_kv_append", "demon_kv_read", "demon_kv_attention", "demon_kv_attention_workspace", "demon_kv_struct_sizes",
 )
 
 _vp = ctypes.c_void_p
@@ -134,6 +134,7 @@ class DemonKvAttnArgs(ctypes.Structure):
         ("table", _vp), ("ld_table", _i64), ("lens", _vp), ("q_lens", _vp),
         ("B", _i32), ("Sq", _i32), ("Hq", _i32), ("W", _i32),
         ("causal", _i32), ("window", _i32), ("scale", _f32), ("reserved", _i32),
+        ("workspace", _vp), ("workspace_bytes", _i64),
     ]
 
 
@@ -184,10 +185,12 @@ def load() -> ctypes.CDLL:
         L.demon_attention.argtypes = [ctypes.POINTER(DemonAttnArgs), _vp]
         # argument blocks packed by kvcache.py (the structures above give their layout)
         L.demon_kv_append.argtypes = L.demon_kv_read.argtypes = L.demon_kv_attention.argtypes = [ctypes.c_char_p, _vp]
+        L.demon_kv_attention_workspace.argtypes = [ctypes.c_char_p]
         L.demon_kv_struct_sizes.argtypes = [ctypes.POINTER(_i64)] * 3
         for name in EXPORTED:
             getattr(L, name).restype = (_i64 if name in ("demon_nvfp4_sf_bytes", "demon_nvfp4_noalloc_scratch_bytes",
-                                                         "demon_attention_args_size") else ctypes.c_int)
+                                                         "demon_attention_args_size",
+                                                         "demon_kv_attention_workspace") else ctypes.c_int)
         g, o = _i64(), _i64()
         L.demon_struct_sizes(ctypes.byref(g), ctypes.byref(o))
         if g.value != ctypes.sizeof(DemonGemmArgs) or o.value != ctypes.sizeof(DemonOdeSlot):

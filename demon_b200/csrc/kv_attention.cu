@@ -8,8 +8,16 @@
 // range of keys in tiles of 64; one warp copies the tiles of K and V codes, as they lie in the
 // pages, into a ring in shared memory (bulk copies of a page's 2 to 8 KB, mbarriers); four warps
 // per row group each take 32 keys of every second tile.  The keys of a row tile are split over a
-// thread-block cluster, which joins its partial results through distributed shared memory: one
-// launch, no workspace.
+// thread-block cluster, which joins its partial results through distributed shared memory (one
+// launch, no workspace), or, for long tables, over as many CTAs as fill the SMs, joined by a second
+// kernel through a workspace.
+//
+// Measured, 16 query heads over 8 (G = 2): one token over 2 x 371 keys 7 us (the launch and two
+// rounds of latency); one token of 48 sequences, 452 MB of codes, 80.5 us (5.6 TB/s); one token of 16
+// sequences of 16,384 keys 91 us (5.9 TB/s); five tokens over 100,001 and 85,000 keys, 379 MB,
+// 92 us (4.1 TB/s: with 10 rows a warp's step has twice the matrix instructions for the same bytes,
+// and registers for three CTAs spill; 168 registers and two CTAs 148 against 140 us at 16 CTAs a unit,
+// six key warps a CTA 155).
 //
 // A warp's step on 32 keys, all in registers (mma.sync m16n8k16, fp32 accumulators), with the keys
 // and V's channels on the 16-wide side of the MMAs and the query rows on the 8-wide one, so that a
@@ -46,6 +54,7 @@ constexpr int kWarpKeys = 32;              // keys per warp and step
 constexpr int kHalf = kTile * kHeadDim;    // one stage's K (or V) codes, 8 KB
 constexpr int kKeyWarps = 4;               // per row group: two per tile, on alternating tiles
 constexpr float kPBias = 14.0f;            // p is scaled by 2^14 (see above)
+constexpr int kPartFloats = kHeadDim + 4;  // a partial result in the workspace: O, M, L, E, 0
 constexpr int kFoldMin = -8;               // smallest V scale, relative to e_ref, folded into P
 
 // NR: 8-row MMA tiles per warp; RT: row groups (of four warps) per CTA.
@@ -133,6 +142,19 @@ __device__ __forceinline__ float join_factor(float m, float M) {
 }
 __device__ __forceinline__ float unit_factor(int e, int E) { return e - E < -126 ? 0.0f : exp2i(imin(e - E, 0)); }
 
+// Four channels of row `grow` of the kv head's rows from its joined sums.
+__device__ __forceinline__ void store_row(const AttnParams& p, int b, int hk, int grow, int nq, int lane, float4 acc, float L,
+                                          int E) {
+  const int i = grow / p.G, gq = grow - i * p.G;
+  // L == 0: the row sees no key (a NaN score makes L NaN, and stays)
+  const float inv = (i < nq && L != 0.0f) ? 1.0f / L : 0.0f;
+  const float un = exp2i(E);
+  uint2 out = make_uint2(0u, 0u);
+  if (inv != 0.0f)
+    out = make_uint2(pack_bf16x2(acc.x * inv * un, acc.y * inv * un), pack_bf16x2(acc.z * inv * un, acc.w * inv * un));
+  *reinterpret_cast<uint2*>(p.o + b * p.o_seq + (int64_t)i * p.o_row + (int64_t)(hk * p.G + gq) * p.o_head + 4 * lane) = out;
+}
+
 template <int NR, int RT>
 __global__ void __launch_bounds__(Cfg<NR, RT>::kThreads) __maxnreg__((Cfg<NR, RT>::kRegs)) attention_small_kernel(const AttnParams p) {
   using C = Cfg<NR, RT>;
@@ -143,10 +165,11 @@ __global__ void __launch_bounds__(Cfg<NR, RT>::kThreads) __maxnreg__((Cfg<NR, RT
   uint64_t* empty = full + kStages;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::offMisc);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t csize = (uint32_t)p.cluster, rank = blockIdx.x % csize;  // clusters lie along x
+  const uint32_t csize = (uint32_t)p.cluster, parts = (uint32_t)p.parts;  // clusters lie along x
+  const uint32_t rank = blockIdx.x % parts;
 
   // unit: row tile fastest, then kv head, then sequence
-  const uint32_t unit = blockIdx.x / csize;
+  const uint32_t unit = blockIdx.x / parts;
   const int rt = (int)(unit % (uint32_t)p.n_rt);
   const uint32_t u1 = unit / (uint32_t)p.n_rt;
   const int hk = (int)(u1 % (uint32_t)p.c.heads), b = (int)(u1 / (uint32_t)p.c.heads);
@@ -161,8 +184,8 @@ __global__ void __launch_bounds__(Cfg<NR, RT>::kThreads) __maxnreg__((Cfg<NR, RT
   ks.lo = ks.hi = ks.lo_all = ks.hi_all = 0;
   if (i0 <= i1) ks = visible(i0, i1, len, nq, p.causal != 0, p.window);
   const int tile_lo = ks.lo / kTile, tile_hi = ks.hi > ks.lo ? (ks.hi + kTile - 1) / kTile : tile_lo;
-  // this CTA's tiles: an even share of the cluster's
-  const int n_all = tile_hi - tile_lo, share = n_all / (int)csize, extra = n_all - share * (int)csize;
+  // this CTA's tiles: an even share
+  const int n_all = tile_hi - tile_lo, share = n_all / (int)parts, extra = n_all - share * (int)parts;
   const int first = tile_lo + (int)rank * share + imin((int)rank, extra), n_tiles = share + ((int)rank < extra ? 1 : 0);
 
   if (threadIdx.x == 0) {
@@ -592,6 +615,12 @@ __global__ void __launch_bounds__(Cfg<NR, RT>::kThreads) __maxnreg__((Cfg<NR, RT
       acc.z = fmaf(v.z, fo, acc.z);
       acc.w = fmaf(v.w, fo, acc.w);
     }
+    if (p.ws) {
+      float* w = p.ws + (((int64_t)unit * (C::kRows * RT) + r) * parts + rank) * kPartFloats;
+      *reinterpret_cast<float4*>(w + 4 * lane) = acc;
+      if (lane == 0) *reinterpret_cast<float4*>(w + kHeadDim) = make_float4(M, L, __int_as_float(E), 0.0f);
+      continue;
+    }
     st_shared_f32x4(sbase + C::offSum + (r * kHeadDim + 4 * lane) * 4, acc.x, acc.y, acc.z, acc.w);
     if (lane == 0) {
       const uint32_t wr = sbase + C::offRow + r * 12;
@@ -600,6 +629,7 @@ __global__ void __launch_bounds__(Cfg<NR, RT>::kThreads) __maxnreg__((Cfg<NR, RT
       st_shared_f32(wr + 8, __int_as_float(E));
     }
   }
+  if (p.ws) return;  // attention_join_kernel does the rest
   if (csize > 1)
     cluster_join();
   else
@@ -626,16 +656,55 @@ __global__ void __launch_bounds__(Cfg<NR, RT>::kThreads) __maxnreg__((Cfg<NR, RT
       acc.z = fmaf(v.z, fo, acc.z);
       acc.w = fmaf(v.w, fo, acc.w);
     }
-    const int i = grow / p.G, gq = grow - i * p.G;
-    // L == 0: the row sees no key (a NaN score makes L NaN, and stays)
-    const float inv = (i < nq && L != 0.0f) ? 1.0f / L : 0.0f;
-    const float un = exp2i(E);
-    uint2 out = make_uint2(0u, 0u);
-    if (inv != 0.0f)
-      out = make_uint2(pack_bf16x2(acc.x * inv * un, acc.y * inv * un), pack_bf16x2(acc.z * inv * un, acc.w * inv * un));
-    *reinterpret_cast<uint2*>(p.o + b * p.o_seq + (int64_t)i * p.o_row + (int64_t)(hk * p.G + gq) * p.o_head + 4 * lane) = out;
+    store_row(p, b, hk, grow, nq, lane, acc, L, E);
   }
   if (csize > 1) cluster_join();  // no CTA leaves while another still reads its results
+}
+
+// The partial results of a row from the workspace: a CTA per row, its warps share the parts.
+constexpr int kJoinWarps = 8;
+__global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const AttnParams p, const int tile_rows) {
+  __shared__ float4 sums[kJoinWarps][32];
+  __shared__ float ls[kJoinWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t unit = blockIdx.x / (uint32_t)tile_rows, rt = unit % (uint32_t)p.n_rt, u1 = unit / (uint32_t)p.n_rt;
+  const int hk = (int)(u1 % (uint32_t)p.c.heads), b = (int)(u1 / (uint32_t)p.c.heads);
+  const int grow = (int)(rt * (uint32_t)tile_rows + blockIdx.x % (uint32_t)tile_rows);
+  if (grow >= p.Sq * p.G) return;
+  const float* w = p.ws + (int64_t)blockIdx.x * p.parts * kPartFloats;
+  float M = -INFINITY, L = 0.0f;
+  int E = kMinExp;
+  for (int k = lane; k < p.parts; k += 32) {
+    const float4 st = *reinterpret_cast<const float4*>(w + (int64_t)k * kPartFloats + kHeadDim);
+    M = fmaxf(M, st.x);
+    E = imax(E, __float_as_int(st.z));
+  }
+#pragma unroll
+  for (int d = 16; d >= 1; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+  E = __reduce_max_sync(0xffffffffu, E);
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+  for (int k = warp; k < p.parts; k += kJoinWarps) {
+    const float* wk = w + (int64_t)k * kPartFloats;
+    const float4 st = *reinterpret_cast<const float4*>(wk + kHeadDim), v = *reinterpret_cast<const float4*>(wk + 4 * lane);
+    const float f = join_factor(st.x, M), fo = f * unit_factor(__float_as_int(st.z), E);
+    L = fmaf(st.y, f, L);
+    acc.x = fmaf(v.x, fo, acc.x);
+    acc.y = fmaf(v.y, fo, acc.y);
+    acc.z = fmaf(v.z, fo, acc.z);
+    acc.w = fmaf(v.w, fo, acc.w);
+  }
+  sums[warp][lane] = acc;
+  if (lane == 0) ls[warp] = L;
+  __syncthreads();
+  if (warp > 0) return;
+  for (int k = 1; k < kJoinWarps; ++k) {
+    const float4 v = sums[k][lane];
+    acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+    L += ls[k];
+  }
+  bool bad = false;  // (reported by the other kernel)
+  store_row(p, b, hk, grow, p.q_lens ? clamp_len(p.q_lens[b], p.Sq, &bad) : p.Sq, lane, acc, L, E);
 }
 
 }  // namespace small
@@ -663,6 +732,45 @@ int kv_attn_check(const DemonKvAttnArgs* a) {
   return DEMON_OK;
 }
 
+// How the small kernel splits a call: `units` row tiles, the keys of each over `parts` CTAs.
+struct SmallPlan {
+  int64_t n_rt, units;
+  int cluster, parts;
+  int64_t ws_bytes;  // for partial results, 0 with a cluster
+};
+
+template <int NR, int RT>
+SmallPlan plan_small(const DemonKvAttnArgs* a, bool workspace) {
+  using C = kv::small::Cfg<NR, RT>;
+  constexpr int kRows = C::kRows * RT, kCtas = 148 * (RT == 1 ? C::kMinCtas : 2);
+  SmallPlan s{};
+  s.n_rt = ((int64_t)a->Sq * (a->Hq / a->cache.heads) + kRows - 1) / kRows;
+  s.units = (int64_t)a->B * a->cache.heads * s.n_rt;
+  int64_t keys = (int64_t)a->W * a->cache.page_size;
+  if (a->window >= 0)  // the band of a row tile's tokens
+    keys = std::min<int64_t>(keys, kRows / (a->Hq / a->cache.heads) + 2 + (a->causal ? 1LL : 2LL) * a->window);
+  const int64_t tiles = (keys + kv::small::kTile - 1) / kv::small::kTile;
+  // Keys split over a cluster as far as all CTAs are resident at once (twice over with 32 rows a CTA),
+  // two tiles or more each: with up to twice as many CTAs, 32 units of 4,096 keys take 22.3 us against
+  // 12.8.  Where nothing more fits, halves all the same: they even out sequences of different lengths
+  // (256 units of 800 to 8,192 keys 56 us, whole 82; all of 4,096 keys 65 us, whole 52).
+  s.cluster = 1;
+  while (s.cluster < 16 && s.units * s.cluster * 2 <= kCtas && tiles >= 4 * s.cluster) s.cluster *= 2;
+  if (s.cluster == 1 && s.units < kCtas && tiles >= 4) s.cluster = 2;
+  s.parts = s.cluster;
+  // Longer tables: as many parts as fill the SMs, any number, joined by a second kernel through a
+  // workspace (the cluster's power of two up to 16 against it: 64 units of 16,384 keys 64.6 and 51 us,
+  // 16 units of 100,000 keys 143 and 92 us, 4 of them 61 and 29 us; below 8,192 keys the second launch
+  // and the workspace cost what they gain).
+  const int64_t parts = s.units > 0 ? std::min<int64_t>(kCtas / s.units, tiles / 6) : 0;
+  if (workspace && tiles >= 128 && parts > s.cluster) {
+    s.cluster = 1;
+    s.parts = (int)parts;
+    s.ws_bytes = s.units * kRows * parts * kv::small::kPartFloats * 4;
+  }
+  return s;
+}
+
 template <int NR, int RT>
 int launch_small(kv::AttnParams p, const DemonKvAttnArgs* a, cudaStream_t st) {
   using C = kv::small::Cfg<NR, RT>;
@@ -675,16 +783,19 @@ int launch_small(kv::AttnParams p, const DemonKvAttnArgs* a, cudaStream_t st) {
   }
   const int64_t rows = (int64_t)a->Sq * p.G;
   DEMON_CHECK_ARG(rows < ((int64_t)1 << 31) - 64, "kv_attention: too many query rows (%lld)", (long long)rows);
-  p.n_rt = (int)((rows + C::kRows * RT - 1) / (C::kRows * RT));
-  const int64_t units = (int64_t)a->B * a->cache.heads * p.n_rt;
-  // Keys split over a cluster until some four waves of CTAs exist, at least two tiles per CTA.
-  const int64_t tiles = ((int64_t)a->W * a->cache.page_size + kv::small::kTile - 1) / kv::small::kTile;
-  int cluster = 1;
-  while (cluster < 16 && units * cluster < 148 * C::kMinCtas && tiles >= 4 * cluster) cluster *= 2;
-  DEMON_CHECK_ARG(units * cluster < ((int64_t)1 << 31), "kv_attention: too many work units (%lld)", (long long)units);
+  const SmallPlan s = plan_small<NR, RT>(a, a->workspace != nullptr);
+  DEMON_CHECK_ARG(((uintptr_t)a->workspace & 15) == 0, "kv_attention: workspace must be 16-byte aligned");
+  DEMON_CHECK_ARG(s.ws_bytes == 0 || a->workspace_bytes >= s.ws_bytes, "kv_attention: workspace of %lld bytes, %lld needed",
+                  (long long)a->workspace_bytes, (long long)s.ws_bytes);
+  p.n_rt = (int)s.n_rt;
+  const int64_t units = s.units;
+  const int cluster = s.cluster;
+  p.parts = s.parts;
+  p.ws = s.ws_bytes > 0 ? (float*)a->workspace : nullptr;
+  DEMON_CHECK_ARG(units * s.parts < ((int64_t)1 << 31), "kv_attention: too many work units (%lld)", (long long)units);
   p.cluster = cluster;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(units * cluster), 1, 1);
+  cfg.gridDim = dim3((unsigned)(units * s.parts), 1, 1);
   cfg.blockDim = dim3(C::kThreads, 1, 1);
   cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = st;
@@ -696,7 +807,41 @@ int launch_small(kv::AttnParams p, const DemonKvAttnArgs* a, cudaStream_t st) {
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 1 ? 1 : 0;
   DEMON_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
+  if (p.ws) {
+    constexpr int kRows = C::kRows * RT;
+    kv::small::attention_join_kernel<<<(unsigned)(units * kRows), kv::small::kJoinWarps * 32, 0, st>>>(p, kRows);
+    DEMON_CUDA(cudaGetLastError());
+  }
   return DEMON_OK;
+}
+
+
+enum class Kernel { kRows8, kRows16, kRows32, kTc };
+
+Kernel kernel_for(const DemonKvAttnArgs* a) {
+  const int G = a->Hq / a->cache.heads, window = a->window;
+  const int64_t rows = (int64_t)a->Sq * G;
+  // DEMON_KV_ATTENTION=small / tc takes one of the two kernels for every call (tests, measurements)
+  const char* force = std::getenv("DEMON_KV_ATTENTION");
+  const bool small_only = force && std::strcmp(force, "small") == 0;
+  if (force && std::strcmp(force, "tc") == 0 && G <= 128) return Kernel::kTc;
+  if (rows <= 8) return Kernel::kRows8;
+  if (rows <= 16) return Kernel::kRows16;
+  // More rows: the small kernel reads the keys once per 32 rows, at about 2 TB/s (60 rows, 4 x 20,000
+  // keys: 129 us; the other kernel 428 us for 80 rows of the same); the tensor-core kernel takes
+  // 2.7 us per tile of 128 keys for 256 rows on one SM (16 x 1,500 rows, 256 keys: 68 us; the small
+  // kernel 597 us).  The lesser estimate is taken, with the keys that the table covers, or those of
+  // the window.
+  if (G <= 128 && !small_only) {
+    const int tokens = 2 * (128 / G);
+    double keys = (double)a->W * a->cache.page_size;
+    if (window >= 0) keys = std::min(keys, (double)tokens + window * (a->causal ? 1.0 : 2.0));
+    const double units = (double)a->B * a->cache.heads * ((a->Sq + tokens - 1) / tokens);
+    const double us_tc = std::ceil(units / 148.0) * std::ceil(keys / 128.0) * 2.7;
+    const double us_small = (double)a->B * a->cache.heads * (double)((rows + 31) / 32) * keys * 256.0 / 2.0e6;
+    if (us_tc < us_small) return Kernel::kTc;
+  }
+  return Kernel::kRows32;
 }
 
 }  // namespace
@@ -720,26 +865,20 @@ extern "C" int demon_kv_attention(const DemonKvAttnArgs* a, void* stream) {
   p.causal = a->causal != 0, p.window = std::min(a->window, kv::kMaxTokens - 2);
   p.scale_log2 = (float)((double)a->scale * 1.4426950408889634);
   p.status = status_word();
-  const int64_t rows = (int64_t)a->Sq * p.G;
-  // DEMON_KV_ATTENTION=small / tc takes one of the two kernels for every call (tests, measurements)
-  const char* force = std::getenv("DEMON_KV_ATTENTION");
-  const bool small_only = force && std::strcmp(force, "small") == 0;
-  if (force && std::strcmp(force, "tc") == 0 && p.G <= 128) return kv::attention_tc(p, (cudaStream_t)stream);
-  if (rows <= 8) return launch_small<1, 1>(p, a, (cudaStream_t)stream);
-  if (rows <= 16) return launch_small<2, 1>(p, a, (cudaStream_t)stream);
-  // More rows: the small kernel reads the keys once per 32 rows, at about 2 TB/s (60 rows, 4 x 20,000
-  // keys: 129 us; the other kernel 428 us for 80 rows of the same); the tensor-core kernel takes
-  // 2.7 us per tile of 128 keys for 256 rows on one SM (16 x 1,500 rows, 256 keys: 68 us; the small
-  // kernel 597 us).  The lesser estimate is taken, with the keys that the table covers, or those of
-  // the window.
-  if (p.G <= 128 && !small_only) {
-    const int tokens = 2 * (128 / p.G);
-    double keys = (double)a->W * a->cache.page_size;
-    if (p.window >= 0) keys = std::min(keys, (double)tokens + p.window * (p.causal ? 1.0 : 2.0));
-    const double units = (double)a->B * a->cache.heads * ((a->Sq + tokens - 1) / tokens);
-    const double us_tc = std::ceil(units / 148.0) * std::ceil(keys / 128.0) * 2.7;
-    const double us_small = (double)a->B * a->cache.heads * (double)((rows + 31) / 32) * keys * 256.0 / 2.0e6;
-    if (us_tc < us_small) return kv::attention_tc(p, (cudaStream_t)stream);
+  switch (kernel_for(a)) {
+    case Kernel::kTc: return kv::attention_tc(p, (cudaStream_t)stream);
+    case Kernel::kRows8: return launch_small<1, 1>(p, a, (cudaStream_t)stream);
+    case Kernel::kRows16: return launch_small<2, 1>(p, a, (cudaStream_t)stream);
+    default: return launch_small<2, 2>(p, a, (cudaStream_t)stream);
   }
-  return launch_small<2, 2>(p, a, (cudaStream_t)stream);
+}
+
+extern "C" int64_t demon_kv_attention_workspace(const DemonKvAttnArgs* a) {
+  if (kv_attn_check(a) != DEMON_OK || a->B == 0 || a->Sq == 0) return 0;  // (the call itself says why)
+  switch (kernel_for(a)) {
+    case Kernel::kTc: return 0;
+    case Kernel::kRows8: return plan_small<1, 1>(a, true).ws_bytes;
+    case Kernel::kRows16: return plan_small<2, 1>(a, true).ws_bytes;
+    default: return plan_small<2, 2>(a, true).ws_bytes;
+  }
 }

@@ -90,7 +90,8 @@ struct AttnParams {
   float scale_log2;    // softmax scale * log2(e)
   int n_rt;            // row tiles (or blocks) per kv head
   int Tt;              // tokens per half block (tensor-core kernel)
-  int cluster;         // CTAs per cluster (small kernel)
+  int cluster, parts;  // CTAs per cluster, CTAs that share the keys of a row tile (small kernel)
+  float* ws;           // their partial results when parts != cluster (small kernel), else null
   unsigned int* status;
 };
 

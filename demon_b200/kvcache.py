@@ -94,12 +94,13 @@ class KVCache:
 _CACHE = "4Pq4i"
 _APPEND = struct.Struct("@" + _CACHE + "P3qP3qPqPP4i")
 _READ = struct.Struct("@" + _CACHE + "P2qP2qPqP4i")
-_ATTN = struct.Struct("@" + _CACHE + "P3qP3qPqPP4i2ifi")
+_ATTN = struct.Struct("@" + _CACHE + "P3qP3qPqPP4i2ifiPq")
 for _s, _c in ((_APPEND, nat.DemonKvAppendArgs), (_READ, nat.DemonKvReadArgs), (_ATTN, nat.DemonKvAttnArgs)):
     assert _s.size == nat.ctypes.sizeof(_c)
 
 _NO_CONTEXT = contextlib.nullcontext()
 _DEFAULT_SCALE = HEAD_DIM ** -0.5
+_WORKSPACE_TOKENS = 8_000  # tables of fewer tokens never ask for a workspace, nor the host for its size
 
 
 def _launch(index: int, stream):
@@ -219,8 +220,14 @@ def attention(q: torch.Tensor, cache: KVCache, table: torch.Tensor, lens: torch.
             oshape, os = _bf16_rows(out, "out", dev)
             if oshape != shape or any(n > 1 and st == 0 for n, st in zip(shape, os)):
                 raise ValueError(f"out must be {tuple(shape)} without overlap, got {tuple(oshape)}, strides {out.stride()}")
-        args = _ATTN.pack(*cache._c, q.data_ptr(), *qs, out.data_ptr(), *os, tp, ld, lp, qp, B, Sq, Hq, W,
-                          1 if causal else 0, -1 if window is None else min(int(window), 1 << 30),
-                          _DEFAULT_SCALE if scale is None else float(scale), 0)
+        fields = (*cache._c, q.data_ptr(), *qs, out.data_ptr(), *os, tp, ld, lp, qp, B, Sq, Hq, W,
+                  1 if causal else 0, -1 if window is None else min(int(window), 1 << 30),
+                  _DEFAULT_SCALE if scale is None else float(scale), 0)
+        args = _ATTN.pack(*fields, 0, 0)
+        if W >= _WORKSPACE_TOKENS // cache._c[6]:
+            n = nat.load().demon_kv_attention_workspace(args)
+            if n:
+                ws = torch.empty(n, dtype=torch.uint8, device=cache._device)
+                args = _ATTN.pack(*fields, ws.data_ptr(), n)
         nat.check(nat.load().demon_kv_attention(args, nat.raw_stream(dev)))
     return out

@@ -463,9 +463,18 @@ typedef struct DemonKvAttnArgs {
   int32_t causal, window; /* window -1: no band */
   float scale;
   int32_t reserved;
+  void* workspace; /* or NULL */
+  int64_t workspace_bytes;
 } DemonKvAttnArgs;
 
 DEMON_API int demon_kv_attention(const DemonKvAttnArgs* args, void* stream);
+/*
+ * Bytes of workspace (16-byte aligned, any contents, free again when the call's work on the stream is
+ * done) with which a call of few rows over a long table runs faster; 0 when none is used.  Without
+ * one (NULL) the keys are split over fewer CTAs, and the result can differ in rounding.  Looks at
+ * sizes only, not at the workspace fields.
+ */
+DEMON_API int64_t demon_kv_attention_workspace(const DemonKvAttnArgs* args);
 
 /* sizeof of the three argument structs as compiled, for binding checks. */
 DEMON_API int demon_kv_struct_sizes(int64_t* append_args, int64_t* read_args, int64_t* attn_args);

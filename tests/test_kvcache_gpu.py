@@ -680,3 +680,92 @@ def test_a_call_of_several_seconds(cuda):
     for i in (0, 77_500, 299_500):
         err = (o[:, i:i + 500].double() - want).abs()
         assert bool((err <= (2.0 ** -8 + 2.0 ** -11) * want.abs() + 2.0 ** -7 * own).all())
+
+
+def attention_args(q, cache, table, lens, out, causal, window=-1, q_lens=None):
+    from demon_b200 import _native as nat
+    from demon_b200 import kvcache
+    B, Sq, Hq, _ = q.shape
+    return nat.DemonKvAttnArgs.from_buffer_copy(kvcache._ATTN.pack(
+        *cache._c, q.data_ptr(), *q.stride()[:3], out.data_ptr(), *out.stride()[:3], table.data_ptr(), table.stride(0),
+        lens.data_ptr(), 0 if q_lens is None else q_lens.data_ptr(), B, Sq, Hq, table.shape[1], int(causal), window,
+        128 ** -0.5, 0, 0, 0))
+
+
+# rows of 8, 16 and (by the environment) 32 per unit; few enough units for a workspace
+@pytest.mark.parametrize("Sq,Hq,Hk,P,lens", [(1, 8, 2, 64, [20_001, 17_000]), (1, 1, 1, 16, [40_000]), (5, 4, 2, 128, [33_000, 0]),
+                                             (3, 12, 3, 32, [16_500]), (10, 6, 2, 64, [30_000]), (64, 1, 1, 16, [17_000])])
+def test_keys_split_over_a_workspace(cuda, Sq, Hq, Hk, P, lens):
+    from demon_b200 import _native as nat
+    cache, ref, table, rows = filled(lens, P, Hk, cuda, 104, v_scale_by=lambda i: torch.exp2((i // 2500 % 3).float() * -9))
+    q = queries(len(lens), Sq, Hq, cuda, Sq)
+    for causal, window, q_lens in ((True, None, None), (False, None, [(Sq + 1) // 2] * len(lens)), (True, 9000, None), (False, 90, None)):
+        check_attention(cuda, cache, ref, rows, table, lens, q, q_lens, causal, window, label=f"{causal} {window}")
+    # with a workspace of any contents, and without one
+    lib, n = nat.load(), i32(lens, cuda)
+    os.environ["DEMON_KV_ATTENTION"] = "small"
+    want = check_one(cuda, cache, ref, rows, table, lens, q, None, True, None, None, "chosen")
+    out = torch.empty_like(q)
+    args = attention_args(q, cache, table, n, out, True)
+    size = lib.demon_kv_attention_workspace(bytes(args))
+    assert size > 0
+    room = torch.full((size + 64,), 255, dtype=torch.uint8, device=cuda)
+    args.workspace, args.workspace_bytes = room.data_ptr(), size
+    nat.check(lib.demon_kv_attention(bytes(args), nat.stream_ptr()))
+    assert torch.equal(out, want) and bool((room[size:] == 255).all())
+    args.workspace_bytes = size - 1
+    with pytest.raises(nat.DemonError, match="workspace"):
+        nat.check(lib.demon_kv_attention(bytes(args), nat.stream_ptr()))
+    args.workspace, args.workspace_bytes = room.data_ptr() + 8, size
+    with pytest.raises(nat.DemonError, match="aligned"):
+        nat.check(lib.demon_kv_attention(bytes(args), nat.stream_ptr()))
+    args.workspace = None
+    out.fill_(3)
+    nat.check(lib.demon_kv_attention(bytes(args), nat.stream_ptr()))
+    for b, L in enumerate(lens):
+        k, v = ref.values(0, rows[b], L), ref.values(1, rows[b], L)
+        exact, own = R.attention(q[b].double(), k, v, Sq, True, None, 128 ** -0.5)
+        assert bool(((out[b].double() - exact).abs() <= R.error_bound(exact, own)).all())
+    ok()
+
+
+def test_nan_across_a_workspace_and_graphs_with_one(cuda):
+    """A NaN score or value met by one part reaches the whole row; captured calls keep workspaces of their own."""
+    from demon_b200 import kvcache
+    lens = [24_000]
+    cache, ref, table, rows = filled(lens, 64, 2, cuda, 105)
+    for kv, pos, d in ((0, 12_345, 7), (1, 20_000, 100)):
+        page, at = rows[0][pos // 64], pos % 64
+        (cache.k if kv == 0 else cache.v).view(torch.uint8)[page, kv, at, d] = 0x7F
+        ref.codes[kv, page, kv, at, d] = torch.nan
+    for Sq in (1, 6):
+        q = queries(1, Sq, 4, cuda, Sq)
+        for causal, window in ((True, None), (True, 3000), (True, 300)):
+            check_attention(cuda, cache, ref, rows, table, lens, q, None, causal, window)
+    n, q = i32(lens, cuda), queries(1, 1, 4, cuda, 9)
+    side, graphs, outs = torch.cuda.Stream(), [], []
+    for window in (2000, None):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(kvcache.attention(q, cache, table, n, causal=True, window=window))
+        graphs.append(g)
+    want = [kvcache.attention(q, cache, table, n, causal=True, window=w) for w in (2000, None)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        graphs[0].replay()
+        with torch.cuda.stream(side):
+            graphs[1].replay()
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            assert torch.equal(o.view(torch.int16), w.view(torch.int16))
+    ok()
+
+
+@pytest.mark.parametrize("Sq,Hq,Hk", [(1, 100, 1), (3, 128, 1), (2, 130, 1), (1, 200, 1), (40, 65, 1)])
+def test_many_query_heads_per_kv_head(cuda, Sq, Hq, Hk):
+    lens = [300, 77]
+    cache, ref, table, rows = filled(lens, 32, Hk, cuda, 106)
+    check_attention(cuda, cache, ref, rows, table, lens, queries(2, Sq, Hq, cuda, Sq), causal=True)
