@@ -12,12 +12,12 @@
 // launch, no workspace), or, for long tables, over as many CTAs as fill the SMs, joined by a second
 // kernel through a workspace.
 //
-// Measured, 16 query heads over 8 (G = 2): one token over 2 x 371 keys 7 us (the launch and two
-// rounds of latency); one token of 48 sequences, 452 MB of codes, 80.5 us (5.6 TB/s); one token of 16
-// sequences of 16,384 keys 91 us (5.9 TB/s); five tokens over 100,001 and 85,000 keys, 379 MB,
-// 92 us (4.1 TB/s: with 10 rows a warp's step has twice the matrix instructions for the same bytes,
-// and registers for three CTAs spill; 168 registers and two CTAs 148 against 140 us at 16 CTAs a unit,
-// six key warps a CTA 155).
+// Measured, 8 kv heads: one token (16 query heads) over 750 keys 7 us, the launch and a few rounds of
+// latency; one token of 48 sequences of up to 8,192 keys (32 query heads), 452 MB of codes, 80.5 us
+// (5.6 TB/s); one token of 16 sequences of 16,384 keys 91 us (5.9 TB/s); five tokens of two sequences
+// of up to 100,001 keys, 379 MB, 92 us (4.1 TB/s: 10 rows take twice the matrix instructions for the
+// same bytes, and registers for three CTAs an SM spill; at 16 CTAs a unit, where it took 140 us, 168
+// registers for two CTAs took 148 and six key warps a CTA 155).
 //
 // A warp's step on 32 keys, all in registers (mma.sync m16n8k16, fp32 accumulators), with the keys
 // and V's channels on the 16-wide side of the MMAs and the query rows on the 8-wide one, so that a
