@@ -54,7 +54,6 @@ constexpr int kWarpKeys = 32;              // keys per warp and step
 constexpr int kHalf = kTile * kHeadDim;    // one stage's K (or V) codes, 8 KB
 constexpr int kKeyWarps = 4;               // per row group: two per tile, on alternating tiles
 constexpr float kPBias = 14.0f;            // p is scaled by 2^14 (see above)
-constexpr int kPartFloats = kHeadDim + 4;  // a partial result in the workspace: O, M, L, E, 0
 constexpr int kFoldMin = -8;               // smallest V scale, relative to e_ref, folded into P
 
 // NR: 8-row MMA tiles per warp; RT: row groups (of four warps) per CTA.
@@ -618,7 +617,7 @@ __global__ void __launch_bounds__(Cfg<NR, RT>::kThreads) __maxnreg__((Cfg<NR, RT
     if (p.ws) {
       float* w = p.ws + (((int64_t)unit * (C::kRows * RT) + r) * parts + rank) * kPartFloats;
       *reinterpret_cast<float4*>(w + 4 * lane) = acc;
-      if (lane == 0) *reinterpret_cast<float4*>(w + kHeadDim) = make_float4(M, L, __int_as_float(E), 0.0f);
+      if (lane == 0) *reinterpret_cast<float4*>(w + kHeadDim) = make_float4(M, L, __int_as_float(E), 1.0f);
       continue;
     }
     st_shared_f32x4(sbase + C::offSum + (r * kHeadDim + 4 * lane) * 4, acc.x, acc.y, acc.z, acc.w);
@@ -687,7 +686,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const A
   for (int k = warp; k < p.parts; k += kJoinWarps) {
     const float* wk = w + (int64_t)k * kPartFloats;
     const float4 st = *reinterpret_cast<const float4*>(wk + kHeadDim), v = *reinterpret_cast<const float4*>(wk + 4 * lane);
-    const float f = join_factor(st.x, M), fo = f * unit_factor(__float_as_int(st.z), E);
+    const float f = join_factor(st.x, M), fo = f * st.w * unit_factor(__float_as_int(st.z), E);
     L = fmaf(st.y, f, L);
     acc.x = fmaf(v.x, fo, acc.x);
     acc.y = fmaf(v.y, fo, acc.y);
@@ -742,7 +741,7 @@ struct SmallPlan {
 template <int NR, int RT>
 SmallPlan plan_small(const DemonKvAttnArgs* a, bool workspace) {
   using C = kv::small::Cfg<NR, RT>;
-  constexpr int kRows = C::kRows * RT, kCtas = 148 * (RT == 1 ? C::kMinCtas : 2);
+  constexpr int kRows = C::kRows * RT;
   SmallPlan s{};
   s.n_rt = ((int64_t)a->Sq * (a->Hq / a->cache.heads) + kRows - 1) / kRows;
   s.units = (int64_t)a->B * a->cache.heads * s.n_rt;
@@ -750,10 +749,11 @@ SmallPlan plan_small(const DemonKvAttnArgs* a, bool workspace) {
   if (a->window >= 0)  // the band of a row tile's tokens
     keys = std::min<int64_t>(keys, kRows / (a->Hq / a->cache.heads) + 2 + (a->causal ? 1LL : 2LL) * a->window);
   const int64_t tiles = (keys + kv::small::kTile - 1) / kv::small::kTile;
-  // Keys split over a cluster as far as all CTAs are resident at once (twice over with 32 rows a CTA),
-  // two tiles or more each: with up to twice as many CTAs, 32 units of 4,096 keys take 22.3 us against
+  // Keys split over a cluster as far as all CTAs are resident at once (twice over with 32 rows a CTA and
+  // 8,192 keys: 24 rows of 8 ragged sequences 103 us, once 117), two tiles or more each: with up to twice as many CTAs, 32 units of 4,096 keys take 22.3 us against
   // 12.8.  Where nothing more fits, halves all the same: they even out sequences of different lengths
   // (256 units of 800 to 8,192 keys 56 us, whole 82; all of 4,096 keys 65 us, whole 52).
+  const int kCtas = 148 * (RT == 1 || tiles < 128 ? C::kMinCtas : 2);
   s.cluster = 1;
   while (s.cluster < 16 && s.units * s.cluster * 2 <= kCtas && tiles >= 4 * s.cluster) s.cluster *= 2;
   if (s.cluster == 1 && s.units < kCtas && tiles >= 4) s.cluster = 2;
@@ -766,9 +766,22 @@ SmallPlan plan_small(const DemonKvAttnArgs* a, bool workspace) {
   if (workspace && tiles >= 128 && parts > s.cluster) {
     s.cluster = 1;
     s.parts = (int)parts;
-    s.ws_bytes = s.units * kRows * parts * kv::small::kPartFloats * 4;
+    s.ws_bytes = s.units * kRows * parts * kv::kPartFloats * 4;
   }
   return s;
+}
+
+int launch_join(const kv::AttnParams& p, int64_t units, int tile_rows, cudaStream_t st) {
+  kv::small::attention_join_kernel<<<(unsigned)(units * tile_rows), kv::small::kJoinWarps * 32, 0, st>>>(p, tile_rows);
+  DEMON_CUDA(cudaGetLastError());
+  return DEMON_OK;
+}
+
+int check_workspace(const DemonKvAttnArgs* a, int64_t bytes) {
+  DEMON_CHECK_ARG(((uintptr_t)a->workspace & 15) == 0, "kv_attention: workspace must be 16-byte aligned");
+  DEMON_CHECK_ARG(a->workspace_bytes >= bytes, "kv_attention: workspace of %lld bytes, %lld needed",
+                  (long long)a->workspace_bytes, (long long)bytes);
+  return DEMON_OK;
 }
 
 template <int NR, int RT>
@@ -784,9 +797,10 @@ int launch_small(kv::AttnParams p, const DemonKvAttnArgs* a, cudaStream_t st) {
   const int64_t rows = (int64_t)a->Sq * p.G;
   DEMON_CHECK_ARG(rows < ((int64_t)1 << 31) - 64, "kv_attention: too many query rows (%lld)", (long long)rows);
   const SmallPlan s = plan_small<NR, RT>(a, a->workspace != nullptr);
-  DEMON_CHECK_ARG(((uintptr_t)a->workspace & 15) == 0, "kv_attention: workspace must be 16-byte aligned");
-  DEMON_CHECK_ARG(s.ws_bytes == 0 || a->workspace_bytes >= s.ws_bytes, "kv_attention: workspace of %lld bytes, %lld needed",
-                  (long long)a->workspace_bytes, (long long)s.ws_bytes);
+  if (s.ws_bytes > 0) {
+    const int rc = check_workspace(a, s.ws_bytes);
+    if (rc != DEMON_OK) return rc;
+  }
   p.n_rt = (int)s.n_rt;
   const int64_t units = s.units;
   const int cluster = s.cluster;
@@ -807,41 +821,78 @@ int launch_small(kv::AttnParams p, const DemonKvAttnArgs* a, cudaStream_t st) {
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 1 ? 1 : 0;
   DEMON_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
-  if (p.ws) {
-    constexpr int kRows = C::kRows * RT;
-    kv::small::attention_join_kernel<<<(unsigned)(units * kRows), kv::small::kJoinWarps * 32, 0, st>>>(p, kRows);
-    DEMON_CUDA(cudaGetLastError());
-  }
-  return DEMON_OK;
+  return p.ws ? launch_join(p, units, C::kRows * RT, st) : DEMON_OK;
 }
 
+
+// The tensor-core kernel's split: blocks of 2 Tt tokens, the keys of each over `parts` units.
+struct TcPlan {
+  int64_t blocks;
+  int parts;
+  double us;         // estimate
+  int64_t ws_bytes;  // 0 with one part
+};
+
+TcPlan plan_tc(const DemonKvAttnArgs* a, bool workspace) {
+  const int G = a->Hq / a->cache.heads, tokens = 2 * (128 / G);
+  double keys = (double)a->W * a->cache.page_size;
+  if (a->window >= 0) keys = std::min(keys, (double)tokens + a->window * (a->causal ? 1.0 : 2.0));
+  const double tiles = std::ceil(keys / 128.0);
+  TcPlan s{};
+  s.blocks = (int64_t)a->B * a->cache.heads * ((a->Sq + tokens - 1) / tokens);
+  s.parts = 1;
+  // 2.7 us per tile of 128 keys for 256 rows on one SM, 2 for a unit's start and output
+  s.us = std::ceil(s.blocks / 148.0) * (tiles * 2.7 + 2.0);
+  // Few blocks: their keys in parts of four tiles or more (512 tokens of 4 heads over 2, 20,000 keys:
+  // 151 us whole, 50 in parts), where that takes a fifth off the estimate
+  // with 4 us for the second kernel and the partial results' way through memory.
+  if (workspace && s.blocks < 148) {
+    const double whole = s.us, rows = (double)s.blocks * tokens * G;
+    for (int parts = 2; parts <= 148 / s.blocks + 1 && parts * 4 <= tiles; ++parts) {
+      const double us = std::ceil(s.blocks * parts / 148.0) * (std::ceil(tiles / parts) * 2.7 + 2.0) + 4.0 +
+                        rows * parts * (2 * kv::kPartFloats * 4) / 4e6;
+      if (us < 0.8 * whole && us < s.us) s.us = us, s.parts = parts;
+    }
+    if (s.parts > 1) s.ws_bytes = s.blocks * tokens * G * s.parts * kv::kPartFloats * 4;
+  }
+  return s;
+}
+
+int launch_tc(kv::AttnParams p, const DemonKvAttnArgs* a, cudaStream_t st) {
+  const TcPlan s = plan_tc(a, a->workspace != nullptr);
+  p.parts = s.parts;
+  if (s.ws_bytes > 0) {
+    const int rc = check_workspace(a, s.ws_bytes);
+    if (rc != DEMON_OK) return rc;
+    p.ws = (float*)a->workspace;
+  }
+  int rc = kv::attention_tc(p, st);
+  if (rc != DEMON_OK || !p.ws) return rc;
+  const int tokens = 2 * (128 / p.G);
+  p.n_rt = (p.Sq + tokens - 1) / tokens;
+  return launch_join(p, s.blocks, tokens * p.G, st);
+}
 
 enum class Kernel { kRows8, kRows16, kRows32, kTc };
 
 Kernel kernel_for(const DemonKvAttnArgs* a) {
-  const int G = a->Hq / a->cache.heads, window = a->window;
+  const int G = a->Hq / a->cache.heads;
   const int64_t rows = (int64_t)a->Sq * G;
   // DEMON_KV_ATTENTION=small / tc takes one of the two kernels for every call (tests, measurements)
   const char* force = std::getenv("DEMON_KV_ATTENTION");
-  const bool small_only = force && std::strcmp(force, "small") == 0;
   if (force && std::strcmp(force, "tc") == 0 && G <= 128) return Kernel::kTc;
   if (rows <= 8) return Kernel::kRows8;
   if (rows <= 16) return Kernel::kRows16;
-  // More rows: the small kernel reads the keys once per 32 rows, at about 2 TB/s (60 rows, 4 x 20,000
-  // keys: 129 us; the other kernel 428 us for 80 rows of the same); the tensor-core kernel takes
-  // 2.7 us per tile of 128 keys for 256 rows on one SM (16 x 1,500 rows, 256 keys: 68 us; the small
-  // kernel 597 us).  The lesser estimate is taken, with the keys that the table covers, or those of
-  // the window.
-  if (G <= 128 && !small_only) {
-    const int tokens = 2 * (128 / G);
-    double keys = (double)a->W * a->cache.page_size;
-    if (window >= 0) keys = std::min(keys, (double)tokens + window * (a->causal ? 1.0 : 2.0));
-    const double units = (double)a->B * a->cache.heads * ((a->Sq + tokens - 1) / tokens);
-    const double us_tc = std::ceil(units / 148.0) * std::ceil(keys / 128.0) * 2.7;
-    const double us_small = (double)a->B * a->cache.heads * (double)((rows + 31) / 32) * keys * 256.0 / 2.0e6;
-    if (us_tc < us_small) return Kernel::kTc;
-  }
-  return Kernel::kRows32;
+  if (G > 128 || (force && std::strcmp(force, "small") == 0)) return Kernel::kRows32;
+  // More rows: the lesser of two estimates, with the keys that the table covers, or those of the
+  // window.  The small kernel reads the keys once per 32 rows, at about 2 TB/s; the tensor-core kernel
+  // see above.  8 kv heads, both measured: 24 rows over 16,384 keys small 31 us, tc 39; 128 rows over
+  // 20,000 keys 81 and 44; 60 rows over 4 x 20,000 keys 130 and 120, 1,500 rows over 16 x 256 keys 597
+  // and 64; 2 heads, 600 rows over 4,096 keys 37 and 38; 1 head, 240 rows over 2,000 keys 22 and 32.
+  double keys = (double)a->W * a->cache.page_size;
+  if (a->window >= 0) keys = std::min(keys, 256.0 / G + a->window * (a->causal ? 1.0 : 2.0));
+  const double us_small = (double)a->B * a->cache.heads * (double)((rows + 31) / 32) * keys * 256.0 / 2.0e6;
+  return plan_tc(a, true).us < us_small ? Kernel::kTc : Kernel::kRows32;
 }
 
 }  // namespace
@@ -866,7 +917,7 @@ extern "C" int demon_kv_attention(const DemonKvAttnArgs* a, void* stream) {
   p.scale_log2 = (float)((double)a->scale * 1.4426950408889634);
   p.status = status_word();
   switch (kernel_for(a)) {
-    case Kernel::kTc: return kv::attention_tc(p, (cudaStream_t)stream);
+    case Kernel::kTc: return launch_tc(p, a, (cudaStream_t)stream);
     case Kernel::kRows8: return launch_small<1, 1>(p, a, (cudaStream_t)stream);
     case Kernel::kRows16: return launch_small<2, 1>(p, a, (cudaStream_t)stream);
     default: return launch_small<2, 2>(p, a, (cudaStream_t)stream);
@@ -876,7 +927,7 @@ extern "C" int demon_kv_attention(const DemonKvAttnArgs* a, void* stream) {
 extern "C" int64_t demon_kv_attention_workspace(const DemonKvAttnArgs* a) {
   if (kv_attn_check(a) != DEMON_OK || a->B == 0 || a->Sq == 0) return 0;  // (the call itself says why)
   switch (kernel_for(a)) {
-    case Kernel::kTc: return 0;
+    case Kernel::kTc: return plan_tc(a, true).ws_bytes;
     case Kernel::kRows8: return plan_small<1, 1>(a, true).ws_bytes;
     case Kernel::kRows16: return plan_small<2, 1>(a, true).ws_bytes;
     default: return plan_small<2, 2>(a, true).ws_bytes;

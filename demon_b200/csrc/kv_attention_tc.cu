@@ -4,7 +4,8 @@
 // The same function as the small kernel in kv_attention.cu (rows, masks, empty rows, NaN).  Work
 // unit: one (sequence, kv head, block of 2 Tt query tokens), Tt = floor(128 / G): each half of the
 // block is Tt tokens times the G query heads of the kv head, up to 128 rows of a tile.  The two
-// halves share every K / V tile of 128 keys.  Persistent CTAs (one per SM), blocks with the most
+// halves share every K / V tile of 128 keys.  Few blocks over long keys: a block's keys are several
+// units, whose partial results the join kernel of kv_attention.cu puts together.  Persistent CTAs (one per SM), blocks with the most
 // keys (the last of a causal prompt) first.
 //
 // Operands.  The codes go from their pages through registers into shared memory as f16, which
@@ -163,6 +164,7 @@ struct Unit {
   int i0;           // first token of the block
   Keys ks;          // keys that some / every row of the block sees
   int tile0, nt;    // key tiles; nt 0: no keys (its rows are zeros), nt -1: no more units
+  int part;         // of the parts that share the block's keys
 };
 
 // The j-th unit of this CTA: rounds go over the CTAs in turn, back and forth, since the units
@@ -172,8 +174,9 @@ __device__ __forceinline__ uint32_t unit_index(uint32_t j) {
 }
 __device__ __forceinline__ Unit decode(const AttnParams& p, uint32_t u, bool* bad) {
   Unit w;
-  const uint32_t bh = (uint32_t)p.B * (uint32_t)p.c.heads;
-  const uint32_t q = u / bh, r = u - q * bh;
+  const uint32_t bh = (uint32_t)p.B * (uint32_t)p.c.heads, block = u / (uint32_t)p.parts;
+  const uint32_t q = block / bh, r = block - q * bh;
+  w.part = (int)(u - block * (uint32_t)p.parts);
   w.b = (int)(r / (uint32_t)p.c.heads);
   w.hk = (int)(r - (uint32_t)w.b * (uint32_t)p.c.heads);
   w.i0 = (p.n_rt - 1 - (int)q) * 2 * p.Tt;
@@ -184,24 +187,31 @@ __device__ __forceinline__ Unit decode(const AttnParams& p, uint32_t u, bool* ba
   if (w.i0 <= i1) w.ks = visible(w.i0, i1, w.len, w.nq, p.causal != 0, p.window);
   w.tile0 = w.ks.lo / kBlk;
   w.nt = w.ks.hi > w.ks.lo ? (w.ks.hi + kBlk - 1) / kBlk - w.tile0 : 0;
+  if (p.parts > 1) {  // an even share of the tiles
+    const int share = w.nt / p.parts, extra = w.nt - share * p.parts;
+    w.tile0 += w.part * share + imin(w.part, extra);
+    w.nt = share + (w.part < extra ? 1 : 0);
+  }
   return w;
 }
 // A unit's record in shared memory.
 __device__ __forceinline__ void put_unit(uint32_t a, const Unit& w) {
   st_shared_v4(a, w.b, w.hk, w.len, w.nq);
   st_shared_v4(a + 16, w.i0, w.ks.lo, w.ks.hi, w.ks.lo_all);
-  st_shared_v4(a + 32, w.ks.hi_all, w.tile0, w.nt, 0);
+  st_shared_v4(a + 32, w.ks.hi_all, w.tile0, w.nt, w.part);
 }
 __device__ __forceinline__ Unit get_unit(uint32_t a) {
   const uint4 x = ld_shared_v4(a), y = ld_shared_v4(a + 16), z = ld_shared_v4(a + 32);
   Unit w;
   w.b = (int)x.x, w.hk = (int)x.y, w.len = (int)x.z, w.nq = (int)x.w;
   w.i0 = (int)y.x, w.ks.lo = (int)y.y, w.ks.hi = (int)y.z, w.ks.lo_all = (int)y.w;
-  w.ks.hi_all = (int)z.x, w.tile0 = (int)z.y, w.nt = (int)z.z;
+  w.ks.hi_all = (int)z.x, w.tile0 = (int)z.y, w.nt = (int)z.z, w.part = (int)z.w;
   return w;
 }
 
-template <int NG>  // 16-key-or-larger groups of a tile with a scale of their own: 128 / min(P, 128)
+// NG: 16-key-or-larger groups of a tile with a scale of their own, 128 / min(P, 128).  Split: partial
+// results to the workspace (a variant of its own: the branch costs the other 5 % in registers).
+template <int NG, bool kSplit>
 __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const AttnParams p,
                                                                     const uint32_t units, const int wide) {
   extern __shared__ uint8_t smem_raw[];
@@ -614,6 +624,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         for (int q = 0; q < 4; ++q) st_global_v4(o + 8 * q, make_uint4(x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]));
       }
     };
+    // the same row's place in the workspace, when several parts share a block's keys
+    auto part_row = [&](const Unit& w, bool* inside) {
+      const int rows = p.Tt * p.G;  // of a half
+      *inside = ri < p.Tt && token_of(w) < p.Sq;
+      const int64_t block = ((int64_t)w.b * p.c.heads + w.hk) * p.n_rt + w.i0 / (2 * p.Tt);
+      return p.ws + ((block * 2 * rows + h * rows + rr) * p.parts + w.part) * kPartFloats;
+    };
     // the next unit; rows of units without keys are zeroed on the way
     uint32_t j = 0;
     auto advance = [&](Unit* w) {
@@ -621,6 +638,15 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         if (w->nt > 0) return true;
         const uint32_t zero[16] = {};
         bool inside;
+        if (kSplit) {  // a part that weighs nothing
+          float* o = part_row(*w, &inside);
+          if (inside) {
+#pragma unroll 1
+            for (int c = 0; c < kHeadDim; c += 4) *reinterpret_cast<float4*>(o + c) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            *reinterpret_cast<float4*>(o + kHeadDim) = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+          }
+          continue;
+        }
         __nv_bfloat16* o = out_row(*w, &inside);
         if (inside) {
 #pragma unroll 1
@@ -849,6 +875,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       }
       bool inside;
       __nv_bfloat16* out = out_row(w, &inside);
+      float* part = kSplit ? part_row(w, &inside) : nullptr;
       if (!warp_wait(&o_full[h], it & 1u, abort_flag, p, 92)) break;
       tc_fence_after();
       const float2 a2 = make_float2(fa, fa), b2 = make_float2(fb, fb);
@@ -866,8 +893,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             const float2 v = mul_f2(
                 mul_f2(make_float2(__uint_as_float(o[32 * d + 2 * q]), __uint_as_float(o[32 * d + 2 * q + 1])), a2), b2);
             x[q] = fb == 0.0f ? 0u : pack_bf16x2(v.x, v.y);  // rows that see nothing: zeros, never 0 * NaN
+            if (kSplit) {
+              if (inside)
+                *reinterpret_cast<float2*>(part + 64 * c + 32 * d + 2 * q) = fb == 0.0f ? make_float2(0.0f, 0.0f) : v;
+            }
           }
-          if (inside) put(out + 64 * c + 32 * d, x);
+          if (inside && !kSplit) put(out + 64 * c + 32 * d, x);
         }
       }
       const uint4 nan = ld_shared_v4(nan_at);
@@ -875,9 +906,16 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
 #pragma unroll 1
         for (int d = 0; d < kHeadDim; ++d) {
           const uint32_t bits = d < 32 ? nan.x : d < 64 ? nan.y : d < 96 ? nan.z : nan.w;
-          if ((bits >> (d & 31)) & 1u) reinterpret_cast<unsigned short*>(out)[d] = 0x7FFF;
+          if ((bits >> (d & 31)) & 1u) {
+            if (kSplit)
+              part[d] = __int_as_float(0x7FFFFFFF);
+            else
+              reinterpret_cast<unsigned short*>(out)[d] = 0x7FFF;
+          }
         }
       }
+      if (kSplit && inside)  // the part's own output, and what it weighs: l 2^m
+        *reinterpret_cast<float4*>(part + kHeadDim) = fb == 0.0f ? make_float4(-INFINITY, 0.0f, 0.0f, 0.0f) : make_float4(m, l, 0.0f, l);
       tc_fence_before();  // O_h is read before this warp publishes the next unit's P_h
       w = nw;
       fr = next_fr;
@@ -891,18 +929,28 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
   if (warp == 12) tmem_dealloc(tmem, kTmemCols);
 }
 
-std::atomic<uint64_t> g_attr{0};
+template <int NG, bool kSplit>
+int launch(const CUtensorMap& tq, const AttnParams& p, uint32_t units, int wide, unsigned grid, cudaStream_t st) {
+  static std::atomic<uint64_t> done{0};
+  const auto kernel = attention_tc_kernel<NG, kSplit>;
+  if (device_pending(done)) {
+    cudaFuncAttributes fa;
+    DEMON_CUDA(cudaFuncGetAttributes(&fa, kernel));
+    if (fa.numRegs != kLaunchRegs) {  // with fewer at launch the setmaxnreg.inc would never return
+      set_error("kv_attention: kernel built with %d registers per thread, the register split needs %d", fa.numRegs, kLaunchRegs);
+      return DEMON_ERR_CUDA;
+    }
+    DEMON_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    mark_device_done(done);
+  }
+  kernel<<<grid, kThreads, kSmem, st>>>(tq, p, units, wide);
+  DEMON_CUDA(cudaGetLastError());
+  return DEMON_OK;
+}
 
 template <int NG>
-int prepare() {
-  cudaFuncAttributes fa;
-  DEMON_CUDA(cudaFuncGetAttributes(&fa, attention_tc_kernel<NG>));
-  if (fa.numRegs != kLaunchRegs) {  // with fewer at launch the setmaxnreg.inc would never return
-    set_error("kv_attention: kernel built with %d registers per thread, the register split needs %d", fa.numRegs, kLaunchRegs);
-    return DEMON_ERR_CUDA;
-  }
-  DEMON_CUDA(cudaFuncSetAttribute(attention_tc_kernel<NG>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
-  return DEMON_OK;
+int launch(const CUtensorMap& tq, const AttnParams& p, uint32_t units, int wide, unsigned grid, cudaStream_t st) {
+  return p.ws ? launch<NG, true>(tq, p, units, wide, grid, st) : launch<NG, false>(tq, p, units, wide, grid, st);
 }
 
 }  // namespace tc
@@ -911,34 +959,25 @@ int attention_tc(AttnParams p, cudaStream_t st) {
   using namespace tc;
   p.Tt = kBlk / p.G;
   p.n_rt = (p.Sq + 2 * p.Tt - 1) / (2 * p.Tt);
-  const int64_t units = (int64_t)p.n_rt * p.B * p.c.heads;
+  const int64_t units = (int64_t)p.n_rt * p.B * p.c.heads * p.parts;
   DEMON_CHECK_ARG(units < ((int64_t)1 << 31), "kv_attention: too many work units (%lld)", (long long)units);
   CUtensorMap tq;
   const int rc0 = make_tmap_4d_bf16(&tq, p.q, {kHeadDim, (uint64_t)p.Hq, (uint64_t)p.Sq, (uint64_t)p.B},
                                     {(uint64_t)p.q_head * 2, (uint64_t)p.q_row * 2, (uint64_t)p.q_seq * 2},
                                     {64, (uint32_t)p.G, (uint32_t)p.Tt, 1});
   if (rc0 != DEMON_OK) return rc0;
-  if (device_pending(g_attr)) {
-    int rc = prepare<1>();
-    if (rc == DEMON_OK) rc = prepare<2>();
-    if (rc == DEMON_OK) rc = prepare<4>();
-    if (rc == DEMON_OK) rc = prepare<8>();
-    if (rc != DEMON_OK) return rc;
-    mark_device_done(g_attr);
-  }
   int dev = 0, sms = 148;
   DEMON_CUDA(cudaGetDevice(&dev));
   DEMON_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
   const unsigned grid = (unsigned)std::min<int64_t>(units, sms);
   const int wide = ((uintptr_t)p.o & 31) == 0 && p.o_seq % 16 == 0 && p.o_row % 16 == 0 && p.o_head % 16 == 0;
+  const uint32_t n = (uint32_t)units;
   switch (p.c.P) {
-    case 16: attention_tc_kernel<8><<<grid, kThreads, kSmem, st>>>(tq, p, (uint32_t)units, wide); break;
-    case 32: attention_tc_kernel<4><<<grid, kThreads, kSmem, st>>>(tq, p, (uint32_t)units, wide); break;
-    case 64: attention_tc_kernel<2><<<grid, kThreads, kSmem, st>>>(tq, p, (uint32_t)units, wide); break;
-    default: attention_tc_kernel<1><<<grid, kThreads, kSmem, st>>>(tq, p, (uint32_t)units, wide); break;
+    case 16: return launch<8>(tq, p, n, wide, grid, st);
+    case 32: return launch<4>(tq, p, n, wide, grid, st);
+    case 64: return launch<2>(tq, p, n, wide, grid, st);
+    default: return launch<1>(tq, p, n, wide, grid, st);
   }
-  DEMON_CUDA(cudaGetLastError());
-  return DEMON_OK;
 }
 
 }  // namespace kv

@@ -76,6 +76,10 @@ __device__ __forceinline__ void st_shared_f32x4(uint32_t a, float x, float y, fl
   asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(a), "f"(x), "f"(y), "f"(z), "f"(w) : "memory");
 }
 
+// A partial result of a row in the workspace: O [128], then the maximum m (log2 units) and the sum l
+// (in units of 2^m), the exponent that O is held in units of, and O's weight beside 2^m.
+constexpr int kPartFloats = kHeadDim + 4;
+
 // One attention call, as both attention kernels see it.
 struct AttnParams {
   Cache c;
@@ -90,8 +94,9 @@ struct AttnParams {
   float scale_log2;    // softmax scale * log2(e)
   int n_rt;            // row tiles (or blocks) per kv head
   int Tt;              // tokens per half block (tensor-core kernel)
-  int cluster, parts;  // CTAs per cluster, CTAs that share the keys of a row tile (small kernel)
-  float* ws;           // their partial results when parts != cluster (small kernel), else null
+  int cluster;         // CTAs per cluster (small kernel)
+  int parts;           // parts that share the keys of a row tile (or block)
+  float* ws;           // their partial results, joined by attention_join_kernel; null: none
   unsigned int* status;
 };
 

@@ -769,3 +769,38 @@ def test_many_query_heads_per_kv_head(cuda, Sq, Hq, Hk):
     lens = [300, 77]
     cache, ref, table, rows = filled(lens, 32, Hk, cuda, 106)
     check_attention(cuda, cache, ref, rows, table, lens, queries(2, Sq, Hq, cuda, Sq), causal=True)
+
+
+@pytest.mark.parametrize("Sq,Hq,Hk,P,lens", [(40, 4, 2, 64, [5000, 3100]), (130, 8, 1, 16, [4000]), (300, 2, 2, 128, [9000, 0]),
+                                             (70, 3, 1, 32, [1300]), (33, 100, 1, 64, [2200])])
+def test_blocks_of_rows_split_over_a_workspace(cuda, Sq, Hq, Hk, P, lens):
+    """The tensor-core kernel with few blocks: parts of their keys, some of which a row does not see."""
+    from demon_b200 import _native as nat
+    cache, ref, table, rows = filled(lens, P, Hk, cuda, 107, v_scale_by=lambda i: torch.exp2((i // 700 % 3).float() * -11))
+    page = rows[0][1000 // P]
+    cache.v.view(torch.uint8)[page, 0, 1000 % P, 5] = 0xFF      # one NaN of V, one of K
+    ref.codes[1, page, 0, 1000 % P, 5] = torch.nan
+    q = queries(len(lens), Sq, Hq, cuda, Sq)
+    for causal, window, q_lens in ((True, None, None), (False, None, [Sq - 7] * len(lens)), (True, 700, None), (False, 2000, None)):
+        check_attention(cuda, cache, ref, rows, table, lens, q, q_lens, causal, window, label=f"{causal} {window}")
+    page = rows[0][1100 // P]
+    cache.k.view(torch.uint8)[page, 0, 1100 % P, 50] = 0x7F
+    ref.codes[0, page, 0, 1100 % P, 50] = torch.nan
+    for causal, window in ((True, None), (True, 150)):
+        check_attention(cuda, cache, ref, rows, table, lens, q, None, causal, window, label=f"NaN {causal} {window}")
+    os.environ["DEMON_KV_ATTENTION"] = "tc"
+    n, out = i32(lens, cuda), torch.empty_like(q)
+    args = attention_args(q, cache, table, n, out, True)
+    size = nat.load().demon_kv_attention_workspace(bytes(args))
+    assert size > 0
+    want = check_one(cuda, cache, ref, rows, table, lens, q, None, True, None, None, "chosen")
+    room = torch.full((size + 64,), 255, dtype=torch.uint8, device=cuda)
+    args.workspace, args.workspace_bytes = room.data_ptr(), size
+    nat.check(nat.load().demon_kv_attention(bytes(args), nat.stream_ptr()))
+    assert torch.equal(out.view(torch.int16), want.view(torch.int16)) and bool((room[size:] == 255).all())
+    args.workspace = None
+    nat.check(nat.load().demon_kv_attention(bytes(args), nat.stream_ptr()))
+    ok()
+    args.workspace, args.workspace_bytes = room.data_ptr(), size - 1
+    with pytest.raises(nat.DemonError, match="workspace"):
+        nat.check(nat.load().demon_kv_attention(bytes(args), nat.stream_ptr()))
