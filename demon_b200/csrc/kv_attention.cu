@@ -685,9 +685,11 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const A
 #pragma unroll 4
   for (int k = warp; k < p.parts; k += kJoinWarps) {
     const float* wk = w + (int64_t)k * kPartFloats;
-    const float4 st = *reinterpret_cast<const float4*>(wk + kHeadDim), v = *reinterpret_cast<const float4*>(wk + 4 * lane);
+    const float4 st = *reinterpret_cast<const float4*>(wk + kHeadDim);
     const float f = join_factor(st.x, M), fo = f * st.w * unit_factor(__float_as_int(st.z), E);
     L = fmaf(st.y, f, L);
+    if (st.x == -INFINITY) continue;  // no key seen (and O perhaps not written)
+    const float4 v = *reinterpret_cast<const float4*>(wk + 4 * lane);
     acc.x = fmaf(v.x, fo, acc.x);
     acc.y = fmaf(v.y, fo, acc.y);
     acc.z = fmaf(v.z, fo, acc.z);

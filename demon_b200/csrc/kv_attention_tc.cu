@@ -5,8 +5,8 @@
 // unit: one (sequence, kv head, block of 2 Tt query tokens), Tt = floor(128 / G): each half of the
 // block is Tt tokens times the G query heads of the kv head, up to 128 rows of a tile.  The two
 // halves share every K / V tile of 128 keys.  Few blocks over long keys: a block's keys are several
-// units, whose partial results the join kernel of kv_attention.cu puts together.  Persistent CTAs (one per SM), blocks with the most
-// keys (the last of a causal prompt) first.
+// units, whose partial results the join kernel of kv_attention.cu puts together.  Persistent CTAs (one
+// per SM), blocks with the most keys (the last of a causal prompt) first.
 //
 // Operands.  The codes go from their pages through registers into shared memory as f16, which
 // holds every E4M3 value: one conversion instruction per two codes, so that the scales stay out
@@ -37,10 +37,11 @@
 // exponentials' rate asks for 1,024) and, for short key ranges (256 keys of a condition are two
 // tiles), by the units' Q conversion and output (Q converted by warpgroup 2 after the unit's first
 // tile: 69 us for 16 x 750 over 256 keys against 64).  Measured, 16 query heads over 8: 6,016 x 6,016
-// 328 to 357 us with the box (0.83 to 0.90 PFLOP/s; the bf16 kernel of attention.cu 264 us), 16 x 750 over 256 keys 64 us (bf16
-// 34 us), 6,001 causal 176 us.  Slower, not kept: steps of 64 keys with two score buffers (Q K^T 64
-// wide takes the tensor core longer, and the overheads of a step double: 396 us); two threads per row
-// (466 us); the next scores loaded ahead of the exponentials (509 us, they come late).
+// 328 to 349 us (0.85 to 0.90 PFLOP/s; the bf16 kernel of attention.cu 264 us), 16 x 750 over 256 keys
+// 64 us (bf16 34 us), 6,001 causal 176 to 181 us.  Slower, not kept: steps of 64 keys with two score
+// buffers (Q K^T 64 wide takes the tensor core longer, and the overheads of a step double: 396 us at
+// 6,016 x 6,016); two threads per row (466 us); the next scores loaded ahead of the exponentials
+// (509 us, they come late).
 #include <algorithm>
 
 #include "demon_host.h"
@@ -163,7 +164,7 @@ struct Unit {
   int b, hk, len, nq;
   int i0;           // first token of the block
   Keys ks;          // keys that some / every row of the block sees
-  int tile0, nt;    // key tiles; nt 0: no keys (its rows are zeros), nt -1: no more units
+  int tile0, nt;    // key tiles; nt 0: no keys (warp 15 writes its zeros, no record), nt -1: no more units
   int part;         // of the parts that share the block's keys
 };
 
@@ -282,9 +283,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
   const int wg = warp >> 2;
-  // The next unit for this warp (*j counts records); false at the end.  Units without keys only
-  // matter to the warps that write rows.
-  auto next_record = [&](uint32_t* j, Unit* w) {
+  // The next unit for this warp (*j counts records); false at the end.  Records are of units with keys
+  // alone: warp 13 waits for the next unit's before it copies the last tile of its own, and the softmax
+  // warps read on only after that tile, so a run of empty records longer than the ring would stop both.
+  auto next_unit = [&](uint32_t* j, Unit* w) {
     const uint32_t s = *j % kUnitSlots;
     if (!warp_wait(&unit_full[s], (*j / kUnitSlots) & 1u, abort_flag, p, 70)) return false;
     *w = get_unit(sbase + offUnit + s * 48);
@@ -292,12 +294,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
     if (lane == 0) mbar_arrive(&unit_empty[s]);
     ++*j;
     return w->nt >= 0;
-  };
-  auto next_unit = [&](uint32_t* j, Unit* w) {
-    do {
-      if (!next_record(j, w)) return false;
-    } while (w->nt == 0);
-    return true;
   };
 
   if (wg == 3) {
@@ -356,7 +352,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
             flush();
             break;
           }
-          if (nt == 0) continue;
           if (!(ok = wait_on(&q_full[0], it & 1u, 75) && wait_on(&kv_full[g % kSlots], (g / kSlots) & 1u, 71))) break;
 #pragma unroll 1
           for (int i = 0; i < nt; ++i) {
@@ -498,6 +493,24 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       __syncwarp();
     } else {
       // ------------------------------------------------------------------ units
+      // a unit without keys: its rows are zeros, or partial results that weigh nothing
+      auto empty_unit = [&](const Unit& u) {
+        const int rows = 2 * p.Tt * p.G;
+        if constexpr (kSplit) {
+          const int64_t block = ((int64_t)u.b * p.c.heads + u.hk) * p.n_rt + u.i0 / (2 * p.Tt);
+          for (int r = lane; r < rows && u.i0 + r / p.G < p.Sq; r += 32)
+            *reinterpret_cast<float4*>(p.ws + ((block * rows + r) * p.parts + u.part) * kPartFloats + kHeadDim) =
+                make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+        } else {
+          for (int r = lane >> 4; r < rows; r += 2) {
+            const int i = u.i0 + r / p.G;
+            if (i >= p.Sq) break;
+            st_global_v4(p.o + u.b * p.o_seq + (int64_t)i * p.o_row + (int64_t)(u.hk * p.G + r % p.G) * p.o_head + (lane & 15) * 8,
+                         make_uint4(0, 0, 0, 0));
+          }
+        }
+        __syncwarp();
+      };
       for (uint32_t j = 0, n = 0;; ++j) {
         bool bad = false;
         Unit w;
@@ -507,6 +520,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
           if (u >= units) continue;
           w = decode(p, u, &bad);
           if (bad && w.hk == 0 && w.i0 == 0 && lane == 0) report(p.status, DEMON_DEV_BAD_ARG, 63);
+          if (w.nt == 0) {
+            empty_unit(w);
+            continue;
+          }
         }
         const uint32_t s = n % kUnitSlots;
         if (!warp_wait(&unit_empty[s], ((n / kUnitSlots) & 1u) ^ 1u, abort_flag, p, 69)) break;
@@ -631,31 +648,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       const int64_t block = ((int64_t)w.b * p.c.heads + w.hk) * p.n_rt + w.i0 / (2 * p.Tt);
       return p.ws + ((block * 2 * rows + h * rows + rr) * p.parts + w.part) * kPartFloats;
     };
-    // the next unit; rows of units without keys are zeroed on the way
     uint32_t j = 0;
-    auto advance = [&](Unit* w) {
-      while (next_record(&j, w)) {
-        if (w->nt > 0) return true;
-        const uint32_t zero[16] = {};
-        bool inside;
-        if (kSplit) {  // a part that weighs nothing
-          float* o = part_row(*w, &inside);
-          if (inside) {
-#pragma unroll 1
-            for (int c = 0; c < kHeadDim; c += 4) *reinterpret_cast<float4*>(o + c) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            *reinterpret_cast<float4*>(o + kHeadDim) = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
-          }
-          continue;
-        }
-        __nv_bfloat16* o = out_row(*w, &inside);
-        if (inside) {
-#pragma unroll 1
-          for (int c = 0; c < 4; ++c) put(o + 32 * c, zero);
-        }
-      }
-      return false;
-    };
-
     const uint32_t s_addr = tmem + lane_addr + kColS + 128 * h;
     // This thread's row of the unit's Q in place, bf16 -> f16 times 2^-e, once the copy has landed;
     // the score factor of the row in *f
@@ -701,7 +694,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
     Unit w, nw;
     float fr = 0.0f, next_fr = 0.0f;
     const uint32_t nan_at = sbase + offNanRow + (h * kBlk + rr) * 16;
-    bool have = advance(&w) && q_convert(0, &fr);
+    bool have = next_unit(&j, &w) && q_convert(0, &fr);
     for (; have; ++it) {
       int jlo = 0, jhi = w.len;  // keys that this row sees: [jlo, jhi)
       bool live;
@@ -865,7 +858,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       }
       if (!ok) break;
       // the next unit's Q, so that its Q K^T runs during this one's output
-      const bool more = advance(&nw);
+      const bool more = next_unit(&j, &nw);
       if (more && !q_convert(it + 1, &next_fr)) break;
       // the output row: O 2^(M - m - 6) / l, the factor in two parts that stay normal
       float fa = 0.0f, fb = 0.0f;

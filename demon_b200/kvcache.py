@@ -223,7 +223,7 @@ def attention(q: torch.Tensor, cache: KVCache, table: torch.Tensor, lens: torch.
                   1 if causal else 0, -1 if window is None else min(int(window), 1 << 30),
                   _DEFAULT_SCALE if scale is None else float(scale), 0)
         args = _ATTN.pack(*fields, 0, 0)
-        if W * cache._c[6] >= (8_000 if Sq * Hq <= 16 * cache._heads else 1_000):  # shorter tables take no workspace
+        if W * cache._c[6] > (8_128 if Sq * Hq <= 16 * cache._heads else 896):  # shorter tables take no workspace
             n = nat.load().demon_kv_attention_workspace(args)
             if n:
                 ws = torch.empty(n, dtype=torch.uint8, device=cache._device)

@@ -804,3 +804,23 @@ def test_blocks_of_rows_split_over_a_workspace(cuda, Sq, Hq, Hk, P, lens):
     args.workspace, args.workspace_bytes = room.data_ptr(), size - 1
     with pytest.raises(nat.DemonError, match="workspace"):
         nat.check(nat.load().demon_kv_attention(bytes(args), nat.stream_ptr()))
+
+
+@pytest.mark.parametrize("lens,Sq,q_lens", [([257] + [0] * 88 + [130], 200, None),                     # long runs of sequences without keys
+                                            ([70, 0, 0] * 40, 150, None),
+                                            ([90] * 60, 300, [1 + (b % 7 == 0) * 299 for b in range(60)]),   # and of blocks without queries
+                                            ([400] * 5 + [0] * 120 + [300], 130, [129] * 126)])
+def test_runs_of_empty_blocks(cuda, lens, Sq, q_lens):
+    """More blocks than SMs, most of them without keys or queries, between others that have them."""
+    cache, ref, table, rows = filled(lens, 32, 8, cuda, 108)
+    q = queries(len(lens), Sq, 16, cuda, Sq)
+    for causal, window in ((False, None), (True, None), (True, 20)):
+        check_attention(cuda, cache, ref, rows, table, lens, q, q_lens, causal, window, label=f"{causal} {window}")
+
+
+@pytest.mark.parametrize("lens,q_lens", [([3000, 0, 0, 0, 0, 0, 2000], None), ([2600] * 6, [1, 1, 200, 1, 1, 70])])
+def test_parts_and_empty_blocks(cuda, lens, q_lens):
+    cache, ref, table, rows = filled(lens, 64, 1, cuda, 109)
+    q = queries(len(lens), 200, 2, cuda, 3)
+    for causal, window in ((False, None), (True, None), (True, 900)):
+        check_attention(cuda, cache, ref, rows, table, lens, q, q_lens, causal, window, label=f"{causal} {window}")
