@@ -67,6 +67,9 @@ class KVCache:
             _c=(k.data_ptr(), v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(), k.shape[0], k.shape[1],
                 k.shape[2], HEAD_DIM, 0))
 
+    def __reduce__(self):  # a copy or an unpickled cache has pointers of its own
+        return type(self), (self.k, self.v, self.k_scale, self.v_scale)
+
     @classmethod
     def empty(cls, pages: int, heads: int, page_size: int = 64, device="cuda") -> "KVCache":
         """A cache of ``pages`` pages, every value zero."""

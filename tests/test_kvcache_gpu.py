@@ -824,3 +824,20 @@ def test_parts_and_empty_blocks(cuda, lens, q_lens):
     q = queries(len(lens), 200, 2, cuda, 3)
     for causal, window in ((False, None), (True, None), (True, 900)):
         check_attention(cuda, cache, ref, rows, table, lens, q, q_lens, causal, window, label=f"{causal} {window}")
+
+
+def test_copies_of_a_cache_are_caches_of_their_own(cuda):
+    import copy
+    import pickle
+
+    from demon_b200 import kvcache
+    cache, _, table, _ = filled([40], 16, 2, cuda, 110)
+    lens = i32([40], cuda)
+    k, v = kvcache.read(cache, table, lens, 40)
+    for other in (copy.deepcopy(cache), pickle.loads(pickle.dumps(cache))):
+        kvcache.append(cache, -k, -v, table, i32([0], cuda))
+        same = kvcache.read(other, table, lens, 40)
+        assert torch.equal(same[0], k) and torch.equal(same[1], v)
+        kvcache.append(cache, k, v, table, i32([0], cuda))
+        assert torch.equal(kvcache.read(cache, table, lens, 40)[0], k)
+    ok()
