@@ -37,8 +37,8 @@
 // exponentials' rate asks for 1,024) and, for short key ranges (256 keys of a condition are two
 // tiles), by the units' Q conversion and output (Q converted by warpgroup 2 after the unit's first
 // tile: 69 us for 16 x 750 over 256 keys against 64).  Measured, 16 query heads over 8: 6,016 x 6,016
-// 328 to 349 us (0.85 to 0.90 PFLOP/s; the bf16 kernel of attention.cu 264 us), 16 x 750 over 256 keys
-// 64 us (bf16 34 us), 6,001 causal 176 to 181 us.  Slower, not kept: steps of 64 keys with two score
+// 327 to 334 us (0.89 to 0.91 PFLOP/s; the bf16 kernel of attention.cu 264 us), 16 x 750 over 256 keys
+// 64 us (bf16 34 us), 6,001 causal 179 to 182 us.  Slower, not kept: steps of 64 keys with two score
 // buffers (Q K^T 64 wide takes the tensor core longer, and the overheads of a step double: 396 us at
 // 6,016 x 6,016); two threads per row (466 us); the next scores loaded ahead of the exponentials
 // (509 us, they come late).
@@ -68,8 +68,9 @@ constexpr float kBias = 6.0f;            // P = 2^(.. + 6)
 constexpr float kRaise = 8.0f;           // offsets are raised when exceeded by more than this
 constexpr float kFast = 60.0f;           // |M - m - ev| up to which l comes from P
 
-// Registers per thread after the split (setmaxnreg): the launch gives 512 x 128.
-constexpr int kLaunchRegs = 128, kSoftmaxRegs = 176, kConvRegs = 80, kIssueRegs = 80;
+// Registers per thread after the split (setmaxnreg): the launch gives 512 x 128.  6,016 x 6,016 keys
+// 334 us; 176 / 80 / 80 341 us, 184 / 72 / 72 339, 160 / 96 / 96 372, 168 / 96 / 80 354.
+constexpr int kLaunchRegs = 128, kSoftmaxRegs = 168, kConvRegs = 88, kIssueRegs = 88;
 static_assert(256 * kSoftmaxRegs + 128 * kConvRegs + 128 * kIssueRegs <= kThreads * kLaunchRegs,
               "register split exceeds the launch's registers (setmaxnreg.inc would wait for good)");
 
@@ -690,14 +691,72 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       return true;
     };
 
-    uint32_t t = 0, it = 0;  // tiles, units
+    uint32_t t = 0;  // tiles
     Unit w, nw;
-    float fr = 0.0f, next_fr = 0.0f;
+    float fr = 0.0f, next_fr = 0.0f, M = -INFINITY, m = -INFINITY, l = 0.0f;
+    bool live = false;
     const uint32_t nan_at = sbase + offNanRow + (h * kBlk + rr) * 16;
-    bool have = next_unit(&j, &w) && q_convert(0, &fr);
-    for (; have; ++it) {
+    for (uint32_t it = 0;; ++it) {  // units, and the output of the last one
+      // the next unit's Q, so that its Q K^T runs during this one's output
+      const bool more = next_unit(&j, &nw);
+      if (more && !q_convert(it, &next_fr)) break;
+      if (it > 0) {
+        // the output row: O 2^(M - m - 6) / l, the factor in two parts that stay normal
+        float fa = 0.0f, fb = 0.0f;
+        if (live && l != 0.0f) {
+          fa = ex2(0.5f * (M - m - kBias));
+          fb = fa / l;
+        }
+        bool inside;
+        __nv_bfloat16* out = out_row(w, &inside);
+        float* part = kSplit ? part_row(w, &inside) : nullptr;
+        if (!warp_wait(&o_full[h], (it - 1) & 1u, abort_flag, p, 92)) break;
+        tc_fence_after();
+        const float2 a2 = make_float2(fa, fa), b2 = make_float2(fb, fb);
+#pragma unroll 1
+        for (int c = 0; c < 2; ++c) {
+          uint32_t o[64];
+          tmem_ld_32x32b_x32(o_addr + 64 * c, *reinterpret_cast<uint32_t(*)[32]>(o));
+          tmem_ld_32x32b_x32(o_addr + 64 * c + 32, *reinterpret_cast<uint32_t(*)[32]>(o + 32));
+          tmem_ld_wait();
+#pragma unroll
+          for (int d = 0; d < 2; ++d) {
+            uint32_t x[16];
+#pragma unroll
+            for (int q = 0; q < 16; ++q) {
+              const float2 v = mul_f2(
+                  mul_f2(make_float2(__uint_as_float(o[32 * d + 2 * q]), __uint_as_float(o[32 * d + 2 * q + 1])), a2), b2);
+              x[q] = fb == 0.0f ? 0u : pack_bf16x2(v.x, v.y);  // rows that see nothing: zeros, never 0 * NaN
+              if (kSplit) {
+                if (inside)
+                  *reinterpret_cast<float2*>(part + 64 * c + 32 * d + 2 * q) = fb == 0.0f ? make_float2(0.0f, 0.0f) : v;
+              }
+            }
+            if (inside && !kSplit) put(out + 64 * c + 32 * d, x);
+          }
+        }
+        const uint4 nan = ld_shared_v4(nan_at);
+        if ((nan.x | nan.y | nan.z | nan.w) && live) {  // channels that met a NaN of V
+#pragma unroll 1
+          for (int d = 0; d < kHeadDim; ++d) {
+            const uint32_t bits = d < 32 ? nan.x : d < 64 ? nan.y : d < 96 ? nan.z : nan.w;
+            if ((bits >> (d & 31)) & 1u) {
+              if (kSplit)
+                part[d] = __int_as_float(0x7FFFFFFF);
+              else
+                reinterpret_cast<unsigned short*>(out)[d] = 0x7FFF;
+            }
+          }
+        }
+        if (kSplit && inside)  // the part's own output, and what it weighs: l 2^m
+          *reinterpret_cast<float4*>(part + kHeadDim) = fb == 0.0f ? make_float4(-INFINITY, 0.0f, 0.0f, 0.0f) : make_float4(m, l, 0.0f, l);
+        tc_fence_before();  // O_h is read before this warp publishes the next unit's P_h
+      }
+      if (!more) break;
+      w = nw;
+      fr = next_fr;
       int jlo = 0, jhi = w.len;  // keys that this row sees: [jlo, jhi)
-      bool live;
+      live = false;
       {
         const int qi = token_of(w);
         live = ri < p.Tt && qi < w.nq;
@@ -707,7 +766,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
           jhi = k.hi;
         }
       }
-      float M = -INFINITY, m = -INFINITY, l = 0.0f;
+      M = m = -INFINITY;
+      l = 0.0f;
       st_shared_v4(nan_at, 0, 0, 0, 0);
       bool ok = true;
       // the keys that every row of the warp sees: tiles within them need no mask
@@ -857,62 +917,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         if (lane == 0) mbar_arrive(&pb_full[h]);
       }
       if (!ok) break;
-      // the next unit's Q, so that its Q K^T runs during this one's output
-      const bool more = next_unit(&j, &nw);
-      if (more && !q_convert(it + 1, &next_fr)) break;
-      // the output row: O 2^(M - m - 6) / l, the factor in two parts that stay normal
-      float fa = 0.0f, fb = 0.0f;
-      if (live && l != 0.0f) {
-        fa = ex2(0.5f * (M - m - kBias));
-        fb = fa / l;
-      }
-      bool inside;
-      __nv_bfloat16* out = out_row(w, &inside);
-      float* part = kSplit ? part_row(w, &inside) : nullptr;
-      if (!warp_wait(&o_full[h], it & 1u, abort_flag, p, 92)) break;
-      tc_fence_after();
-      const float2 a2 = make_float2(fa, fa), b2 = make_float2(fb, fb);
-#pragma unroll 1
-      for (int c = 0; c < 2; ++c) {
-        uint32_t o[64];
-        tmem_ld_32x32b_x32(o_addr + 64 * c, *reinterpret_cast<uint32_t(*)[32]>(o));
-        tmem_ld_32x32b_x32(o_addr + 64 * c + 32, *reinterpret_cast<uint32_t(*)[32]>(o + 32));
-        tmem_ld_wait();
-#pragma unroll
-        for (int d = 0; d < 2; ++d) {
-          uint32_t x[16];
-#pragma unroll
-          for (int q = 0; q < 16; ++q) {
-            const float2 v = mul_f2(
-                mul_f2(make_float2(__uint_as_float(o[32 * d + 2 * q]), __uint_as_float(o[32 * d + 2 * q + 1])), a2), b2);
-            x[q] = fb == 0.0f ? 0u : pack_bf16x2(v.x, v.y);  // rows that see nothing: zeros, never 0 * NaN
-            if (kSplit) {
-              if (inside)
-                *reinterpret_cast<float2*>(part + 64 * c + 32 * d + 2 * q) = fb == 0.0f ? make_float2(0.0f, 0.0f) : v;
-            }
-          }
-          if (inside && !kSplit) put(out + 64 * c + 32 * d, x);
-        }
-      }
-      const uint4 nan = ld_shared_v4(nan_at);
-      if ((nan.x | nan.y | nan.z | nan.w) && live) {  // channels that met a NaN of V
-#pragma unroll 1
-        for (int d = 0; d < kHeadDim; ++d) {
-          const uint32_t bits = d < 32 ? nan.x : d < 64 ? nan.y : d < 96 ? nan.z : nan.w;
-          if ((bits >> (d & 31)) & 1u) {
-            if (kSplit)
-              part[d] = __int_as_float(0x7FFFFFFF);
-            else
-              reinterpret_cast<unsigned short*>(out)[d] = 0x7FFF;
-          }
-        }
-      }
-      if (kSplit && inside)  // the part's own output, and what it weighs: l 2^m
-        *reinterpret_cast<float4*>(part + kHeadDim) = fb == 0.0f ? make_float4(-INFINITY, 0.0f, 0.0f, 0.0f) : make_float4(m, l, 0.0f, l);
-      tc_fence_before();  // O_h is read before this warp publishes the next unit's P_h
-      w = nw;
-      fr = next_fr;
-      have = more;
     }
   }
 

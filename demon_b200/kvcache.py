@@ -68,7 +68,7 @@ class KVCache:
                 k.shape[2], HEAD_DIM, 0))
 
     def __reduce__(self):  # a copy or an unpickled cache has pointers of its own
-        return type(self), (self.k, self.v, self.k_scale, self.v_scale)
+        return _from_bytes, (self.k.view(torch.uint8), self.v.view(torch.uint8), self.k_scale, self.v_scale)
 
     @classmethod
     def empty(cls, pages: int, heads: int, page_size: int = 64, device="cuda") -> "KVCache":
@@ -89,6 +89,11 @@ class KVCache:
     @property
     def page_size(self) -> int:
         return self.k.shape[2]
+
+
+def _from_bytes(k, v, k_scale, v_scale) -> KVCache:
+    """A cache whose codes come as bytes (torch pickles those; its 8-bit floats it does not read back)."""
+    return KVCache(k.view(torch.float8_e4m3fn), v.view(torch.float8_e4m3fn), k_scale, v_scale)
 
 
 # The argument blocks of include/demon_b200.h as struct formats (native sizes, no implicit padding:
