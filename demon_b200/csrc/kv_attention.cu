@@ -15,9 +15,8 @@
 // Measured, 8 kv heads: one token (16 query heads) over 750 keys 7 us, the launch and a few rounds of
 // latency; one token of 48 sequences of up to 8,192 keys (32 query heads), 452 MB of codes, 80.5 us
 // (5.6 TB/s); one token of 16 sequences of 16,384 keys 91 us (5.9 TB/s); five tokens of two sequences
-// of up to 100,001 keys, 379 MB, 92 us (4.1 TB/s: 10 rows take twice the matrix instructions for the
-// same bytes, and registers for three CTAs an SM spill; at 16 CTAs a unit, where it took 140 us, 168
-// registers for two CTAs took 148 and six key warps a CTA 155).
+// of up to 100,001 keys, 379 MB, 82 us (4.6 TB/s: 10 rows take twice the matrix instructions for the
+// same bytes; six key warps a CTA were slower, 155 against 140 us at 16 CTAs a unit).
 //
 // A warp's step on 32 keys, all in registers (mma.sync m16n8k16, fp32 accumulators), with the keys
 // and V's channels on the 16-wide side of the MMAs and the query rows on the 8-wide one, so that a
@@ -66,10 +65,11 @@ struct Cfg {
   // The two warps of a tile see every second one: with an even number of stages they meet every
   // phase of the stages they use.  (With three, a warp one phase ahead took the phase before as its own.)
   static_assert(kStages % 2 == 0, "a stage must always belong to the same warps");
-  static constexpr int kMinCtas = RT == 1 ? 3 : 1;
+  static constexpr int kMinCtas = NR == 1 ? 3 : RT == 1 ? 2 : 1;
   // Registers: a scheduler's quarter of the file holds whole warps, so 128 let three CTAs of five
-  // warps in (200 would leave one), 168 one of nine.
-  static constexpr int kRegs = RT == 1 ? 128 : 168;
+  // warps in, 168 two (200 would leave one), 168 one of nine.  16 rows with 128 spill 460 bytes: 92
+  // against 82 us for five tokens over 100,000 keys.
+  static constexpr int kRegs = NR == 1 ? 128 : 168;
   static constexpr bool kQShared = NR > 1;                // Q operands in shared memory, for those registers
   static constexpr int offScale = kStages * 2 * kHalf;    // [stage][piece][K, V] fp32
   static constexpr int offBar = offScale + kStages * 4 * 2 * 4;  // full[stage], empty[stage]
@@ -762,7 +762,7 @@ SmallPlan plan_small(const DemonKvAttnArgs* a, bool workspace) {
   s.parts = s.cluster;
   // Longer tables: as many parts as fill the SMs, any number, joined by a second kernel through a
   // workspace (the cluster's power of two up to 16 against it: 64 units of 16,384 keys 64.6 and 51 us,
-  // 16 units of 100,000 keys 143 and 92 us, 4 of them 61 and 29 us; below 8,192 keys the second launch
+  // 16 units of 100,000 keys 143 and 82 us, 4 of them 61 and 29 us; below 8,192 keys the second launch
   // and the workspace cost what they gain).
   const int64_t parts = s.units > 0 ? std::min<int64_t>(kCtas / s.units, tiles / 6) : 0;
   if (workspace && tiles >= 128 && parts > s.cluster) {
