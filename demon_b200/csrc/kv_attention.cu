@@ -850,7 +850,8 @@ TcPlan plan_tc(const DemonKvAttnArgs* a, bool workspace) {
   // with 4 us for the second kernel and the partial results' way through memory.
   if (workspace && s.blocks < 148) {
     const double whole = s.us, rows = (double)s.blocks * tokens * G;
-    for (int parts = 2; parts <= 148 / s.blocks + 1 && parts * 4 <= tiles; ++parts) {
+    const int64_t most = std::max<int64_t>(148 / s.blocks, 8);  // (8: 80 blocks of 76 tiles 265 us whole, 180 in parts)
+    for (int parts = 2; parts <= most && parts * 4 <= tiles; ++parts) {
       const double us = std::ceil(s.blocks * parts / 148.0) * (std::ceil(tiles / parts) * 2.7 + 2.0) + 4.0 +
                         rows * parts * (2 * kv::kPartFloats * 4) / 4e6;
       if (us < 0.8 * whole && us < s.us) s.us = us, s.parts = parts;
