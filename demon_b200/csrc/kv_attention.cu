@@ -752,9 +752,10 @@ SmallPlan plan_small(const DemonKvAttnArgs* a, bool workspace) {
     keys = std::min<int64_t>(keys, kRows / (a->Hq / a->cache.heads) + 2 + (a->causal ? 1LL : 2LL) * a->window);
   const int64_t tiles = (keys + kv::small::kTile - 1) / kv::small::kTile;
   // Keys split over a cluster as far as all CTAs are resident at once (twice over with 32 rows a CTA and
-  // 8,192 keys: 24 rows of 8 ragged sequences 103 us, once 117), two tiles or more each: with up to twice as many CTAs, 32 units of 4,096 keys take 22.3 us against
-  // 12.8.  Where nothing more fits, halves all the same: they even out sequences of different lengths
-  // (256 units of 800 to 8,192 keys 56 us, whole 82; all of 4,096 keys 65 us, whole 52).
+  // 8,192 keys: 24 rows of 8 ragged sequences 103 us, once 117), two tiles or more each: with up to
+  // twice as many CTAs, 32 units of 4,096 keys take 22.3 us against 12.8.  Where nothing more fits,
+  // halves all the same: they even out sequences of different lengths (256 units of 800 to 8,192 keys
+  // 56 us, whole 82; all of 4,096 keys 65 us, whole 52).
   const int kCtas = 148 * (RT == 1 || tiles < 128 ? C::kMinCtas : 2);
   s.cluster = 1;
   while (s.cluster < 16 && s.units * s.cluster * 2 <= kCtas && tiles >= 4 * s.cluster) s.cluster *= 2;
