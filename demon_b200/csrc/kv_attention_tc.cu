@@ -828,7 +828,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         const float m1 = up ? mt : m, M1 = UP ? Mt : M;
         const float mo = M1 == -INFINITY ? 0.0f : M1, ml = m1 == -INFINITY ? 0.0f : m1;
         const float D = mo - ml;
-        const bool far = D - tail.x > kFast || tail.y - D > kFast;
+        // (rows without a token do not vote: theirs are leftovers of shared memory, and the second
+        // exponential rounds the other rows' sums differently)
+        const bool far = live && (D - tail.x > kFast || tail.y - D > kFast);
         float lw = D;
         if (__any_sync(0xffffffffu, up || UP || far)) {
           if (up) l *= ex2(m - m1);

@@ -841,3 +841,21 @@ def test_copies_of_a_cache_are_caches_of_their_own(cuda):
         kvcache.append(cache, k, v, table, i32([0], cuda))
         assert torch.equal(kvcache.read(cache, table, lens, 40)[0], k)
     ok()
+
+
+# 128 rows of a tile are not a multiple of these heads: the rows behind them hold what shared memory held
+@pytest.mark.parametrize("G", [3, 5, 6, 7, 12, 100])
+def test_rows_that_no_token_has_change_nothing(cuda, G):
+    """Equal bits whatever ran on the SMs before, in the blocks' own rows and behind a workspace."""
+    from demon_b200 import kvcache
+    os.environ["DEMON_KV_ATTENTION"] = "tc"
+    cache, ref, table, rows = filled([864, 400, 3000], 16, 2, cuda, 120)
+    other, _, table2, _ = filled([500] * 40, 16, 2, cuda, 121)
+    lens, q = i32([864, 400, 3000], cuda), queries(3, 59, 2 * G, cuda, G)
+    first = check_one(cuda, cache, ref, rows, table, [864, 400, 3000], q, None, True, None, None, f"G={G}")
+    short = kvcache.attention(q, cache, table[:, :55].contiguous(), lens.clamp(max=880), causal=True)
+    for by in (1e38, 1e-3, 1e20):
+        kvcache.attention(queries(40, 260, 4, cuda, 9, by), other, table2, i32([500] * 40, cuda))
+        assert torch.equal(kvcache.attention(q, cache, table, lens, causal=True), first), by
+        assert torch.equal(kvcache.attention(q, cache, table[:, :55].contiguous(), lens.clamp(max=880), causal=True), short), by
+    ok()
