@@ -859,3 +859,19 @@ def test_rows_that_no_token_has_change_nothing(cuda, G):
         assert torch.equal(kvcache.attention(q, cache, table, lens, causal=True), first), by
         assert torch.equal(kvcache.attention(q, cache, table[:, :55].contiguous(), lens.clamp(max=880), causal=True), short), by
     ok()
+
+
+def test_a_second_part_on_an_sm(cuda):
+    """The tensor-core kernel with more parts of blocks than SMs: a CTA takes several, of different blocks."""
+    from demon_b200 import _native as nat
+    lens, Sq, Hq, Hk = [9640, 5000, 9000, 0, 7001], 87, 24, 8
+    cache, ref, table, rows = filled(lens, 64, Hk, cuda, 118, v_scale_by=lambda i: torch.exp2((i // 1700 % 3).float() * -7))
+    q = queries(len(lens), Sq, Hq, cuda, 5)
+    os.environ["DEMON_KV_ATTENTION"] = "tc"
+    args = attention_args(q, cache, table, i32(lens, cuda), q, True)
+    tokens, blocks = 2 * (128 // 3), 2 * len(lens) * Hk
+    parts, rest = divmod(nat.load().demon_kv_attention_workspace(bytes(args)), blocks * tokens * 3 * (128 + 4) * 4)
+    assert rest == 0 and parts * blocks > 148 and parts * blocks % 148 > 0
+    for causal, window, q_lens in ((True, None, None), (False, None, [Sq, 1, 70, 3, 0]), (True, 6000, None)):
+        first = check_one(cuda, cache, ref, rows, table, lens, q, q_lens, causal, window, None, f"{causal} {window}")
+        assert torch.equal(first, check_one(cuda, cache, ref, rows, table, lens, q, q_lens, causal, window, None, "again"))
