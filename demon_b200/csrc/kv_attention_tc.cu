@@ -651,6 +651,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
     };
     uint32_t j = 0;
     const uint32_t s_addr = tmem + lane_addr + kColS + 128 * h;
+    if (ri >= p.Tt) {
+      // Rows behind the last whole token: no copy writes their Q.  Zeros, since what shared memory held
+      // could vote for the second exponential below, which rounds the sums of the warp's other rows
+      // differently.  (That vote by rows with a token only: prompt 180 -> 183.5 us.)
+      for (int k = 0; k < 16; ++k) st_shared_v4(sbase + offQ + h * kTile + rr * 128 + (k >> 3) * kBox + (k & 7) * 16, 0, 0, 0, 0);
+    }
     // This thread's row of the unit's Q in place, bf16 -> f16 times 2^-e, once the copy has landed;
     // the score factor of the row in *f
     auto q_convert = [&](uint32_t unit, float* f) {
@@ -828,9 +834,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         const float m1 = up ? mt : m, M1 = UP ? Mt : M;
         const float mo = M1 == -INFINITY ? 0.0f : M1, ml = m1 == -INFINITY ? 0.0f : m1;
         const float D = mo - ml;
-        // (rows without a token do not vote: theirs are leftovers of shared memory, and the second
-        // exponential rounds the other rows' sums differently)
-        const bool far = live && (D - tail.x > kFast || tail.y - D > kFast);
+        const bool far = D - tail.x > kFast || tail.y - D > kFast;
         float lw = D;
         if (__any_sync(0xffffffffu, up || UP || far)) {
           if (up) l *= ex2(m - m1);
