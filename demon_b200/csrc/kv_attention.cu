@@ -660,35 +660,44 @@ __global__ void __launch_bounds__(Cfg<NR, RT>::kThreads) __maxnreg__((Cfg<NR, RT
   if (csize > 1) cluster_join();  // no CTA leaves while another still reads its results
 }
 
-// The partial results of a row from the workspace: a CTA per row, its warps share the parts.
+// The partial results of a row from the workspace: a CTA per row, its warps share the parts.  A part of
+// the tensor-core kernel is the row's output over its keys and may be as large as V's largest value, next
+// to fp32's: the parts' weights are summed first, and each is multiplied by its share of them.
 constexpr int kJoinWarps = 8;
 __global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const AttnParams p, const int tile_rows) {
   __shared__ float4 sums[kJoinWarps][32];
-  __shared__ float ls[kJoinWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t unit = blockIdx.x / (uint32_t)tile_rows, rt = unit % (uint32_t)p.n_rt, u1 = unit / (uint32_t)p.n_rt;
   const int hk = (int)(u1 % (uint32_t)p.c.heads), b = (int)(u1 / (uint32_t)p.c.heads);
   const int grow = (int)(rt * (uint32_t)tile_rows + blockIdx.x % (uint32_t)tile_rows);
   if (grow >= p.Sq * p.G) return;
   const float* w = p.ws + (int64_t)blockIdx.x * p.parts * kPartFloats;
+  // maximum, unit and sum of weights: every warp the same
   float M = -INFINITY, L = 0.0f;
   int E = kMinExp;
   for (int k = lane; k < p.parts; k += 32) {
     const float4 st = *reinterpret_cast<const float4*>(w + (int64_t)k * kPartFloats + kHeadDim);
-    M = fmaxf(M, st.x);
+    const float n = fmaxf(M, st.x);
+    L = fmaf(st.y, join_factor(st.x, n), L * join_factor(M, n));
+    M = n;
     E = imax(E, __float_as_int(st.z));
   }
+  float top = M;
 #pragma unroll
-  for (int d = 16; d >= 1; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+  for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+  L *= join_factor(M, top);
+  M = top;
+#pragma unroll
+  for (int d = 16; d >= 1; d >>= 1) L += __shfl_xor_sync(0xffffffffu, L, d);
   E = __reduce_max_sync(0xffffffffu, E);
+  const float inv = L != 0.0f ? 1.0f / L : 0.0f;
   float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
   for (int k = warp; k < p.parts; k += kJoinWarps) {
     const float* wk = w + (int64_t)k * kPartFloats;
     const float4 st = *reinterpret_cast<const float4*>(wk + kHeadDim);
-    const float f = join_factor(st.x, M), fo = f * st.w * unit_factor(__float_as_int(st.z), E);
-    L = fmaf(st.y, f, L);
     if (st.x == -INFINITY) continue;  // no key seen (and O perhaps not written)
+    const float fo = join_factor(st.x, M) * st.w * inv * unit_factor(__float_as_int(st.z), E);
     const float4 v = *reinterpret_cast<const float4*>(wk + 4 * lane);
     acc.x = fmaf(v.x, fo, acc.x);
     acc.y = fmaf(v.y, fo, acc.y);
@@ -696,14 +705,13 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const A
     acc.w = fmaf(v.w, fo, acc.w);
   }
   sums[warp][lane] = acc;
-  if (lane == 0) ls[warp] = L;
   __syncthreads();
   if (warp > 0) return;
   for (int k = 1; k < kJoinWarps; ++k) {
     const float4 v = sums[k][lane];
     acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
-    L += ls[k];
   }
+  if (L == L && L != 0.0f) L = 1.0f;  // (divided by already; a NaN stays)
   bool bad = false;  // (reported by the other kernel)
   store_row(p, b, hk, grow, p.q_lens ? clamp_len(p.q_lens[b], p.Sq, &bad) : p.Sq, lane, acc, L, E);
 }

@@ -875,3 +875,32 @@ def test_a_second_part_on_an_sm(cuda):
     for causal, window, q_lens in ((True, None, None), (False, None, [Sq, 1, 70, 3, 0]), (True, 6000, None)):
         first = check_one(cuda, cache, ref, rows, table, lens, q, q_lens, causal, window, None, f"{causal} {window}")
         assert torch.equal(first, check_one(cuda, cache, ref, rows, table, lens, q, q_lens, causal, window, None, "again"))
+
+
+# ------------------------------------------------------------------------- values far from one
+
+def held(k, v, lens, P, dev, seed):
+    """A cache holding k / v [B, S, heads, 128] at these lengths, its twin, and the table."""
+    from demon_b200 import kvcache
+    table, rows, pages = make_table([k.shape[1]] * len(lens), P, dev, seed)
+    cache, ref = kvcache.KVCache.empty(pages, k.shape[2], P, dev), R.RefCache(pages, k.shape[2], P, dev)
+    k, v = k.to(torch.bfloat16).to(dev), v.to(torch.bfloat16).to(dev)
+    kvcache.append(cache, k, v, table, i32([0] * len(lens), dev), i32(lens, dev))
+    ref.append(k, v, rows, [0] * len(lens), lens)
+    return cache, ref, table, rows
+
+
+@pytest.mark.parametrize("signs", [False, True])
+@pytest.mark.parametrize("Sq,Hq,Hk,P,lens", [(300, 2, 2, 128, [9000, 4100]), (40, 8, 2, 64, [5000]), (70, 1, 1, 16, [1300]),
+                                             (1, 8, 2, 64, [20_001, 17_000]), (10, 6, 2, 32, [30_000])])
+def test_large_values_in_parts(cuda, Sq, Hq, Hk, P, lens, signs):
+    """V of 5e37 to 2e38 over keys whose parts are joined: no partial sum leaves fp32, which ends at 3.4e38."""
+    g = torch.Generator().manual_seed(Sq)
+    k = torch.randn(len(lens), max(lens), Hk, 128, generator=g)
+    v = (1 + 3 * torch.rand(k.shape, generator=g)) * 5e37
+    if signs:  # by channel: what overflows does not meet its opposite
+        v = v * (1 - 2 * (torch.arange(128) % 2))
+    cache, ref, table, rows = held(k, v, lens, P, cuda, 111)
+    q = queries(len(lens), Sq, Hq, cuda, Sq)
+    for causal, window in ((True, None), (False, 9000)):
+        check_attention(cuda, cache, ref, rows, table, lens, q, None, causal, window, label=f"{causal} {window}")
