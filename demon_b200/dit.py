@@ -104,8 +104,9 @@ class CrossCache:
         """The same pages for another batch: entry i is condition ``index[i]`` (a condition may
         stand in several sequences; nothing is copied but its page numbers)."""
         index = torch.as_tensor(index)
-        if index.dtype == torch.bool or index.dtype.is_floating_point or index.dim() != 1:
+        if index.dtype == torch.bool or index.dtype.is_floating_point or index.dtype.is_complex or index.dim() != 1:
             raise ValueError("rows: index must be a list or 1-D tensor of integers")
+        index = index.long()  # (torch takes a uint8 index for a mask)
         n = self.table.shape[0]
         if index.is_cuda:  # no look at its values from here: an index out of range sees no page
             inside = (index >= 0) & (index < n)

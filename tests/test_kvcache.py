@@ -199,3 +199,15 @@ def test_rows_of_a_condition_cache_refuses_what_is_not_a_condition():
     for bad in (1, [[0]], [0.5], torch.tensor([True, False, True])):
         with pytest.raises(ValueError, match="index"):
             kv.rows(bad)
+
+
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64, torch.uint16])
+def test_rows_takes_every_integer_type_for_numbers(dtype):
+    """torch takes a uint8 index for a mask; here it numbers conditions like any other."""
+    from demon_b200.dit import CrossCache
+    kv = CrossCache(None, torch.arange(6, dtype=torch.int32).view(3, 2), torch.tensor([5, 6, 7], dtype=torch.int32))
+    for index in ([1, 1, 1], [0, 1, 1], [2, 0], [1, 0, 1, 2]):
+        got = kv.rows(torch.tensor(index, dtype=dtype))
+        assert got.table.tolist() == [[2 * i, 2 * i + 1] for i in index] and got.lens.tolist() == [5 + i for i in index]
+    with pytest.raises(ValueError, match="index"):
+        kv.rows(torch.tensor([1j]))

@@ -904,3 +904,14 @@ def test_large_values_in_parts(cuda, Sq, Hq, Hk, P, lens, signs):
     q = queries(len(lens), Sq, Hq, cuda, Sq)
     for causal, window in ((True, None), (False, 9000)):
         check_attention(cuda, cache, ref, rows, table, lens, q, None, causal, window, label=f"{causal} {window}")
+
+
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int16, torch.int32])
+def test_condition_rows_by_a_device_index_of_other_types(cuda, dtype):
+    from demon_b200.dit import CrossCache
+    cache, _, table, _ = filled([60, 50, 40], 16, 2, cuda, 122)
+    kv = CrossCache(cache, table, i32([60, 50, 40], cuda))
+    for index in ([1, 1, 1], [0, 1, 1], [2, 0]):
+        for where in (cuda, "cpu"):
+            r = kv.rows(torch.tensor(index, dtype=dtype, device=where))
+            assert torch.equal(r.table, table[torch.tensor(index, device=cuda)]) and r.lens.tolist() == [60 - 10 * i for i in index]
