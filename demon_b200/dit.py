@@ -108,14 +108,21 @@ class CrossCache:
             raise ValueError("rows: index must be a list or 1-D tensor of integers")
         index = index.long()  # (torch takes a uint8 index for a mask)
         n = self.table.shape[0]
-        if index.is_cuda:  # no look at its values from here: an index out of range sees no page
-            inside = (index >= 0) & (index < n)
-            index = torch.where(inside, index, 0)
-            return CrossCache(self.cache, torch.where(inside[:, None], self.table[index], -1), self.lens[index])
+        if index.is_cuda:  # no look at its values from here
+            return self._chosen(index)
         if index.numel() and not (0 <= int(index.min()) and int(index.max()) < n):
             raise IndexError(f"rows: index out of range for {n} conditions")
         index = index.to(self.table.device)
         return CrossCache(self.cache, self.table[index].contiguous(), self.lens[index].contiguous())
+
+    def _chosen(self, index) -> "CrossCache":
+        """Rows by an index that may be out of range: such an entry becomes a sequence of one token
+        without a page, which sees nothing and which attention reports."""
+        n, W = self.table.shape
+        table = torch.cat([self.table, self.table.new_full((1, W), -1)])
+        lens = torch.cat([self.lens, self.lens.new_ones(1)])
+        index = torch.where((index >= 0) & (index < n), index, n)
+        return CrossCache(self.cache, table[index], lens[index])
 
 
 class TimestepEmbedding(nn.Module):

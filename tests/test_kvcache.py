@@ -211,3 +211,17 @@ def test_rows_takes_every_integer_type_for_numbers(dtype):
         assert got.table.tolist() == [[2 * i, 2 * i + 1] for i in index] and got.lens.tolist() == [5 + i for i in index]
     with pytest.raises(ValueError, match="index"):
         kv.rows(torch.tensor([1j]))
+
+
+@pytest.mark.parametrize("n,W", [(3, 2), (1, 1), (0, 2), (0, 0)])
+def test_rows_by_an_unread_index_never_leaves_the_conditions(n, W):
+    """What a device index does, on the CPU: out of range is one token without a page, of no conditions too."""
+    from demon_b200.dit import CrossCache
+    table = torch.arange(n * W, dtype=torch.int32).view(n, W)
+    kv = CrossCache(None, table, torch.zeros(n, dtype=torch.int32))     # (conditions without tokens: still reported)
+    index = [-1, 0, n - 1, n, n + 7, -(1 << 40), 1 << 40]
+    got = kv._chosen(torch.tensor(index))
+    for row, length, i in zip(got.table.tolist(), got.lens.tolist(), index):
+        assert (row, length) == ((table[i].tolist(), 0) if 0 <= i < n else ([-1] * W, 1))
+    assert got.table.dtype == got.lens.dtype == torch.int32 and got.table.is_contiguous()
+    assert kv._chosen(torch.zeros(0, dtype=torch.int64)).table.shape == (0, W)

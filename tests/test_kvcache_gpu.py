@@ -915,3 +915,19 @@ def test_condition_rows_by_a_device_index_of_other_types(cuda, dtype):
         for where in (cuda, "cpu"):
             r = kv.rows(torch.tensor(index, dtype=dtype, device=where))
             assert torch.equal(r.table, table[torch.tensor(index, device=cuda)]) and r.lens.tolist() == [60 - 10 * i for i in index]
+
+
+def test_condition_rows_of_no_conditions_by_a_device_index(cuda):
+    """Every index is out of range: zeros, and reported, also where the first condition has no tokens."""
+    from demon_b200 import _native as nat
+    from demon_b200 import kvcache
+    from demon_b200.dit import CrossCache
+    cache, _, table, _ = filled([60], 16, 2, cuda, 123)
+    index, q = torch.tensor([0, 1], device=cuda), queries(2, 2, 4, cuda, 1)
+    for kv in (CrossCache(cache, table[:0], i32([], cuda)), CrossCache(cache, table[:0, :0], i32([], cuda)),
+               CrossCache(cache, table, i32([0], cuda))):
+        r = kv.rows(index)
+        assert not bool(kvcache.attention(q, r.cache, r.table, r.lens).any())
+        assert nat.device_status()[0] == BAD_ARG
+        assert kv.rows(index[:0]).table.shape[0] == 0
+    ok()
