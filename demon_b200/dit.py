@@ -103,7 +103,7 @@ class CrossCache:
     def rows(self, index) -> "CrossCache":
         """The same pages for another batch: entry i is condition ``index[i]`` (a condition may
         stand in several sequences; nothing is copied but its page numbers)."""
-        index = torch.as_tensor(index)
+        index = torch.as_tensor(index, dtype=torch.int64 if isinstance(index, (list, tuple)) and not index else None)
         if index.dtype == torch.bool or index.dtype.is_floating_point or index.dtype.is_complex or index.dim() != 1:
             raise ValueError("rows: index must be a list or 1-D tensor of integers")
         index = index.long()  # (torch takes a uint8 index for a mask)

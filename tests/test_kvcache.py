@@ -225,3 +225,13 @@ def test_rows_by_an_unread_index_never_leaves_the_conditions(n, W):
         assert (row, length) == ((table[i].tolist(), 0) if 0 <= i < n else ([-1] * W, 1))
     assert got.table.dtype == got.lens.dtype == torch.int32 and got.table.is_contiguous()
     assert kv._chosen(torch.zeros(0, dtype=torch.int64)).table.shape == (0, W)
+
+
+def test_rows_of_an_empty_list():
+    from demon_b200.dit import CrossCache
+    kv = CrossCache(None, torch.arange(6, dtype=torch.int32).view(3, 2), torch.tensor([5, 6, 7], dtype=torch.int32))
+    for none in ([], ()):
+        got = kv.rows(none)
+        assert got.table.shape == (0, 2) and got.lens.shape == (0,)
+    with pytest.raises(ValueError, match="index"):
+        kv.rows([[]])
