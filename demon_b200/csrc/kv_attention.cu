@@ -30,7 +30,8 @@
 //   O^T += V^T P^T: the codes of V go in unscaled; O is held in units of 2^e_ref, the largest V
 //     scale met so far.  Keys of a page with a smaller scale 2^e have P multiplied by
 //     2^(e - e_ref), exactly; if that is below 2^-8, their product goes through accumulators of
-//     its own, so that P's precision never depends on the scales.
+//     its own, so that P's precision never depends on the scales.  (V scales more than 2^64 apart:
+//     row_of_wide_scales.)
 // The f16 conversions take one instruction per two codes (and one more for the upper half of a
 // word), and only a byte permute stands between V's rows and the operand layout: the keys and
 // channels of a step may be taken in any order as long as both operands agree.
@@ -54,6 +55,7 @@ constexpr int kHalf = kTile * kHeadDim;    // one stage's K (or V) codes, 8 KB
 constexpr int kKeyWarps = 4;               // per row group: two per tile, on alternating tiles
 constexpr float kPBias = 14.0f;            // p is scaled by 2^14 (see above)
 constexpr int kFoldMin = -8;               // smallest V scale, relative to e_ref, folded into P
+constexpr int kSpread = 64;                // V exponents of a CTA's keys up to which its rows share e_ref
 
 // NR: 8-row MMA tiles per warp; RT: row groups (of four warps) per CTA.
 template <int NR, int RT>
@@ -73,7 +75,7 @@ struct Cfg {
   static constexpr bool kQShared = NR > 1;                // Q operands in shared memory, for those registers
   static constexpr int offScale = kStages * 2 * kHalf;    // [stage][piece][K, V] fp32
   static constexpr int offBar = offScale + kStages * 4 * 2 * 4;  // full[stage], empty[stage]
-  static constexpr int offMisc = offBar + kStages * 2 * 8;       // abort flag
+  static constexpr int offMisc = offBar + kStages * 2 * 8;       // abort flag, wide flag
   static constexpr int offQ = offMisc + 16;               // [row group][k-step][lane] Q operands
   static constexpr int kSmem = offQ + (kQShared ? RT * 8 * 32 * 16 : 0);
   // After the key loop the ring holds the partial results: per warp O [rows][128] fp32, then the
@@ -154,6 +156,63 @@ __device__ __forceinline__ void store_row(const AttnParams& p, int b, int hk, in
   *reinterpret_cast<uint2*>(p.o + b * p.o_seq + (int64_t)i * p.o_row + (int64_t)(hk * p.G + gq) * p.o_head + 4 * lane) = out;
 }
 
+// One row over keys [from, to) by one warp, four channels a lane, on the codes where they lie: what a CTA
+// falls back on when V's exponents lie more than kSpread apart among its keys.  The key loop holds O of all
+// its rows in units of the largest exponent met; a row that does not see that one, and whose own lie far
+// below, would leave fp32's range.  Here the unit is that of the keys that the row sees.  Statistics and
+// biases as there.  (Units for each row in the key loop cost every call 2 to 5 %.)
+__device__ __forceinline__ void row_of_wide_scales(const AttnParams& p, int b, int hk, int grow, int len, int nq, int from,
+                                                   int to, int lane, float& m, float& l, int& unit, float4& acc) {
+  const int i = grow / p.G, gq = grow - i * p.G;
+  m = -INFINITY;
+  l = 0.0f;
+  unit = kMinExp;
+  acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (i < nq) {
+    const uint2 w = __ldg(reinterpret_cast<const uint2*>(p.q + b * p.q_seq + (int64_t)i * p.q_row +
+                                                         (int64_t)(hk * p.G + gq) * p.q_head + 4 * lane));
+    const float2 q0 = bf2_f2(w.x), q1 = bf2_f2(w.y);
+    const uint32_t x = w.x & 0x7FFF7FFFu, y = w.y & 0x7FFF7FFFu;  // the largest finite magnitude, as in the key loop
+    uint32_t mx = __vmaxu2(x & __vcmpltu2(x, 0x7F807F80u), y & __vcmpltu2(y, 0x7F807F80u));
+    mx = __reduce_max_sync(0xffffffffu, max(mx & 0xFFFFu, mx >> 16));
+    const int k = imax((int)(mx >> 7) - 127 - 13, -126);
+    const float by = exp2i(-k), fac = exp2i(k) * p.scale_log2;
+    const Keys see = visible(i, i, len, nq, p.causal != 0, p.window);
+    const int lo = imax(see.lo, from), hi = imin(see.hi, to);
+    for (int j0 = lo & ~15; j0 < hi; j0 += 16) {
+      const int pid = page_id(p.table + b * p.ld_table, p.W, j0 / p.c.P, p.c.pages);
+      if (pid < 0) continue;  // (reported by the copying warp)
+      const int64_t ph = (int64_t)pid * p.c.heads + hk, at = (ph * p.c.P + j0 % p.c.P) * kHeadDim + 4 * lane;
+      const float f = fac * fabsf(__ldg(p.c.scale[0] + ph));
+      const int ev = scale_exp(__ldg(p.c.scale[1] + ph));
+      const int is = imax(unit, ev);
+      const float vf = unit_factor(ev, is);
+      float back = unit_factor(unit, is);
+      unit = is;
+      for (int j = imax(j0, lo); j < imin(j0 + 16, hi); ++j) {
+        uint32_t a[2], c[2];
+        e4m3x4_f16(__ldg(reinterpret_cast<const uint32_t*>(p.c.codes[0] + at + (j - j0) * kHeadDim)), a[0], a[1]);
+        e4m3x4_f16(__ldg(reinterpret_cast<const uint32_t*>(p.c.codes[1] + at + (j - j0) * kHeadDim)), c[0], c[1]);
+        const float2 k0 = f16x2_f32(a[0]), k1 = f16x2_f32(a[1]), v0 = f16x2_f32(c[0]), v1 = f16x2_f32(c[1]);
+        float t = fmaf(q0.x * by, k0.x, fmaf(q0.y * by, k0.y, fmaf(q1.x * by, k1.x, q1.y * by * k1.y)));
+#pragma unroll
+        for (int d = 16; d >= 1; d >>= 1) t += __shfl_xor_sync(0xffffffffu, t, d);
+        t *= f;
+        const float n = fmaxf(m, t), s = n == -INFINITY ? 1.0f : ex2(m - n);
+        const float e = ex2(t + (kPBias - (n == -INFINITY ? 0.0f : n)));
+        m = n;
+        l = fmaf(l, s, e);
+        const float so = s * back, eo = e * vf;
+        back = 1.0f;
+        acc.x = fmaf(acc.x, so, v0.x * eo);
+        acc.y = fmaf(acc.y, so, v0.y * eo);
+        acc.z = fmaf(acc.z, so, v1.x * eo);
+        acc.w = fmaf(acc.w, so, v1.y * eo);
+      }
+    }
+  }
+}
+
 template <int NR, int RT>
 __global__ void __launch_bounds__(Cfg<NR, RT>::kThreads) __maxnreg__((Cfg<NR, RT>::kRegs)) attention_small_kernel(const AttnParams p) {
   using C = Cfg<NR, RT>;
@@ -163,6 +222,7 @@ __global__ void __launch_bounds__(Cfg<NR, RT>::kThreads) __maxnreg__((Cfg<NR, RT
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::offBar);
   uint64_t* empty = full + kStages;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::offMisc);
+  volatile int* wide_flag = abort_flag + 1;  // V exponents more than kSpread apart
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t csize = (uint32_t)p.cluster, parts = (uint32_t)p.parts;  // clusters lie along x
   const uint32_t rank = blockIdx.x % parts;
@@ -193,6 +253,7 @@ __global__ void __launch_bounds__(Cfg<NR, RT>::kThreads) __maxnreg__((Cfg<NR, RT
       mbar_init(&empty[s], 2 * RT);
     }
     *abort_flag = 0;
+    *wide_flag = 0;
     fence_mbar_init();
   }
   __syncthreads();
@@ -221,6 +282,7 @@ __global__ void __launch_bounds__(Cfg<NR, RT>::kThreads) __maxnreg__((Cfg<NR, RT
     const int n_pieces = n_tiles * pieces;
     bool ok = true;
     int issued = 0;  // tiles whose copies were started
+    int e_lo = kMaxExp, e_hi = kMinExp;  // V exponents
     for (int base = 0; ok && base < n_pieces; base += 32) {
       const int pc = base + lane;
       int pid = -1, key = 0;
@@ -236,6 +298,10 @@ __global__ void __launch_bounds__(Cfg<NR, RT>::kThreads) __maxnreg__((Cfg<NR, RT
             report(p.status, DEMON_DEV_BAD_ARG, 64);
           }
         }
+      }
+      if (pid >= 0) {
+        e_lo = imin(e_lo, scale_exp(sv));
+        e_hi = imax(e_hi, scale_exp(sv));
       }
       const int n_here = imin(32, n_pieces - base);
       for (int t = 0; t < n_here && ok; t += pieces) {
@@ -264,6 +330,9 @@ __global__ void __launch_bounds__(Cfg<NR, RT>::kThreads) __maxnreg__((Cfg<NR, RT
         __syncwarp();
       }
     }
+    e_lo = __reduce_min_sync(0xffffffffu, e_lo);
+    e_hi = __reduce_max_sync(0xffffffffu, e_hi);
+    if (lane == 0 && e_hi - e_lo > kSpread) *wide_flag = 1;
     if (!ok) {  // gave up: no copy may be in flight when the CTA leaves
       volatile int never = 0;
       for (int t = imax(issued - kStages, 0); t < issued; ++t)
@@ -577,7 +646,8 @@ __global__ void __launch_bounds__(Cfg<NR, RT>::kThreads) __maxnreg__((Cfg<NR, RT
         if (g == 0) {
           st_shared_f32(ws + row * 12, m[r][x]);
           st_shared_f32(ws + row * 12 + 4, l[r][x]);
-          st_shared_f32(ws + row * 12 + 8, __int_as_float(e_ref));
+          // (a unit that others of the warp need must not count for a row that has seen nothing)
+          st_shared_f32(ws + row * 12 + 8, __int_as_float(m[r][x] == -INFINITY ? kMinExp : e_ref));
         }
 #pragma unroll
         for (int q = 0; q < 4; ++q)
@@ -589,30 +659,35 @@ __global__ void __launch_bounds__(Cfg<NR, RT>::kThreads) __maxnreg__((Cfg<NR, RT
   // the CTA's four partial results of each row into one: a warp per row, four channels a lane
   constexpr int n_warps = kKeyWarps * RT + 1;
   const int rows_here = imin(C::kRows * RT, n_rows - row0);
+  const bool wide = *wide_flag != 0;
   for (int r = warp; r < rows_here; r += n_warps) {
     const int wt = r / C::kRows, rr = r % C::kRows;
     float mm[kKeyWarps], M = -INFINITY, L = 0.0f;
     int ee[kKeyWarps], E = kMinExp;
-#pragma unroll
-    for (int k = 0; k < kKeyWarps; ++k) {
-      const uint32_t ws = sbase + C::offStat + ((wt * kKeyWarps + k) * C::kRows + rr) * 12;
-      mm[k] = ld_shared_f32(ws);
-      ee[k] = __float_as_int(ld_shared_f32(ws + 8));
-      M = fmaxf(M, mm[k]);
-      E = imax(E, ee[k]);
-    }
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (wide) {
+      row_of_wide_scales(p, b, hk, row0 + r, len, nq, first * kTile, (first + n_tiles) * kTile, lane, M, L, E, acc);
+    } else {
 #pragma unroll
-    for (int k = 0; k < kKeyWarps; ++k) {
-      const uint32_t ws = sbase + C::offStat + ((wt * kKeyWarps + k) * C::kRows + rr) * 12;
-      const float f = join_factor(mm[k], M);
-      L = fmaf(ld_shared_f32(ws + 4), f, L);
-      const float fo = f * unit_factor(ee[k], E);
-      const float4 v = ld_shared_f32x4(sbase + (wt * kKeyWarps + k) * C::kWarpO + (rr * kHeadDim + 4 * lane) * 4);
-      acc.x = fmaf(v.x, fo, acc.x);
-      acc.y = fmaf(v.y, fo, acc.y);
-      acc.z = fmaf(v.z, fo, acc.z);
-      acc.w = fmaf(v.w, fo, acc.w);
+      for (int k = 0; k < kKeyWarps; ++k) {
+        const uint32_t ws = sbase + C::offStat + ((wt * kKeyWarps + k) * C::kRows + rr) * 12;
+        mm[k] = ld_shared_f32(ws);
+        ee[k] = __float_as_int(ld_shared_f32(ws + 8));
+        M = fmaxf(M, mm[k]);
+        E = imax(E, ee[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < kKeyWarps; ++k) {
+        const uint32_t ws = sbase + C::offStat + ((wt * kKeyWarps + k) * C::kRows + rr) * 12;
+        const float f = join_factor(mm[k], M);
+        L = fmaf(ld_shared_f32(ws + 4), f, L);
+        const float fo = f * unit_factor(ee[k], E);
+        const float4 v = ld_shared_f32x4(sbase + (wt * kKeyWarps + k) * C::kWarpO + (rr * kHeadDim + 4 * lane) * 4);
+        acc.x = fmaf(v.x, fo, acc.x);
+        acc.y = fmaf(v.y, fo, acc.y);
+        acc.z = fmaf(v.z, fo, acc.z);
+        acc.w = fmaf(v.w, fo, acc.w);
+      }
     }
     if (p.ws) {
       float* w = p.ws + (((int64_t)unit * (C::kRows * RT) + r) * parts + rank) * kPartFloats;

@@ -110,3 +110,32 @@ def error_bound(o, bound):
     """Largest allowed |kernel - o| for a bf16 output: half a step of bf16, 2^-8 of the value
     (2^-134 where bf16 is subnormal), and the kernel's own error."""
     return 2.0 ** -8 * (o.abs() + bound) + bound + 2.0 ** -134
+
+
+def seen_bound(q, k, v, v_unit, nq, causal, window, scale):
+    """The error that an attention kernel may make in fp32 with f16 probabilities, from the keys that
+    each row sees alone: as in `attention`, with its last term by row.  v_unit [heads, n]: the scale
+    of each key's V.  p below 2^-28 of the row's largest is off by half of f16's smallest step, which
+    is 2^-31 of the largest weight at most (V's scales are folded into p down to 2^-8), and weighs a
+    code of up to 448 in units of the largest V scale that the row sees."""
+    Sq, Hq, _ = q.shape
+    Hk, n, _ = k.shape
+    bound = torch.zeros_like(q)
+    if nq == 0 or n == 0:
+        return bound
+    pos = torch.arange(n - nq, n, device=q.device)[:, None]
+    j = torch.arange(n, device=q.device)[None, :]
+    see = torch.ones(nq, n, dtype=torch.bool, device=q.device)
+    if causal:
+        see &= j <= pos
+    if window is not None:
+        see &= (j - pos).abs() <= window
+    zero = torch.zeros((), dtype=torch.float64, device=q.device)
+    for h in range(Hq):
+        kh, vh, unit = k[h * Hk // Hq], v[h * Hk // Hq], v_unit[h * Hk // Hq]
+        s = torch.where(see, (q[:nq, h] @ kh.T) * scale, -torch.inf)
+        p = torch.where(see.any(1)[:, None], torch.softmax(s, -1), zero)
+        ds = torch.where(see, 2.0 ** -16 * (q[:nq, h].abs() @ kh.abs().T) * scale, zero).amax(-1, keepdim=True)
+        top = torch.where(see, 448.0 * unit, zero).amax(-1, keepdim=True)
+        bound[:nq, h] = (2.0 ** -11 + 2.0 ** -13 + 2 * ds) * (p @ vh.abs()) + 2.0 ** -31 * see.sum(-1, keepdim=True) * top
+    return bound

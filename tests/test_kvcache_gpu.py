@@ -931,3 +931,51 @@ def test_condition_rows_of_no_conditions_by_a_device_index(cuda):
         assert nat.device_status()[0] == BAD_ARG
         assert kv.rows(index[:0]).table.shape[0] == 0
     ok()
+
+
+def check_seen(cuda, cache, ref, rows, table, lens, q, causal, window):
+    """Through both kernels, with the allowed error of each row from the keys that it sees alone."""
+    from demon_b200 import kvcache
+    for name in ("small", "tc"):
+        os.environ["DEMON_KV_ATTENTION"] = name
+        o = kvcache.attention(q, cache, table, i32(lens, cuda), causal=causal, window=window)
+        for b, n in enumerate(lens):
+            k, v = ref.values(0, rows[b], n), ref.values(1, rows[b], n)
+            pid = torch.tensor(rows[b][:-(-n // ref.P)], device=cuda)
+            unit = torch.exp2(ref.exp[1][pid].double()).repeat_interleave(ref.P, 0)[:n].T
+            want, _ = R.attention(q[b].double(), k, v, q.shape[1], causal, window, 128 ** -0.5)
+            room = R.error_bound(want, R.seen_bound(q[b].double(), k, v, unit, q.shape[1], causal, window, 128 ** -0.5))
+            err = (o[b].double() - want).abs()
+            assert bool((err <= room).all()), f"{name} {causal} {window} b={b}: {float((err / room).nan_to_num(nan=9e9).max()):.3f}"
+    ok()
+
+
+@pytest.mark.parametrize("Sq,Hq,Hk,P,lens", [(40, 2, 1, 16, [200, 77]), (5, 3, 1, 16, [66, 34]), (150, 4, 2, 32, [300, 64]),
+                                             (9, 1, 1, 16, [9000]), (33, 2, 2, 64, [9100])])
+@pytest.mark.parametrize("low,high", [(-120, 110), (110, -120), (-60, 70), (-3, 4)])
+def test_scales_of_pages_that_a_row_does_not_see(cuda, Sq, Hq, Hk, P, lens, low, high):
+    """V around 2^low before the middle of the rows' last positions and 2^high from there: a row's result
+    has the precision of the pages that it sees, whatever the scales of those that its neighbours see."""
+    g = torch.Generator().manual_seed(Sq)
+    n = max(lens)
+    k, v = (torch.randn(len(lens), n, Hk, 128, generator=g) for _ in range(2))
+    for b, L in enumerate(lens):
+        turn = (L - min(Sq, L) // 2) // P * P
+        v[b] *= torch.exp2(torch.where(torch.arange(n) < turn, low, high).double()).float()[:, None, None]
+    cache, ref, table, rows = held(k, v, lens, P, cuda, 112)
+    q = queries(len(lens), Sq, Hq, cuda, Sq)
+    for causal, window in ((True, None), (True, 11), (False, 3), (False, 20)):
+        check_seen(cuda, cache, ref, rows, table, lens, q, causal, window)
+
+
+@pytest.mark.parametrize("Sq", [1, 9, 150])
+@pytest.mark.parametrize("step", [3, 11, 40, -3, -11, -40])
+def test_page_scales_far_apart_row_by_row(cuda, Sq, step):
+    """V's scale rises or falls by 2^step from page to page, each row held to what it sees."""
+    n = 16 * max(2, 80 // abs(step))
+    g = torch.Generator().manual_seed(113)
+    k, v = (torch.randn(1, n, 1, 128, generator=g) for _ in range(2))
+    v = v * torch.exp2((torch.arange(n) // 16).double() * step).float()[None, :, None, None]
+    cache, ref, table, rows = held(k, v, [n], 16, cuda, 113)
+    for causal, window in ((True, None), (False, 17)):
+        check_seen(cuda, cache, ref, rows, table, [n], queries(1, Sq, 2, cuda, 4), causal, window)
