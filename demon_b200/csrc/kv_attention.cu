@@ -55,6 +55,7 @@ constexpr int kHalf = kTile * kHeadDim;    // one stage's K (or V) codes, 8 KB
 constexpr int kKeyWarps = 4;               // per row group: two per tile, on alternating tiles
 constexpr float kPBias = 14.0f;            // p is scaled by 2^14 (see above)
 constexpr int kFoldMin = -8;               // smallest V scale, relative to e_ref, folded into P
+constexpr float kMaxFactor = 1.3e36f;      // of a score: a zero score stays zero (its page's scale may be a hidden key's)
 constexpr int kSpread = 64;                // V exponents of a CTA's keys up to which its rows share e_ref
 
 // NR: 8-row MMA tiles per warp; RT: row groups (of four warps) per CTA.
@@ -183,7 +184,7 @@ __device__ __forceinline__ void row_of_wide_scales(const AttnParams& p, int b, i
       const int pid = page_id(p.table + b * p.ld_table, p.W, j0 / p.c.P, p.c.pages);
       if (pid < 0) continue;  // (reported by the copying warp)
       const int64_t ph = (int64_t)pid * p.c.heads + hk, at = (ph * p.c.P + j0 % p.c.P) * kHeadDim + 4 * lane;
-      const float f = fac * fabsf(__ldg(p.c.scale[0] + ph));
+      const float f = fminf(fac * fabsf(__ldg(p.c.scale[0] + ph)), kMaxFactor);
       const int ev = scale_exp(__ldg(p.c.scale[1] + ph));
       const int is = imax(unit, ev);
       const float vf = unit_factor(ev, is);
@@ -463,7 +464,7 @@ __global__ void __launch_bounds__(Cfg<NR, RT>::kThreads) __maxnreg__((Cfg<NR, RT
         for (int z = 0; z < 2; ++z)
 #pragma unroll
           for (int r = 0; r < NR; ++r) {
-            const float f0 = fac[r][0] * sk[z], f1 = fac[r][1] * sk[z];
+            const float f0 = fminf(fac[r][0] * sk[z], kMaxFactor), f1 = fminf(fac[r][1] * sk[z], kMaxFactor);
             sa[z][r][0] *= f0;
             sa[z][r][1] *= f1;
             sa[z][r][2] *= f0;

@@ -979,3 +979,15 @@ def test_page_scales_far_apart_row_by_row(cuda, Sq, step):
     cache, ref, table, rows = held(k, v, [n], 16, cuda, 113)
     for causal, window in ((True, None), (False, 17)):
         check_seen(cuda, cache, ref, rows, table, [n], queries(1, Sq, 2, cuda, 4), causal, window)
+
+
+@pytest.mark.parametrize("Sq", [1, 5, 150])
+@pytest.mark.parametrize("big", [1e38, 3e30])
+def test_a_page_scale_from_keys_that_are_not_seen(cuda, Sq, big):
+    """Zero keys in a page whose scale comes from keys behind the length: the scores are zero, not 0 * inf."""
+    g = torch.Generator().manual_seed(Sq)
+    k, v = torch.zeros(1, 48, 1, 128), torch.randn(1, 48, 1, 128, generator=g)
+    k[:, 40:] = big
+    cache, ref, table, rows = held(k, v, [48], 16, cuda, 114)
+    q = torch.full((1, Sq, 2, 128), big, dtype=torch.bfloat16, device=cuda)
+    check_attention(cuda, cache, ref, rows, table, [40], q)
