@@ -963,7 +963,8 @@ int launch_tc(kv::AttnParams p, const DemonKvAttnArgs* a, cudaStream_t st) {
 
 enum class Kernel { kRows8, kRows16, kRows32, kTc };
 
-Kernel kernel_for(const DemonKvAttnArgs* a) {
+// `workspace`: there is one (its size is checked when the kernel that takes it is launched).
+Kernel kernel_for(const DemonKvAttnArgs* a, bool workspace) {
   const int G = a->Hq / a->cache.heads;
   const int64_t rows = (int64_t)a->Sq * G;
   // DEMON_KV_ATTENTION=small / tc takes one of the two kernels for every call (tests, measurements)
@@ -974,13 +975,14 @@ Kernel kernel_for(const DemonKvAttnArgs* a) {
   if (G > 128 || (force && std::strcmp(force, "small") == 0)) return Kernel::kRows32;
   // More rows: the lesser of two estimates, with the keys that the table covers, or those of the
   // window.  The small kernel reads the keys once per 32 rows, at about 2 TB/s; the tensor-core kernel
-  // see above.  8 kv heads, both measured: 24 rows over 16,384 keys small 31 us, tc 39; 128 rows over
+  // see above (without a workspace it takes whole key ranges: 64 tokens of 8 heads over one kv head and
+  // 20,000 keys 387 us, the small kernel 82, parts 41).  8 kv heads, both measured: 24 rows over 16,384 keys small 31 us, tc 39; 128 rows over
   // 20,000 keys 81 and 44; 60 rows over 4 x 20,000 keys 130 and 120, 1,500 rows over 16 x 256 keys 597
   // and 64; 2 heads, 600 rows over 4,096 keys 37 and 38; 1 head, 240 rows over 2,000 keys 22 and 32.
   double keys = (double)a->W * a->cache.page_size;
   if (a->window >= 0) keys = std::min(keys, 256.0 / G + a->window * (a->causal ? 1.0 : 2.0));
   const double us_small = (double)a->B * a->cache.heads * (double)((rows + 31) / 32) * keys * 256.0 / 2.0e6;
-  return plan_tc(a, true).us < us_small ? Kernel::kTc : Kernel::kRows32;
+  return plan_tc(a, workspace).us < us_small ? Kernel::kTc : Kernel::kRows32;
 }
 
 }  // namespace
@@ -1004,7 +1006,7 @@ extern "C" int demon_kv_attention(const DemonKvAttnArgs* a, void* stream) {
   p.causal = a->causal != 0, p.window = std::min(a->window, kv::kMaxTokens - 2);
   p.scale_log2 = (float)((double)a->scale * 1.4426950408889634);
   p.status = status_word();
-  switch (kernel_for(a)) {
+  switch (kernel_for(a, a->workspace != nullptr)) {
     case Kernel::kTc: return launch_tc(p, a, (cudaStream_t)stream);
     case Kernel::kRows8: return launch_small<1, 1>(p, a, (cudaStream_t)stream);
     case Kernel::kRows16: return launch_small<2, 1>(p, a, (cudaStream_t)stream);
@@ -1014,7 +1016,7 @@ extern "C" int demon_kv_attention(const DemonKvAttnArgs* a, void* stream) {
 
 extern "C" int64_t demon_kv_attention_workspace(const DemonKvAttnArgs* a) {
   if (kv_attn_check(a) != DEMON_OK || a->B == 0 || a->Sq == 0) return 0;  // (the call itself says why)
-  switch (kernel_for(a)) {
+  switch (kernel_for(a, true)) {
     case Kernel::kTc: return plan_tc(a, true).ws_bytes;
     case Kernel::kRows8: return plan_small<1, 1>(a, true).ws_bytes;
     case Kernel::kRows16: return plan_small<2, 1>(a, true).ws_bytes;

@@ -470,9 +470,10 @@ typedef struct DemonKvAttnArgs {
 DEMON_API int demon_kv_attention(const DemonKvAttnArgs* args, void* stream);
 /*
  * Bytes of workspace (16-byte aligned, any contents, free again when the call's work on the stream is
- * done) with which a call of few rows over a long table runs faster; 0 when none is used.  Without
- * one (NULL) the keys are split over fewer CTAs, and the result can differ in rounding.  Looks at
- * sizes only, not at the workspace fields.
+ * done) with which a call of few rows or row blocks over a long table runs faster, its keys in parts
+ * that a second kernel joins; 0 when none is used.  At most 160 MB.  Without one (NULL) the keys are
+ * split over fewer CTAs, another kernel may be the faster one, and the result can differ in rounding.
+ * Looks at sizes only, not at the workspace fields.
  */
 DEMON_API int64_t demon_kv_attention_workspace(const DemonKvAttnArgs* args);
 

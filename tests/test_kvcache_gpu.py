@@ -991,3 +991,23 @@ def test_a_page_scale_from_keys_that_are_not_seen(cuda, Sq, big):
     cache, ref, table, rows = held(k, v, [48], 16, cuda, 114)
     q = torch.full((1, Sq, 2, 128), big, dtype=torch.bfloat16, device=cuda)
     check_attention(cuda, cache, ref, rows, table, [40], q)
+
+
+# long tables of few blocks: with a workspace the tensor-core kernel's parts are the faster choice
+@pytest.mark.parametrize("Sq,Hq,Hk,L", [(64, 8, 1, 20_000), (40, 16, 8, 12_000), (130, 4, 2, 16_000)])
+def test_the_kernel_without_a_workspace_is_chosen_for_that(cuda, Sq, Hq, Hk, L):
+    """A C caller without a workspace is not sent to a kernel that is only faster with one."""
+    from demon_b200 import _native as nat
+    cache, ref, table, rows = filled([L], 128, Hk, cuda, 115)
+    q, n, got = queries(1, Sq, Hq, cuda, Sq), i32([L], cuda), {}
+    for name in ("", "small", "tc"):
+        os.environ["DEMON_KV_ATTENTION"] = name
+        got[name] = torch.full_like(q, 3)
+        args = attention_args(q, cache, table, n, got[name], False)
+        nat.check(nat.load().demon_kv_attention(bytes(args), nat.stream_ptr()))
+        want, own = R.attention(q[0].double(), ref.values(0, rows[0], L), ref.values(1, rows[0], L), Sq, False, None, 128 ** -0.5)
+        assert bool(((got[name][0].double() - want).abs() <= R.error_bound(want, own)).all())
+    os.environ["DEMON_KV_ATTENTION"] = ""
+    assert nat.load().demon_kv_attention_workspace(bytes(args)) > 0
+    assert not torch.equal(got["small"], got["tc"]) and torch.equal(got[""], got["small"])
+    ok()
