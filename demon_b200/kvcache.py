@@ -211,6 +211,8 @@ def attention(q: torch.Tensor, cache: KVCache, table: torch.Tensor, lens: torch.
     ``out`` may be ``q`` itself; it must not overlap other rows of it.
     """
     dev = cache._index
+    if window is not None and window < 0:  # (-1 is the C struct's word for none)
+        raise nat.DemonError(nat.DEMON_ERR_INVALID, f"kv_attention: window must be None or at least 0 (got {window})")
     shape, qs = _bf16_rows(q, "q", dev)
     B, Sq, Hq, _ = shape
     tp, ld, W = _table(table, B, dev)

@@ -235,3 +235,13 @@ def test_rows_of_an_empty_list():
         assert got.table.shape == (0, 2) and got.lens.shape == (0,)
     with pytest.raises(ValueError, match="index"):
         kv.rows([[]])
+
+
+@pytest.mark.parametrize("window", [-1, -2, -(1 << 40)])
+def test_a_negative_window_is_refused(window):
+    from types import SimpleNamespace
+
+    from demon_b200 import _native as nat
+    from demon_b200.kvcache import attention
+    with pytest.raises(nat.DemonError, match="window"):
+        attention(torch.zeros(1, 1, 1, 128), SimpleNamespace(_index=0), None, None, window=window)

@@ -1011,3 +1011,13 @@ def test_the_kernel_without_a_workspace_is_chosen_for_that(cuda, Sq, Hq, Hk, L):
     assert nat.load().demon_kv_attention_workspace(bytes(args)) > 0
     assert not torch.equal(got["small"], got["tc"]) and torch.equal(got[""], got["small"])
     ok()
+
+
+@pytest.mark.parametrize("window", [-1, -2, -(1 << 40)])
+def test_a_negative_window_is_refused(cuda, window):
+    """None is no band; a negative one is a mistake, -1 (which means none in the C struct) as much as others."""
+    from demon_b200 import _native as nat
+    from demon_b200 import kvcache
+    cache, _, table, _ = filled([40], 16, 2, cuda, 116)
+    with pytest.raises(nat.DemonError, match="window"):
+        kvcache.attention(queries(1, 1, 4, cuda, 1), cache, table, i32([40], cuda), window=window)
