@@ -265,6 +265,8 @@ extern "C" int demon_kv_append(const DemonKvAppendArgs* a, void* stream) {
   DEMON_CHECK_ARG(a->S >= 0 && a->S <= kv::kMaxTokens, "kv_append: bad token count S=%d", a->S);
   if (a->B == 0 || a->S == 0) return DEMON_OK;
   DEMON_CHECK_ARG(a->k && a->v && a->start, "kv_append: null k / v / start");
+  DEMON_CHECK_ARG(a->cache.k != a->cache.v && a->cache.k_scale != a->cache.v_scale,
+                  "kv_append: the cache's K and V are one buffer");
   DEMON_CHECK_ARG(al16(a->k) && al16(a->v), "kv_append: k and v must be 16-byte aligned");
   DEMON_CHECK_ARG(a->k_seq % 8 == 0 && a->k_row % 8 == 0 && a->k_head % 8 == 0 && a->v_seq % 8 == 0 &&
                       a->v_row % 8 == 0 && a->v_head % 8 == 0,

@@ -157,7 +157,7 @@ def append(cache: KVCache, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor
     and head the scale is the smallest power of two that covers every token written since the
     page was empty; when it grows, the page's earlier tokens are rounded again.  k and v are read
     through their strides (multiples of 8 elements; columns of a fused projection work as they
-    are).  The pages a call writes must belong to one sequence each.
+    are).  The pages a call writes must belong to one sequence each and stand in its table once.
     """
     dev = cache._index
     shape, ks = _bf16_rows(k, "k", dev)

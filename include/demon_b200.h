@@ -401,7 +401,7 @@ typedef struct DemonKvCache {
  * 448 * 2^119, saturate; NaN stays NaN), and when e grew the earlier tokens' codes are rounded
  * to it.  Tokens of a page at or after start[b] + count[b]
  * keep their codes (they mean nothing under a new scale).  The pages that one call writes must
- * be different for different sequences.
+ * be different for different sequences, and for the positions of one; K and V must not be one buffer.
  */
 typedef struct DemonKvAppendArgs {
   DemonKvCache cache;

@@ -1021,3 +1021,16 @@ def test_a_negative_window_is_refused(cuda, window):
     cache, _, table, _ = filled([40], 16, 2, cuda, 116)
     with pytest.raises(nat.DemonError, match="window"):
         kvcache.attention(queries(1, 1, 4, cuda, 1), cache, table, i32([40], cuda), window=window)
+
+
+def test_append_refuses_one_buffer_for_k_and_v(cuda):
+    """K and V may be one buffer for reading and attention, but not to write both into."""
+    from demon_b200 import _native as nat
+    from demon_b200 import kvcache
+    cache, _, table, _ = filled([40], 16, 2, cuda, 117)
+    x = queries(1, 3, 2, cuda, 1)
+    for one in (kvcache.KVCache(cache.k, cache.k, cache.k_scale, cache.k_scale),
+                kvcache.KVCache(cache.k, cache.v, cache.k_scale, cache.k_scale)):
+        with pytest.raises(nat.DemonError, match="one buffer"):
+            kvcache.append(one, x, x, table, i32([5], cuda))
+    ok()
