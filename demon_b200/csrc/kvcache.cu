@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(kReadThreads) read_kernel(const ReadParams p) 
 static bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 int kv_cache_check(const DemonKvCache* c, const char* who) {
-  DEMON_CHECK_ARG(c->k && c->v && c->k_scale && c->v_scale, "%s: null cache buffer", who);
+  DEMON_CHECK_ARG(c->pages == 0 || (c->k && c->v && c->k_scale && c->v_scale), "%s: null cache buffer", who);
   DEMON_CHECK_ARG(al16(c->k) && al16(c->v), "%s: cache codes must be 16-byte aligned", who);
   DEMON_CHECK_ARG(((uintptr_t)c->k_scale & 3) == 0 && ((uintptr_t)c->v_scale & 3) == 0,
                   "%s: cache scales must be 4-byte aligned", who);
@@ -265,7 +265,7 @@ extern "C" int demon_kv_append(const DemonKvAppendArgs* a, void* stream) {
   DEMON_CHECK_ARG(a->S >= 0 && a->S <= kv::kMaxTokens, "kv_append: bad token count S=%d", a->S);
   if (a->B == 0 || a->S == 0) return DEMON_OK;
   DEMON_CHECK_ARG(a->k && a->v && a->start, "kv_append: null k / v / start");
-  DEMON_CHECK_ARG(a->cache.k != a->cache.v && a->cache.k_scale != a->cache.v_scale,
+  DEMON_CHECK_ARG(a->cache.pages == 0 || (a->cache.k != a->cache.v && a->cache.k_scale != a->cache.v_scale),
                   "kv_append: the cache's K and V are one buffer");
   DEMON_CHECK_ARG(al16(a->k) && al16(a->v), "kv_append: k and v must be 16-byte aligned");
   DEMON_CHECK_ARG(a->k_seq % 8 == 0 && a->k_row % 8 == 0 && a->k_head % 8 == 0 && a->v_seq % 8 == 0 &&

@@ -1034,3 +1034,22 @@ def test_append_refuses_one_buffer_for_k_and_v(cuda):
         with pytest.raises(nat.DemonError, match="one buffer"):
             kvcache.append(one, x, x, table, i32([5], cuda))
     ok()
+
+
+def test_a_cache_without_pages(cuda, which):
+    """No page at all: nothing to append to, zeros read, rows that see no key."""
+    from demon_b200 import _native as nat
+    from demon_b200 import kvcache
+    cache = kvcache.KVCache.empty(0, 2, 16, cuda)
+    table, zero, one = i32([[-1, -1]], cuda), i32([0], cuda), i32([1], cuda)
+    x = queries(1, 3, 2, cuda, 1)
+    kvcache.append(cache, x, x, table, zero, zero)
+    for Sq in (1, 140):
+        assert not bool(kvcache.attention(queries(1, Sq, 4, cuda, 1), cache, table, zero).any())
+    assert not bool(kvcache.read(cache, table, zero, 9)[0].any())
+    ok()
+    kvcache.append(cache, x, x, table, zero, one)
+    for Sq in (1, 140):
+        assert not bool(kvcache.attention(queries(1, Sq, 4, cuda, 1), cache, table, one).any())
+    torch.cuda.synchronize()
+    assert nat.device_status()[0] == BAD_ARG
