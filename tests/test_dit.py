@@ -267,3 +267,47 @@ def test_cross_attention_from_the_8_bit_cache(cuda):
         assert torch.equal(same, run((first, L)))
     with pytest.raises(ValueError, match="e4m3"):
         m.encoder_kv(enc, cache="int8")
+
+
+@pytest.mark.gpu
+def test_each_layer_attends_over_its_own_cached_condition(cuda, monkeypatch):
+    """What every cross-attention gives to its o_proj is the attention of its queries over its layer's
+    cached K / V of the condition that rows() names, within the kernel's own rounding (the whole-forward
+    bar above is that of the NVFP4 linears behind it)."""
+    import kv_reference as R
+    from demon_b200 import dit, kvcache
+    d = _fixture()
+    m = _model(d, cuda)
+    enc, t = d["enc"].to(cuda), d["t"].to(cuda)
+    L, n = enc.shape[1], d["x"].shape[0]
+    g = torch.Generator().manual_seed(7)
+    enc = torch.cat([enc[:1], torch.randn(2, *enc.shape[1:], generator=g).to(enc)])      # three different conditions
+    index = [2, 0, 1, 2, 0][:n]
+    queries, outputs = [], []
+    attend, out = kvcache.attention, dit.Attention._out
+
+    def attention(q, *args, **kw):
+        queries.append(q.clone())
+        return attend(q, *args, **kw)
+
+    def _out(self, o, *args):
+        if self.cross:
+            outputs.append(o.clone())
+        return out(self, o, *args)
+    monkeypatch.setattr(kvcache, "attention", attention)
+    monkeypatch.setattr(dit.Attention, "_out", _out)
+    with torch.no_grad():
+        kv, _ = m.encoder_kv(enc, cache="e4m3", page_size=32)
+        plain, _ = m.encoder_kv(enc)
+        m(hidden_states=d["x"].to(cuda), timestep=t, timestep_r=t, context_latents=d["ctx"].to(cuda),
+          encoder_kv=([c.rows(index) for c in kv], L))
+    assert len(queries) == len(outputs) == len(m.layers)
+    for layer, (q, o) in enumerate(zip(queries, outputs)):
+        k, v = kvcache.read(kv[layer].cache, kv[layer].table, kv[layer].lens, L)
+        raw = plain[layer].float().view(3, L, 2, -1, 128)
+        for x, r in ((k, raw[:, :, 0]), (v, raw[:, :, 1])):   # that layer's values: half a step of E4M3 off at most
+            assert bool(((x.float() - r).abs() <= torch.maximum(r.abs() * 2.0 ** -4, r.abs().max() * 2.0 ** -17)).all())
+        for b, i in enumerate(index):
+            want, own = R.attention(q[b].double(), k[i].transpose(0, 1).double(), v[i].transpose(0, 1).double(), q.shape[1], False,
+                                    None, 128 ** -0.5)
+            assert bool(((o.view(q.shape)[b].double() - want).abs() <= R.error_bound(want, own)).all()), (layer, b)

@@ -245,3 +245,29 @@ def test_a_negative_window_is_refused(window):
     from demon_b200.kvcache import attention
     with pytest.raises(nat.DemonError, match="window"):
         attention(torch.zeros(1, 1, 1, 128), SimpleNamespace(_index=0), None, None, window=window)
+
+
+def _attention_args(B, Sq, Hq, Hk, W, P, window=-1):
+    """An argument block of these sizes; the planner looks at no buffer (only that there are some)."""
+    from demon_b200 import _native as nat
+    a = nat.DemonKvAttnArgs(B=B, Sq=Sq, Hq=Hq, W=W, window=window, causal=1, scale=0.1, q=16, o=16, table=16, ld_table=W, lens=16)
+    a.cache = nat.DemonKvCache(k=16, v=16, k_scale=16, v_scale=16, pages=1, heads=Hk, page_size=P, head_dim=128)
+    return bytes(a)
+
+
+def test_workspaces_of_every_size_of_call():
+    """Where the Python call does not ask for a workspace the planner would use none, and none exceeds 160 MB."""
+    from demon_b200 import _build, _native as nat
+    _build.build()
+    size = nat.load().demon_kv_attention_workspace
+    used = most = 0
+    for Hk, G in ((1, 1), (8, 2), (4, 3), (2, 7), (1, 16), (8, 8), (1, 128), (1, 130)):
+        for B in (1, 2, 3, 5, 9, 16, 18, 40, 73, 147):
+            for Sq in (1, 2, 3, 5, 8, 16, 17, 33, 64, 100, 200, 500, 1000, 4000):
+                few = Sq * G <= 16
+                for keys in (16, 128, 512, 896, 912, 1024, 2048, 8128, 8192, 9600, 20000, 100000, 1 << 20):
+                    for window in (-1, 500, 6000, 50000):
+                        n = size(_attention_args(B, Sq, Hk * G, Hk, keys // 16, 16, window))
+                        assert n >= 0 and (n == 0 or keys > (8_128 if few else 896)), (Hk, G, B, Sq, keys, window)
+                        used, most = used + (n > 0), max(most, n)
+    assert used > 1000 and 2 ** 26 < most <= 160_000_000

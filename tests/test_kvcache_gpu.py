@@ -1053,3 +1053,53 @@ def test_a_cache_without_pages(cuda, which):
         assert not bool(kvcache.attention(queries(1, Sq, 4, cuda, 1), cache, table, one).any())
     torch.cuda.synchronize()
     assert nat.device_status()[0] == BAD_ARG
+
+
+@pytest.mark.parametrize("Sq,Hq,Hk,P,lens", [(40, 4, 2, 64, [5000, 3100]), (130, 8, 1, 16, [4000]), (300, 2, 2, 128, [9000, 0]),
+                                             (70, 3, 1, 32, [1300]), (33, 100, 1, 64, [2200])])
+def test_blocks_of_rows_without_a_workspace(cuda, Sq, Hq, Hk, P, lens):
+    """The tensor-core kernel over whole key ranges where it would take parts with a workspace."""
+    from demon_b200 import _native as nat
+    cache, ref, table, rows = filled(lens, P, Hk, cuda, 119)
+    q, n = queries(len(lens), Sq, Hq, cuda, Sq), i32(lens, cuda)
+    os.environ["DEMON_KV_ATTENTION"] = "tc"
+    out = torch.full_like(q, 3)
+    args = attention_args(q, cache, table, n, out, True)
+    assert nat.load().demon_kv_attention_workspace(bytes(args)) > 0
+    nat.check(nat.load().demon_kv_attention(bytes(args), nat.stream_ptr()))
+    for b, L in enumerate(lens):
+        k, v = ref.values(0, rows[b], L), ref.values(1, rows[b], L)
+        exact, own = R.attention(q[b].double(), k, v, Sq, True, None, 128 ** -0.5)
+        assert bool(((out[b].double() - exact).abs() <= R.error_bound(exact, own)).all())
+    ok()
+
+
+@pytest.mark.parametrize("Sq,Hq", [(1, 16), (12, 2), (20_000, 16)])
+def test_values_over_a_million_keys(cuda, Sq, Hq, which):
+    """V of 1 + noise, so that an output is near 1 and the tolerance below means something: the table
+    names 8 pages again and again, and every row equals the row over these 8 pages.
+
+    Tolerance: two bf16 outputs, 2^-8 each at most; f16 probabilities 2^-11 of sum p |v| twice; the long
+    call adds at most 2^16 matrix instructions of 16 keys into an fp32 accumulator, each dropping at most
+    2^-23 of sum p |v|, and as many fp32 additions into the softmax sum (2^-24 each).
+    """
+    from demon_b200 import kvcache
+    if Sq == 20_000 and which == "small":
+        pytest.skip("the few-row kernel takes minutes for that many rows")
+    table, rows, pages = make_table([1024], 128, cuda, 124)
+    g = torch.Generator().manual_seed(124)
+    cache, ref = kvcache.KVCache.empty(pages, 1, 128, cuda), R.RefCache(pages, 1, 128, cuda)
+    k, v = torch.randn(1, 1024, 1, 128, generator=g), 1 + 0.25 * torch.randn(1, 1024, 1, 128, generator=g)
+    k, v = k.to(torch.bfloat16).to(cuda), v.to(torch.bfloat16).to(cuda)
+    kvcache.append(cache, k, v, table, i32([0], cuda))
+    ref.append(k, v, rows, [0], [1024])
+    q = queries(1, min(Sq, 500), Hq, cuda, 5)
+    long = table[:, :8].repeat(1, 1024).contiguous()
+    o = kvcache.attention(q.repeat(1, -(-Sq // 500), 1, 1), cache, long, i32([1 << 20], cuda))
+    want, _ = R.attention(q[0].double(), ref.values(0, rows[0], 1024), ref.values(1, rows[0], 1024), q.shape[1], False, None, 128 ** -0.5)
+    ok()
+    mass, _ = R.attention(q[0].double(), ref.values(0, rows[0], 1024), ref.values(1, rows[0], 1024).abs(), q.shape[1], False, None,
+                          128 ** -0.5)
+    room = 2.0 ** -8 * want.abs() + (2.0 ** -10 + 2.0 ** 16 * (2.0 ** -23 + 2.0 ** -24)) * mass
+    for i in range(0, Sq, 500 * 13):
+        assert bool(((o[0, i:i + 500].double() - want[:o.shape[1] - i]).abs() <= room[:o.shape[1] - i]).all()), i
