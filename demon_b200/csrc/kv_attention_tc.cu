@@ -134,6 +134,14 @@ __device__ __forceinline__ void setmaxnreg_dec() {
 __device__ __forceinline__ void st_shared_u16(uint32_t a, uint32_t x) {
   asm volatile("st.shared.u16 [%0], %1;" ::"r"(a), "h"((unsigned short)x) : "memory");
 }
+__device__ __forceinline__ void st_shared_b32(uint32_t a, uint32_t x) {
+  asm volatile("st.shared.b32 [%0], %1;" ::"r"(a), "r"(x) : "memory");
+}
+__device__ __forceinline__ uint32_t ld_shared_b32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
 // 4-D tiled load.
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tmap, uint64_t* bar, int32_t x, int32_t y, int32_t z,
                                             int32_t u) {

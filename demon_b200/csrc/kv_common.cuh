@@ -58,26 +58,9 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
 // 0x80 in every byte of w that is E4M3's NaN.
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
 
-__device__ __forceinline__ void st_shared_b32(uint32_t a, uint32_t x) {
-  asm volatile("st.shared.b32 [%0], %1;" ::"r"(a), "r"(x) : "memory");
-}
-__device__ __forceinline__ uint32_t ld_shared_b32(uint32_t a) {
-  uint32_t v;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
-  return v;
-}
 __device__ __forceinline__ float ld_shared_f32(uint32_t a) {
   float v;
   asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
-  return v;
-}
-
-__device__ __forceinline__ void st_shared_f32x2(uint32_t a, float x, float y) {
-  asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(a), "f"(x), "f"(y) : "memory");
-}
-__device__ __forceinline__ float2 ld_shared_f32x2(uint32_t a) {
-  float2 v;
-  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
   return v;
 }
 __device__ __forceinline__ void st_shared_f32x4(uint32_t a, float x, float y, float z, float w) {

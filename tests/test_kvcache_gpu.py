@@ -951,7 +951,8 @@ def check_seen(cuda, cache, ref, rows, table, lens, q, causal, window):
 
 
 @pytest.mark.parametrize("Sq,Hq,Hk,P,lens", [(40, 2, 1, 16, [200, 77]), (5, 3, 1, 16, [66, 34]), (150, 4, 2, 32, [300, 64]),
-                                             (9, 1, 1, 16, [9000]), (33, 2, 2, 64, [9100])])
+                                             (9, 1, 1, 16, [9000]), (33, 2, 2, 64, [9100]),
+                                             (4, 2, 1, 16, [70, 18]), (8, 1, 1, 32, [9000, 40])])
 @pytest.mark.parametrize("low,high", [(-120, 110), (110, -120), (-60, 70), (-3, 4)])
 def test_scales_of_pages_that_a_row_does_not_see(cuda, Sq, Hq, Hk, P, lens, low, high):
     """V around 2^low before the middle of the rows' last positions and 2^high from there: a row's result
