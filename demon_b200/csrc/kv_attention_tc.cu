@@ -475,7 +475,15 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       uint32_t issued = 0;  // halves
       Unit w;
       bool ok = true;
-      const uint32_t bytes = (uint32_t)(p.Tt * p.G) * kHeadDim * 2;
+      const int q_rows = p.Tt * p.G;
+      const uint32_t bytes = (uint32_t)q_rows * kHeadDim * 2;
+      // Rows behind the last whole token: no copy writes them.  Zeros, since what shared memory held could
+      // vote for the softmax's second exponential, which rounds the sums of the warp's other rows
+      // differently.  (Zeroed by all threads at the start: 6,016 x 6,016 keys 333 -> 347 us, by the softmax
+      // warps 341: the compiler's choices in their loop.)
+      for (int i = lane; i < (kBlk - q_rows) * 32; i += 32)
+        st_shared_v4(sbase + offQ + ((i >> 4) & 1) * kTile + ((i >> 3) & 1) * kBox + (q_rows + (i >> 5)) * 128 + (i & 7) * 16, 0, 0, 0, 0);
+      __syncwarp();
       for (; ok && next_unit(&j, &w); ++it)
         for (int h = 0; h < 2; ++h) {
           if (!(ok = warp_wait(&q_empty[h], (it & 1u) ^ 1u, abort_flag, p, 91))) break;
@@ -651,12 +659,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
     };
     uint32_t j = 0;
     const uint32_t s_addr = tmem + lane_addr + kColS + 128 * h;
-    if (ri >= p.Tt) {
-      // Rows behind the last whole token: no copy writes their Q.  Zeros, since what shared memory held
-      // could vote for the second exponential below, which rounds the sums of the warp's other rows
-      // differently.  (That vote by rows with a token only: prompt 180 -> 183.5 us.)
-      for (int k = 0; k < 16; ++k) st_shared_v4(sbase + offQ + h * kTile + rr * 128 + (k >> 3) * kBox + (k & 7) * 16, 0, 0, 0, 0);
-    }
     // This thread's row of the unit's Q in place, bf16 -> f16 times 2^-e, once the copy has landed;
     // the score factor of the row in *f
     auto q_convert = [&](uint32_t unit, float* f) {
