@@ -180,6 +180,7 @@ __device__ __forceinline__ void row_of_wide_scales(const AttnParams& p, int b, i
     const float by = exp2i(-k), fac = exp2i(k) * p.scale_log2;
     const Keys see = visible(i, i, len, nq, p.causal != 0, p.window);
     const int lo = imax(see.lo, from), hi = imin(see.hi, to);
+#pragma unroll 1
     for (int j0 = lo & ~15; j0 < hi; j0 += 16) {
       const int pid = page_id(p.table + b * p.ld_table, p.W, j0 / p.c.P, p.c.pages);
       if (pid < 0) continue;  // (reported by the copying warp)
@@ -190,6 +191,7 @@ __device__ __forceinline__ void row_of_wide_scales(const AttnParams& p, int b, i
       const float vf = unit_factor(ev, is);
       float back = unit_factor(unit, is);
       unit = is;
+#pragma unroll 1
       for (int j = imax(j0, lo); j < imin(j0 + 16, hi); ++j) {
         uint32_t a[2], c[2];
         e4m3x4_f16(__ldg(reinterpret_cast<const uint32_t*>(p.c.codes[0] + at + (j - j0) * kHeadDim)), a[0], a[1]);
@@ -660,15 +662,26 @@ __global__ void __launch_bounds__(Cfg<NR, RT>::kThreads) __maxnreg__((Cfg<NR, RT
   // the CTA's four partial results of each row into one: a warp per row, four channels a lane
   constexpr int n_warps = kKeyWarps * RT + 1;
   const int rows_here = imin(C::kRows * RT, n_rows - row0);
-  const bool wide = *wide_flag != 0;
-  for (int r = warp; r < rows_here; r += n_warps) {
-    const int wt = r / C::kRows, rr = r % C::kRows;
-    float mm[kKeyWarps], M = -INFINITY, L = 0.0f;
-    int ee[kKeyWarps], E = kMinExp;
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (wide) {
-      row_of_wide_scales(p, b, hk, row0 + r, len, nq, first * kTile, (first + n_tiles) * kTile, lane, M, L, E, acc);
-    } else {
+  const auto put_row = [&](int r, float M, float L, int E, const float4& acc) {
+    if (p.ws) {
+      float* w = p.ws + (((int64_t)unit * (C::kRows * RT) + r) * parts + rank) * kPartFloats;
+      *reinterpret_cast<float4*>(w + 4 * lane) = acc;
+      if (lane == 0) *reinterpret_cast<float4*>(w + kHeadDim) = make_float4(M, L, __int_as_float(E), 1.0f);
+      return;
+    }
+    st_shared_f32x4(sbase + C::offSum + (r * kHeadDim + 4 * lane) * 4, acc.x, acc.y, acc.z, acc.w);
+    if (lane == 0) {
+      const uint32_t wr = sbase + C::offRow + r * 12;
+      st_shared_f32(wr, M);
+      st_shared_f32(wr + 4, L);
+      st_shared_f32(wr + 8, __int_as_float(E));
+    }
+  };
+  if (__builtin_expect(*wide_flag == 0, 1)) {
+    for (int r = warp; r < rows_here; r += n_warps) {
+      const int wt = r / C::kRows, rr = r % C::kRows;
+      float mm[kKeyWarps], M = -INFINITY, L = 0.0f;
+      int ee[kKeyWarps], E = kMinExp;
 #pragma unroll
       for (int k = 0; k < kKeyWarps; ++k) {
         const uint32_t ws = sbase + C::offStat + ((wt * kKeyWarps + k) * C::kRows + rr) * 12;
@@ -677,6 +690,7 @@ __global__ void __launch_bounds__(Cfg<NR, RT>::kThreads) __maxnreg__((Cfg<NR, RT
         M = fmaxf(M, mm[k]);
         E = imax(E, ee[k]);
       }
+      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
       for (int k = 0; k < kKeyWarps; ++k) {
         const uint32_t ws = sbase + C::offStat + ((wt * kKeyWarps + k) * C::kRows + rr) * 12;
@@ -689,19 +703,15 @@ __global__ void __launch_bounds__(Cfg<NR, RT>::kThreads) __maxnreg__((Cfg<NR, RT
         acc.z = fmaf(v.z, fo, acc.z);
         acc.w = fmaf(v.w, fo, acc.w);
       }
+      put_row(r, M, L, E, acc);
     }
-    if (p.ws) {
-      float* w = p.ws + (((int64_t)unit * (C::kRows * RT) + r) * parts + rank) * kPartFloats;
-      *reinterpret_cast<float4*>(w + 4 * lane) = acc;
-      if (lane == 0) *reinterpret_cast<float4*>(w + kHeadDim) = make_float4(M, L, __int_as_float(E), 1.0f);
-      continue;
-    }
-    st_shared_f32x4(sbase + C::offSum + (r * kHeadDim + 4 * lane) * 4, acc.x, acc.y, acc.z, acc.w);
-    if (lane == 0) {
-      const uint32_t wr = sbase + C::offRow + r * 12;
-      st_shared_f32(wr, M);
-      st_shared_f32(wr + 4, L);
-      st_shared_f32(wr + 8, __int_as_float(E));
+  } else {
+    for (int r = warp; r < rows_here; r += n_warps) {
+      float M, L;
+      int E;
+      float4 acc;
+      row_of_wide_scales(p, b, hk, row0 + r, len, nq, first * kTile, (first + n_tiles) * kTile, lane, M, L, E, acc);
+      put_row(r, M, L, E, acc);
     }
   }
   if (p.ws) return;  // attention_join_kernel does the rest
@@ -751,12 +761,22 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const A
   // maximum, unit and sum of weights: every warp the same
   float M = -INFINITY, L = 0.0f;
   int E = kMinExp;
-  for (int k = lane; k < p.parts; k += 32) {
-    const float4 st = *reinterpret_cast<const float4*>(w + (int64_t)k * kPartFloats + kHeadDim);
-    const float n = fmaxf(M, st.x);
-    L = fmaf(st.y, join_factor(st.x, n), L * join_factor(M, n));
+  for (int k0 = 0; k0 < p.parts; k0 += 128) {
+    float4 st[4];  // (loads first: in a chain with the sums they took a microsecond of 30)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int k = k0 + 32 * i + lane;
+      st[i] = k < p.parts ? *reinterpret_cast<const float4*>(w + (int64_t)k * kPartFloats + kHeadDim)
+                          : make_float4(-INFINITY, 0.0f, __int_as_float(kMinExp), 0.0f);
+    }
+    const float n = fmaxf(fmaxf(fmaxf(M, st[0].x), fmaxf(st[1].x, st[2].x)), st[3].x);
+    L *= join_factor(M, n);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      L = fmaf(st[i].y, join_factor(st[i].x, n), L);
+      E = imax(E, __float_as_int(st[i].z));
+    }
     M = n;
-    E = imax(E, __float_as_int(st.z));
   }
   float top = M;
 #pragma unroll
