@@ -12,10 +12,10 @@
 // launch, no workspace), or, for long tables, over as many CTAs as fill the SMs, joined by a second
 // kernel through a workspace.
 //
-// Measured, 8 kv heads: one token (16 query heads) over 750 keys 7 us, the launch and a few rounds of
-// latency; one token of 48 sequences of up to 8,192 keys (32 query heads), 452 MB of codes, 80.5 us
-// (5.6 TB/s); one token of 16 sequences of 16,384 keys 91 us (5.9 TB/s); five tokens of two sequences
-// of up to 100,001 keys, 379 MB, 82 us (4.6 TB/s: 10 rows take twice the matrix instructions for the
+// Measured, 8 kv heads: one token (16 query heads) over 750 keys 7.5 us, the launch and a few rounds of
+// latency; one token of 48 sequences of up to 8,192 keys (32 query heads), 452 MB of codes, 81 us
+// (5.6 TB/s); one token of 16 sequences of 16,384 keys 93 us (5.8 TB/s); five tokens of two sequences
+// of up to 100,001 keys, 379 MB, 83.5 us (4.5 TB/s: 10 rows take twice the matrix instructions for the
 // same bytes; six key warps a CTA were slower, 155 against 140 us at 16 CTAs a unit).
 //
 // A warp's step on 32 keys, all in registers (mma.sync m16n8k16, fp32 accumulators), with the keys

@@ -33,12 +33,12 @@
 //   warp 15           the list of units: lengths and masks into a ring of records that every role reads.
 // Tensor memory as in attention.cu: S_h at 128 h, P_h over its upper half, O_h at 256 + 128 h.
 //
-// Bound by the softmax warps' path from S to P (some 3,000 clocks per tile and half, of which the
+// Bound by the softmax warps' path from S to P (2,830 clocks per tile and half, of which the
 // exponentials' rate asks for 1,024) and, for short key ranges (256 keys of a condition are two
 // tiles), by the units' Q conversion and output (Q converted by warpgroup 2 after the unit's first
 // tile: 69 us for 16 x 750 over 256 keys against 64).  Measured, 16 query heads over 8: 6,016 x 6,016
-// 327 to 334 us (0.89 to 0.91 PFLOP/s; the bf16 kernel of attention.cu 264 us), 16 x 750 over 256 keys
-// 64 us (bf16 34 us), 6,001 causal 179 to 182 us.  Slower, not kept: steps of 64 keys with two score
+// 333 us (0.89 PFLOP/s; the bf16 kernel of attention.cu 267 us), 16 x 750 over 256 keys 64.5 us (bf16
+// 34.5 us), 6,001 causal 180 us.  Slower, not kept: steps of 64 keys with two score
 // buffers (Q K^T 64 wide takes the tensor core longer, and the overheads of a step double: 396 us at
 // 6,016 x 6,016); two threads per row (466 us); the next scores loaded ahead of the exponentials
 // (509 us, they come late).

@@ -453,9 +453,11 @@ class DemonDiT(nn.Module):
         ``cache="e4m3"`` keeps them in the paged 8-bit cache (:mod:`demon_b200.kvcache`), half the
         memory of bf16 (24 layers of 256 tokens: 12.6 MB a condition), as one :class:`CrossCache`
         per layer; ``[c.rows(index) for c in kv]`` lets several sequences share a condition's
-        pages.  E4M3 rounds every K and V element by up to 2^-4 of itself, and the cache's
-        attention picks its kernel by the whole call's size, so a sequence's bits may then
-        depend on the batch it is computed in.
+        pages.  It saves memory, not time: attention over it takes 64.5 us where the bf16 kernel
+        takes 34.5 (16 x 750 queries over 256 tokens).  An element of K or V is off by up to 2^-4
+        of itself or 2^-10 of its page's scale, whichever is more (the scale is at most 1/224 of
+        the page's largest), and the cache's attention picks its kernel by the whole call's size,
+        so a sequence's bits may then depend on the batch it is computed in.
         """
         if cache not in (None, "e4m3"):
             raise ValueError(f"encoder_kv: cache must be None or 'e4m3', got {cache!r}")
