@@ -996,9 +996,10 @@ Kernel kernel_for(const DemonKvAttnArgs* a, bool workspace) {
   // More rows: the lesser of two estimates, with the keys that the table covers, or those of the
   // window.  The small kernel reads the keys once per 32 rows, at about 2 TB/s; the tensor-core kernel
   // see above (without a workspace it takes whole key ranges: 64 tokens of 8 heads over one kv head and
-  // 20,000 keys 387 us, the small kernel 82, parts 41).  8 kv heads, both measured: 24 rows over 16,384 keys small 31 us, tc 39; 128 rows over
-  // 20,000 keys 81 and 44; 60 rows over 4 x 20,000 keys 130 and 120, 1,500 rows over 16 x 256 keys 597
-  // and 64; 2 heads, 600 rows over 4,096 keys 37 and 38; 1 head, 240 rows over 2,000 keys 22 and 32.
+  // 20,000 keys 387 us, the small kernel 82, parts 41).  8 kv heads, both measured: 24 rows over 16,384
+  // keys small 32 us, tc 39; 128 rows over 20,000 keys 81 and 45; 60 rows over 4 x 20,000 keys 130 and
+  // 122, 1,500 rows over 16 x 256 keys 597 and 64; 2 heads, 600 rows over 4,096 keys 37 and 38; 1 head,
+  // 240 rows over 2,000 keys 22 and 32.
   double keys = (double)a->W * a->cache.page_size;
   if (a->window >= 0) keys = std::min(keys, 256.0 / G + a->window * (a->causal ? 1.0 : 2.0));
   const double us_small = (double)a->B * a->cache.heads * (double)((rows + 31) / 32) * keys * 256.0 / 2.0e6;
